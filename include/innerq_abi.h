@@ -387,6 +387,83 @@ int iq_decode_attention_noalloc(const void* q, int64_t sq_b, int64_t sq_h, const
                                 int B, int Hq, int Hkv, int T, int D, float scale,
                                 void* out, int64_t so_b, int64_t so_h, void* stream);
 
+/* ---- Many sequences of different lengths: 4-bit pages and packed prompts --------------------------------
+ *
+ * A pool of pages is shared by S sequences.  A page holds 64 tokens of every KV head, K and V in 4-bit asym groups
+ * of 32 along head_dim (quant.py:58-77 of each token's row: the same codes, scales and zero points).  One (page,
+ * head) is 2 * 64 * (D/8 + D/32) 32-bit words (U = D/8, G = D/32):
+ *     K codes  uint32 [64 tokens][U]             word o: codes of dims 8o .. 8o+7, code i at bits 4i
+ *     K meta   uint16 [64 tokens][G][2]          {scale, zero}
+ *     V codes  uint32 [8 blocks][U][8 tokens]    token t of the page: block t/32*4 + t%16/4, place t%4 + t/16%2*4
+ *     V meta   uint16 [8 blocks][G][2][8 tokens] scales, then zeros
+ * A code stands for c*s + z, rounded to the activation dtype.
+ *
+ * table[s * s_table + i] is the page of sequence s's tokens [64 i, 64 i + 64), lens[s] its token count (see each
+ * call), both read on the device: a captured call follows their values.  What they hold is checked there, before any
+ * access: an entry that names no page of the pool, or a token past P * 64 (or past the rotation's rows, or of a
+ * negative length), is not accessed, and the call ORs IQ_PAGED_BAD_* into *status, which nothing here clears.  Two
+ * sequences may share pages that no call writes. */
+enum iq_paged_status {
+  IQ_PAGED_BAD_PAGE = 1,  /* a table entry outside [0, n_pages) was needed */
+  IQ_PAGED_BAD_TOKEN = 2  /* a token past the table's P * 64 or past the rotation's rows, or a negative length */
+};
+
+typedef struct iq_paged {
+  uint32_t* pages;       /* [n_pages][H][words], 16-byte aligned */
+  int64_t n_pages;
+  const int32_t* table;  /* [S][P], row stride s_table */
+  int64_t s_table;
+  const int32_t* lens;   /* [S] */
+  int32_t* status;       /* one word */
+  int S, P, H, D;
+  int mode;              /* IQ_MODE_ASYM, IQ_MODE_BF16 for bf16 activations */
+} iq_paged;
+
+/* Bytes of one page (H heads). */
+int iq_page_bytes(int H, int D, int64_t* bytes);
+
+/* Appends N new tokens: those of sequence s are rows [cu[s], cu[s+1]) of k and v [N, H, D] (cu int32 [S+1] on the
+ * device, non-decreasing; NULL: one token per sequence, N = S) and become its tokens lens[s] + i (lens: tokens held
+ * before).  Rows outside [cu[0], cu[S]) are left out.  cos, sin (both or neither): fp32 [n_pos][R/2]; k's first R
+ * dims (R <= D, a multiple of 16) are rotated by row lens[s] + i before they are quantized,
+ *     y[d] = x[d] cos[d] - x[d + R/2] sin[d],  y[d + R/2] = x[d + R/2] cos[d] + x[d] sin[d],  d < R/2,
+ * in fp32 with each product rounded, then rounded to the activation dtype.  q [N, Hq, D] (or NULL) is written rotated
+ * (unrotated without cos) to q_out, which may be q.  Strides in elements, multiples of 8; D contiguous, 16-byte
+ * aligned.  A sequence's rows must not lie in a page that another sequence's rows of this call lie in. */
+int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, const void* k, int64_t sk_n, int64_t sk_h,
+                    const void* v, int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int64_t n_pos, int R,
+                    const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* q_out, int64_t so_n, int64_t so_h,
+                    void* stream);
+
+/* The values of tokens lens[s] + i of every sequence (i < cu[s+1] - cu[s], as iq_paged_append), written to rows
+ * cu[s] + i of k_out and v_out [N, H, D]; NaN for a token that the checks above refuse; rows outside [cu[0], cu[S])
+ * are not written. */
+int iq_paged_read(const iq_paged* p, const int32_t* cu, int N, void* k_out, int64_t sk_n, int64_t sk_h, void* v_out,
+                  int64_t sv_n, int64_t sv_h, void* stream);
+
+/* softmax(q K^T scale) V over the pages for m (1 .. 16) new tokens per sequence: q [S, m, Hq, D], lens[s] the tokens
+ * held with the new ones, so token j of the m sees keys below lens[s] - (m - 1 - j), with window > 0 only the last
+ * `window` of them.  Logits, softmax statistics and sums in fp32, the weights rounded to the activation dtype for
+ * their product with V.  A row that sees no key is 0; a sequence that needs a page outside the pool gives NaN.  Any
+ * Hq that H divides.  workspace: iq_paged_attention_workspace_bytes (0: none needed), 16-byte aligned. */
+size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D);
+int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
+                       float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* softmax(q K^T scale) V of S prompts that lie one behind the other: q, out [N, Hq, D], k, v [Nk, H, D] (fp16, or
+ * bf16 with mode IQ_MODE_BF16; strides in elements, multiples of 8; D contiguous, 16-byte aligned).  Rows [cu_q[s],
+ * cu_q[s+1]) attend to keys [cu_k[s], cu_k[s+1]) (int32 [S+1] on the device, non-decreasing; bounds outside [0, N] or
+ * [0, Nk] are moved to them).  causal: the last row sees all keys, row i of lq all but the lq - 1 - i last of lk;
+ * window > 0 (causal only): only the last `window` of those.  Logits, softmax statistics and sums in fp32, the weights
+ * rounded to the activation dtype for their product with V.  A row that sees no key is 0; rows of q outside
+ * [cu_q[0], cu_q[S]) are not written.  k and v may be NULL
+ * with Nk = 0.  Key strides below 2^23.  Any Hq that H divides; no workspace. */
+int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
+                        const void* v, int64_t sv_n, int64_t sv_h, const int32_t* cu_q, const int32_t* cu_k, int S, int N,
+                        int Nk, int Hq, int H, int D, int mode, float scale, int causal, int window, void* out,
+                        int64_t so_n, int64_t so_h, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

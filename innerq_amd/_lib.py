@@ -74,6 +74,14 @@ class iq_split_plan(ctypes.Structure):
                 ("pair_e0", ctypes.c_int), ("bf16", ctypes.c_int), ("reserved", ctypes.c_int * 2)]
 
 
+class iq_paged(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_void_p), ("n_pages", ctypes.c_int64),
+                ("table", ctypes.c_void_p), ("s_table", ctypes.c_int64),
+                ("lens", ctypes.c_void_p), ("status", ctypes.c_void_p),
+                ("S", ctypes.c_int), ("P", ctypes.c_int), ("H", ctypes.c_int), ("D", ctypes.c_int),
+                ("mode", ctypes.c_int)]
+
+
 SIGNATURES = {
     "iq_abi_version": (I, []),
     "iq_strerror": (ctypes.c_char_p, [I]),
@@ -106,6 +114,12 @@ SIGNATURES = {
     "iq_decode_attention_splits_live": (I, [P, L, L, P, ctypes.POINTER(iq_segment), ctypes.POINTER(iq_segment),
                                             I, I, I, I, I, F, P, S, ctypes.POINTER(iq_split_plan), P]),
     "iq_decode_attention_combine_live": (I, [ctypes.POINTER(iq_split_plan), I, I, I, I, P, L, L, P, S, P]),
+    "iq_page_bytes": (I, [I, I, ctypes.POINTER(L)]),
+    "iq_paged_append": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P, P, L, I, P, L, L, I, P, L, L, P]),
+    "iq_paged_read": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P]),
+    "iq_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I]),
+    "iq_paged_attention": (I, [ctypes.POINTER(iq_paged), P, L, L, L, I, I, F, I, P, L, L, L, P, S, P]),
+    "iq_prompt_attention": (I, [P, L, L, P, L, L, P, L, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P]),
     "iq_decode_noalloc_max_bytes": (S, []),
     "iq_decode_attention_noalloc": (I, [P, L, L, P, ctypes.POINTER(iq_segment), ctypes.POINTER(iq_segment),
                                         I, I, I, I, I, F, P, L, L, P]),

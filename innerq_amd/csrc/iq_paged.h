@@ -1,0 +1,107 @@
+// 4-bit pages (gfx950), shared by iq_paged.hip (append, read) and iq_paged_attn.hip.
+//
+// A page holds 64 tokens of every KV head, K and V both in 4-bit asym groups of 32 along head_dim, so a token is
+// whole in its page as soon as it is appended: sequences of any lengths append one token or many without an fp16
+// window, and no two tokens share a word.  One (page, head) is one run of 32-bit words (U = D/8, G = D/32):
+//
+//   K codes  [64 tokens][U]            a token's row: one 16-byte load per lane is one group (D = 128)
+//   K meta   [64 tokens][G]            {scale, zero} halves
+//   V codes  [8 blocks][U][8 tokens]   one lane's two 16-byte loads are 8 dims of the 8 tokens of an MFMA operand
+//   V meta   [8 blocks][G][8 scales | 8 zeros]
+//
+// A word is 8 codes of one token (dims 8o .. 8o+7, code i at bits 4i).  V block b = t/32*4 + t%16/4 holds the tokens
+// whose logits one lane of the QK^T product's result holds (t%4 and t/16%2 give the place in it), so the softmax
+// weights are the next product's operand where they are, with no exchange between lanes.
+#pragma once
+#include "iq_common.h"
+#include "iq_device.h"
+
+namespace iq {
+
+constexpr int PAGE = 64, PGROUP = 32;
+__host__ __device__ constexpr int page_km(int D) { return PAGE * (D / 8); }                 // K meta's first word
+__host__ __device__ constexpr int page_vc(int D) { return PAGE * (D / 8 + D / 32); }        // V codes'
+__host__ __device__ constexpr int page_vm(int D) { return page_vc(D) + PAGE * (D / 8); }    // V meta's
+__host__ __device__ constexpr int page_words(int D) { return 2 * PAGE * (D / 8 + D / 32); }
+__host__ __device__ constexpr int v_block(int t) { return t / 32 * 4 + t % 16 / 4; }
+__host__ __device__ constexpr int v_place(int t) { return t % 4 + t / 16 % 2 * 4; }
+
+// bits of a store's status word (iq_paged.status)
+constexpr int32_t PAGED_BAD_PAGE = IQ_PAGED_BAD_PAGE, PAGED_BAD_TOKEN = IQ_PAGED_BAD_TOKEN;
+
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+typedef float fl2_t __attribute__((ext_vector_type(2)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+
+// two floats rounded to the activation dtype (nearest even), as one dword
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const fl2_t x = {a, b};
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf2_t));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, h2_t));
+}
+
+template <bool BF>
+__device__ __forceinline__ float lo_half(uint32_t w) { return BF ? __uint_as_float(w << 16) : float(__builtin_bit_cast(h2_t, w).x); }
+template <bool BF>
+__device__ __forceinline__ float hi_half(uint32_t w) {
+  return BF ? __uint_as_float(w & 0xffff0000u) : float(__builtin_bit_cast(h2_t, w).y);
+}
+
+// ---- values of packed codes: RN(c s + z) in the activation dtype ---------------------------------------------
+// fp16: codes become fp16 integers by an exponent pattern or-ed over their bits (1024 + c, or 64 + c for a field at
+// bit 4), the pattern's value is subtracted (exact), and one packed fma rounds c s + z once.  bf16 has no packed
+// arithmetic on gfx950: fp32 (c s is exact there, the sum rounds to 24 bits first, as the reference's fp32
+// dequantization followed by a cast).
+
+// the four pairs {code i of a, code i of b}, i = 0..3, of two 16-bit fields a (low half) and b (high half)
+__device__ __forceinline__ void pairs4(uint32_t x, h2_t (&c)[4]) {
+  const h2_t b0 = {_Float16(1024.f), _Float16(1024.f)}, b1 = {_Float16(64.f), _Float16(64.f)};
+  const uint32_t y = x >> 8;
+  c[0] = __builtin_bit_cast(h2_t, (x & 0x000f000fu) | 0x64006400u) - b0;
+  c[1] = __builtin_bit_cast(h2_t, (x & 0x00f000f0u) | 0x54005400u) - b1;
+  c[2] = __builtin_bit_cast(h2_t, (y & 0x000f000fu) | 0x64006400u) - b0;
+  c[3] = __builtin_bit_cast(h2_t, (y & 0x00f000f0u) | 0x54005400u) - b1;
+}
+// the values of one token's word w with meta {s, z}: dwords of the pairs (0,4), (1,5), (2,6), (3,7)
+template <bool BF>
+__device__ __forceinline__ u4_t k_values(uint32_t w, uint32_t meta) {
+  u4_t r;
+  if constexpr (!BF) {
+    const h2_t m = __builtin_bit_cast(h2_t, meta), s = {m.x, m.x}, z = {m.y, m.y};
+    h2_t c[4];
+    pairs4(w, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[i], s, z));
+  } else {
+    const float s = __uint_as_float(meta << 16), z = __uint_as_float(meta & 0xffff0000u);
+    const uint32_t e = w & 0x0f0f0f0fu, o = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6 and 1 3 5 7
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = i & 1 ? o : e;
+      const int b = i / 2 * 8;
+      r[i] = pack2<true>(__builtin_fmaf(float((x >> b) & 0xffu), s, z), __builtin_fmaf(float((x >> (b + 16)) & 0xffu), s, z));
+    }
+  }
+  return r;
+}
+
+// ---- sequences -----------------------------------------------------------------------------------------------
+// token n of a flat list belongs to sequence s at place i (cu null: one token each); false: to none
+__device__ __forceinline__ bool sequence_of(const int32_t* cu, int S, int n, int& s, int& i) {
+  if (!cu) { s = n; i = 0; return n < S; }
+  int lo = 0, hi = S;  // cu[lo] <= n < cu[hi], where there is such a sequence
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (cu[mid] <= n) lo = mid; else hi = mid;
+  }
+  s = lo;
+  i = n - cu[lo];
+  return i >= 0 && n < cu[lo + 1];
+}
+
+}  // namespace iq

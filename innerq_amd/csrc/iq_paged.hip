@@ -1,0 +1,267 @@
+// Appending to and reading 4-bit pages (gfx950): iq_paged_append, iq_paged_read.
+//
+// append: U = D/8 lanes hold one token of one head, 8 values each.  A lane that rotates reads its own 8 values and
+// the 8 of its partner half (the second read hits L1), so neither the rotation nor a q rotated in place needs LDS;
+// the group's minimum and maximum go over the 4 lanes of a group by DPP.
+#include "iq_paged.h"
+#include "iq_quantize.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+struct AppendArgs {
+  iq_paged p;
+  const int32_t* cu;
+  int N, Hq;
+  const uint16_t *k, *v, *q;
+  int64_t sk_n, sk_h, sv_n, sv_h, sq_n, sq_h;
+  uint16_t* qo;
+  int64_t so_n, so_h;
+  const float *cos, *sin;
+  int64_t n_pos;
+  int R;
+};
+
+template <bool BF>
+__device__ __forceinline__ void load8(const uint16_t* x, float (&f)[8]) {
+  const u4_t w = *reinterpret_cast<const u4_t*>(x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = lo16(w[i], BF);
+    f[2 * i + 1] = hi16(w[i], BF);
+  }
+}
+
+// min / max over the 4 lanes of a quad, NaN propagating
+__device__ __forceinline__ float quad_min(float x) {
+  x = __builtin_elementwise_minimum(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, true)));
+  return __builtin_elementwise_minimum(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float quad_max(float x) {
+  x = __builtin_elementwise_maximum(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, true)));
+  return __builtin_elementwise_maximum(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, true)));
+}
+
+// the 4-bit word of 8 values and its group's meta word (quant.py's asymmetric form, every op rounded to the type)
+template <bool BF>
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& meta) {
+  float mn = x[0], mx = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    mn = __builtin_elementwise_minimum(mn, x[i]);
+    mx = __builtin_elementwise_maximum(mx, x[i]);
+  }
+  const GroupQ g = group_params<4, IQ_MODE_ASYM, BF>(quad_min(mn), quad_max(mx), 0.f);
+  uint32_t w = 0;
+  if (!g.slow) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = round_act(__fmul_rn(round_act(x[i] - g.z, BF), g.r), BF);
+      w |= uint32_t(__float2int_rn(fminf(y, 15.f))) << (4 * i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= asym_field_b(asym_code_b(x[i], g.z, g.s, 4, BF), 4) << (4 * i);
+  }
+  meta = meta_word(g.s, g.z, BF);
+  return w;
+}
+
+// rotation of the 8 values f (dims 8o ..) with their partners p: fp32 products, each rounded, as separate torch ops
+template <bool BF>
+__device__ __forceinline__ void rotate8(float (&f)[8], const float (&p)[8], const float (&c)[8], const float (&s)[8],
+                                        bool second) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = f[i] * c[i], b = p[i] * s[i];
+    f[i] = round_act(second ? a + b : a - b, BF);
+  }
+}
+
+template <int D, bool BF>
+__global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a, int heads_per_block) {
+  constexpr int U = D / 8, TOK = THREADS / U;
+  const int o = threadIdx.x % U, n = blockIdx.x * TOK + threadIdx.x / U;
+  int s, i;
+  if (n >= a.N || !sequence_of(a.cu, a.p.S, n, s, i)) return;
+  const int held = a.p.lens[s];
+  const int64_t at = int64_t(held) + i;
+  const int H = a.p.H, heads = 2 * H + (a.q ? a.Hq : 0);
+  int32_t bad = 0, page = -1;
+  if (held < 0 || at >= int64_t(a.p.P) * PAGE || (a.cos && at >= a.n_pos)) bad = PAGED_BAD_TOKEN;
+  else {
+    page = a.p.table[s * a.p.s_table + at / PAGE];
+    if (page < 0 || page >= a.p.n_pages) bad = PAGED_BAD_PAGE;
+  }
+  if (bad) {  // the token is left out
+    if (o == 0 && blockIdx.y == 0) atomicOr(a.p.status, bad);
+    return;
+  }
+  const int row = int(at % PAGE);
+  const bool turn = a.cos && 8 * o < a.R, second = 16 * o >= a.R;
+  float c[8], sn[8];
+  if (turn) {
+    const int64_t d = at * (a.R / 2) + 8 * o - (second ? a.R / 2 : 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f4_t x = *reinterpret_cast<const f4_t*>(a.cos + d + 4 * j), y = *reinterpret_cast<const f4_t*>(a.sin + d + 4 * j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { c[4 * j + e] = x[e]; sn[4 * j + e] = y[e]; }
+    }
+  }
+  const int partner = (second ? -a.R : a.R) / 2;
+  const int h1 = min(heads, int(blockIdx.y + 1) * heads_per_block);
+  for (int h = blockIdx.y * heads_per_block; h < h1; ++h) {
+    const bool isv = h >= H && h < 2 * H, isq = h >= 2 * H;
+    const int hh = isq ? h - 2 * H : isv ? h - H : h;
+    const uint16_t* x = isq ? a.q + n * a.sq_n + hh * a.sq_h : isv ? a.v + n * a.sv_n + hh * a.sv_h
+                                                                   : a.k + n * a.sk_n + hh * a.sk_h;
+    x += 8 * o;
+    float f[8];
+    load8<BF>(x, f);
+    if (turn && !isv) {
+      float p[8];
+      load8<BF>(x + partner, p);
+      rotate8<BF>(f, p, c, sn, second);
+    }
+    if (isq) {
+      u4_t w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack2<BF>(f[2 * j], f[2 * j + 1]);
+      *reinterpret_cast<u4_t*>(a.qo + n * a.so_n + hh * a.so_h + 8 * o) = w;
+      continue;
+    }
+    uint32_t meta;
+    const uint32_t w = quantize8<BF>(f, meta);
+    uint32_t* pg = a.p.pages + (int64_t(page) * H + hh) * page_words(D);
+    if (!isv) {
+      pg[row * U + o] = w;
+      if (o % 4 == 0) pg[page_km(D) + row * (D / 32) + o / 4] = meta;
+    } else {
+      const int b = v_block(row), e = v_place(row);
+      pg[page_vc(D) + (b * U + o) * 8 + e] = w;
+      if (o % 4 == 0) {
+        uint16_t* m = reinterpret_cast<uint16_t*>(pg + page_vm(D)) + (b * (D / 32) + o / 4) * 16 + e;
+        m[0] = uint16_t(meta);
+        m[8] = uint16_t(meta >> 16);
+      }
+    }
+  }
+}
+
+struct ReadArgs {
+  iq_paged p;
+  const int32_t* cu;
+  int N;
+  uint16_t *k, *v;
+  int64_t sk_n, sk_h, sv_n, sv_h;
+};
+
+// a lane: 8 values of one token of one head of K or V
+template <int D, bool BF>
+__global__ __launch_bounds__(THREADS) void read_kernel(ReadArgs a) {
+  constexpr int U = D / 8, TOK = THREADS / U;
+  const int o = threadIdx.x % U, n = blockIdx.x * TOK + threadIdx.x / U;
+  int s, i;
+  if (n >= a.N || !sequence_of(a.cu, a.p.S, n, s, i)) return;
+  const int held = a.p.lens[s];
+  const int64_t at = int64_t(held) + i;
+  const int H = a.p.H, hh = blockIdx.y % H;
+  const bool isv = int(blockIdx.y) >= H;
+  int32_t bad = 0, page = -1;
+  if (held < 0 || at >= int64_t(a.p.P) * PAGE) bad = PAGED_BAD_TOKEN;
+  else {
+    page = a.p.table[s * a.p.s_table + at / PAGE];
+    if (page < 0 || page >= a.p.n_pages) bad = PAGED_BAD_PAGE;
+  }
+  uint16_t* out = (isv ? a.v + n * a.sv_n + hh * a.sv_h : a.k + n * a.sk_n + hh * a.sk_h) + 8 * o;
+  u4_t r;
+  if (bad) {  // no such token: NaN
+    if (o == 0 && blockIdx.y == 0) atomicOr(a.p.status, bad);
+    r = u4_t{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+  } else {
+    const int row = int(at % PAGE);
+    const uint32_t* pg = a.p.pages + (int64_t(page) * H + hh) * page_words(D);
+    uint32_t w, meta;
+    if (!isv) {
+      w = pg[row * U + o];
+      meta = pg[page_km(D) + row * (D / 32) + o / 4];
+    } else {
+      const int b = v_block(row), e = v_place(row);
+      w = pg[page_vc(D) + (b * U + o) * 8 + e];
+      const uint16_t* m = reinterpret_cast<const uint16_t*>(pg + page_vm(D)) + (b * (D / 32) + o / 4) * 16 + e;
+      meta = uint32_t(m[0]) | uint32_t(m[8]) << 16;
+    }
+    const u4_t x = k_values<BF>(w, meta);  // pairs (0,4) (1,5) (2,6) (3,7) -> (0,1) (2,3) (4,5) (6,7)
+    r = u4_t{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
+             __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+  }
+  *reinterpret_cast<u4_t*>(out) = r;
+}
+
+inline bool rows_ok(const void* p, int64_t s_n, int64_t s_h) { return aligned(p, 16) && s_n % 8 == 0 && s_h % 8 == 0; }
+
+template <typename F>
+int by_format(int D, int mode, F&& f) {
+  if (D == 128) return mode & IQ_MODE_BF16 ? f.template operator()<128, true>() : f.template operator()<128, false>();
+  return mode & IQ_MODE_BF16 ? f.template operator()<64, true>() : f.template operator()<64, false>();
+}
+
+}  // namespace
+
+namespace iq {
+int check_paged(const iq_paged* p) {
+  IQ_CHECK(p && p->pages && p->table && p->lens && p->status, IQ_ERR_NULL);
+  IQ_CHECK(base_mode(p->mode) == IQ_MODE_ASYM, IQ_ERR_MODE);
+  IQ_CHECK(d_ok(p->D) && p->H > 0 && p->H <= 4096 && p->S > 0 && p->P > 0 && p->n_pages > 0, IQ_ERR_SHAPE);
+  IQ_CHECK(p->P <= INT32_MAX / PAGE && p->n_pages <= INT32_MAX && p->s_table >= 0, IQ_ERR_SHAPE);
+  IQ_CHECK(aligned(p->pages, 16) && aligned(p->table, 4) && aligned(p->lens, 4) && aligned(p->status, 4), IQ_ERR_ALIGN);
+  return IQ_OK;
+}
+}  // namespace iq
+
+extern "C" int iq_page_bytes(int H, int D, int64_t* bytes) {
+  IQ_CHECK(bytes, IQ_ERR_NULL);
+  IQ_CHECK(d_ok(D) && H > 0 && H <= 4096, IQ_ERR_SHAPE);
+  *bytes = int64_t(H) * page_words(D) * 4;
+  return IQ_OK;
+}
+
+extern "C" int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, const void* k, int64_t sk_n, int64_t sk_h,
+                               const void* v, int64_t sv_n, int64_t sv_h, const float* cos, const float* sin,
+                               int64_t n_pos, int R, const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* q_out,
+                               int64_t so_n, int64_t so_h, void* stream) {
+  if (const int st = iq::check_paged(p)) return st;
+  IQ_CHECK((N == 0 || (k && v && (!q || q_out))) && (!cos == !sin), IQ_ERR_NULL);
+  IQ_CHECK(N >= 0 && (cu || N == p->S), IQ_ERR_SHAPE);
+  IQ_CHECK(!q || (Hq > 0 && Hq <= 4096), IQ_ERR_SHAPE);
+  IQ_CHECK(!cos || (R > 0 && R <= p->D && R % 16 == 0 && n_pos > 0), IQ_ERR_SHAPE);
+  IQ_CHECK(rows_ok(k, sk_n, sk_h) && rows_ok(v, sv_n, sv_h) && aligned(cos, 16) && aligned(sin, 16), IQ_ERR_ALIGN);
+  IQ_CHECK(!q || (rows_ok(q, sq_n, sq_h) && rows_ok(q_out, so_n, so_h)), IQ_ERR_ALIGN);
+  if (N == 0) return IQ_OK;
+  const AppendArgs a{*p, cu, N, Hq, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)q, sk_n, sk_h, sv_n, sv_h,
+                     sq_n, sq_h, (uint16_t*)q_out, so_n, so_h, cos, sin, n_pos, R};
+  return by_format(p->D, p->mode, [&]<int D, bool BF>() {
+    const int tiles = int(ceil_div(N, THREADS / (D / 8))), heads = 2 * p->H + (q ? Hq : 0);
+    const int hpb = tiles >= 256 ? 8 : 1;
+    append_kernel<D, BF><<<dim3(tiles, unsigned(ceil_div(heads, hpb))), THREADS, 0, (hipStream_t)stream>>>(a, hpb);
+    return launch_status();
+  });
+}
+
+extern "C" int iq_paged_read(const iq_paged* p, const int32_t* cu, int N, void* k_out, int64_t sk_n, int64_t sk_h,
+                             void* v_out, int64_t sv_n, int64_t sv_h, void* stream) {
+  if (const int st = iq::check_paged(p)) return st;
+  IQ_CHECK(N == 0 || (k_out && v_out), IQ_ERR_NULL);
+  IQ_CHECK(N >= 0 && (cu || N == p->S), IQ_ERR_SHAPE);
+  IQ_CHECK(rows_ok(k_out, sk_n, sk_h) && rows_ok(v_out, sv_n, sv_h), IQ_ERR_ALIGN);
+  if (N == 0) return IQ_OK;
+  const ReadArgs a{*p, cu, N, (uint16_t*)k_out, (uint16_t*)v_out, sk_n, sk_h, sv_n, sv_h};
+  return by_format(p->D, p->mode, [&]<int D, bool BF>() {
+    const unsigned tiles = unsigned(ceil_div(N, THREADS / (D / 8)));
+    read_kernel<D, BF><<<dim3(tiles, 2u * p->H), THREADS, 0, (hipStream_t)stream>>>(a);
+    return launch_status();
+  });
+}

@@ -1,0 +1,609 @@
+// Attention of one or a few new tokens per sequence over 4-bit pages (gfx950): iq_paged_attention.
+//
+// Flash decoding over a ragged batch: the pages of all (sequence, KV head, tile of 16 query rows) lie behind one
+// another in one list, which the workgroups share out evenly (read from the sequences' lengths on the device, so a
+// captured call follows them); a workgroup's four waves take its pages in turn, each with its own running maximum,
+// sum and accumulators, merged over LDS at the end of each (sequence, head).  Where a (sequence, head) spans several
+// workgroups, their fp32 partials go to the workspace and a second launch merges them in a fixed order.
+//
+// One page, one wave: K's words become the A operands of v_mfma_f32_16x16x32 (16 tokens x 32 dims; the B operand is
+// the query rows, held in registers), whose result has a query row per lane and 4 tokens per lane; its exponentials,
+// rounded to the activation dtype, are the B operand of V^T P^T as they are (iq_paged.h's V blocks).
+#include "iq_paged.h"
+
+using namespace iq;
+
+namespace {
+
+constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 16;
+constexpr float NEG_INF = -__builtin_inff();
+
+struct AttnArgs {
+  iq_paged p;
+  const uint16_t* q;
+  int64_t sq_s, sq_m, sq_h;
+  uint16_t* out;
+  int64_t so_s, so_m, so_h;
+  int m, nrep, tiles;  // new tokens per sequence, query heads per KV head, tiles of 16 rows (row = token * nrep + head)
+  float scale;         // times log2(e)
+  int window;          // 0: none
+  int grid;
+  float* ws;
+  int split;           // 0: a workgroup takes a whole (sequence, head, tile)
+};
+
+// pages that sequence s reads: [lo, lo + n)
+__device__ __forceinline__ int pages_of(const AttnArgs& a, int s, int& lo) {
+  const int len = min(a.p.lens[s], a.p.P * PAGE);
+  lo = a.window ? max(0, len - a.m + 1 - a.window) / PAGE : 0;
+  return len > 0 ? (len + PAGE - 1) / PAGE - lo : 0;
+}
+
+// inclusive scan over the wave's 64 lanes
+__device__ __forceinline__ int wave_scan(int v) {
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int x = __shfl_up(v, o, 64);
+    if (int(threadIdx.x & 63) >= o) v += x;
+  }
+  return v;
+}
+
+// units (pages times heads and tiles) of all sequences
+__device__ __forceinline__ int total_units(const AttnArgs& a) {
+  int t = 0, lo;
+  for (int s0 = 0; s0 < a.p.S; s0 += 64) {
+    const int s = s0 + int(threadIdx.x & 63);
+    t += s < a.p.S ? pages_of(a, s, lo) : 0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+  return __builtin_amdgcn_readfirstlane(t) * a.p.H * a.tiles;
+}
+// the sequence that holds unit u, and its first unit (u < total)
+__device__ __forceinline__ void find_unit(const AttnArgs& a, int u, int& s, int& first) {
+  const int per = a.p.H * a.tiles;
+  int base = 0, lo;
+  for (int s0 = 0; s0 < a.p.S; s0 += 64) {
+    const int i = s0 + int(threadIdx.x & 63);
+    const int n = i < a.p.S ? pages_of(a, i, lo) * per : 0;
+    const int end = base + wave_scan(n);
+    const uint64_t past = __ballot(end > u);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      s = s0 + l;
+      first = __builtin_amdgcn_readlane(end - n, l);
+      return;
+    }
+    base = __builtin_amdgcn_readlane(end, 63);
+  }
+  s = a.p.S;
+  first = base;
+}
+__device__ __forceinline__ int units_per_group(int total, int grid) {
+  return max((total + grid - 1) / grid, 4);  // a page per wave at least
+}
+
+// row r of tile t of sequence s: its query head offset (head in the group, token)
+struct Row {
+  int token, head;
+  bool real;
+};
+__device__ __forceinline__ Row row_of(const AttnArgs& a, int tile, int r) {
+  const int i = tile * ROWS + r, token = i / a.nrep;
+  return {token, i - token * a.nrep, token < a.m};
+}
+
+// one lane's part of a page: its K words and meta (4 tiles of 16 tokens), its V words and meta (2 blocks)
+struct KRegs {
+  u4_t c[4];  // D = 64: two words used
+  uint32_t m[4];
+};
+struct VRegs {
+  u4_t c[2][2], s[2], z[2];
+};
+
+// A page is read through a buffer descriptor of its own (one page's bytes; none for a page outside the pool): lane
+// offsets stay in 32 bits and the offsets within a page in the instructions' immediates.  Each byte is read once:
+// the loads leave the caches to others.
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr int STREAM = 2;  // non-temporal
+
+template <int D>
+struct Lane {
+  uint32_t kc, km, vc, vm;  // the lane's byte offsets into a page
+  __device__ __forceinline__ Lane() {
+    constexpr int U = D / 8, G = D / 32;
+    const uint32_t lane = threadIdx.x & 63, l = lane & 15, quarter = lane >> 4;
+    const uint32_t octet = D == 128 ? l : l / 2;
+    kc = (l * U + quarter * (U / 4)) * 4;
+    km = (page_km(D) + l * G + (D == 128 ? quarter : quarter / 2)) * 4;
+    vc = (page_vc(D) + (quarter * U + octet) * 8) * 4;
+    vm = (page_vm(D) + (quarter * G + octet / 4) * 8) * 4;
+  }
+};
+__device__ __forceinline__ u4_t bload4(rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, STREAM));
+}
+
+template <int D>
+__device__ __forceinline__ void load_k(rsrc_t pg, const Lane<D>& at, KRegs& r) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t c = at.kc + t * 16 * (D / 8) * 4;
+    if constexpr (D == 128) {
+      r.c[t] = bload4(pg, c);
+    } else {
+      const u2_t x = __builtin_bit_cast(u2_t, __builtin_amdgcn_raw_buffer_load_b64(pg, c, 0, STREAM));
+      r.c[t] = u4_t{x.x, x.y, 0, 0};
+    }
+    r.m[t] = __builtin_amdgcn_raw_buffer_load_b32(pg, at.km + t * 16 * (D / 32) * 4, 0, STREAM);
+  }
+}
+template <int D>
+__device__ __forceinline__ void load_v(rsrc_t pg, const Lane<D>& at, VRegs& r) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t c = at.vc + h * 4 * (D / 8) * 32, m = at.vm + h * 4 * (D / 32) * 32;
+    r.c[h][0] = bload4(pg, c);
+    r.c[h][1] = bload4(pg, c + 16);
+    r.s[h] = bload4(pg, m);
+    r.z[h] = bload4(pg, m + 16);
+  }
+}
+
+template <bool BF>
+__device__ __forceinline__ f4_t mma(u4_t a, u4_t b, f4_t c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+}
+
+// the A operands of V^T for 32 tokens: x[j] holds, for the lane's dim j, its 8 tokens (D/16 dims per lane)
+template <int D, bool BF>
+__device__ __forceinline__ void v_operands(const u4_t (&c)[2], u4_t s, u4_t z, u4_t (&x)[D / 16]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int pr = 0; pr < 4; ++pr) {  // tokens 2 pr, 2 pr + 1
+    const uint32_t w0 = c[pr / 2][pr % 2 * 2], w1 = c[pr / 2][pr % 2 * 2 + 1];
+    const uint32_t sp = s[pr], zp = z[pr];  // (a bit_cast of a vector's element would take its first one)
+#pragma unroll
+    for (int half = 0; half < D / 64; ++half) {
+      uint32_t f;  // 16-bit fields of the two tokens: 4 dims
+      if constexpr (D == 128) f = __builtin_amdgcn_perm(w1, w0, half ? 0x07060302u : 0x05040100u);
+      else f = __builtin_amdgcn_perm(w1, w0, lane & 1 ? 0x07060302u : 0x05040100u);
+      if constexpr (!BF) {
+        h2_t cc[4];
+        pairs4(f, cc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[half * 4 + i][pr] = __builtin_bit_cast(
+              uint32_t, __builtin_elementwise_fma(cc[i], __builtin_bit_cast(h2_t, sp), __builtin_bit_cast(h2_t, zp)));
+      } else {
+        const float s0 = lo_half<BF>(sp), s1 = hi_half<BF>(sp);
+        const float z0 = lo_half<BF>(zp), z1 = hi_half<BF>(zp);
+        const uint32_t e = f & 0x0f0f0f0fu, o = (f >> 4) & 0x0f0f0f0fu;  // dims 0 2 (token 0), 0 2 (token 1); 1 3
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t y = i & 1 ? o : e;
+          const int b = i / 2 * 8;
+          x[half * 4 + i][pr] = pack2<true>(__builtin_fmaf(float((y >> b) & 0xffu), s0, z0),
+                                            __builtin_fmaf(float((y >> (b + 16)) & 0xffu), s1, z1));
+        }
+      }
+    }
+  }
+}
+
+template <int D, bool BF>
+struct Acc {
+  f4_t o[D / 16];  // dims row * D/16 + j of query row lane % 16, row = lane/16 * 4 + i
+  float m, l;
+};
+
+// the logits of a page's 64 tokens: s[t][i] of token 16 t + 4 (lane/16) + i for query row lane % 16
+template <int D, bool BF>
+__device__ __forceinline__ void logits(const KRegs& r, const u4_t (&q)[D / 32], float scale, f4_t (&s)[4]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    s[t] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) s[t] = mma<BF>(k_values<BF>(r.c[t][j], r.m[t]), q[j], s[t]);
+    s[t] *= scale;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// the running softmax over 64 more logits; s becomes the weights
+template <int D, bool BF>
+__device__ __forceinline__ void weights(f4_t (&s)[4], Acc<D, BF>& acc) {
+  float mx = acc.m;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
+  {
+    auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    x = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  }
+  const float base = mx == NEG_INF ? 0.f : mx;  // a row that has seen nothing yet
+  if (__any(mx != acc.m)) {
+    const float f = __builtin_amdgcn_exp2f(acc.m - base);
+    acc.l *= f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) acc.o[j] *= f;
+    acc.m = mx;
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
+      sum += s[t][i];
+    }
+  acc.l += sum;
+}
+
+// is any value of the tokens with these scales and zeros (pairs) an infinity or NaN?  It is where z or 15 s + z is.
+template <bool BF>
+__device__ __forceinline__ bool odd_values(uint32_t s, uint32_t z) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float zz = i ? hi_half<BF>(z) : lo_half<BF>(z), ss = i ? hi_half<BF>(s) : lo_half<BF>(s);
+    const float top = __builtin_fmaf(15.f, ss, zz);
+    const uint32_t t = pack2<BF>(top, zz);  // rounded as the values are
+    const uint32_t e = BF ? 0x7f80u : 0x7c00u;
+    odd |= (t & e) == e || ((t >> 16) & e) == e;
+  }
+  return odd;
+}
+
+// Readies 32 tokens of a page that not every row sees all of (k0: the first token's number; the row sees [low, lim),
+// no row sees tokens outside [lo, len)): tokens that no row sees, whose page rows may hold anything, get values 0.
+// A token whose values hold an infinity or NaN is taken by itself, into the rows that see it (the product would carry
+// it into every row, as 0 * inf), and then gets values 0 too.
+template <int D, bool BF>
+__device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t& z, u4_t p, Acc<D, BF>& acc, int k0, int lim,
+                                              int low, int lo, int len) {
+  const int quarter = (threadIdx.x & 63) >> 4;
+  bool odd = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t keep = 0;
+#pragma unroll
+    for (int e = 2 * w; e < 2 * w + 2; ++e) {
+      const int k = k0 + e / 4 * 16 + quarter * 4 + e % 4;
+      if (k < len && k >= lo) keep |= e & 1 ? 0xffff0000u : 0x0000ffffu;
+    }
+    s[w] &= keep;
+    z[w] &= keep;
+    odd |= odd_values<BF>(s[w], z[w]);
+  }
+  if (!__any(odd)) return;
+#pragma clang loop unroll(disable)
+  for (int t = 0; t < 32; ++t) {
+    const int qd = t / 8, e = t % 8, k = k0 + e / 4 * 16 + qd * 4 + e % 4;
+    const uint32_t half = quarter == qd ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+    u4_t st, zt, pt;
+    odd = false;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t at = w == e / 2 ? half : 0u;
+      st[w] = s[w] & at;
+      zt[w] = z[w] & at;
+      pt[w] = p[w] & at;
+      odd |= odd_values<BF>(st[w], zt[w]);
+    }
+    if (!__any(odd)) continue;
+    const bool sees = k < lim && k >= low;
+    u4_t x[D / 16];
+    v_operands<D, BF>(c, st, zt, x);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      const f4_t y = mma<BF>(x[j], pt, acc.o[j]);
+      if (sees) acc.o[j] = y;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t at = w == e / 2 ? half : 0u;
+      s[w] &= ~at;
+      z[w] &= ~at;
+    }
+  }
+}
+
+template <int D, bool BF>
+__device__ __forceinline__ void values(VRegs& r, const f4_t (&s)[4], Acc<D, BF>& acc, bool mask, int tok0, int lim, int low,
+                                       int lo, int len) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const u4_t p = {pack2<BF>(s[2 * h][0], s[2 * h][1]), pack2<BF>(s[2 * h][2], s[2 * h][3]),
+                    pack2<BF>(s[2 * h + 1][0], s[2 * h + 1][1]), pack2<BF>(s[2 * h + 1][2], s[2 * h + 1][3])};
+    if (mask) unseen_values<D, BF>(r.c[h], r.s[h], r.z[h], p, acc, tok0 + h * 32, lim, low, lo, len);
+    u4_t x[D / 16];
+    v_operands<D, BF>(r.c[h], r.s[h], r.z[h], x);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) acc.o[j] = mma<BF>(x[j], p, acc.o[j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// a slot of the workspace: 16 rows of D sums, 16 maxima, 16 sums of weights
+template <int D>
+__device__ __forceinline__ float* slot_of(float* ws, int i) { return ws + int64_t(i) * (ROWS * D + 2 * ROWS); }
+
+template <int D, bool BF>
+__device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, int tile, int r, int d, const float (&v)[8],
+                                          float inv) {
+  const Row w = row_of(a, tile, r);
+  if (!w.real) return;
+  u4_t x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = pack2<BF>(v[2 * i] * inv, v[2 * i + 1] * inv);
+  *reinterpret_cast<u4_t*>(a.out + s * a.so_s + w.token * a.so_m + (int64_t(head) * a.nrep + w.head) * a.so_h + d) = x;
+}
+
+template <int D, bool BF>
+__global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
+  constexpr int J = D / 16;
+  __shared__ float so[WAVES][ROWS][D + 4];
+  __shared__ float sm[WAVES][ROWS], sl[WAVES][ROWS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15,
+            quarter = lane >> 4;
+  const int H = a.p.H;
+  int u, u1, s = 0, first = 0;
+  if (a.split) {
+    const int total = total_units(a), per = units_per_group(total, a.grid);
+    u = min(int64_t(blockIdx.x) * per, int64_t(total));
+    u1 = min(u + per, total);
+    if (u < u1) find_unit(a, u, s, first);
+  } else {
+    s = blockIdx.x / (H * a.tiles);
+    int lo;
+    const int n = pages_of(a, s, lo);
+    u = first = 0;
+    const int hr = blockIdx.x - s * H * a.tiles;
+    u = hr * n;
+    u1 = u + n;
+  }
+  // sequences without tokens: rows of zeros
+  for (int e = a.split ? blockIdx.x : s; e < (a.split ? a.p.S : s + 1); e += a.grid) {
+    int lo;
+    if (pages_of(a, e, lo) > 0) continue;
+    const float zero[8] = {};
+    const int rows = a.m * a.nrep, nh = a.split ? H : 1;
+    for (int i = threadIdx.x; i < nh * rows * (D / 8); i += THREADS) {
+      const int d = i % (D / 8) * 8, r = i / (D / 8) % rows;
+      const int h = a.split ? i / (D / 8) / rows : blockIdx.x / a.tiles % H;
+      store_row<D, BF>(a, e, h, r / ROWS, r % ROWS, d, zero, 0.f);
+    }
+  }
+  while (u < u1) {
+    int lo;
+    int n = __builtin_amdgcn_readfirstlane(pages_of(a, s, lo));
+    if (n <= 0) { ++s; continue; }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int hr = (u - first) / n, p0 = (u - first) - hr * n, cnt = min(n - p0, u1 - u);
+    const int head = hr / a.tiles, tile = hr - head * a.tiles;
+    const int len = __builtin_amdgcn_readfirstlane(min(a.p.lens[s], a.p.P * PAGE));
+    const Row row = row_of(a, tile, l);
+    const int lim = len - (a.m - 1 - row.token), low = a.window ? lim - a.window : 0;  // the row sees keys [low, lim)
+    // the query row of this lane, its octets in the order of k_values' pairs
+    u4_t q[D / 32];
+    {
+      const uint16_t* x = a.q + s * a.sq_s + row.token * a.sq_m + (int64_t(head) * a.nrep + row.head) * a.sq_h +
+                          quarter * (D / 4);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        u4_t w = {0, 0, 0, 0};
+        if (row.real) w = *reinterpret_cast<const u4_t*>(x + 8 * j);
+        q[j] = u4_t{__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
+                    __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
+      }
+    }
+    Acc<D, BF> acc;
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc.o[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+    acc.m = NEG_INF;
+    acc.l = 0.f;
+    const int32_t* table = a.p.table + s * a.p.s_table + lo + p0;
+    const int mine = wave < cnt ? (cnt - wave + WAVES - 1) / WAVES : 0;  // this wave's pages: wave, wave + 4, ...
+    int ids = 0;
+    const uint32_t* pages = a.p.pages + int64_t(head) * page_words(D);
+    const int64_t stride = int64_t(H) * page_words(D);
+    // the page of the wave's turn i: one outside the pool is not read and counts as NaN
+    bool bad = false;
+    auto page_of = [&](int i) {
+      if ((i & 63) == 0) {
+        const int k = wave + (i + lane) * WAVES;
+        ids = k < cnt ? table[k] : 0;
+      }
+      const int id = __builtin_amdgcn_readlane(ids, i & 63);
+      const bool b = id < 0 || id >= a.p.n_pages;
+      bad |= b;
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(pages + (b ? 0 : id) * stride), 0,
+                                               b ? 0 : page_words(D) * 4, 0x00020000);
+    };
+    // K of the next page is on its way from the moment this page's logits are done, V from its product's end
+    const Lane<D> at;
+    KRegs kr;
+    VRegs vr;
+    if (mine > 0) {
+      const rsrc_t pg = page_of(0);
+      load_k<D>(pg, at, kr);
+      load_v<D>(pg, at, vr);
+    }
+    const int see0 = a.window ? max(0, len - a.m + 1 - a.window) : 0;  // the first key that any row sees
+    for (int i = 0; i < mine; ++i) {
+      const int tok0 = (lo + p0 + wave + i * WAVES) * PAGE;
+      const bool mask = tok0 + PAGE > len - a.m + 1 || (a.window && tok0 < len - a.window);
+      f4_t w[4];
+      logits<D, BF>(kr, q, a.scale, w);
+      const bool more = i + 1 < mine;
+      rsrc_t next;
+      if (more) {
+        next = page_of(i + 1);
+        load_k<D>(next, at, kr);
+      }
+      if (mask) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = tok0 + t * 16 + quarter * 4 + e;
+            if (k >= lim || k < low) w[t][e] = NEG_INF;
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      weights<D, BF>(w, acc);
+      __builtin_amdgcn_sched_barrier(0);
+      values<D, BF>(vr, w, acc, mask, tok0, lim, low, see0, len);
+      if (more) load_v<D>(next, at, vr);
+    }
+    if (bad) {
+      acc.l = __builtin_nanf("");
+      if (lane == 0) atomicOr(a.p.status, PAGED_BAD_PAGE);
+    }
+    // the four waves' sums
+    {
+      auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc.l), __float_as_uint(acc.l), false, false);
+      acc.l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+      x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc.l), __float_as_uint(acc.l), false, false);
+      acc.l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    if (quarter == 0) {
+      sm[wave][l] = acc.m;
+      sl[wave][l] = acc.l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < J; j += 4)
+        *reinterpret_cast<f4_t*>(&so[wave][l][(quarter * 4 + i) * J + j]) =
+            f4_t{acc.o[j][i], acc.o[j + 1][i], acc.o[j + 2][i], acc.o[j + 3][i]};
+    __syncthreads();
+    const bool whole = cnt == n;
+    float* slot = whole ? nullptr : slot_of<D>(a.ws, 2 * blockIdx.x + (p0 == 0 ? 1 : 0));
+    for (int i = threadIdx.x; i < ROWS * (D / 8); i += THREADS) {
+      const int rr = i / (D / 8), d = i % (D / 8) * 8;
+      float mx = NEG_INF;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, sm[w][rr]);
+      float sum = 0.f, v[8] = {};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float f = sm[w][rr] == NEG_INF ? 0.f : exp2f(sm[w][rr] - mx);
+        sum += sl[w][rr] == 0.f ? 0.f : sl[w][rr] * (sl[w][rr] != sl[w][rr] ? 1.f : f);
+        if (f != 0.f)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += f * so[w][rr][d + e];
+      }
+      if (whole) {
+        store_row<D, BF>(a, s, head, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) slot[rr * D + d + e] = v[e];
+        if (d == 0) {
+          slot[ROWS * D + rr] = mx;
+          slot[ROWS * D + ROWS + rr] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    u += cnt;
+    if (a.split && u - first >= n * H * a.tiles) {
+      first += n * H * a.tiles;
+      ++s;
+    }
+  }
+}
+
+// one workgroup per (sequence, head, tile) that several workgroups computed: merges their slots in order
+template <int D, bool BF>
+__global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
+  const int per_seq = a.p.H * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
+  const int total = total_units(a), per = units_per_group(total, a.grid);
+  int lo, first = 0;
+  for (int s0 = 0; s0 < s; s0 += 64) {
+    const int i = s0 + int(threadIdx.x & 63);
+    int n = i < s ? pages_of(a, i, lo) * per_seq : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    first += n;
+  }
+  const int n = pages_of(a, s, lo);
+  if (n <= 0) return;
+  const int u0 = first + hr * n, g0 = u0 / per, g1 = (u0 + n - 1) / per;
+  if (g0 == g1) return;
+  const int rr = threadIdx.x / (D / 8), d = threadIdx.x % (D / 8) * 8;
+  float mx = NEG_INF;
+  for (int g = g0; g <= g1; ++g) mx = fmaxf(mx, slot_of<D>(a.ws, 2 * g + (g == g0 ? 1 : 0))[ROWS * D + rr]);
+  float sum = 0.f, v[8] = {};
+  for (int g = g0; g <= g1; ++g) {
+    const float* p = slot_of<D>(a.ws, 2 * g + (g == g0 ? 1 : 0));
+    const float m = p[ROWS * D + rr], l = p[ROWS * D + ROWS + rr];
+    const float f = m == NEG_INF ? 0.f : exp2f(m - mx);
+    sum += l != l ? l : f * l;
+    if (f != 0.f)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += f * p[rr * D + d + e];
+  }
+  store_row<D, BF>(a, s, hr / a.tiles, hr % a.tiles, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+}
+
+constexpr int GRID = 512;  // two workgroups per CU
+
+// tiles of (sequence, head) items; whether a workgroup takes a whole one: those of few pages
+struct Launch {
+  int tiles, split, grid;
+};
+inline Launch plan_of(int S, int P, int m, int nrep, int H) {
+  Launch p;
+  p.tiles = int(ceil_div(int64_t(m) * nrep, ROWS));
+  p.split = P > WAVES;
+  p.grid = p.split ? GRID : S * H * p.tiles;
+  return p;
+}
+
+}  // namespace
+
+namespace iq {
+int check_paged(const iq_paged* p);
+}
+
+extern "C" size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D) {
+  if (S <= 0 || P <= 0 || m <= 0 || Hq <= 0 || H <= 0 || Hq % H || !d_ok(D)) return 0;
+  if (!plan_of(S, P, m, Hq / H, H).split) return 0;
+  return size_t(2 * GRID) * (ROWS * D + 2 * ROWS) * sizeof(float);
+}
+
+extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
+                                  float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int st = iq::check_paged(p)) return st;
+  IQ_CHECK(q && out, IQ_ERR_NULL);
+  IQ_CHECK(m > 0 && m <= 16 && Hq > 0 && Hq % p->H == 0 && Hq <= 4096 && window >= 0, IQ_ERR_SHAPE);
+  IQ_CHECK(aligned(q, 16) && aligned(out, 16) && sq_s % 8 == 0 && sq_m % 8 == 0 && sq_h % 8 == 0 && so_s % 8 == 0 &&
+               so_m % 8 == 0 && so_h % 8 == 0, IQ_ERR_ALIGN);
+  const int nrep = Hq / p->H;
+  const Launch pl = plan_of(p->S, p->P, m, nrep, p->H);
+  IQ_CHECK(int64_t(p->S) * p->P * p->H * pl.tiles <= INT32_MAX, IQ_ERR_SHAPE);
+  const size_t need = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
+  IQ_CHECK(!need || (workspace && workspace_bytes >= need), IQ_ERR_WORKSPACE);
+  IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
+  const AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, m, nrep, pl.tiles,
+                   scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, pl.split};
+  auto launch = [&]<int D, bool BF>() {
+    attn_kernel<D, BF><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
+    if (const int st = launch_status()) return st;
+    if (pl.split)
+      combine_kernel<D, BF><<<p->S * p->H * pl.tiles, ROWS * (D / 8), 0, (hipStream_t)stream>>>(a);
+    return launch_status();
+  };
+  const bool bf = act_bf16(p->mode);
+  if (p->D == 128) return bf ? launch.operator()<128, true>() : launch.operator()<128, false>();
+  return bf ? launch.operator()<64, true>() : launch.operator()<64, false>();
+}

@@ -1,0 +1,322 @@
+// Attention over packed prompts (gfx950): iq_prompt_attention.
+//
+// Sequences of different lengths lie one behind the other; a workgroup takes 128 query rows of one head of one
+// sequence (four waves of 32 rows) and walks over the sequence's keys in tiles of 64, staged through LDS.  Both
+// products run transposed on v_mfma_f32_32x32x16: S^T = K Q^T leaves a query row per lane and its keys in the lane's
+// registers, where the running softmax needs one exchange (with the lane of the other half-wave) per tile, and the
+// exponentials, rounded to the activation dtype, are the B operand of O^T += V^T P^T as they are: V^T's A operand
+// reads LDS with ds_read_b64_tr_b16 in the same order of keys.
+#include "iq_paged.h"
+
+using namespace iq;
+
+namespace {
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+
+constexpr int WAVES = 4, THREADS = 64 * WAVES, BM = 32 * WAVES, BN = 64;
+constexpr float NEG_INF = -__builtin_inff();
+
+struct PromptArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* out;
+  int64_t sq_n, sq_h, sk_n, sk_h, sv_n, sv_h, so_n, so_h;
+  const int32_t *cu_q, *cu_k;
+  int S, N, Nk, Hq, nrep, slots;
+  float c;              // |scale| log2(e); 1 for a scale of 0
+  uint32_t keep, sign;  // and-ed, xor-ed into the queries: a scale of 0 clears them, a negative one flips their signs
+  int causal, window;
+};
+
+// rows [r0, r1) of sequence s in a packed tensor of n rows (whatever cu holds)
+__device__ __forceinline__ void rows_of(const int32_t* cu, int s, int n, int& r0, int& r1) {
+  r0 = min(max(cu[s], 0), n);
+  r1 = min(max(cu[s + 1], r0), n);
+}
+
+template <bool BF>
+__device__ __forceinline__ f16_t mma32(u4_t a, u4_t b, f16_t c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+}
+
+// 16-byte chunk c of row r in an LDS tile: spread so that neither K's reads (one chunk of 16 rows) nor V's transposed
+// ones (four chunks of 4 rows) meet in a bank
+template <int D>
+__device__ __forceinline__ int chunk_at(int r, int c) {
+  if constexpr (D == 128) return r * 16 + (c ^ ((r & 3) << 2 | (r >> 2 & 3)));
+  else return r * 8 + (c ^ ((r >> 1 & 1) << 2 | (r >> 2 & 3)));
+}
+
+template <int D, bool BF>
+__global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
+#pragma clang fp contract(off)  // logits times c and the maximum times c round alike
+  constexpr int CH = D / 8, KS = D / 16, DB = D / 32;  // chunks per row, k steps of S, blocks of 32 dims
+  constexpr int LOADS = BN * CH / THREADS;             // chunks per thread and tile
+  __shared__ u4_t lk[BN * CH], lv[BN * CH];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
+
+  // this workgroup's (KV head, slot, head in the group); blocks go round robin over the 8 XCDs, so each XCD takes a
+  // run of items: the same keys
+  const int total = gridDim.x, x = blockIdx.x % 8, base = total / 8, rest = total % 8;
+  const int item = x * base + min(x, rest) + blockIdx.x / 8;
+  const int g = item % a.nrep, slot = item / a.nrep % a.slots, kvh = item / a.nrep / a.slots, head = kvh * a.nrep + g;
+
+  // the slot's sequence and tile of rows, the last tiles (the longest) first
+  int s = -1, tile = 0, q0 = 0, q1 = 0;
+  {
+    int before = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+      int r0 = 0, r1 = 0;
+      if (s0 + lane < a.S) rows_of(a.cu_q, s0 + lane, a.N, r0, r1);
+      const int t = (r1 - r0 + BM - 1) / BM;
+      int end = t;
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) {
+        const int y = __shfl_up(end, o, 64);
+        if (lane >= o) end += y;
+      }
+      end += before;
+      const uint64_t past = __ballot(end > slot);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        s = s0 + l;
+        tile = __builtin_amdgcn_readlane(end, l) - 1 - slot;
+        q0 = __builtin_amdgcn_readlane(r0, l);
+        q1 = __builtin_amdgcn_readlane(r1, l);
+        break;
+      }
+      before = __builtin_amdgcn_readlane(end, 63);
+    }
+  }
+  if (s < 0) return;
+  int k0, k1;
+  rows_of(a.cu_k, s, a.Nk, k0, k1);
+  k0 = __builtin_amdgcn_readfirstlane(k0);
+  k1 = __builtin_amdgcn_readfirstlane(k1);
+  const int lq = q1 - q0, keys = k1 - k0, off = keys - lq;
+  const int row = tile * BM + wave * 32 + n;  // this lane's query row in the sequence
+  const bool real = row < lq;
+  // key j is seen iff first <= j < last
+  const int last = a.causal ? min(row + off + 1, keys) : keys, first = a.window ? max(row + off + 1 - a.window, 0) : 0;
+  // the tiles of keys that any row of the workgroup sees
+  const int row_a = tile * BM, row_z = min(row_a + BM, lq) - 1;
+  const int j_end = a.causal ? min(row_z + off + 1, keys) : keys, j_begin = a.window ? max(row_a + off + 1 - a.window, 0) : 0;
+  const int t_begin = j_begin / BN, t_end = j_end > j_begin ? (j_end + BN - 1) / BN : t_begin;
+
+  u4_t q[KS];  // B operand: row n, dims 16 ks + 8 hi + e
+  {
+    const uint16_t* p = a.q + int64_t(q0 + row) * a.sq_n + head * a.sq_h + 8 * hi;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      q[ks] = u4_t{0, 0, 0, 0};
+      if (real) q[ks] = (*reinterpret_cast<const u4_t*>(p + 16 * ks) & a.keep) ^ a.sign;
+    }
+  }
+  f16_t o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+  float m = NEG_INF, l = 0.f;
+
+  // a tile's rows past the last key that the workgroup sees read as zeros (the descriptor's bound)
+  const uint16_t *kp = a.k + int64_t(k0) * a.sk_n + kvh * a.sk_h, *vp = a.v + int64_t(k0) * a.sv_n + kvh * a.sv_h;
+  u4_t rk[LOADS], rv[LOADS];
+  auto fetch = [&](int t) {
+    const int rows = min(j_end - t * BN, BN);
+    const rsrc_t dk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kp + int64_t(t) * BN * a.sk_n), 0,
+                                                        int((rows - 1) * a.sk_n + D) * 2, 0x00020000);
+    const rsrc_t dv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vp + int64_t(t) * BN * a.sv_n), 0,
+                                                        int((rows - 1) * a.sv_n + D) * 2, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int e = threadIdx.x + i * THREADS, r = e / CH, c = e % CH;
+      const bool in = r < rows;  // (overlapping rows, of a stride below D, end before the bound)
+      rk[i] = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(dk, in ? (r * int(a.sk_n) + c * 8) * 2 : -16, 0, 0));
+      rv[i] = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(dv, in ? (r * int(a.sv_n) + c * 8) * 2 : -16, 0, 0));
+    }
+  };
+  if (t_begin < t_end) fetch(t_begin);
+  for (int t = t_begin; t < t_end; ++t) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int e = threadIdx.x + i * THREADS, r = e / CH, c = e % CH;
+      lk[chunk_at<D>(r, c)] = rk[i];
+      lv[chunk_at<D>(r, c)] = rv[i];
+    }
+    __syncthreads();
+    if (t + 1 < t_end) fetch(t + 1);
+    const int j0 = t * BN;
+    // this wave's rows: does any see the tile, do all see all of it?
+    const int wa = row_a + wave * 32, wz = min(wa + 31, lq - 1);
+    const int w_last = a.causal ? min(wz + off + 1, keys) : keys, w_first = a.window ? max(wa + off + 1 - a.window, 0) : 0;
+    if (wa >= lq || w_last <= j0 || w_first >= j0 + BN) continue;
+    const bool mask = (a.causal ? min(wa + off + 1, keys) : keys) < j0 + BN || (a.window && wz + off + 1 - a.window > j0);
+
+    f16_t st[2];  // st[kb][i]: key 32 kb + 8 (i/4) + 4 hi + i%4 of the tile
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) st[kb] = mma32<BF>(lk[chunk_at<D>(kb * 32 + n, 2 * ks + hi)], q[ks], st[kb]);
+    }
+    if (mask) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = j0 + 32 * kb + 8 * (i / 4) + 4 * hi + i % 4;
+          if (j >= last || j < first) st[kb][i] = NEG_INF;
+        }
+    }
+    float mx = m;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[kb][i]);
+    {
+      const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    }
+    // weights relative to 2^base, base = RN(max c): the fma form leaves a common factor of 2^(error of base), which the
+    // sum shares; where base is so large that the factor would leave [1/2, 2], logits are rounded as base is
+    const float was = m == NEG_INF ? 0.f : m * a.c, base = mx == NEG_INF ? 0.f : mx * a.c;
+    if (__any(mx != m)) {
+      const float f = __builtin_amdgcn_exp2f(m == NEG_INF ? NEG_INF : was - base);
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] *= f;
+      m = mx;
+    }
+    float sum = 0.f;
+    if (__any(fabsf(base) > 65536.f)) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[kb][i] = st[kb][i] * a.c - base;
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[kb][i] = __builtin_fmaf(st[kb][i], a.c, -base);
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        st[kb][i] = __builtin_amdgcn_exp2f(st[kb][i]);
+        sum += st[kb][i];
+      }
+    l += sum;
+    u4_t p[4];  // keys 16 kc + 8 (e/4) + 4 hi + e%4, e = 0..7
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[kc][i] = pack2<BF>(st[kc / 2][8 * (kc % 2) + 2 * i], st[kc / 2][8 * (kc % 2) + 2 * i + 1]);
+    // V^T's operand: dim 32 b + n, the keys of p
+    auto v_operand = [&](int kc, int b) {
+      u4_t y;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = lane & 15, r = kc * 16 + h * 8 + hi * 4 + j / 4, d = b * 32 + (lane >> 4 & 1) * 16 + j % 4 * 4;
+        const char* at = reinterpret_cast<const char*>(&lv[chunk_at<D>(r, d / 8)]) + d % 8 * 2;
+        const u2_t w = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                    (__attribute__((address_space(3))) s4_t*)(uintptr_t)(uint32_t)(uintptr_t)at));
+        y[2 * h] = w.x;
+        y[2 * h + 1] = w.y;
+      }
+      return y;
+    };
+    bool odd = false;
+    if (mask) {  // does V hold an infinity or NaN (0 * inf would carry it into rows that do not see its key)?
+      const uint32_t e = BF ? 0x7f80u : 0x7c00u;
+      for (int i = lane; i < BN * CH; i += 64) {
+        const u4_t w = lv[i];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) odd |= (w[y] & e) == e || ((w[y] >> 16) & e) == e;
+      }
+    }
+    if (!__any(odd)) {
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[b] = mma32<BF>(v_operand(kc, b), p[kc], o[b]);
+    } else {  // key by key, into the rows that see it
+#pragma clang loop unroll(disable)
+      for (int key = 0; key < BN; ++key) {
+        const int at = key / 16 * 4 + key % 16 / 8 * 2 + key % 4 / 2, of = key % 8 / 4;  // p's word, in the lanes hi == of
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i == at) w = p[i / 4][i % 4];
+        const auto y = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        w = of ? y[1] : y[0];
+        const float pk = key & 1 ? hi_half<BF>(w) : lo_half<BF>(w);
+        if (j0 + key < last && j0 + key >= first) {
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const u2_t x = reinterpret_cast<const u2_t*>(&lv[chunk_at<D>(key, 4 * b + i)])[hi];
+              const uint32_t x0 = x.x, x1 = x.y;
+              o[b][4 * i] = __builtin_fmaf(pk, lo_half<BF>(x0), o[b][4 * i]);
+              o[b][4 * i + 1] = __builtin_fmaf(pk, hi_half<BF>(x0), o[b][4 * i + 1]);
+              o[b][4 * i + 2] = __builtin_fmaf(pk, lo_half<BF>(x1), o[b][4 * i + 2]);
+              o[b][4 * i + 3] = __builtin_fmaf(pk, hi_half<BF>(x1), o[b][4 * i + 3]);
+            }
+        }
+      }
+    }
+  }
+  {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+  }
+  if (!real) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = a.out + int64_t(q0 + row) * a.so_n + head * a.so_h + 4 * hi;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<u2_t*>(out + 32 * b + 8 * i) = u2_t{pack2<BF>(o[b][4 * i] * inv, o[b][4 * i + 1] * inv),
+                                                            pack2<BF>(o[b][4 * i + 2] * inv, o[b][4 * i + 3] * inv)};
+}
+
+}  // namespace
+
+extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
+                                   const void* v, int64_t sv_n, int64_t sv_h, const int32_t* cu_q, const int32_t* cu_k,
+                                   int S, int N, int Nk, int Hq, int H, int D, int mode, float scale, int causal, int window,
+                                   void* out, int64_t so_n, int64_t so_h, void* stream) {
+  IQ_CHECK(cu_q && cu_k && (N == 0 || (q && out)) && (Nk == 0 || (k && v)), IQ_ERR_NULL);
+  IQ_CHECK(base_mode(mode) == 0, IQ_ERR_MODE);
+  IQ_CHECK(d_ok(D) && H > 0 && Hq > 0 && Hq % H == 0 && Hq <= 4096 && S > 0 && N >= 0 && Nk >= 0 && window >= 0, IQ_ERR_SHAPE);
+  IQ_CHECK(!window || causal, IQ_ERR_MODE);
+  for (const int64_t s : {sk_n, sv_n}) IQ_CHECK(s >= 0 && s < (1 << 23), IQ_ERR_SHAPE);  // a tile of rows in 32 bits
+  for (const int64_t s : {sq_n, sq_h, sk_n, sk_h, sv_n, sv_h, so_n, so_h}) IQ_CHECK(s % 8 == 0, IQ_ERR_ALIGN);
+  IQ_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, 4) && aligned(cu_k, 4),
+           IQ_ERR_ALIGN);
+  if (N == 0) return IQ_OK;
+  const int64_t slots = int64_t(N) / BM + S;  // a sequence has at most rows / 128 + 1 tiles
+  IQ_CHECK(slots * Hq <= INT32_MAX, IQ_ERR_SHAPE);
+  const float c = scale * 1.44269504088896340736f;
+  PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
+               sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), c == 0 ? 1.f : c < 0 ? -c : c, c == 0 ? 0u : ~0u,
+               c < 0 ? 0x80008000u : 0u,
+               causal ? 1 : 0, window};
+  auto launch = [&]<int D_, bool BF>() {
+    prompt_kernel<D_, BF><<<unsigned(slots * Hq), THREADS, 0, (hipStream_t)stream>>>(a);
+    return launch_status();
+  };
+  const bool bf = act_bf16(mode);
+  if (D == 128) return bf ? launch.operator()<128, true>() : launch.operator()<128, false>();
+  return bf ? launch.operator()<64, true>() : launch.operator()<64, false>();
+}

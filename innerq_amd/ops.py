@@ -6,6 +6,7 @@ path: a CPU tensor or a missing library raises.
 """
 from __future__ import annotations
 
+import contextlib
 import copy
 import ctypes
 from typing import Optional, Sequence
@@ -75,6 +76,28 @@ def require_act(t: torch.Tensor, name: str, dtype=None) -> None:
     """A HIP device tensor of an activation dtype (fp16 or bf16; exactly ``dtype`` when given)."""
     require_device(t, name, dtype)
     act_flag(t.dtype)
+
+
+def on_device(device: torch.device):
+    """The device as the current one while a call launches there (nothing to do where it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def rows_aligned(t: torch.Tensor) -> bool:
+    """Whether every row over the last dim is contiguous and starts on a 16-byte boundary (16-bit types)."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in t.stride()[:-1])
+
+
+def check_cu(cu: torch.Tensor, name: str, S: Optional[int], device: torch.device) -> torch.Tensor:
+    """Cumulative lengths: int32 [S + 1] on ``device``, contiguous."""
+    require_device(cu, name, torch.int32)
+    if cu.dim() != 1 or cu.shape[0] < 2 or (S is not None and cu.shape[0] != S + 1) or cu.device != device \
+            or not cu.is_contiguous():
+        _shape_error(f"{name} must be a contiguous int32 [{'S' if S is None else S} + 1] tensor on {device}, got "
+                     f"{tuple(cu.shape)} on {cu.device}")
+    return cu
 
 
 def require_f16_store(store, role: str) -> None:
@@ -850,6 +873,57 @@ def decode_attention_combine_live(plan, B: int, Hq: int, T: int, D: int, device,
     ws = _workspace(device, _lib.lib().iq_decode_workspace_bytes(B, Hq, T, D))
     call("iq_decode_attention_combine_live", ctypes.byref(plan), B, Hq, T, D, _p(out), out.stride(0), out.stride(1),
          _p(ws), ws.numel(), _stream(device))
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float,
+                     cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = True, window: Optional[int] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(q K^T * scale) V of prompts of different lengths that lie one behind the other.
+
+    q [N, Hq, D]; k, v [Nk, H, D] of q's dtype (fp16 or bf16), Hq a multiple of H, D 64 or 128.  Sequence s is rows
+    cu_seqlens[s] .. cu_seqlens[s+1] (int32 [S+1] on the device, read by the kernel: a captured call follows its
+    values) of q and, by cu_seqlens_k (default: the same), of k and v.  causal: a sequence's last row sees all its
+    keys, each row before it one less (a chunk of a prompt behind its earlier keys has more keys than rows); window:
+    only the last ``window`` of the keys up to its own.  Rows that see no key are 0; rows outside the sequences are
+    not written.  Inference only: tensors that autograd follows are refused."""
+    require_act(q, "q")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise NotImplementedError("prompt_attention has no backward: call it under torch.no_grad()")
+    if q.dim() != 3 or k.dim() != 3:
+        _shape_error(f"q must be [N, Hq, D] and k [Nk, H, D], got {tuple(q.shape)} and {tuple(k.shape)}")
+    (N, Hq, D), (Nk, H), dev = q.shape, k.shape[:2], q.device
+    if D not in (64, 128):
+        _shape_error(f"prompt_attention takes head_dim 64 or 128, got {D}")
+    check_gqa(Hq, H)
+    if not Hq:
+        _shape_error("q has no heads")
+    rows = []
+    for t, name, shape in ((q, "q", (N, Hq, D)), (k, "k", (Nk, H, D)), (v, "v", (Nk, H, D))):
+        require_device(t, name, q.dtype)
+        check_out(t.shape, shape, name)
+        if t.device != dev:
+            _shape_error(f"{name} is on {t.device}, q on {dev}")
+        rows.append(t if rows_aligned(t) and t.stride(0) < 2 ** 23 else t.contiguous())
+    q, k, v = rows
+    cu_q = check_cu(cu_seqlens, "cu_seqlens", None, dev)
+    S = cu_q.shape[0] - 1
+    cu_k = cu_q if cu_seqlens_k is None else check_cu(cu_seqlens_k, "cu_seqlens_k", S, dev)
+    if cu_seqlens_k is None and Nk != N:
+        _shape_error(f"{N} rows of q and {Nk} of k need a cu_seqlens_k of their own")
+    if window is not None and (not causal or not 0 < window < 2 ** 31):
+        raise ValueError(f"a window is positive and causal, got window={window}, causal={causal}")
+    if out is None:
+        out = torch.empty(N, Hq, D, dtype=q.dtype, device=dev)
+    else:
+        require_device(out, "out", q.dtype)
+        check_out(out.shape, (N, Hq, D))
+        if out.device != dev or not rows_aligned(out):
+            _shape_error("out needs a contiguous head_dim, rows on 16-byte boundaries and q's device")
+    with on_device(dev):
+        call("iq_prompt_attention", _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
+             v.stride(1), _p(cu_q), _p(cu_k), S, N, Nk, Hq, H, D, act_flag(q.dtype), float(scale), 1 if causal else 0,
+             window or 0, _p(out), out.stride(0), out.stride(1), _stream(dev))
     return out
 
 
