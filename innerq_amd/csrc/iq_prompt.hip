@@ -57,7 +57,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
 #pragma clang fp contract(off)  // logits times c and the maximum times c round alike
   constexpr int CH = D / 8, KS = D / 16, DB = D / 32;  // chunks per row, k steps of S, blocks of 32 dims
   constexpr int LOADS = BN * CH / THREADS;             // chunks per thread and tile
-  __shared__ u4_t lk[BN * CH], lv[BN * CH];
+  __shared__ u4_t lk0[BN * CH], lk1[BN * CH], lv0[BN * CH], lv1[BN * CH];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
 
   // this workgroup's (KV head, slot, head in the group); blocks go round robin over the 8 XCDs, so each XCD takes a
@@ -108,14 +108,13 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   const int j_end = a.causal ? min(row_z + off + 1, keys) : keys, j_begin = a.window ? max(row_a + off + 1 - a.window, 0) : 0;
   const int t_begin = j_begin / BN, t_end = j_end > j_begin ? (j_end + BN - 1) / BN : t_begin;
 
-  u4_t q[KS];  // B operand: row n, dims 16 ks + 8 hi + e
+  u4_t q[KS];  // B operand: row n, dims 16 ks + 8 hi + e (rows past the end repeat the last one and are not stored)
   {
-    const uint16_t* p = a.q + int64_t(q0 + row) * a.sq_n + head * a.sq_h + 8 * hi;
+    const uint16_t* p = a.q + int64_t(q0 + min(row, lq - 1)) * a.sq_n + head * a.sq_h + 8 * hi;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      q[ks] = u4_t{0, 0, 0, 0};
-      if (real) q[ks] = (*reinterpret_cast<const u4_t*>(p + 16 * ks) & a.keep) ^ a.sign;
-    }
+    for (int ks = 0; ks < KS; ++ks) q[ks] = *reinterpret_cast<const u4_t*>(p + 16 * ks);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[ks] = (q[ks] & a.keep) ^ a.sign;
   }
   f16_t o[DB];
 #pragma unroll
@@ -124,39 +123,44 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
   float m = NEG_INF, l = 0.f;
 
-  // a tile's rows past the last key that the workgroup sees read as zeros (the descriptor's bound)
+  // Tiles go from memory to LDS without registers, one tile ahead.  LDS is written in lane order, so the spreading of
+  // chunk_at is in the source address: a thread's chunk of every pass of THREADS chunks has the same place in its row.
+  // Rows past the last key that the workgroup sees are past the descriptor's bound and read as zeros.
   const uint16_t *kp = a.k + int64_t(k0) * a.sk_n + kvh * a.sk_h, *vp = a.v + int64_t(k0) * a.sv_n + kvh * a.sv_h;
-  u4_t rk[LOADS], rv[LOADS];
-  auto fetch = [&](int t) {
+  const int sk = int(a.sk_n) * 2, sv = int(a.sv_n) * 2, fr = threadIdx.x / CH, fc = (chunk_at<D>(fr, threadIdx.x % CH) % CH) * 16;
+  const int vk = fr * sk + fc, vv = fr * sv + fc;
+  auto fetch = [&](int t, u4_t* lk, u4_t* lv) {
     const int rows = min(j_end - t * BN, BN);
     const rsrc_t dk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kp + int64_t(t) * BN * a.sk_n), 0,
-                                                        int((rows - 1) * a.sk_n + D) * 2, 0x00020000);
+                                                        (rows - 1) * sk + D * 2, 0x00020000);
     const rsrc_t dv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vp + int64_t(t) * BN * a.sv_n), 0,
-                                                        int((rows - 1) * a.sv_n + D) * 2, 0x00020000);
+                                                        (rows - 1) * sv + D * 2, 0x00020000);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int e = threadIdx.x + i * THREADS, r = e / CH, c = e % CH;
-      const bool in = r < rows;  // (overlapping rows, of a stride below D, end before the bound)
-      rk[i] = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(dk, in ? (r * int(a.sk_n) + c * 8) * 2 : -16, 0, 0));
-      rv[i] = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(dv, in ? (r * int(a.sv_n) + c * 8) * 2 : -16, 0, 0));
+      constexpr int ROWS = THREADS / CH;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(dk, (__attribute__((address_space(3))) void*)(lk + i * THREADS + wave * 64), 16,
+                                               vk, i * ROWS * sk, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(dv, (__attribute__((address_space(3))) void*)(lv + i * THREADS + wave * 64), 16,
+                                               vv, i * ROWS * sv, 0, 0);
     }
   };
-  if (t_begin < t_end) fetch(t_begin);
-  for (int t = t_begin; t < t_end; ++t) {
-    __syncthreads();
+  // this lane's operands in a tile, in bytes; blocks of 32 keys (K), of 16 (V) are at fixed distances from them
+  int ka[KS], va[DB][2];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int e = threadIdx.x + i * THREADS, r = e / CH, c = e % CH;
-      lk[chunk_at<D>(r, c)] = rk[i];
-      lv[chunk_at<D>(r, c)] = rv[i];
+  for (int ks = 0; ks < KS; ++ks) ka[ks] = chunk_at<D>(n, 2 * ks + hi) * 16;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = lane & 15, d = b * 32 + (lane >> 4 & 1) * 16 + j % 4 * 4;
+      va[b][h] = chunk_at<D>(h * 8 + hi * 4 + j / 4, d / 8) * 16 + d % 8 * 2;
     }
-    __syncthreads();
-    if (t + 1 < t_end) fetch(t + 1);
+  auto step = [&](int t, const u4_t* lk, const u4_t* lv) {
     const int j0 = t * BN;
     // this wave's rows: does any see the tile, do all see all of it?
     const int wa = row_a + wave * 32, wz = min(wa + 31, lq - 1);
     const int w_last = a.causal ? min(wz + off + 1, keys) : keys, w_first = a.window ? max(wa + off + 1 - a.window, 0) : 0;
-    if (wa >= lq || w_last <= j0 || w_first >= j0 + BN) continue;
+    if (wa >= lq || w_last <= j0 || w_first >= j0 + BN) return;
     const bool mask = (a.causal ? min(wa + off + 1, keys) : keys) < j0 + BN || (a.window && wz + off + 1 - a.window > j0);
 
     f16_t st[2];  // st[kb][i]: key 32 kb + 8 (i/4) + 4 hi + i%4 of the tile
@@ -165,7 +169,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) st[kb] = mma32<BF>(lk[chunk_at<D>(kb * 32 + n, 2 * ks + hi)], q[ks], st[kb]);
+      for (int ks = 0; ks < KS; ++ks) st[kb] = mma32<BF>(*reinterpret_cast<const u4_t*>(reinterpret_cast<const char*>(lk) + ka[ks] + kb * 32 * CH * 16), q[ks], st[kb]);
     }
     if (mask) {
 #pragma unroll
@@ -225,10 +229,9 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
       u4_t y;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int j = lane & 15, r = kc * 16 + h * 8 + hi * 4 + j / 4, d = b * 32 + (lane >> 4 & 1) * 16 + j % 4 * 4;
-        const char* at = reinterpret_cast<const char*>(&lv[chunk_at<D>(r, d / 8)]) + d % 8 * 2;
-        const u2_t w = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                    (__attribute__((address_space(3))) s4_t*)(uintptr_t)(uint32_t)(uintptr_t)at));
+        const char* at = reinterpret_cast<const char*>(lv) + va[b][h] + kc * 16 * CH * 16;
+        const u2_t w = __builtin_bit_cast(
+            u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)at));
         y[2 * h] = w.x;
         y[2 * h + 1] = w.y;
       }
@@ -274,6 +277,16 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
         }
       }
     }
+  };
+  if (t_begin < t_end) fetch(t_begin, lk0, lv0);
+  for (int t = t_begin; t < t_end; t += 2) {
+    __syncthreads();  // the tile is there, and no wave reads the other buffer any more
+    if (t + 1 < t_end) fetch(t + 1, lk1, lv1);
+    step(t, lk0, lv0);
+    if (t + 1 >= t_end) break;
+    __syncthreads();
+    if (t + 2 < t_end) fetch(t + 2, lk0, lv0);
+    step(t + 1, lk1, lv1);
   }
   {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
