@@ -1,7 +1,7 @@
 // Attention of one or a few new tokens per sequence over 4-bit pages (gfx950): iq_paged_attention.
 //
-// Flash decoding over a ragged batch: the pages of all (sequence, KV head, tile of 16 query rows) lie behind one
-// another in one list, which the workgroups share out evenly (read from the sequences' lengths on the device, so a
+// Flash decoding over a ragged batch: the pages of all (sequence, KV head, tile of 16 query rows), each with PAD
+// units before them, lie behind one another in one list, which the workgroups share out evenly (read from the sequences' lengths on the device, so a
 // captured call follows them); a workgroup's four waves take its pages in turn, each with its own running maximum,
 // sum and accumulators, merged over LDS at the end of each (sequence, head).  Where a (sequence, head) spans several
 // workgroups, their fp32 partials go to the workspace and a second launch merges them in a fixed order.
@@ -16,6 +16,10 @@ using namespace iq;
 namespace {
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 16;
+// What a (sequence, head, tile) costs beside its pages, in pages: its queries, its first page's latency and the
+// merge of the waves.  Counted where the workgroups share out the list; without it a workgroup whose share was many
+// short sequences came last (48 sequences of 130 .. 16001 tokens, bf16: 181 us against 82).
+constexpr int PAD = 8;
 constexpr float NEG_INF = -__builtin_inff();
 
 struct AttnArgs {
@@ -49,39 +53,39 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// units (pages times heads and tiles) of all sequences
-__device__ __forceinline__ int total_units(const AttnArgs& a) {
-  int t = 0, lo;
-  for (int s0 = 0; s0 < a.p.S; s0 += 64) {
-    const int s = s0 + int(threadIdx.x & 63);
-    t += s < a.p.S ? pages_of(a, s, lo) : 0;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-  return __builtin_amdgcn_readfirstlane(t) * a.p.H * a.tiles;
+// Where a lane's sequence s0 + lane ends in the list of units (a unit: a page of one head and tile), s0 a multiple of
+// 64 and `base` the units before it; n: the sequence's units.
+struct Part {
+  int n, end;
+};
+__device__ __forceinline__ Part part_at(const AttnArgs& a, int s0, int base) {
+  int lo;
+  const int s = s0 + int(threadIdx.x & 63), pages = s < a.p.S ? pages_of(a, s, lo) : 0;
+  const int n = pages > 0 ? (pages + PAD) * a.p.H * a.tiles : 0;
+  return {n, base + wave_scan(n)};
 }
-// the sequence that holds unit u, and its first unit (u < total)
-__device__ __forceinline__ void find_unit(const AttnArgs& a, int u, int& s, int& first) {
-  const int per = a.p.H * a.tiles;
-  int base = 0, lo;
-  for (int s0 = 0; s0 < a.p.S; s0 += 64) {
-    const int i = s0 + int(threadIdx.x & 63);
-    const int n = i < a.p.S ? pages_of(a, i, lo) * per : 0;
-    const int end = base + wave_scan(n);
-    const uint64_t past = __ballot(end > u);
+__device__ __forceinline__ int total_units(const AttnArgs& a, const Part& first) {
+  int end = __builtin_amdgcn_readlane(first.end, 63);
+  for (int s0 = 64; s0 < a.p.S; s0 += 64) end = __builtin_amdgcn_readlane(part_at(a, s0, end).end, 63);
+  return end;
+}
+// the sequence that holds unit u < total, and its first unit
+__device__ __forceinline__ void find_unit(const AttnArgs& a, Part p, int u, int& s, int& first) {
+  for (int s0 = 0;;) {
+    const uint64_t past = __ballot(p.end > u);
     if (past) {
       const int l = __builtin_ctzll(past);
       s = s0 + l;
-      first = __builtin_amdgcn_readlane(end - n, l);
+      first = __builtin_amdgcn_readlane(p.end - p.n, l);
       return;
     }
-    base = __builtin_amdgcn_readlane(end, 63);
+    s0 += 64;
+    if (s0 >= a.p.S) return;
+    p = part_at(a, s0, __builtin_amdgcn_readlane(p.end, 63));
   }
-  s = a.p.S;
-  first = base;
 }
 __device__ __forceinline__ int units_per_group(int total, int grid) {
-  return max((total + grid - 1) / grid, 4);  // a page per wave at least
+  return max((total + grid - 1) / grid, WAVES);  // a page per wave at least
 }
 
 // row r of tile t of sequence s: its query head offset (head in the group, token)
@@ -356,18 +360,19 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
   const int H = a.p.H;
   int u, u1, s = 0, first = 0;
   if (a.split) {
-    const int total = total_units(a), per = units_per_group(total, a.grid);
+    const Part part = part_at(a, 0, 0);
+    const int total = total_units(a, part), per = units_per_group(total, a.grid);
     u = min(int64_t(blockIdx.x) * per, int64_t(total));
     u1 = min(u + per, total);
-    if (u < u1) find_unit(a, u, s, first);
+    if (u < u1) find_unit(a, part, u, s, first);
   } else {
     s = blockIdx.x / (H * a.tiles);
     int lo;
     const int n = pages_of(a, s, lo);
     u = first = 0;
     const int hr = blockIdx.x - s * H * a.tiles;
-    u = hr * n;
-    u1 = u + n;
+    u = hr * (n + PAD);
+    u1 = n > 0 ? u + n + PAD : u;
   }
   // sequences without tokens: rows of zeros
   for (int e = a.split ? blockIdx.x : s; e < (a.split ? a.p.S : s + 1); e += a.grid) {
@@ -386,68 +391,69 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
     int n = __builtin_amdgcn_readfirstlane(pages_of(a, s, lo));
     if (n <= 0) { ++s; continue; }
     lo = __builtin_amdgcn_readfirstlane(lo);
-    const int hr = (u - first) / n, p0 = (u - first) - hr * n, cnt = min(n - p0, u1 - u);
+    const int hr = (u - first) / (n + PAD), x0 = (u - first) - hr * (n + PAD), x1 = min(n + PAD, x0 + u1 - u);
+    const int p0 = max(x0 - PAD, 0), cnt = x1 - PAD - p0;  // this workgroup's pages of the head and tile
+    u += x1 - x0;
+    const bool over = a.split && u - first >= (n + PAD) * H * a.tiles;
+    if (cnt <= 0) continue;
     const int head = hr / a.tiles, tile = hr - head * a.tiles;
     const int len = __builtin_amdgcn_readfirstlane(min(a.p.lens[s], a.p.P * PAGE));
     const Row row = row_of(a, tile, l);
     const int lim = len - (a.m - 1 - row.token), low = a.window ? lim - a.window : 0;  // the row sees keys [low, lim)
     // the query row of this lane, its octets in the order of k_values' pairs
-    u4_t q[D / 32];
+    u4_t q[D / 32];  // (rows past the last repeat it and are not stored)
     {
-      const uint16_t* x = a.q + s * a.sq_s + row.token * a.sq_m + (int64_t(head) * a.nrep + row.head) * a.sq_h +
-                          quarter * (D / 4);
+      const int token = min(row.token, a.m - 1), h = row.real ? row.head : a.nrep - 1;
+      const uint16_t* x = a.q + s * a.sq_s + token * a.sq_m + (int64_t(head) * a.nrep + h) * a.sq_h + quarter * (D / 4);
+      u4_t w[D / 32];
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        u4_t w = {0, 0, 0, 0};
-        if (row.real) w = *reinterpret_cast<const u4_t*>(x + 8 * j);
-        q[j] = u4_t{__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
-                    __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
-      }
+      for (int j = 0; j < D / 32; ++j) w[j] = *reinterpret_cast<const u4_t*>(x + 8 * j);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        q[j] = u4_t{__builtin_amdgcn_perm(w[j][2], w[j][0], 0x05040100u), __builtin_amdgcn_perm(w[j][2], w[j][0], 0x07060302u),
+                    __builtin_amdgcn_perm(w[j][3], w[j][1], 0x05040100u), __builtin_amdgcn_perm(w[j][3], w[j][1], 0x07060302u)};
     }
     Acc<D, BF> acc;
 #pragma unroll
     for (int j = 0; j < J; ++j) acc.o[j] = f4_t{0.f, 0.f, 0.f, 0.f};
     acc.m = NEG_INF;
     acc.l = 0.f;
-    const int32_t* table = a.p.table + s * a.p.s_table + lo + p0;
-    const int mine = wave < cnt ? (cnt - wave + WAVES - 1) / WAVES : 0;  // this wave's pages: wave, wave + 4, ...
-    int ids = 0;
+    // (read as constants, by scalar loads: a vector load here would wait for the pages under way)
+    typedef const __attribute__((address_space(4))) int32_t* consts_t;
+    const consts_t table = (consts_t)(a.p.table + s * a.p.s_table + lo + p0);
+    const int mine = wave < cnt ? (cnt - wave + WAVES - 1) / WAVES : 0;  // this wave's pages: wave, wave + WAVES, ...
     const uint32_t* pages = a.p.pages + int64_t(head) * page_words(D);
     const int64_t stride = int64_t(H) * page_words(D);
     // the page of the wave's turn i: one outside the pool is not read and counts as NaN
     bool bad = false;
-    auto page_of = [&](int i) {
-      if ((i & 63) == 0) {
-        const int k = wave + (i + lane) * WAVES;
-        ids = k < cnt ? table[k] : 0;
-      }
-      const int id = __builtin_amdgcn_readlane(ids, i & 63);
+    // past its last page a wave loads from a descriptor of no bytes: the loop has no branch that a load depends on,
+    // which the wait counts would have to allow for
+    auto id_of = [&](int i) { return i < mine ? table[wave + i * WAVES] : 0; };
+    auto page_of = [&](int id, bool there) {
       const bool b = id < 0 || id >= a.p.n_pages;
       bad |= b;
       return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(pages + (b ? 0 : id) * stride), 0,
-                                               b ? 0 : page_words(D) * 4, 0x00020000);
+                                               b || !there ? 0 : page_words(D) * 4, 0x00020000);
     };
     // K of the next page is on its way from the moment this page's logits are done, V from its product's end
     const Lane<D> at;
     KRegs kr;
     VRegs vr;
-    if (mine > 0) {
-      const rsrc_t pg = page_of(0);
+    {
+      const rsrc_t pg = page_of(id_of(0), mine > 0);
       load_k<D>(pg, at, kr);
       load_v<D>(pg, at, vr);
     }
     const int see0 = a.window ? max(0, len - a.m + 1 - a.window) : 0;  // the first key that any row sees
+    int id = id_of(1);
     for (int i = 0; i < mine; ++i) {
       const int tok0 = (lo + p0 + wave + i * WAVES) * PAGE;
       const bool mask = tok0 + PAGE > len - a.m + 1 || (a.window && tok0 < len - a.window);
       f4_t w[4];
       logits<D, BF>(kr, q, a.scale, w);
-      const bool more = i + 1 < mine;
-      rsrc_t next;
-      if (more) {
-        next = page_of(i + 1);
-        load_k<D>(next, at, kr);
-      }
+      const rsrc_t next = page_of(id, i + 1 < mine);
+      id = id_of(i + 2);
+      load_k<D>(next, at, kr);
       if (mask) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -461,13 +467,13 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
       weights<D, BF>(w, acc);
       __builtin_amdgcn_sched_barrier(0);
       values<D, BF>(vr, w, acc, mask, tok0, lim, low, see0, len);
-      if (more) load_v<D>(next, at, vr);
+      load_v<D>(next, at, vr);
     }
     if (bad) {
       acc.l = __builtin_nanf("");
       if (lane == 0) atomicOr(a.p.status, PAGED_BAD_PAGE);
     }
-    // the four waves' sums
+    // the waves' sums
     {
       auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc.l), __float_as_uint(acc.l), false, false);
       acc.l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
@@ -513,45 +519,81 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
       }
     }
     __syncthreads();
-    u += cnt;
-    if (a.split && u - first >= n * H * a.tiles) {
-      first += n * H * a.tiles;
+    if (over) {
+      first += (n + PAD) * H * a.tiles;
       ++s;
     }
   }
 }
 
-// one workgroup per (sequence, head, tile) that several workgroups computed: merges their slots in order
+// one workgroup per (sequence, head, tile): merges the slots of those that several workgroups computed, in order
 template <int D, bool BF>
 __global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
   const int per_seq = a.p.H * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
-  const int total = total_units(a), per = units_per_group(total, a.grid);
-  int lo, first = 0;
-  for (int s0 = 0; s0 < s; s0 += 64) {
-    const int i = s0 + int(threadIdx.x & 63);
-    int n = i < s ? pages_of(a, i, lo) * per_seq : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-    first += n;
-  }
-  const int n = pages_of(a, s, lo);
+  Part part = part_at(a, 0, 0);
+  const int total = total_units(a, part), per = units_per_group(total, a.grid);
+  for (int s0 = 64; s0 <= s; s0 += 64) part = part_at(a, s0, __builtin_amdgcn_readlane(part.end, 63));
+  const int units = __builtin_amdgcn_readlane(part.n, s & 63), n = units / per_seq;
   if (n <= 0) return;
-  const int u0 = first + hr * n, g0 = u0 / per, g1 = (u0 + n - 1) / per;
+  const int u0 = __builtin_amdgcn_readlane(part.end, s & 63) - units + hr * n, g0 = (u0 + PAD) / per, g1 = (u0 + n - 1) / per;
   if (g0 == g1) return;
-  const int rr = threadIdx.x / (D / 8), d = threadIdx.x % (D / 8) * 8;
-  float mx = NEG_INF;
-  for (int g = g0; g <= g1; ++g) mx = fmaxf(mx, slot_of<D>(a.ws, 2 * g + (g == g0 ? 1 : 0))[ROWS * D + rr]);
-  float sum = 0.f, v[8] = {};
-  for (int g = g0; g <= g1; ++g) {
-    const float* p = slot_of<D>(a.ws, 2 * g + (g == g0 ? 1 : 0));
-    const float m = p[ROWS * D + rr], l = p[ROWS * D + ROWS + rr];
-    const float f = m == NEG_INF ? 0.f : exp2f(m - mx);
-    sum += l != l ? l : f * l;
-    if (f != 0.f)
+  // lanes of D/8 take a row's dims, `parts` of them its slots in runs
+  const int tile = hr % a.tiles, rows = min(ROWS, a.m * a.nrep - tile * ROWS), parts = g1 - g0 < 4 ? 1 : ROWS / rows;
+  const int grp = threadIdx.x / (D / 8), part_i = grp / rows, rr = grp - part_i * rows, d = threadIdx.x % (D / 8) * 8;
+  const int run = (g1 - g0 + parts) / parts, ga = g0 + part_i * run, gz = part_i < parts ? min(ga + run - 1, g1) : -1;
+  constexpr int B = 4;  // slots whose loads are under way together
+  float mx = NEG_INF, sum = 0.f, v[8] = {};
+  for (int g = ga; g <= gz; g += B) {
+    float m[B], l[B];
+    f4_t x[B][2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += f * p[rr * D + d + e];
+    for (int i = 0; i < B; ++i) {
+      const int gi = min(g + i, gz);
+      const float* p = slot_of<D>(a.ws, 2 * gi + (gi == g0 ? 1 : 0));
+      m[i] = p[ROWS * D + rr];
+      l[i] = p[ROWS * D + ROWS + rr];
+      x[i][0] = *reinterpret_cast<const f4_t*>(p + rr * D + d);
+      x[i][1] = *reinterpret_cast<const f4_t*>(p + rr * D + d + 4);
+    }
+    const float was = mx;
+#pragma unroll
+    for (int i = 0; i < B; ++i) mx = fmaxf(mx, m[i]);
+    const float keep = was == NEG_INF ? 0.f : exp2f(was - mx);
+    sum *= keep;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (g + i > gz) break;
+      const float f = m[i] == NEG_INF ? 0.f : exp2f(m[i] - mx);
+      sum += l[i] != l[i] ? l[i] : f * l[i];
+      if (f != 0.f)  // (a slot that saw nothing, or nothing that counts)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += f * x[i][e / 4][e % 4];
+    }
   }
-  store_row<D, BF>(a, s, hr / a.tiles, hr % a.tiles, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+  __shared__ float sv[ROWS][D], sm[ROWS], sl[ROWS];
+  if (parts > 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sv[grp][d + e] = v[e];
+    if (d == 0) {
+      sm[grp] = mx;
+      sl[grp] = sum;
+    }
+    __syncthreads();
+    if (part_i > 0) return;
+    for (int i = 1; i < parts; ++i) {
+      const int o = i * rows + rr;
+      const float was = mx;
+      mx = fmaxf(mx, sm[o]);
+      const float keep = was == NEG_INF ? 0.f : exp2f(was - mx), f = sm[o] == NEG_INF ? 0.f : exp2f(sm[o] - mx);
+      sum = (was == NEG_INF ? sum : sum * keep) + (sl[o] != sl[o] ? sl[o] : f * sl[o]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = keep * v[e] + (f != 0.f ? f * sv[o][d + e] : 0.f);
+    }
+  }
+  if (part_i > 0) return;
+  store_row<D, BF>(a, s, hr / a.tiles, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
 }
 
 constexpr int GRID = 512;  // two workgroups per CU
@@ -563,7 +605,7 @@ struct Launch {
 inline Launch plan_of(int S, int P, int m, int nrep, int H) {
   Launch p;
   p.tiles = int(ceil_div(int64_t(m) * nrep, ROWS));
-  p.split = P > WAVES;
+  p.split = P > 2 * WAVES;
   p.grid = p.split ? GRID : S * H * p.tiles;
   return p;
 }
@@ -590,7 +632,7 @@ extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s
                so_m % 8 == 0 && so_h % 8 == 0, IQ_ERR_ALIGN);
   const int nrep = Hq / p->H;
   const Launch pl = plan_of(p->S, p->P, m, nrep, p->H);
-  IQ_CHECK(int64_t(p->S) * p->P * p->H * pl.tiles <= INT32_MAX, IQ_ERR_SHAPE);
+  IQ_CHECK(int64_t(p->S) * (p->P + PAD) * p->H * pl.tiles <= INT32_MAX, IQ_ERR_SHAPE);
   const size_t need = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
   IQ_CHECK(!need || (workspace && workspace_bytes >= need), IQ_ERR_WORKSPACE);
   IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
