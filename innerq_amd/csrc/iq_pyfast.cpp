@@ -1,6 +1,7 @@
 // Native front of the per-token calls: the argument checks, segment structures
 // and launches of ops.decode_attention, ops.qk_gemv, ops.av_gemv and
-// ops.window_append for the ordinary case, without Python between them.
+// ops.window_append for the ordinary case, without Python between them; and of
+// ops.prompt_attention and paged.PagedStore's append, read and attend.
 //
 // The Python wrappers build ~40 ctypes fields and ~30 small objects per call,
 // and short calls waited for them: a decode of one sequence over 1000 tokens
@@ -21,6 +22,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 
 #include "../../include/innerq_abi.h"
 
@@ -477,8 +480,279 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
   Py_RETURN_NONE;
 }
 
+// ---- many sequences: 4-bit pages and packed prompts ----
+typedef int (*paged_append_t)(const iq_paged*, const int32_t*, int, const void*, int64_t, int64_t, const void*, int64_t,
+                              int64_t, const float*, const float*, int64_t, int, const void*, int64_t, int64_t, int, void*,
+                              int64_t, int64_t, void*);
+typedef int (*paged_read_t)(const iq_paged*, const int32_t*, int, void*, int64_t, int64_t, void*, int64_t, int64_t, void*);
+typedef size_t (*paged_ws_t)(int, int, int, int, int, int);
+typedef int (*paged_attend_t)(const iq_paged*, const void*, int64_t, int64_t, int64_t, int, int, float, int, void*, int64_t,
+                              int64_t, int64_t, void*, size_t, void*);
+typedef int (*prompt_t)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, const void*, int64_t, int64_t,
+                        const int32_t*, const int32_t*, int, int, int, int, int, int, int, float, int, int, void*, int64_t,
+                        int64_t, void*);
+struct Serving {
+  paged_append_t append;
+  paged_read_t read;
+  paged_ws_t ws;
+  paged_attend_t attend;
+  prompt_t prompt;
+} sv{};
+
+// whether a call on `device` may launch as things are: it is the current device
+bool current(int device) { return c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice().index() == device; }
+bool followed(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+
+// a tensor of 16-bit rows as the kernels read them: D contiguous, rows on 16-byte boundaries
+const at::Tensor* rows_of(PyObject* o, int64_t dims, at::ScalarType dt, int device, int64_t D) {
+  const at::Tensor* t = tensor_of(o);
+  if (!t || t->dim() != dims || t->scalar_type() != dt || t->get_device() != device || t->size(dims - 1) != D ||
+      t->stride(dims - 1) != 1 || (uintptr_t(t->data_ptr()) & 15) || followed(*t))
+    return nullptr;
+  for (int64_t i = 0; i + 1 < dims; ++i)
+    if (t->stride(i) % 8) return nullptr;
+  return t;
+}
+// a contiguous int32 vector of n values on the device
+const at::Tensor* ints_of(PyObject* o, int64_t n, int device) {
+  const at::Tensor* t = tensor_of(o);
+  return t && t->dim() == 1 && t->scalar_type() == at::kInt && t->get_device() == device && t->size(0) == n &&
+                 t->is_contiguous() ? t : nullptr;
+}
+// a[0..5] of a PagedStore call: its pages, D, dtype and status, the call's table and lens
+bool paged_of(PyObject* const* a, iq_paged* p, at::ScalarType* dt, int* dev) {
+  const at::Tensor *pages = tensor_of(a[0]), *status = tensor_of(a[3]), *table = tensor_of(a[4]);
+  if (!pages || !status || !table || !PyLong_Check(a[1]) || !THPDtype_Check(a[2]) || pages->dim() != 3 ||
+      table->dim() != 2 || table->scalar_type() != at::kInt || table->size(0) < 1 || table->size(1) < 1 ||
+      table->stride(1) != 1 || table->size(0) > INT32_MAX || table->size(1) > INT32_MAX)
+    return false;
+  *dev = pages->get_device();
+  *dt = ((THPDtype*)a[2])->scalar_type;
+  const at::Tensor* lens = ints_of(a[5], table->size(0), *dev);
+  if (!lens || table->get_device() != *dev || status->get_device() != *dev || !act_dtype(*dt) || !current(*dev)) return false;
+  p->pages = (uint32_t*)pages->data_ptr();
+  p->n_pages = pages->size(0);
+  p->table = (const int32_t*)table->data_ptr();
+  p->s_table = table->stride(0);
+  p->lens = (const int32_t*)lens->data_ptr();
+  p->status = (int32_t*)status->data_ptr();
+  p->S = int(table->size(0)); p->P = int(table->size(1));
+  p->H = int(pages->size(1)); p->D = int(PyLong_AsLong(a[1]));
+  p->mode = act_flag(*dt);
+  return true;
+}
+// cu_seqlens of S sequences over N rows (None: N = S)
+bool cu_of(PyObject* o, int64_t S, int64_t N, int device, const int32_t** cu) {
+  *cu = nullptr;
+  if (o == Py_None) return N == S;
+  const at::Tensor* t = ints_of(o, S + 1, device);
+  if (t) *cu = (const int32_t*)t->data_ptr();
+  return t != nullptr;
+}
+bool window_of(PyObject* o, int64_t* w) {
+  *w = 0;
+  return o == Py_None || (ints(&o, {0}, w) && *w > 0 && *w <= INT32_MAX);
+}
+at::Tensor like(const at::Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
+
+// paged_append(pages, D, dtype, status, table, lens, k, v, cu, cos, sin, q, q_out): (q_out or None,), or None
+PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  iq_paged p{};
+  at::ScalarType dt;
+  int dev;
+  if (na != 13 || !paged_of(a, &p, &dt, &dev)) Py_RETURN_NONE;
+  const at::Tensor *k = rows_of(a[6], 3, dt, dev, p.D), *v = rows_of(a[7], 3, dt, dev, p.D);
+  const int32_t* cu;
+  if (!k || !v || k->size(0) < 1 || k->size(0) > INT32_MAX || k->size(1) != p.H || v->sizes() != k->sizes() ||
+      !cu_of(a[8], p.S, k->size(0), dev, &cu))
+    Py_RETURN_NONE;
+  const float* tab[2] = {nullptr, nullptr};
+  int64_t n_pos = 0, half = 0;
+  for (int i = 0; i < 2; ++i) {
+    if ((a[9] == Py_None) != (a[10] == Py_None)) Py_RETURN_NONE;
+    if (a[9] == Py_None) break;
+    const at::Tensor* t = tensor_of(a[9 + i]);
+    if (!t || t->dim() != 2 || t->scalar_type() != at::kFloat || t->get_device() != dev || !t->is_contiguous() || followed(*t) ||
+        (i && (t->size(0) != n_pos || t->size(1) != half)))
+      Py_RETURN_NONE;
+    n_pos = t->size(0);
+    half = t->size(1);
+    tab[i] = (const float*)t->data_ptr();
+  }
+  if (half > 128) Py_RETURN_NONE;
+  const at::Tensor* q = nullptr;
+  at::Tensor out;
+  if (a[11] != Py_None) {
+    q = rows_of(a[11], 3, dt, dev, p.D);
+    if (!q || q->size(0) != k->size(0) || q->size(1) < 1 || q->size(1) > 4096) Py_RETURN_NONE;
+    if (a[12] != Py_None) {
+      const at::Tensor* o = rows_of(a[12], 3, dt, dev, p.D);
+      if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
+      out = *o;
+    }
+  } else if (a[12] != Py_None) Py_RETURN_NONE;
+  void* stream;
+  PyObject* key;
+  if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
+  Py_DECREF(key);
+  if (q && !out.defined()) {
+    try { out = like(*q); } catch (...) { Py_RETURN_NONE; }
+  }
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = sv.append(&p, cu, int(k->size(0)), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1),
+                 tab[0], tab[1], n_pos, int(2 * half), q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+                 q ? int(q->size(1)) : 0, q ? out.data_ptr() : nullptr, q ? out.stride(0) : 0, q ? out.stride(1) : 0, stream);
+  Py_END_ALLOW_THREADS
+  if (st != IQ_OK) return not_ok("iq_paged_append", st);
+  if (!q) return PyTuple_Pack(1, Py_None);
+  if (a[12] != Py_None) return PyTuple_Pack(1, a[12]);
+  PyObject* w = THPVariable_Wrap(std::move(out));
+  PyObject* r = w ? PyTuple_Pack(1, w) : nullptr;
+  Py_XDECREF(w);
+  return r;
+}
+
+// paged_read(pages, D, dtype, status, table, lens, cu, n): (k, v), new tensors, or None
+PyObject* paged_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  iq_paged p{};
+  at::ScalarType dt;
+  int dev;
+  int64_t n;
+  const int32_t* cu;
+  if (na != 8 || !ints(a, {7}, &n) || n < 1 || n > INT32_MAX || !paged_of(a, &p, &dt, &dev) || !cu_of(a[6], p.S, n, dev, &cu))
+    Py_RETURN_NONE;
+  void* stream;
+  PyObject* key;
+  if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
+  Py_DECREF(key);
+  at::Tensor k, v;
+  try {
+    k = at::empty({n, p.H, p.D}, at::TensorOptions().dtype(dt).device(c10::Device(c10::DeviceType::CUDA, dev)));
+    v = like(k);
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = sv.read(&p, cu, int(n), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), stream);
+  Py_END_ALLOW_THREADS
+  if (st != IQ_OK) return not_ok("iq_paged_read", st);
+  PyObject *kw = THPVariable_Wrap(std::move(k)), *vw = THPVariable_Wrap(std::move(v));
+  PyObject* r = kw && vw ? PyTuple_Pack(2, kw, vw) : nullptr;
+  Py_XDECREF(kw);
+  Py_XDECREF(vw);
+  return r;
+}
+
+// paged_attend(pages, D, dtype, status, table, lens, q, scale, window, out): the output, or None
+PyObject* paged_attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  iq_paged p{};
+  at::ScalarType dt;
+  int dev;
+  int64_t window;
+  if (na != 10 || !paged_of(a, &p, &dt, &dev) || !window_of(a[8], &window)) Py_RETURN_NONE;
+  const at::Tensor* q = tensor_of(a[6]);
+  if (!q || (q->dim() != 3 && q->dim() != 4)) Py_RETURN_NONE;
+  const int nd = int(q->dim());
+  q = rows_of(a[6], nd, dt, dev, p.D);
+  if (!q || q->size(0) != p.S) Py_RETURN_NONE;
+  const int64_t m = nd == 3 ? 1 : q->size(1), Hq = q->size(nd - 2);
+  if (m < 1 || m > 16 || Hq < 1 || Hq > 4096 || p.H < 1 || Hq % p.H) Py_RETURN_NONE;
+  const double scale = PyFloat_AsDouble(a[7]);
+  if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  at::Tensor out;
+  if (a[9] != Py_None) {
+    const at::Tensor* o = rows_of(a[9], nd, dt, dev, p.D);
+    if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
+    out = *o;
+  }
+  void* stream;
+  PyObject* key;
+  if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
+  Py_DECREF(key);
+  const size_t wsb = sv.ws(p.S, p.P, int(m), int(Hq), p.H, p.D);
+  at::Tensor ws;
+  try {
+    if (!out.defined()) out = like(*q);
+    if (wsb) ws = at::empty({int64_t(wsb)}, q->options().dtype(at::kByte).requires_grad(false));
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+  const int64_t sm = nd == 3 ? 0 : q->stride(1), om = nd == 3 ? 0 : out.stride(1);
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = sv.attend(&p, q->data_ptr(), q->stride(0), sm, q->stride(nd - 2), int(m), int(Hq), float(scale), int(window),
+                 out.data_ptr(), out.stride(0), om, out.stride(nd - 2), wsb ? ws.data_ptr() : nullptr, wsb, stream);
+  Py_END_ALLOW_THREADS
+  if (st != IQ_OK) return not_ok("iq_paged_attention", st);
+  if (a[9] != Py_None) { Py_INCREF(a[9]); return a[9]; }
+  return THPVariable_Wrap(std::move(out));
+}
+
+// prompt(q, k, v, cu, scale, cu_k, causal, window, out): the output, or None
+PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 9 || !PyBool_Check(a[6])) Py_RETURN_NONE;
+  const at::Tensor *q = tensor_of(a[0]), *cu = tensor_of(a[3]);
+  if (!q || !cu || q->dim() != 3 || !act_dtype(q->scalar_type()) || cu->dim() != 1) Py_RETURN_NONE;
+  const at::ScalarType dt = q->scalar_type();
+  const int dev = q->get_device();
+  const int64_t D = q->size(2), N = q->size(0), Hq = q->size(1), S = cu->size(0) - 1;
+  q = rows_of(a[0], 3, dt, dev, D);
+  const at::Tensor *k = rows_of(a[1], 3, dt, dev, D), *v = rows_of(a[2], 3, dt, dev, D);
+  int64_t window;
+  if (!q || !k || !v || S < 1 || S > INT32_MAX || N < 1 || N > INT32_MAX || Hq < 1 || k->size(0) < 1 ||
+      k->size(0) > INT32_MAX || k->size(1) < 1 || Hq % k->size(1) || v->sizes() != k->sizes() || (D != 64 && D != 128) ||
+      k->stride(0) >= 1 << 23 || v->stride(0) >= 1 << 23 || !ints_of(a[3], S + 1, dev) || !window_of(a[7], &window) ||
+      (window && a[6] == Py_False) || !current(dev))
+    Py_RETURN_NONE;
+  const at::Tensor* cu_k = cu;
+  if (a[5] != Py_None) cu_k = ints_of(a[5], S + 1, dev);
+  if (!cu_k || (a[5] == Py_None && k->size(0) != N)) Py_RETURN_NONE;
+  const double scale = PyFloat_AsDouble(a[4]);
+  if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  at::Tensor out;
+  if (a[8] != Py_None) {
+    const at::Tensor* o = rows_of(a[8], 3, dt, dev, D);
+    if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
+    out = *o;
+  }
+  void* stream;
+  PyObject* key;
+  if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
+  Py_DECREF(key);
+  if (!out.defined()) {
+    try { out = at::empty(q->sizes(), q->options().requires_grad(false)); } catch (...) { Py_RETURN_NONE; }
+  }
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = sv.prompt(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(),
+                 v->stride(0), v->stride(1), (const int32_t*)cu->data_ptr(), (const int32_t*)cu_k->data_ptr(), int(S), int(N),
+                 int(k->size(0)), int(Hq), int(k->size(1)), int(D), act_flag(dt), float(scale), a[6] == Py_True, int(window),
+                 out.data_ptr(), out.stride(0), out.stride(1), stream);
+  Py_END_ALLOW_THREADS
+  if (st != IQ_OK) return not_ok("iq_prompt_attention", st);
+  if (a[8] != Py_None) { Py_INCREF(a[8]); return a[8]; }
+  return THPVariable_Wrap(std::move(out));
+}
+
+// bind_serving(addresses): after bind()
+PyObject* bind_serving(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 1 || !PyTuple_Check(a[0]) || PyTuple_Size(a[0]) != 5) {
+    PyErr_SetString(PyExc_TypeError, "bind_serving(five addresses)");
+    return nullptr;
+  }
+  void* p[5];
+  for (int i = 0; i < 5; ++i) p[i] = PyLong_AsVoidPtr(PyTuple_GetItem(a[0], i));
+  if (PyErr_Occurred()) return nullptr;
+  sv = {(paged_append_t)p[0], (paged_read_t)p[1], (paged_ws_t)p[2], (paged_attend_t)p[3], (prompt_t)p[4]};
+  Py_RETURN_NONE;
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(bind), FAST(decode), FAST(qk), FAST(av), FAST(window_append), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FAST(bind), FAST(decode), FAST(qk), FAST(av), FAST(window_append),
+                         FAST(bind_serving), FAST(paged_append), FAST(paged_read), FAST(paged_attend), FAST(prompt),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_iqfast", nullptr, -1, methods};
 
 }  // namespace

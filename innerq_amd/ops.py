@@ -52,6 +52,9 @@ def _native(t):
              "iq_av_workspace_bytes", "iq_av_gemv", "iq_window_append")
     m.bind(tuple(ctypes.cast(getattr(h, n), ctypes.c_void_p).value for n in names), _WS,
            torch._C._cuda_getCurrentRawStream)
+    names = ("iq_paged_append", "iq_paged_read", "iq_paged_attention_workspace_bytes", "iq_paged_attention",
+             "iq_prompt_attention")
+    m.bind_serving(tuple(ctypes.cast(getattr(h, n), ctypes.c_void_p).value for n in names))
     _fast = m
     return m
 
@@ -887,6 +890,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     keys, each row before it one less (a chunk of a prompt behind its earlier keys has more keys than rows); window:
     only the last ``window`` of the keys up to its own.  Rows that see no key are 0; rows outside the sequences are
     not written.  Inference only: tensors that autograd follows are refused."""
+    fast = _native(q)
+    if fast is not None:
+        r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out)
+        if r is not None:
+            return r
     require_act(q, "q")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise NotImplementedError("prompt_attention has no backward: call it under torch.no_grad()")

@@ -147,6 +147,12 @@ class PagedStore:
         token's row (pairs d, d + R/2).  Returns q [N, Hq, D] rotated, written to ``q_out`` (which may be q) or a new
         tensor; None without q.  Rows outside the sequences are neither appended nor written to q_out.  Sequences
         that append must not share the pages they append to."""
+        fast = ops._native(k)
+        if fast is not None:
+            r = fast.paged_append(self.pages, self.D, self.dtype, self.status, table, lens, k, v, cu_seqlens, cos, sin, q,
+                                  q_out)
+            if r is not None:
+                return r[0]
         _no_grad(k, v, q, cos, sin)
         p = self._args(table, lens)
         if k.dim() != 3:
@@ -192,6 +198,11 @@ class PagedStore:
              k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
         """K and V [n, H, D] of tokens lens[s] + i of every sequence, at rows cu_seqlens[s] + i (as ``append`` takes
         them; n rows in all).  Rows outside the sequences are not written."""
+        fast = ops._native(self.pages)
+        if fast is not None and k_out is None and v_out is None:
+            r = fast.paged_read(self.pages, self.D, self.dtype, self.status, table, lens, cu_seqlens, n)
+            if r is not None:
+                return r
         p = self._args(table, lens)
         cu = self._cu(cu_seqlens, p.S, n)
         want = (n, self.H, self.D)
@@ -210,6 +221,11 @@ class PagedStore:
         """softmax(q K^T * scale) V over each sequence's first lens[s] tokens, the new ones among them.  q [S, Hq, D]
         (one new token) or [S, m, Hq, D] (m <= 16: token j sees all but the m - 1 - j after it); window: only the last
         ``window`` tokens up to its own.  Rows that see no token are 0.  Returns a tensor of q's shape."""
+        fast = ops._native(q)
+        if fast is not None:
+            r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out)
+            if r is not None:
+                return r
         _no_grad(q)
         p = self._args(table, lens)
         if q.dim() not in (3, 4) or q.shape[0] != p.S:

@@ -502,3 +502,33 @@ def test_refusals():
         paged.PagedStore(4, 2, 64, DEV, torch.float32)
     with pytest.raises(ValueError):
         st.read(table, lens, cu, 3, k_out=k[:2])
+
+
+def test_the_native_front_and_the_general_path_agree(monkeypatch):
+    """The same calls through csrc/iq_pyfast.cpp and through the Python path: the same bits."""
+    g, rng = torch.Generator().manual_seed(13), random.Random(13)
+    H, Hq, D, lens = 2, 8, 64, [70, 3, 129]
+    cos, sin = (t.to(DEV) for t in angles(200, 32))
+    k, v = normal(g, 202, H, D).to(DEV), normal(g, 202, H, D).to(DEV)
+    q = normal(g, 202, Hq, D).to(DEV)
+    _, table = tables(rng, [n + 1 for n in lens])
+    cu = i32([0, 70, 73, 202])
+    results = []
+    for general in (False, True):
+        with monkeypatch.context() as m:
+            if general:
+                m.setattr(ops, "_native", lambda t: None)
+            st = paged.PagedStore(int(table.max()) + 1, H, D, DEV)
+            st.pages.zero_()
+            a = st.append(k, v, table, i32([0] * 3), cu, cos, sin, q=q)
+            b = st.append(k[:3], v[:3], table, i32(lens), q=q[:3], q_out=torch.empty_like(q[:3]))
+            c = st.read(table, i32([0] * 3), cu, 202)
+            d = st.attend(b, table, i32(lens) + 1, 0.125)
+            e = st.attend(q[:6].view(3, 2, Hq, D), table, i32(lens) + 1, 0.125, window=40, out=torch.empty(3, 2, Hq, D, device=DEV).half())
+            f = ops.prompt_attention(a, c[0], c[1], cu, 0.125)
+            h = ops.prompt_attention(a, c[0], c[1], cu, 0.125, cu_seqlens_k=cu, window=30, out=torch.empty_like(a))
+            n = ops.prompt_attention(a, c[0], c[1], cu, 0.125, causal=False)
+            assert st.append(k[:3], v[:3], table, i32(lens)) is None
+            results.append([st.pages, a, b, *c, d, e, f, h, n])
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
