@@ -155,22 +155,117 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
       const int j = lane & 15, d = b * 32 + (lane >> 4 & 1) * 16 + j % 4 * 4;
       va[b][h] = chunk_at<D>(h * 8 + hi * 4 + j / 4, d / 8) * 16 + d % 8 * 2;
     }
-  auto step = [&](int t, const u4_t* lk, const u4_t* lv) {
+  // S^T of a tile: st[kb][i] is key 32 kb + 8 (i/4) + 4 hi + i%4.  All of one block's operands are on their way before
+  // its products begin, the next block's take their places.
+  auto scores = [&](const u4_t* lk, f16_t (&st)[2]) {
+    auto at = [&](int kb, int ks) { return *reinterpret_cast<const u4_t*>(reinterpret_cast<const char*>(lk) + ka[ks] + kb * 32 * CH * 16); };
+    u4_t x[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) x[ks] = at(0, ks);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        st[kb] = mma32<BF>(x[ks], q[ks], st[kb]);
+        if (kb == 0) x[ks] = at(1, ks);
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);  // LDS reads
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
+  };
+  // V^T's operand: dim 32 b + n, keys 16 kc + 8 (e/4) + 4 hi + e%4
+  auto v_operand = [&](const u4_t* lv, int kc, int b) {
+    u4_t y;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const char* at = reinterpret_cast<const char*>(lv) + va[b][h] + kc * 16 * CH * 16;
+      const u2_t w = __builtin_bit_cast(
+          u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)at));
+      y[2 * h] = w.x;
+      y[2 * h + 1] = w.y;
+    }
+    return y;
+  };
+  // the running maximum over a tile (in both halves of the wave)
+  auto maximum = [&](const f16_t (&st)[2]) {
+    float x[4] = {m, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i % 4] = fmaxf(x[i % 4], st[kb][i]);
+    const float y = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
+  };
+  // Weights are relative to 2^base, base = RN(max c).
+  auto base_of = [&](float x) { return x == NEG_INF ? 0.f : x * a.c; };
+  auto rescale = [&](float mx, float base) {
+    if (__any(mx != m)) {
+      const float f = __builtin_amdgcn_exp2f(m == NEG_INF ? NEG_INF : m * a.c - base);
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] *= f;
+      m = mx;
+    }
+  };
+  // exponents to weights: their sum into l, rounded and in pairs into p (keys as v_operand's)
+  auto weigh = [&](f16_t (&st)[2], u4_t (&p)[4]) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        st[kb][i] = __builtin_amdgcn_exp2f(st[kb][i]);
+        sum[i % 4] += st[kb][i];
+      }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[kc][i] = pack2<BF>(st[kc / 2][8 * (kc % 2) + 2 * i], st[kc / 2][8 * (kc % 2) + 2 * i + 1]);
+  };
+  auto products = [&](const u4_t* lv, const u4_t (&p)[4]) {
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] = mma32<BF>(v_operand(lv, kc, b), p[kc], o[b]);
+  };
+
+  // A tile that every row of the workgroup sees whole.  False (and nothing done) where logits are so large that one fma
+  // per logit, whose weights share a factor of 2^(the error of base), will not do.
+  auto whole_tile = [&](const u4_t* lk, const u4_t* lv) {
+    f16_t st[2];
+    scores(lk, st);
+    const float mx = maximum(st), base = base_of(mx);
+    if (__any(fabsf(base) > 65536.f)) return false;
+    rescale(mx, base);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[kb][i] = __builtin_fmaf(st[kb][i], a.c, -base);
+    u4_t p[4];
+    weigh(st, p);
+    products(lv, p);
+    return true;
+  };
+
+  // Any tile: logits times c rounded as base is; keys that a row does not see have weight 0.
+  auto any_tile = [&](int t, const u4_t* lk, const u4_t* lv) {
     const int j0 = t * BN;
     // this wave's rows: does any see the tile, do all see all of it?
     const int wa = row_a + wave * 32, wz = min(wa + 31, lq - 1);
     const int w_last = a.causal ? min(wz + off + 1, keys) : keys, w_first = a.window ? max(wa + off + 1 - a.window, 0) : 0;
     if (wa >= lq || w_last <= j0 || w_first >= j0 + BN) return;
     const bool mask = (a.causal ? min(wa + off + 1, keys) : keys) < j0 + BN || (a.window && wz + off + 1 - a.window > j0);
-
-    f16_t st[2];  // st[kb][i]: key 32 kb + 8 (i/4) + 4 hi + i%4 of the tile
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) st[kb] = mma32<BF>(*reinterpret_cast<const u4_t*>(reinterpret_cast<const char*>(lk) + ka[ks] + kb * 32 * CH * 16), q[ks], st[kb]);
-    }
+    f16_t st[2];
+    scores(lk, st);
     if (mask) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -180,63 +275,14 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
           if (j >= last || j < first) st[kb][i] = NEG_INF;
         }
     }
-    float mx = m;
+    const float mx = maximum(st), base = base_of(mx);
+    rescale(mx, base);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[kb][i]);
-    {
-      const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-      mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-    }
-    // weights relative to 2^base, base = RN(max c): the fma form leaves a common factor of 2^(error of base), which the
-    // sum shares; where base is so large that the factor would leave [1/2, 2], logits are rounded as base is
-    const float was = m == NEG_INF ? 0.f : m * a.c, base = mx == NEG_INF ? 0.f : mx * a.c;
-    if (__any(mx != m)) {
-      const float f = __builtin_amdgcn_exp2f(m == NEG_INF ? NEG_INF : was - base);
-      l *= f;
-#pragma unroll
-      for (int b = 0; b < DB; ++b) o[b] *= f;
-      m = mx;
-    }
-    float sum = 0.f;
-    if (__any(fabsf(base) > 65536.f)) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[kb][i] = st[kb][i] * a.c - base;
-    } else {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[kb][i] = __builtin_fmaf(st[kb][i], a.c, -base);
-    }
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        st[kb][i] = __builtin_amdgcn_exp2f(st[kb][i]);
-        sum += st[kb][i];
-      }
-    l += sum;
-    u4_t p[4];  // keys 16 kc + 8 (e/4) + 4 hi + e%4, e = 0..7
-#pragma unroll
-    for (int kc = 0; kc < 4; ++kc)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[kc][i] = pack2<BF>(st[kc / 2][8 * (kc % 2) + 2 * i], st[kc / 2][8 * (kc % 2) + 2 * i + 1]);
-    // V^T's operand: dim 32 b + n, the keys of p
-    auto v_operand = [&](int kc, int b) {
-      u4_t y;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const char* at = reinterpret_cast<const char*>(lv) + va[b][h] + kc * 16 * CH * 16;
-        const u2_t w = __builtin_bit_cast(
-            u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)at));
-        y[2 * h] = w.x;
-        y[2 * h + 1] = w.y;
-      }
-      return y;
-    };
+      for (int i = 0; i < 16; ++i) st[kb][i] = st[kb][i] * a.c - base;
+    u4_t p[4];
+    weigh(st, p);
     bool odd = false;
     if (mask) {  // does V hold an infinity or NaN (0 * inf would carry it into rows that do not see its key)?
       const uint32_t e = BF ? 0x7f80u : 0x7c00u;
@@ -247,46 +293,63 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
       }
     }
     if (!__any(odd)) {
-#pragma unroll
-      for (int kc = 0; kc < 4; ++kc)
-#pragma unroll
-        for (int b = 0; b < DB; ++b) o[b] = mma32<BF>(v_operand(kc, b), p[kc], o[b]);
-    } else {  // key by key, into the rows that see it
+      products(lv, p);
+      return;
+    }
+    // key by key, into the rows that see it
 #pragma clang loop unroll(disable)
-      for (int key = 0; key < BN; ++key) {
-        const int at = key / 16 * 4 + key % 16 / 8 * 2 + key % 4 / 2, of = key % 8 / 4;  // p's word, in the lanes hi == of
-        uint32_t w = 0;
+    for (int key = 0; key < BN; ++key) {
+      const int at = key / 16 * 4 + key % 16 / 8 * 2 + key % 4 / 2, of = key % 8 / 4;  // p's word, in the lanes hi == of
+      uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (i == at) w = p[i / 4][i % 4];
-        const auto y = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-        w = of ? y[1] : y[0];
-        const float pk = key & 1 ? hi_half<BF>(w) : lo_half<BF>(w);
-        if (j0 + key < last && j0 + key >= first) {
+      for (int i = 0; i < 16; ++i)
+        if (i == at) w = p[i / 4][i % 4];
+      const auto y = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+      w = of ? y[1] : y[0];
+      const float pk = key & 1 ? hi_half<BF>(w) : lo_half<BF>(w);
+      if (j0 + key < last && j0 + key >= first) {
 #pragma unroll
-          for (int b = 0; b < DB; ++b)
+        for (int b = 0; b < DB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const u2_t x = reinterpret_cast<const u2_t*>(&lv[chunk_at<D>(key, 4 * b + i)])[hi];
-              const uint32_t x0 = x.x, x1 = x.y;
-              o[b][4 * i] = __builtin_fmaf(pk, lo_half<BF>(x0), o[b][4 * i]);
-              o[b][4 * i + 1] = __builtin_fmaf(pk, hi_half<BF>(x0), o[b][4 * i + 1]);
-              o[b][4 * i + 2] = __builtin_fmaf(pk, lo_half<BF>(x1), o[b][4 * i + 2]);
-              o[b][4 * i + 3] = __builtin_fmaf(pk, hi_half<BF>(x1), o[b][4 * i + 3]);
-            }
-        }
+          for (int i = 0; i < 4; ++i) {
+            const u2_t x = reinterpret_cast<const u2_t*>(&lv[chunk_at<D>(key, 4 * b + i)])[hi];
+            const uint32_t x0 = x.x, x1 = x.y;
+            o[b][4 * i] = __builtin_fmaf(pk, lo_half<BF>(x0), o[b][4 * i]);
+            o[b][4 * i + 1] = __builtin_fmaf(pk, hi_half<BF>(x0), o[b][4 * i + 1]);
+            o[b][4 * i + 2] = __builtin_fmaf(pk, lo_half<BF>(x1), o[b][4 * i + 2]);
+            o[b][4 * i + 3] = __builtin_fmaf(pk, hi_half<BF>(x1), o[b][4 * i + 3]);
+          }
       }
     }
   };
-  if (t_begin < t_end) fetch(t_begin, lk0, lv0);
-  for (int t = t_begin; t < t_end; t += 2) {
+
+  // The tiles' order: [whole_a, whole_z), which every row sees whole, then the others; tile number i of it goes through
+  // buffer i % 2, and every wave passes the same barriers.
+  int whole_a = a.window ? (max(row_z + off + 1 - a.window, 0) + BN - 1) / BN : 0;
+  int whole_z = (a.causal ? min(row_a + off + 1, keys) : keys) / BN;
+  if (whole_a >= whole_z || t_begin >= t_end) whole_a = whole_z = t_begin;
+  const int nw = whole_z - whole_a, tail = t_end - whole_z, count = t_end - t_begin;
+  auto tile_at = [&](int i) { return i < nw ? whole_a + i : i < nw + tail ? whole_z + i - nw : t_begin + i - nw - tail; };
+  bool ready = false;  // tile i is in LDS and waits to be done
+  int i = 0;
+  if (count > 0) fetch(tile_at(0), lk0, lv0);
+  while (i < nw) {
     __syncthreads();  // the tile is there, and no wave reads the other buffer any more
-    if (t + 1 < t_end) fetch(t + 1, lk1, lv1);
-    step(t, lk0, lv0);
-    if (t + 1 >= t_end) break;
+    if (i + 1 < count) fetch(tile_at(i + 1), lk1, lv1);
+    if (!whole_tile(lk0, lv0)) { ready = true; break; }
+    if (++i >= nw) break;
     __syncthreads();
-    if (t + 2 < t_end) fetch(t + 2, lk0, lv0);
-    step(t + 1, lk1, lv1);
+    if (i + 1 < count) fetch(tile_at(i + 1), lk0, lv0);
+    if (!whole_tile(lk1, lv1)) { ready = true; break; }
+    ++i;
+  }
+  for (; i < count; ++i, ready = false) {
+    u4_t *lk = i & 1 ? lk1 : lk0, *lv = i & 1 ? lv1 : lv0;
+    if (!ready) {
+      __syncthreads();
+      if (i + 1 < count) fetch(tile_at(i + 1), i & 1 ? lk0 : lk1, i & 1 ? lv0 : lv1);
+    }
+    any_tile(tile_at(i), lk, lv);
   }
   {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
