@@ -1,7 +1,7 @@
 // Attention over packed prompts (gfx950): iq_prompt_attention.
 //
-// Sequences of different lengths lie one behind the other; a workgroup takes 128 query rows of one head of one
-// sequence (four waves of 32 rows) and walks over the sequence's keys in tiles of 64, staged through LDS.  Both
+// Sequences of different lengths lie one behind the other; a workgroup takes 128 rows of one KV head of one sequence
+// (query rows times the heads that share the KV head; four waves of 32) and walks over the sequence's keys in tiles of 64, staged through LDS.  Both
 // products run transposed on v_mfma_f32_32x32x16: S^T = K Q^T leaves a query row per lane and its keys in the lane's
 // registers, where the running softmax needs one exchange (with the lane of the other half-wave) per tile, and the
 // exponentials, rounded to the activation dtype, are the B operand of O^T += V^T P^T as they are: V^T's A operand
@@ -36,12 +36,20 @@ __device__ __forceinline__ void rows_of(const int32_t* cu, int s, int n, int& r0
   r1 = min(max(cu[s + 1], r0), n);
 }
 
+// tiles of BM rows that a KV head's share of a sequence of lq query rows makes
+__device__ __forceinline__ int tiles_of(int lq, int nrep) { return int((int64_t(lq) * nrep + BM - 1) / BM); }
+
 template <bool BF>
 __device__ __forceinline__ f16_t mma32(u4_t a, u4_t b, f16_t c) {
   if constexpr (BF)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+  typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2_t, a), __builtin_bit_cast(us2_t, b)));
 }
 
 // 16-byte chunk c of row r in an LDS tile: spread so that neither K's reads (one chunk of 16 rows) nor V's transposed
@@ -58,13 +66,13 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   constexpr int CH = D / 8, KS = D / 16, DB = D / 32;  // chunks per row, k steps of S, blocks of 32 dims
   constexpr int LOADS = BN * CH / THREADS;             // chunks per thread and tile
   __shared__ u4_t lk0[BN * CH], lk1[BN * CH], lv0[BN * CH], lv1[BN * CH];
+  __shared__ int lodd[2][WAVES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
 
-  // this workgroup's (KV head, slot, head in the group); blocks go round robin over the 8 XCDs, so each XCD takes a
-  // run of items: the same keys
+  // this workgroup's KV head and slot; blocks go round robin over the 8 XCDs, so each XCD takes a run of items: the
+  // same keys
   const int total = gridDim.x, x = blockIdx.x % 8, base = total / 8, rest = total % 8;
-  const int item = x * base + min(x, rest) + blockIdx.x / 8;
-  const int g = item % a.nrep, slot = item / a.nrep % a.slots, kvh = item / a.nrep / a.slots, head = kvh * a.nrep + g;
+  const int item = x * base + min(x, rest) + blockIdx.x / 8, slot = item % a.slots, kvh = item / a.slots;
 
   // the slot's sequence and tile of rows, the last tiles (the longest) first
   int s = -1, tile = 0, q0 = 0, q1 = 0;
@@ -73,7 +81,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     for (int s0 = 0; s0 < a.S; s0 += 64) {
       int r0 = 0, r1 = 0;
       if (s0 + lane < a.S) rows_of(a.cu_q, s0 + lane, a.N, r0, r1);
-      const int t = (r1 - r0 + BM - 1) / BM;
+      const int t = tiles_of(r1 - r0, a.nrep);
       int end = t;
 #pragma unroll
       for (int o = 1; o < 64; o *= 2) {
@@ -98,19 +106,19 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   rows_of(a.cu_k, s, a.Nk, k0, k1);
   k0 = __builtin_amdgcn_readfirstlane(k0);
   k1 = __builtin_amdgcn_readfirstlane(k1);
-  const int lq = q1 - q0, keys = k1 - k0, off = keys - lq;
-  const int row = tile * BM + wave * 32 + n;  // this lane's query row in the sequence
-  const bool real = row < lq;
+  const int lq = q1 - q0, keys = k1 - k0, off = keys - lq, rows = lq * a.nrep;
+  // this lane's row of the KV head's rows, which are its query rows' heads one behind the other: row * nrep + head
+  const int vrow = tile * BM + wave * 32 + n, row = min(vrow, rows - 1) / a.nrep, head = kvh * a.nrep + min(vrow, rows - 1) % a.nrep;
   // key j is seen iff first <= j < last
   const int last = a.causal ? min(row + off + 1, keys) : keys, first = a.window ? max(row + off + 1 - a.window, 0) : 0;
   // the tiles of keys that any row of the workgroup sees
-  const int row_a = tile * BM, row_z = min(row_a + BM, lq) - 1;
+  const int row_a = tile * BM / a.nrep, row_z = (min(tile * BM + BM, rows) - 1) / a.nrep;
   const int j_end = a.causal ? min(row_z + off + 1, keys) : keys, j_begin = a.window ? max(row_a + off + 1 - a.window, 0) : 0;
   const int t_begin = j_begin / BN, t_end = j_end > j_begin ? (j_end + BN - 1) / BN : t_begin;
 
   u4_t q[KS];  // B operand: row n, dims 16 ks + 8 hi + e (rows past the end repeat the last one and are not stored)
   {
-    const uint16_t* p = a.q + int64_t(q0 + min(row, lq - 1)) * a.sq_n + head * a.sq_h + 8 * hi;
+    const uint16_t* p = a.q + int64_t(q0 + row) * a.sq_n + head * a.sq_h + 8 * hi;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[ks] = *reinterpret_cast<const u4_t*>(p + 16 * ks);
 #pragma unroll
@@ -257,23 +265,28 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   };
 
   // Any tile: logits times c rounded as base is; keys that a row does not see have weight 0.
-  auto any_tile = [&](int t, const u4_t* lk, const u4_t* lv) {
+  // odd: V holds an infinity or NaN, which 0 * inf would carry into rows that do not see its key.
+  auto any_tile = [&](int t, const u4_t* lk, const u4_t* lv, bool odd) {
     const int j0 = t * BN;
     // this wave's rows: does any see the tile, do all see all of it?
-    const int wa = row_a + wave * 32, wz = min(wa + 31, lq - 1);
+    const int va = tile * BM + wave * 32, wa = va / a.nrep, wz = min(va + 31, rows - 1) / a.nrep;
     const int w_last = a.causal ? min(wz + off + 1, keys) : keys, w_first = a.window ? max(wa + off + 1 - a.window, 0) : 0;
-    if (wa >= lq || w_last <= j0 || w_first >= j0 + BN) return;
+    if (va >= rows || w_last <= j0 || w_first >= j0 + BN) return;
     const bool mask = (a.causal ? min(wa + off + 1, keys) : keys) < j0 + BN || (a.window && wz + off + 1 - a.window > j0);
     f16_t st[2];
     scores(lk, st);
     if (mask) {
+      const int z = last - j0 - 4 * hi, f = first - j0 - 4 * hi;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = j0 + 32 * kb + 8 * (i / 4) + 4 * hi + i % 4;
-          if (j >= last || j < first) st[kb][i] = NEG_INF;
-        }
+        for (int i = 0; i < 16; ++i) st[kb][i] = 32 * kb + 8 * (i / 4) + i % 4 >= z ? NEG_INF : st[kb][i];
+      if (a.window) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st[kb][i] = 32 * kb + 8 * (i / 4) + i % 4 < f ? NEG_INF : st[kb][i];
+      }
     }
     const float mx = maximum(st), base = base_of(mx);
     rescale(mx, base);
@@ -283,16 +296,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
       for (int i = 0; i < 16; ++i) st[kb][i] = st[kb][i] * a.c - base;
     u4_t p[4];
     weigh(st, p);
-    bool odd = false;
-    if (mask) {  // does V hold an infinity or NaN (0 * inf would carry it into rows that do not see its key)?
-      const uint32_t e = BF ? 0x7f80u : 0x7c00u;
-      for (int i = lane; i < BN * CH; i += 64) {
-        const u4_t w = lv[i];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) odd |= (w[y] & e) == e || ((w[y] >> 16) & e) == e;
-      }
-    }
-    if (!__any(odd)) {
+    if (!mask || !odd) {
       products(lv, p);
       return;
     }
@@ -345,17 +349,33 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   }
   for (; i < count; ++i, ready = false) {
     u4_t *lk = i & 1 ? lk1 : lk0, *lv = i & 1 ? lv1 : lv0;
+    bool odd = false;
     if (!ready) {
+      // each wave looks through the part of V that it has loaded itself
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < LOADS; ++c) {
+        const u4_t w = lv[c * THREADS + threadIdx.x];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) top = max_halves(top, w[y] & 0x7fff7fffu);
+      }
+      const uint32_t e = BF ? 0x7f80u : 0x7c00u;
+      const bool mine = __any((top & 0xffffu) >= e || (top >> 16) >= e);
+      if (lane == 0) lodd[i & 1][wave] = mine;
       __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) odd |= lodd[i & 1][w] != 0;
+      odd = __builtin_amdgcn_readfirstlane(odd);
       if (i + 1 < count) fetch(tile_at(i + 1), i & 1 ? lk0 : lk1, i & 1 ? lv0 : lv1);
     }
-    any_tile(tile_at(i), lk, lv);
+    any_tile(tile_at(i), lk, lv, odd);
   }
   {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(y[0]) + __uint_as_float(y[1]);
   }
-  if (!real) return;
+  if (vrow >= rows) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* out = a.out + int64_t(q0 + row) * a.so_n + head * a.so_h + 4 * hi;
 #pragma unroll
@@ -381,15 +401,15 @@ extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, co
   IQ_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, 4) && aligned(cu_k, 4),
            IQ_ERR_ALIGN);
   if (N == 0) return IQ_OK;
-  const int64_t slots = int64_t(N) / BM + S;  // a sequence has at most rows / 128 + 1 tiles
-  IQ_CHECK(slots * Hq <= INT32_MAX, IQ_ERR_SHAPE);
+  const int64_t slots = int64_t(N) * (Hq / H) / BM + S;  // a sequence has at most rows / 128 + 1 tiles
+  IQ_CHECK(slots * H <= INT32_MAX && int64_t(N) * (Hq / H) <= INT32_MAX - BM, IQ_ERR_SHAPE);
   const float c = scale * 1.44269504088896340736f;
   PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
                sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), c == 0 ? 1.f : c < 0 ? -c : c, c == 0 ? 0u : ~0u,
                c < 0 ? 0x80008000u : 0u,
                causal ? 1 : 0, window};
   auto launch = [&]<int D_, bool BF>() {
-    prompt_kernel<D_, BF><<<unsigned(slots * Hq), THREADS, 0, (hipStream_t)stream>>>(a);
+    prompt_kernel<D_, BF><<<unsigned(slots * H), THREADS, 0, (hipStream_t)stream>>>(a);
     return launch_status();
   };
   const bool bf = act_bf16(mode);
