@@ -26,6 +26,7 @@ struct PromptArgs {
   const int32_t *cu_q, *cu_k;
   int S, N, Nk, Hq, nrep, slots;
   float c;              // |scale| log2(e); 1 for a scale of 0
+  float slack;          // 8 / c
   uint32_t keep, sign;  // and-ed, xor-ed into the queries: a scale of 0 clears them, a negative one flips their signs
   int causal, window;
 };
@@ -212,16 +213,21 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
     return fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
   };
-  // Weights are relative to 2^base, base = RN(max c).
+  // Weights are relative to 2^base, base = RN(m c), m a maximum that is replaced when a row's has grown past it by 8 in
+  // the exponent: weights stay below 2^8, and the accumulators are rescaled once or twice in a row's life.
   auto base_of = [&](float x) { return x == NEG_INF ? 0.f : x * a.c; };
-  auto rescale = [&](float mx, float base) {
-    if (__any(mx != m)) {
-      const float f = __builtin_amdgcn_exp2f(m == NEG_INF ? NEG_INF : m * a.c - base);
+  auto rescaled = [&](float mx) {  // base for a tile of maximum mx
+    const bool grown = __any(mx > m + a.slack);
+    mx = grown ? mx : m;
+    const float base = base_of(mx);
+    if (grown) {
+      const float f = __builtin_amdgcn_exp2f(m == NEG_INF ? NEG_INF : base_of(m) - base);
       l *= f;
 #pragma unroll
       for (int b = 0; b < DB; ++b) o[b] *= f;
-      m = mx;
     }
+    m = mx;
+    return base;
   };
   // exponents to weights: their sum into l, rounded and in pairs into p (keys as v_operand's)
   auto weigh = [&](f16_t (&st)[2], u4_t (&p)[4]) {
@@ -246,14 +252,13 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
       for (int b = 0; b < DB; ++b) o[b] = mma32<BF>(v_operand(lv, kc, b), p[kc], o[b]);
   };
 
-  // A tile that every row of the workgroup sees whole.  False (and nothing done) where logits are so large that one fma
+  // A tile that every row of the workgroup sees whole.  False (the tile is not done) where logits are so large that one fma
   // per logit, whose weights share a factor of 2^(the error of base), will not do.
   auto whole_tile = [&](const u4_t* lk, const u4_t* lv) {
     f16_t st[2];
     scores(lk, st);
-    const float mx = maximum(st), base = base_of(mx);
+    const float base = rescaled(maximum(st));
     if (__any(fabsf(base) > 65536.f)) return false;
-    rescale(mx, base);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -288,8 +293,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
           for (int i = 0; i < 16; ++i) st[kb][i] = 32 * kb + 8 * (i / 4) + i % 4 < f ? NEG_INF : st[kb][i];
       }
     }
-    const float mx = maximum(st), base = base_of(mx);
-    rescale(mx, base);
+    const float base = rescaled(maximum(st));
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -405,7 +409,7 @@ extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, co
   IQ_CHECK(slots * H <= INT32_MAX && int64_t(N) * (Hq / H) <= INT32_MAX - BM, IQ_ERR_SHAPE);
   const float c = scale * 1.44269504088896340736f;
   PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
-               sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), c == 0 ? 1.f : c < 0 ? -c : c, c == 0 ? 0u : ~0u,
+               sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), c == 0 ? 1.f : c < 0 ? -c : c, c == 0 ? 8.f : 8.f / (c < 0 ? -c : c), c == 0 ? 0u : ~0u,
                c < 0 ? 0x80008000u : 0u,
                causal ? 1 : 0, window};
   auto launch = [&]<int D_, bool BF>() {
