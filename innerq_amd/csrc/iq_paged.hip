@@ -9,6 +9,7 @@
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int BATCH = 4;  // heads whose loads are under way together
 
 struct AppendArgs {
   iq_paged p;
@@ -24,8 +25,7 @@ struct AppendArgs {
 };
 
 template <bool BF>
-__device__ __forceinline__ void load8(const uint16_t* x, float (&f)[8]) {
-  const u4_t w = *reinterpret_cast<const u4_t*>(x);
+__device__ __forceinline__ void unpack8(u4_t w, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     f[2 * i] = lo16(w[i], BF);
@@ -43,6 +43,12 @@ __device__ __forceinline__ float quad_max(float x) {
   return __builtin_elementwise_maximum(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, true)));
 }
 
+// 8 floats rounded to the activation dtype, in pairs (a conversion instruction per pair)
+template <bool BF>
+__device__ __forceinline__ u4_t pack8(const float (&f)[8]) {
+  return u4_t{pack2<BF>(f[0], f[1]), pack2<BF>(f[2], f[3]), pack2<BF>(f[4], f[5]), pack2<BF>(f[6], f[7])};
+}
+
 // the 4-bit word of 8 values and its group's meta word (quant.py's asymmetric form, every op rounded to the type)
 template <bool BF>
 __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& meta) {
@@ -55,11 +61,17 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& met
   const GroupQ g = group_params<4, IQ_MODE_ASYM, BF>(quad_min(mn), quad_max(mx), 0.f);
   uint32_t w = 0;
   if (!g.slow) {
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = round_act(__fmul_rn(round_act(x[i] - g.z, BF), g.r), BF);
-      w |= uint32_t(__float2int_rn(fminf(y, 15.f))) << (4 * i);
-    }
+    for (int i = 0; i < 8; ++i) y[i] = x[i] - g.z;
+    unpack8<BF>(pack8<BF>(y), y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(y[i], g.r);
+    unpack8<BF>(pack8<BF>(y), y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // the code is in the low bits of clamp_rne's pattern
+      w += __float_as_uint(clamp_rne<4>(y[i], false)) << (4 * i);
+    w -= shifted_sum(RNE_BITS, 8, 4);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w |= asym_field_b(asym_code_b(x[i], g.z, g.s, 4, BF), 4) << (4 * i);
@@ -68,15 +80,14 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], uint32_t& met
   return w;
 }
 
-// rotation of the 8 values f (dims 8o ..) with their partners p: fp32 products, each rounded, as separate torch ops
-template <bool BF>
-__device__ __forceinline__ void rotate8(float (&f)[8], const float (&p)[8], const float (&c)[8], const float (&s)[8],
-                                        bool second) {
+// rotation of the 8 values f (dims 8o ..) with their partners p (s negated in the first half): fp32 products, each
+// rounded, as separate torch ops
+__device__ __forceinline__ void rotate8(float (&f)[8], const float (&p)[8], const float (&c)[8], const float (&s)[8]) {
 #pragma clang fp contract(off)
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float a = f[i] * c[i], b = p[i] * s[i];
-    f[i] = round_act(second ? a + b : a - b, BF);
+    f[i] = a + b;
   }
 }
 
@@ -108,44 +119,53 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a, int heads
     for (int j = 0; j < 2; ++j) {
       const f4_t x = *reinterpret_cast<const f4_t*>(a.cos + d + 4 * j), y = *reinterpret_cast<const f4_t*>(a.sin + d + 4 * j);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { c[4 * j + e] = x[e]; sn[4 * j + e] = y[e]; }
+      for (int e = 0; e < 4; ++e) { c[4 * j + e] = x[e]; sn[4 * j + e] = second ? y[e] : -y[e]; }
     }
   }
-  const int partner = (second ? -a.R : a.R) / 2;
-  const int h1 = min(heads, int(blockIdx.y + 1) * heads_per_block);
-  for (int h = blockIdx.y * heads_per_block; h < h1; ++h) {
-    const bool isv = h >= H && h < 2 * H, isq = h >= 2 * H;
-    const int hh = isq ? h - 2 * H : isv ? h - H : h;
-    const uint16_t* x = isq ? a.q + n * a.sq_n + hh * a.sq_h : isv ? a.v + n * a.sv_n + hh * a.sv_h
-                                                                   : a.k + n * a.sk_n + hh * a.sk_h;
-    x += 8 * o;
-    float f[8];
-    load8<BF>(x, f);
-    if (turn && !isv) {
-      float p[8];
-      load8<BF>(x + partner, p);
-      rotate8<BF>(f, p, c, sn, second);
-    }
-    if (isq) {
-      u4_t w;
+  const int partner = (second ? -a.R : a.R) / 2, h1 = min(heads, int(blockIdx.y + 1) * heads_per_block);
+  for (int h0 = blockIdx.y * heads_per_block; h0 < h1; h0 += BATCH) {
+    u4_t own[BATCH], other[BATCH];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack2<BF>(f[2 * j], f[2 * j + 1]);
-      *reinterpret_cast<u4_t*>(a.qo + n * a.so_n + hh * a.so_h + 8 * o) = w;
-      continue;
+    for (int i = 0; i < BATCH; ++i) {  // (past the block's last head: that one again)
+      const int h = min(h0 + i, h1 - 1);
+      const uint16_t* x = h < H ? a.k + n * a.sk_n + h * a.sk_h : h < 2 * H ? a.v + n * a.sv_n + (h - H) * a.sv_h
+                                                                           : a.q + n * a.sq_n + (h - 2 * H) * a.sq_h;
+      own[i] = *reinterpret_cast<const u4_t*>(x + 8 * o);
+      other[i] = turn ? *reinterpret_cast<const u4_t*>(x + 8 * o + partner) : u4_t{0, 0, 0, 0};
     }
-    uint32_t meta;
-    const uint32_t w = quantize8<BF>(f, meta);
-    uint32_t* pg = a.p.pages + (int64_t(page) * H + hh) * page_words(D);
-    if (!isv) {
-      pg[row * U + o] = w;
-      if (o % 4 == 0) pg[page_km(D) + row * (D / 32) + o / 4] = meta;
-    } else {
-      const int b = v_block(row), e = v_place(row);
-      pg[page_vc(D) + (b * U + o) * 8 + e] = w;
-      if (o % 4 == 0) {
-        uint16_t* m = reinterpret_cast<uint16_t*>(pg + page_vm(D)) + (b * (D / 32) + o / 4) * 16 + e;
-        m[0] = uint16_t(meta);
-        m[8] = uint16_t(meta >> 16);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i;
+      if (h >= h1) break;
+      const bool isv = h >= H && h < 2 * H;
+      float f[8];
+      u4_t x = own[i];
+      if (turn && !isv) {
+        float p[8];
+        unpack8<BF>(x, f);
+        unpack8<BF>(other[i], p);
+        rotate8(f, p, c, sn);
+        x = pack8<BF>(f);
+      }
+      if (h >= 2 * H) {
+        *reinterpret_cast<u4_t*>(a.qo + n * a.so_n + (h - 2 * H) * a.so_h + 8 * o) = x;
+        continue;
+      }
+      unpack8<BF>(x, f);
+      uint32_t meta;
+      const uint32_t w = quantize8<BF>(f, meta);
+      uint32_t* pg = a.p.pages + (int64_t(page) * H + (isv ? h - H : h)) * page_words(D);
+      if (!isv) {
+        pg[row * U + o] = w;
+        if (o % 4 == 0) pg[page_km(D) + row * (D / 32) + o / 4] = meta;
+      } else {
+        const int b = v_block(row), e = v_place(row);
+        pg[page_vc(D) + (b * U + o) * 8 + e] = w;
+        if (o % 4 == 0) {
+          uint16_t* m = reinterpret_cast<uint16_t*>(pg + page_vm(D)) + (b * (D / 32) + o / 4) * 16 + e;
+          m[0] = uint16_t(meta);
+          m[8] = uint16_t(meta >> 16);
+        }
       }
     }
   }
@@ -159,47 +179,59 @@ struct ReadArgs {
   int64_t sk_n, sk_h, sv_n, sv_h;
 };
 
-// a lane: 8 values of one token of one head of K or V
+// a lane: 8 values of one token, for each of the block's heads of K and V
 template <int D, bool BF>
-__global__ __launch_bounds__(THREADS) void read_kernel(ReadArgs a) {
+__global__ __launch_bounds__(THREADS) void read_kernel(ReadArgs a, int heads_per_block) {
   constexpr int U = D / 8, TOK = THREADS / U;
   const int o = threadIdx.x % U, n = blockIdx.x * TOK + threadIdx.x / U;
   int s, i;
   if (n >= a.N || !sequence_of(a.cu, a.p.S, n, s, i)) return;
   const int held = a.p.lens[s];
   const int64_t at = int64_t(held) + i;
-  const int H = a.p.H, hh = blockIdx.y % H;
-  const bool isv = int(blockIdx.y) >= H;
-  int32_t bad = 0, page = -1;
+  const int H = a.p.H;
+  int32_t bad = 0, page = 0;
   if (held < 0 || at >= int64_t(a.p.P) * PAGE) bad = PAGED_BAD_TOKEN;
   else {
     page = a.p.table[s * a.p.s_table + at / PAGE];
     if (page < 0 || page >= a.p.n_pages) bad = PAGED_BAD_PAGE;
   }
-  uint16_t* out = (isv ? a.v + n * a.sv_n + hh * a.sv_h : a.k + n * a.sk_n + hh * a.sk_h) + 8 * o;
-  u4_t r;
-  if (bad) {  // no such token: NaN
-    if (o == 0 && blockIdx.y == 0) atomicOr(a.p.status, bad);
-    r = u4_t{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
-  } else {
-    const int row = int(at % PAGE);
-    const uint32_t* pg = a.p.pages + (int64_t(page) * H + hh) * page_words(D);
-    uint32_t w, meta;
-    if (!isv) {
-      w = pg[row * U + o];
-      meta = pg[page_km(D) + row * (D / 32) + o / 4];
-    } else {
-      const int b = v_block(row), e = v_place(row);
-      w = pg[page_vc(D) + (b * U + o) * 8 + e];
-      const uint16_t* m = reinterpret_cast<const uint16_t*>(pg + page_vm(D)) + (b * (D / 32) + o / 4) * 16 + e;
-      meta = uint32_t(m[0]) | uint32_t(m[8]) << 16;
+  if (bad && o == 0 && blockIdx.y == 0) atomicOr(a.p.status, bad);
+  const int row = int(at % PAGE), b = v_block(row), e = v_place(row);
+  const int h1 = min(2 * H, int(blockIdx.y + 1) * heads_per_block);
+  for (int h0 = blockIdx.y * heads_per_block; h0 < h1; h0 += BATCH) {
+    uint32_t w[BATCH], s16[BATCH], z16[BATCH];
+    if (!bad) {
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {  // (past the block's last head: that one again)
+        const int h = min(h0 + i, h1 - 1);
+        const bool isv = h >= H;
+        const uint32_t* pg = a.p.pages + (int64_t(page) * H + (isv ? h - H : h)) * page_words(D);
+        const uint16_t* m = reinterpret_cast<const uint16_t*>(pg);
+        w[i] = pg[isv ? page_vc(D) + (b * U + o) * 8 + e : row * U + o];
+        const int at16 = isv ? 2 * page_vm(D) + (b * (D / 32) + o / 4) * 16 + e : 2 * (page_km(D) + row * (D / 32) + o / 4);
+        s16[i] = m[at16];
+        z16[i] = m[at16 + (isv ? 8 : 1)];
+      }
     }
-    const u4_t x = k_values<BF>(w, meta);  // pairs (0,4) (1,5) (2,6) (3,7) -> (0,1) (2,3) (4,5) (6,7)
-    r = u4_t{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
-             __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i;
+      if (h >= h1) break;
+      u4_t r = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // no such token: NaN
+      if (!bad) {
+        const u4_t x = k_values<BF>(w[i], s16[i] | z16[i] << 16);  // pairs (0,4) (1,5) (2,6) (3,7) -> (0,1) (2,3) (4,5) (6,7)
+        r = u4_t{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
+                 __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+      }
+      uint16_t* out = h >= H ? a.v + n * a.sv_n + (h - H) * a.sv_h : a.k + n * a.sk_n + h * a.sk_h;
+      *reinterpret_cast<u4_t*>(out + 8 * o) = r;
+    }
   }
-  *reinterpret_cast<u4_t*>(out) = r;
 }
+
+// Heads that a block does for its tokens: 8 where the tokens alone fill the card (the look-up of a token, three or more
+// loads that wait for each other, then serves 8 heads), one where there are few.
+inline int heads_per_block(int tiles) { return tiles >= 256 ? 8 : 1; }
 
 inline bool rows_ok(const void* p, int64_t s_n, int64_t s_h) { return aligned(p, 16) && s_n % 8 == 0 && s_h % 8 == 0; }
 
@@ -245,7 +277,7 @@ extern "C" int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, cons
                      sq_n, sq_h, (uint16_t*)q_out, so_n, so_h, cos, sin, n_pos, R};
   return by_format(p->D, p->mode, [&]<int D, bool BF>() {
     const int tiles = int(ceil_div(N, THREADS / (D / 8))), heads = 2 * p->H + (q ? Hq : 0);
-    const int hpb = tiles >= 256 ? 8 : 1;
+    const int hpb = heads_per_block(tiles);
     append_kernel<D, BF><<<dim3(tiles, unsigned(ceil_div(heads, hpb))), THREADS, 0, (hipStream_t)stream>>>(a, hpb);
     return launch_status();
   });
@@ -260,8 +292,8 @@ extern "C" int iq_paged_read(const iq_paged* p, const int32_t* cu, int N, void* 
   if (N == 0) return IQ_OK;
   const ReadArgs a{*p, cu, N, (uint16_t*)k_out, (uint16_t*)v_out, sk_n, sk_h, sv_n, sv_h};
   return by_format(p->D, p->mode, [&]<int D, bool BF>() {
-    const unsigned tiles = unsigned(ceil_div(N, THREADS / (D / 8)));
-    read_kernel<D, BF><<<dim3(tiles, 2u * p->H), THREADS, 0, (hipStream_t)stream>>>(a);
+    const int tiles = int(ceil_div(N, THREADS / (D / 8))), hpb = heads_per_block(tiles);
+    read_kernel<D, BF><<<dim3(tiles, unsigned(ceil_div(2 * p->H, hpb))), THREADS, 0, (hipStream_t)stream>>>(a, hpb);
     return launch_status();
   });
 }
