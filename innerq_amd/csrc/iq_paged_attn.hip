@@ -636,6 +636,7 @@ extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s
   const size_t need = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
   IQ_CHECK(!need || (workspace && workspace_bytes >= need), IQ_ERR_WORKSPACE);
   IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
+  if (window >= p->P * PAGE) window = 0;  // hides nothing
   const AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, m, nrep, pl.tiles,
                    scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, pl.split};
   auto launch = [&]<int D, bool BF>() {

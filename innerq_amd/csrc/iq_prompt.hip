@@ -138,20 +138,18 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   const uint16_t *kp = a.k + int64_t(k0) * a.sk_n + kvh * a.sk_h, *vp = a.v + int64_t(k0) * a.sv_n + kvh * a.sv_h;
   const int sk = int(a.sk_n) * 2, sv = int(a.sv_n) * 2, fr = threadIdx.x / CH, fc = (chunk_at<D>(fr, threadIdx.x % CH) % CH) * 16;
   const int vk = fr * sk + fc, vv = fr * sv + fc;
-  auto fetch = [&](int t, u4_t* lk, u4_t* lv) {
+  auto fetch1 = [&](const uint16_t* p, int64_t stride, int bytes, int at, int t, u4_t* lds) {
     const int rows = min(j_end - t * BN, BN);
-    const rsrc_t dk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kp + int64_t(t) * BN * a.sk_n), 0,
-                                                        (rows - 1) * sk + D * 2, 0x00020000);
-    const rsrc_t dv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vp + int64_t(t) * BN * a.sv_n), 0,
-                                                        (rows - 1) * sv + D * 2, 0x00020000);
+    const rsrc_t d = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p + int64_t(t) * BN * stride), 0,
+                                                       (rows - 1) * bytes + D * 2, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      constexpr int ROWS = THREADS / CH;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(dk, (__attribute__((address_space(3))) void*)(lk + i * THREADS + wave * 64), 16,
-                                               vk, i * ROWS * sk, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(dv, (__attribute__((address_space(3))) void*)(lv + i * THREADS + wave * 64), 16,
-                                               vv, i * ROWS * sv, 0, 0);
-    }
+    for (int i = 0; i < LOADS; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)(lds + i * THREADS + wave * 64), 16,
+                                               at, i * (THREADS / CH) * bytes, 0, 0);
+  };
+  auto fetch = [&](int t, u4_t* lk, u4_t* lv) {
+    fetch1(kp, a.sk_n, sk, vk, t, lk);
+    fetch1(vp, a.sv_n, sv, vv, t, lv);
   };
   // this lane's operands in a tile, in bytes; blocks of 32 keys (K), of 16 (V) are at fixed distances from them
   int ka[KS], va[DB][2];
@@ -252,24 +250,24 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
       for (int b = 0; b < DB; ++b) o[b] = mma32<BF>(v_operand(lv, kc, b), p[kc], o[b]);
   };
 
-  // A tile that every row of the workgroup sees whole.  False (the tile is not done) where logits are so large that one fma
-  // per logit, whose weights share a factor of 2^(the error of base), will not do.
-  auto whole_tile = [&](const u4_t* lk, const u4_t* lv) {
-    f16_t st[2];
-    scores(lk, st);
+  // logits to weights.  One fma per logit leaves all weights of a row a common factor of 2^(the error of base), which the
+  // sum shares; where base is so large that this shows in a rounded weight, logits are rounded as base is.
+  auto softmax = [&](f16_t (&st)[2], u4_t (&p)[4]) {
     const float base = rescaled(maximum(st));
-    if (__any(fabsf(base) > 65536.f)) return false;
+    float c = a.c;
+    if (__any(fabsf(base) > 65536.f)) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) st[kb] *= a.c;
+      c = 1.f;
+    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) st[kb][i] = __builtin_fmaf(st[kb][i], a.c, -base);
-    u4_t p[4];
+      for (int i = 0; i < 16; ++i) st[kb][i] = __builtin_fmaf(st[kb][i], c, -base);
     weigh(st, p);
-    products(lv, p);
-    return true;
   };
 
-  // Any tile: logits times c rounded as base is; keys that a row does not see have weight 0.
+  // Any tile: keys that a row does not see have weight 0.
   // odd: V holds an infinity or NaN, which 0 * inf would carry into rows that do not see its key.
   auto any_tile = [&](int t, const u4_t* lk, const u4_t* lv, bool odd) {
     const int j0 = t * BN;
@@ -293,13 +291,8 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
           for (int i = 0; i < 16; ++i) st[kb][i] = 32 * kb + 8 * (i / 4) + i % 4 < f ? NEG_INF : st[kb][i];
       }
     }
-    const float base = rescaled(maximum(st));
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st[kb][i] = st[kb][i] * a.c - base;
     u4_t p[4];
-    weigh(st, p);
+    softmax(st, p);
     if (!mask || !odd) {
       products(lv, p);
       return;
@@ -338,41 +331,50 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   if (whole_a >= whole_z || t_begin >= t_end) whole_a = whole_z = t_begin;
   const int nw = whole_z - whole_a, tail = t_end - whole_z, count = t_end - t_begin;
   auto tile_at = [&](int i) { return i < nw ? whole_a + i : i < nw + tail ? whole_z + i - nw : t_begin + i - nw - tail; };
-  bool ready = false;  // tile i is in LDS and waits to be done
   int i = 0;
+  auto whole_tile = [&](const u4_t* lk, const u4_t* lv) {
+    f16_t st[2];
+    u4_t p[4];
+    scores(lk, st);
+    softmax(st, p);
+    products(lv, p);
+  };
+  // This wave's loads to LDS are there.  Every barrier that hands a tile over is behind such a wait: the compiler's own
+  // does not cover them on all paths.
+  auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
   if (count > 0) fetch(tile_at(0), lk0, lv0);
   while (i < nw) {
+    arrived();
     __syncthreads();  // the tile is there, and no wave reads the other buffer any more
     if (i + 1 < count) fetch(tile_at(i + 1), lk1, lv1);
-    if (!whole_tile(lk0, lv0)) { ready = true; break; }
+    whole_tile(lk0, lv0);
     if (++i >= nw) break;
+    arrived();
     __syncthreads();
     if (i + 1 < count) fetch(tile_at(i + 1), lk0, lv0);
-    if (!whole_tile(lk1, lv1)) { ready = true; break; }
+    whole_tile(lk1, lv1);
     ++i;
   }
-  for (; i < count; ++i, ready = false) {
+  for (; i < count; ++i) {
     u4_t *lk = i & 1 ? lk1 : lk0, *lv = i & 1 ? lv1 : lv0;
-    bool odd = false;
-    if (!ready) {
-      // each wave looks through the part of V that it has loaded itself
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      uint32_t top = 0;
+    // each wave looks through the part of V that it has loaded itself for infinities and NaN
+    arrived();
+    uint32_t top = 0;
 #pragma unroll
-      for (int c = 0; c < LOADS; ++c) {
-        const u4_t w = lv[c * THREADS + threadIdx.x];
+    for (int c = 0; c < LOADS; ++c) {
+      const u4_t w = lv[c * THREADS + threadIdx.x];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) top = max_halves(top, w[y] & 0x7fff7fffu);
-      }
-      const uint32_t e = BF ? 0x7f80u : 0x7c00u;
-      const bool mine = __any((top & 0xffffu) >= e || (top >> 16) >= e);
-      if (lane == 0) lodd[i & 1][wave] = mine;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) odd |= lodd[i & 1][w] != 0;
-      odd = __builtin_amdgcn_readfirstlane(odd);
-      if (i + 1 < count) fetch(tile_at(i + 1), i & 1 ? lk0 : lk1, i & 1 ? lv0 : lv1);
+      for (int y = 0; y < 4; ++y) top = max_halves(top, w[y] & 0x7fff7fffu);
     }
+    const uint32_t e = BF ? 0x7f80u : 0x7c00u;
+    const bool mine = __any((top & 0xffffu) >= e || (top >> 16) >= e);
+    if (lane == 0) lodd[i & 1][wave] = mine;
+    __syncthreads();
+    bool odd = false;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) odd |= lodd[i & 1][w] != 0;
+    odd = __builtin_amdgcn_readfirstlane(odd);
+    if (i + 1 < count) fetch(tile_at(i + 1), i & 1 ? lk0 : lk1, i & 1 ? lv0 : lv1);
     any_tile(tile_at(i), lk, lv, odd);
   }
   {
@@ -405,8 +407,11 @@ extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, co
   IQ_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, 4) && aligned(cu_k, 4),
            IQ_ERR_ALIGN);
   if (N == 0) return IQ_OK;
-  const int64_t slots = int64_t(N) * (Hq / H) / BM + S;  // a sequence has at most rows / 128 + 1 tiles
-  IQ_CHECK(slots * H <= INT32_MAX && int64_t(N) * (Hq / H) <= INT32_MAX - BM, IQ_ERR_SHAPE);
+  const int64_t rows = int64_t(N) * (Hq / H);
+  IQ_CHECK(rows <= INT32_MAX - BM && int64_t(N) + Nk <= INT32_MAX, IQ_ERR_SHAPE);
+  const int64_t slots = rows / BM + S;  // a sequence has at most rows / BM + 1 tiles
+  IQ_CHECK(slots * H <= INT32_MAX, IQ_ERR_SHAPE);
+  if (window >= Nk) window = 0;  // hides nothing
   const float c = scale * 1.44269504088896340736f;
   PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
                sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), c == 0 ? 1.f : c < 0 ? -c : c, c == 0 ? 8.f : 8.f / (c < 0 ? -c : c), c == 0 ? 0u : ~0u,

@@ -234,7 +234,7 @@ def test_attend_drafts_and_windows(dtype, D, m, Hq, window):
     check_attend(st, table, cu, lens, normal(g, len(lens), m, Hq, D, dtype=dtype, outliers=False), D ** -0.5, window)
 
 
-@pytest.mark.parametrize("window", [None, 1, 64, 700])
+@pytest.mark.parametrize("window", [None, 1, 64, 700, 2 ** 31 - 1])
 def test_attend_one_token_windows(window):
     g, rng = torch.Generator().manual_seed(3), random.Random(3)
     lens = [1, 64, 65, 1500, 0, 129]

@@ -85,6 +85,13 @@ def test_long():
         assert bool(((out[i] - want[0]).abs() <= bound[0]).all()), i
 
 
+def test_windows_past_every_length():
+    lq, lk = [70, 3], [20, 90]
+    q, k, v = inputs(6, lq, lk, 2, 1, 64, torch.float16)
+    for window in (90, 110, 2 ** 31 - 1):
+        check(q, k, v, lq, lk, 0.125, True, window)
+
+
 def test_many_sequences():
     rng = random.Random(2)
     lens = [rng.choice([0, 1, 2, 7, 40]) for _ in range(200)]
@@ -194,6 +201,18 @@ def test_another_stream_same_result():
         for _ in range(3):
             assert torch.equal(ops.prompt_attention(q, k, v, i32([0, 900]), 0.09), want)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_are_waited_for(D):
+    """Tiles reach LDS behind the program's back: many runs, each on memory that was just written, give the same bits."""
+    lens = [900, 5, 257, 640]
+    q, k, v = (t.to(DEV) for t in inputs(16, lens, lens, 8, 2, D, torch.float16))
+    cu = i32(starts(lens))
+    want = ops.prompt_attention(q, k, v, cu, 0.09)
+    for _ in range(30):
+        a, b, c = q.clone(), k.clone(), v.clone()
+        assert torch.equal(ops.prompt_attention(a, b, c, cu, 0.09), want)
 
 
 def test_refusals():
