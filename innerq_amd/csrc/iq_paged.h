@@ -67,6 +67,10 @@ __device__ __forceinline__ void pairs4(uint32_t x, h2_t (&c)[4]) {
   c[2] = __builtin_bit_cast(h2_t, (y & 0x000f000fu) | 0x64006400u) - b0;
   c[3] = __builtin_bit_cast(h2_t, (y & 0x00f000f0u) | 0x54005400u) - b1;
 }
+// codes in bytes 0, 1 (HI: 2, 3) of x as floats: a byte 0 .. 15 is, as an OCP e4m3 number, exactly its code times 2^-9
+template <bool HI>
+__device__ __forceinline__ fl2_t codes2(uint32_t x) { return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x, 512.f, HI); }
+
 // the values of one token's word w with meta {s, z}: dwords of the pairs (0,4), (1,5), (2,6), (3,7)
 template <bool BF>
 __device__ __forceinline__ u4_t k_values(uint32_t w, uint32_t meta) {
@@ -80,12 +84,9 @@ __device__ __forceinline__ u4_t k_values(uint32_t w, uint32_t meta) {
   } else {
     const float s = __uint_as_float(meta << 16), z = __uint_as_float(meta & 0xffff0000u);
     const uint32_t e = w & 0x0f0f0f0fu, o = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6 and 1 3 5 7
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t x = i & 1 ? o : e;
-      const int b = i / 2 * 8;
-      r[i] = pack2<true>(__builtin_fmaf(float((x >> b) & 0xffu), s, z), __builtin_fmaf(float((x >> (b + 16)) & 0xffu), s, z));
-    }
+    const fl2_t c02 = codes2<false>(e), c46 = codes2<true>(e), c13 = codes2<false>(o), c57 = codes2<true>(o);
+    auto two = [&](float a, float b) { return pack2<true>(__builtin_fmaf(a, s, z), __builtin_fmaf(b, s, z)); };
+    r = u4_t{two(c02.x, c46.x), two(c13.x, c57.x), two(c02.y, c46.y), two(c13.y, c57.y)};
   }
   return r;
 }

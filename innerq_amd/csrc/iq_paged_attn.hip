@@ -188,13 +188,12 @@ __device__ __forceinline__ void v_operands(const u4_t (&c)[2], u4_t s, u4_t z, u
         const float s0 = lo_half<BF>(sp), s1 = hi_half<BF>(sp);
         const float z0 = lo_half<BF>(zp), z1 = hi_half<BF>(zp);
         const uint32_t e = f & 0x0f0f0f0fu, o = (f >> 4) & 0x0f0f0f0fu;  // dims 0 2 (token 0), 0 2 (token 1); 1 3
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t y = i & 1 ? o : e;
-          const int b = i / 2 * 8;
-          x[half * 4 + i][pr] = pack2<true>(__builtin_fmaf(float((y >> b) & 0xffu), s0, z0),
-                                            __builtin_fmaf(float((y >> (b + 16)) & 0xffu), s1, z1));
-        }
+        const fl2_t e0 = codes2<false>(e), e1 = codes2<true>(e), o0 = codes2<false>(o), o1 = codes2<true>(o);
+        auto two = [&](float a, float b) { return pack2<true>(__builtin_fmaf(a, s0, z0), __builtin_fmaf(b, s1, z1)); };
+        x[half * 4][pr] = two(e0.x, e1.x);
+        x[half * 4 + 1][pr] = two(o0.x, o1.x);
+        x[half * 4 + 2][pr] = two(e0.y, e1.y);
+        x[half * 4 + 3][pr] = two(o0.y, o1.y);
       }
     }
   }
