@@ -429,7 +429,8 @@ int iq_page_bytes(int H, int D, int64_t* bytes);
  *     y[d] = x[d] cos[d] - x[d + R/2] sin[d],  y[d + R/2] = x[d + R/2] cos[d] + x[d] sin[d],  d < R/2,
  * in fp32 with each product rounded, then rounded to the activation dtype.  q [N, Hq, D] (or NULL) is written rotated
  * (unrotated without cos) to q_out, which may be q.  Strides in elements, multiples of 8; D contiguous, 16-byte
- * aligned.  A sequence's rows must not lie in a page that another sequence's rows of this call lie in. */
+ * aligned.  A sequence's rows must not lie in a page that another sequence's rows of this call lie in.
+ * At most 2^27 rows a call. */
 int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, const void* k, int64_t sk_n, int64_t sk_h,
                     const void* v, int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int64_t n_pos, int R,
                     const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* q_out, int64_t so_n, int64_t so_h,
@@ -444,7 +445,8 @@ int iq_paged_read(const iq_paged* p, const int32_t* cu, int N, void* k_out, int6
 /* softmax(q K^T scale) V over the pages for m (1 .. 16) new tokens per sequence: q [S, m, Hq, D], lens[s] the tokens
  * held with the new ones, so token j of the m sees keys below lens[s] - (m - 1 - j), with window > 0 only the last
  * `window` of them.  Logits, softmax statistics and sums in fp32, the weights rounded to the activation dtype for
- * their product with V.  A row that sees no key is 0; a sequence that needs a page outside the pool gives NaN.  Any
+ * their product with V.  A row that sees no key is 0; a sequence that needs a page outside the pool, or holds more
+ * than P * 64 tokens, gives NaN.  Any
  * Hq that H divides.  workspace: iq_paged_attention_workspace_bytes (0: none needed), 16-byte aligned. */
 size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D);
 int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,

@@ -91,6 +91,17 @@ __device__ __forceinline__ u4_t k_values(uint32_t w, uint32_t meta) {
   return r;
 }
 
+// inclusive sum over the wave's 64 lanes (of ints; every lane takes part): within rows of 16, then from row to row
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // ---- sequences -----------------------------------------------------------------------------------------------
 // token n of a flat list belongs to sequence s at place i (cu null: one token each); false: to none
 __device__ __forceinline__ bool sequence_of(const int32_t* cu, int S, int n, int& s, int& i) {

@@ -9,6 +9,7 @@
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int MOST_TOKENS = 1 << 27;  // of a call: a grid has less than 2^32 threads
 constexpr int BATCH = 4;  // heads whose loads are under way together
 
 struct AppendArgs {
@@ -267,7 +268,7 @@ extern "C" int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, cons
                                int64_t so_n, int64_t so_h, void* stream) {
   if (const int st = iq::check_paged(p)) return st;
   IQ_CHECK((N == 0 || (k && v && (!q || q_out))) && (!cos == !sin), IQ_ERR_NULL);
-  IQ_CHECK(N >= 0 && (cu || N == p->S), IQ_ERR_SHAPE);
+  IQ_CHECK(N >= 0 && N <= MOST_TOKENS && (cu || N == p->S), IQ_ERR_SHAPE);
   IQ_CHECK(!q || (Hq > 0 && Hq <= 4096), IQ_ERR_SHAPE);
   IQ_CHECK(!cos || (R > 0 && R <= p->D && R % 16 == 0 && n_pos > 0), IQ_ERR_SHAPE);
   IQ_CHECK(rows_ok(k, sk_n, sk_h) && rows_ok(v, sv_n, sv_h) && aligned(cos, 16) && aligned(sin, 16), IQ_ERR_ALIGN);
@@ -287,7 +288,7 @@ extern "C" int iq_paged_read(const iq_paged* p, const int32_t* cu, int N, void* 
                              void* v_out, int64_t sv_n, int64_t sv_h, void* stream) {
   if (const int st = iq::check_paged(p)) return st;
   IQ_CHECK(N == 0 || (k_out && v_out), IQ_ERR_NULL);
-  IQ_CHECK(N >= 0 && (cu || N == p->S), IQ_ERR_SHAPE);
+  IQ_CHECK(N >= 0 && N <= MOST_TOKENS && (cu || N == p->S), IQ_ERR_SHAPE);
   IQ_CHECK(rows_ok(k_out, sk_n, sk_h) && rows_ok(v_out, sv_n, sv_h), IQ_ERR_ALIGN);
   if (N == 0) return IQ_OK;
   const ReadArgs a{*p, cu, N, (uint16_t*)k_out, (uint16_t*)v_out, sk_n, sk_h, sv_n, sv_h};

@@ -33,6 +33,7 @@ struct AttnArgs {
   int window;          // 0: none
   int grid;
   float* ws;
+  int each;            // sequences per lane where a wave adds up their pages (Part)
   int split;           // 0: a workgroup takes a whole (sequence, head, tile)
 };
 
@@ -43,43 +44,58 @@ __device__ __forceinline__ int pages_of(const AttnArgs& a, int s, int& lo) {
   return len > 0 ? (len + PAGE - 1) / PAGE - lo : 0;
 }
 
-// inclusive scan over the wave's 64 lanes
-__device__ __forceinline__ int wave_scan(int v) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int x = __shfl_up(v, o, 64);
-    if (int(threadIdx.x & 63) >= o) v += x;
-  }
-  return v;
-}
-
-// Where a lane's sequence s0 + lane ends in the list of units (a unit: a page of one head and tile), s0 a multiple of
-// 64 and `base` the units before it; n: the sequence's units.
+// Where a lane's `each` sequences from s0 + each * lane on end in the list of units (a unit: a page of one head and
+// tile), `base` the units before s0; n: the sequences' units.  A lane takes one sequence where there are at most 64,
+// four (their loads under way together) where there are more.
+constexpr int EACH = 4;
 struct Part {
-  int n, end;
+  int n[EACH], end;
 };
 __device__ __forceinline__ Part part_at(const AttnArgs& a, int s0, int base) {
-  int lo;
-  const int s = s0 + int(threadIdx.x & 63), pages = s < a.p.S ? pages_of(a, s, lo) : 0;
-  const int n = pages > 0 ? (pages + PAD) * a.p.H * a.tiles : 0;
-  return {n, base + wave_scan(n)};
+  Part p;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    p.n[i] = 0;
+    if (i >= a.each) continue;
+    int lo;
+    const int s = s0 + int(threadIdx.x & 63) * a.each + i, pages = pages_of(a, min(s, a.p.S - 1), lo);
+    p.n[i] = s < a.p.S && pages > 0 ? (pages + PAD) * a.p.H * a.tiles : 0;
+    sum += p.n[i];
+  }
+  p.end = base + wave_scan(sum);
+  return p;
 }
 __device__ __forceinline__ int total_units(const AttnArgs& a, const Part& first) {
   int end = __builtin_amdgcn_readlane(first.end, 63);
-  for (int s0 = 64; s0 < a.p.S; s0 += 64) end = __builtin_amdgcn_readlane(part_at(a, s0, end).end, 63);
+  for (int s0 = 64 * a.each; s0 < a.p.S; s0 += 64 * a.each) end = __builtin_amdgcn_readlane(part_at(a, s0, end).end, 63);
   return end;
+}
+// of the lane that holds sequence s: its units, and the unit after them
+__device__ __forceinline__ void units_of(const AttnArgs& a, const Part& p, int s, int& n, int& end) {
+  const int l = s / a.each % 64, k = s % a.each;
+  end = __builtin_amdgcn_readlane(p.end, l);
+  n = 0;
+#pragma unroll
+  for (int i = EACH - 1; i >= 0; --i) {
+    const int x = __builtin_amdgcn_readlane(p.n[i], l);
+    if (i > k) end -= x;
+    if (i == k) n = x;
+  }
 }
 // the sequence that holds unit u < total, and its first unit
 __device__ __forceinline__ void find_unit(const AttnArgs& a, Part p, int u, int& s, int& first) {
   for (int s0 = 0;;) {
     const uint64_t past = __ballot(p.end > u);
     if (past) {
-      const int l = __builtin_ctzll(past);
-      s = s0 + l;
-      first = __builtin_amdgcn_readlane(p.end - p.n, l);
-      return;
+      s = s0 + __builtin_ctzll(past) * a.each + a.each - 1;  // the lane's last one that begins at or before u
+      for (int n, end;; --s) {
+        units_of(a, p, s, n, end);
+        first = end - n;
+        if (first <= u && n > 0) return;
+      }
     }
-    s0 += 64;
+    s0 += 64 * a.each;
     if (s0 >= a.p.S) return;
     p = part_at(a, s0, __builtin_amdgcn_readlane(p.end, 63));
   }
@@ -377,6 +393,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
   for (int e = a.split ? blockIdx.x : s; e < (a.split ? a.p.S : s + 1); e += a.grid) {
     int lo;
     if (pages_of(a, e, lo) > 0) continue;
+    if (a.p.lens[e] < 0 && threadIdx.x == 0) atomicOr(a.p.status, PAGED_BAD_TOKEN);
     const float zero[8] = {};
     const int rows = a.m * a.nrep, nh = a.split ? H : 1;
     for (int i = threadIdx.x; i < nh * rows * (D / 8); i += THREADS) {
@@ -425,12 +442,19 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
     const int64_t stride = int64_t(H) * page_words(D);
     // the page of the wave's turn i: one outside the pool is not read and counts as NaN
     bool bad = false;
+    if (a.p.lens[s] > a.p.P * PAGE) {  // more tokens than the table has pages for: NaN too
+      bad = true;
+      if (threadIdx.x == 0) atomicOr(a.p.status, PAGED_BAD_TOKEN);
+    }
     // past its last page a wave loads from a descriptor of no bytes: the loop has no branch that a load depends on,
     // which the wait counts would have to allow for
     auto id_of = [&](int i) { return i < mine ? table[wave + i * WAVES] : 0; };
     auto page_of = [&](int id, bool there) {
       const bool b = id < 0 || id >= a.p.n_pages;
-      bad |= b;
+      if (b && there) {
+        bad = true;
+        if (lane == 0) atomicOr(a.p.status, PAGED_BAD_PAGE);
+      }
       return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(pages + (b ? 0 : id) * stride), 0,
                                                b || !there ? 0 : page_words(D) * 4, 0x00020000);
     };
@@ -468,10 +492,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
       values<D, BF>(vr, w, acc, mask, tok0, lim, low, see0, len);
       load_v<D>(next, at, vr);
     }
-    if (bad) {
-      acc.l = __builtin_nanf("");
-      if (lane == 0) atomicOr(a.p.status, PAGED_BAD_PAGE);
-    }
+    if (bad) acc.l = __builtin_nanf("");
     // the waves' sums
     {
       auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc.l), __float_as_uint(acc.l), false, false);
@@ -531,10 +552,12 @@ __global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
   const int per_seq = a.p.H * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
   Part part = part_at(a, 0, 0);
   const int total = total_units(a, part), per = units_per_group(total, a.grid);
-  for (int s0 = 64; s0 <= s; s0 += 64) part = part_at(a, s0, __builtin_amdgcn_readlane(part.end, 63));
-  const int units = __builtin_amdgcn_readlane(part.n, s & 63), n = units / per_seq;
+  for (int s0 = 64 * a.each; s0 <= s; s0 += 64 * a.each) part = part_at(a, s0, __builtin_amdgcn_readlane(part.end, 63));
+  int units, end;
+  units_of(a, part, s, units, end);
+  const int n = units / per_seq;
   if (n <= 0) return;
-  const int u0 = __builtin_amdgcn_readlane(part.end, s & 63) - units + hr * n, g0 = (u0 + PAD) / per, g1 = (u0 + n - 1) / per;
+  const int u0 = end - units + hr * n, g0 = (u0 + PAD) / per, g1 = (u0 + n - 1) / per;
   if (g0 == g1) return;
   // lanes of D/8 take a row's dims, `parts` of them its slots in runs
   const int tile = hr % a.tiles, rows = min(ROWS, a.m * a.nrep - tile * ROWS), parts = g1 - g0 < 4 ? 1 : ROWS / rows;
@@ -631,13 +654,14 @@ extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s
                so_m % 8 == 0 && so_h % 8 == 0, IQ_ERR_ALIGN);
   const int nrep = Hq / p->H;
   const Launch pl = plan_of(p->S, p->P, m, nrep, p->H);
-  IQ_CHECK(int64_t(p->S) * (p->P + PAD) * p->H * pl.tiles <= INT32_MAX, IQ_ERR_SHAPE);
+  IQ_CHECK(int64_t(p->S) * (p->P + PAD) * p->H * pl.tiles <= INT32_MAX &&
+               int64_t(p->S) * p->H * pl.tiles <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
   const size_t need = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
   IQ_CHECK(!need || (workspace && workspace_bytes >= need), IQ_ERR_WORKSPACE);
   IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   if (window >= p->P * PAGE) window = 0;  // hides nothing
   const AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, m, nrep, pl.tiles,
-                   scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, pl.split};
+                   scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, p->S > 64 ? EACH : 1, pl.split};
   auto launch = [&]<int D, bool BF>() {
     attn_kernel<D, BF><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
     if (const int st = launch_status()) return st;

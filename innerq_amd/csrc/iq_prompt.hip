@@ -75,34 +75,43 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   const int total = gridDim.x, x = blockIdx.x % 8, base = total / 8, rest = total % 8;
   const int item = x * base + min(x, rest) + blockIdx.x / 8, slot = item % a.slots, kvh = item / a.slots;
 
-  // the slot's sequence and tile of rows, the last tiles (the longest) first
-  int s = -1, tile = 0, q0 = 0, q1 = 0;
-  {
-    int before = 0;
-    for (int s0 = 0; s0 < a.S; s0 += 64) {
-      int r0 = 0, r1 = 0;
-      if (s0 + lane < a.S) rows_of(a.cu_q, s0 + lane, a.N, r0, r1);
-      const int t = tiles_of(r1 - r0, a.nrep);
-      int end = t;
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) {
-        const int y = __shfl_up(end, o, 64);
-        if (lane >= o) end += y;
-      }
-      end += before;
-      const uint64_t past = __ballot(end > slot);
+  // The slot's sequence and tile of rows, a sequence's last tiles (the longest) first.
+  int s = 0, q0, q1, tile;
+  if (a.S <= 256) {  // the sequences' tiles lie behind one another (128 prompts of 16 tokens: 18 us, with the search 20)
+    uint64_t past;
+    for (int before = 0;; s += 64) {
+      rows_of(a.cu_q, min(s + lane, a.S - 1), a.N, q0, q1);
+      const int end = before + wave_scan(s + lane < a.S ? tiles_of(q1 - q0, a.nrep) : 0);
+      past = __ballot(end > slot);
       if (past) {
         const int l = __builtin_ctzll(past);
-        s = s0 + l;
+        s += l;
+        q0 = __builtin_amdgcn_readlane(q0, l);
+        q1 = __builtin_amdgcn_readlane(q1, l);
         tile = __builtin_amdgcn_readlane(end, l) - 1 - slot;
-        q0 = __builtin_amdgcn_readlane(r0, l);
-        q1 = __builtin_amdgcn_readlane(r1, l);
         break;
       }
+      if (s + 64 >= a.S) return;
       before = __builtin_amdgcn_readlane(end, 63);
     }
+  } else {
+    // Sequence s has the slots from first_slot(s) to first_slot(s + 1), at least as many as it has tiles: found among 64
+    // starts at a time, without a sum over the sequences before it.
+    auto first_slot = [&](int i) { return int(int64_t(min(max(a.cu_q[i], 0), a.N)) * a.nrep / BM) + i; };
+    for (int n = a.S; n > 1;) {  // it is among the n from s on
+      const int step = (n + 63) / 64, i = min(s + lane * step, a.S);
+      const int at = 63 - __builtin_clzll(__ballot(lane * step < n && first_slot(i) <= slot) | 1);
+      n = min(step, n - at * step);
+      s += at * step;
+    }
+    rows_of(a.cu_q, s, a.N, q0, q1);
+    tile = tiles_of(q1 - q0, a.nrep) - 1 - (slot - first_slot(s));
+    if (tile < 0 || tile >= tiles_of(q1 - q0, a.nrep)) return;
   }
-  if (s < 0) return;
+  s = __builtin_amdgcn_readfirstlane(s);  // (uniform, which the compiler does not see: it would loop over lanes at each load)
+  q0 = __builtin_amdgcn_readfirstlane(q0);
+  q1 = __builtin_amdgcn_readfirstlane(q1);
+  tile = __builtin_amdgcn_readfirstlane(tile);
   int k0, k1;
   rows_of(a.cu_k, s, a.Nk, k0, k1);
   k0 = __builtin_amdgcn_readfirstlane(k0);
@@ -409,8 +418,8 @@ extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, co
   if (N == 0) return IQ_OK;
   const int64_t rows = int64_t(N) * (Hq / H);
   IQ_CHECK(rows <= INT32_MAX - BM && int64_t(N) + Nk <= INT32_MAX, IQ_ERR_SHAPE);
-  const int64_t slots = rows / BM + S;  // a sequence has at most rows / BM + 1 tiles
-  IQ_CHECK(slots * H <= INT32_MAX, IQ_ERR_SHAPE);
+  const int64_t slots = rows / BM + S;  // first_slot(S) at most
+  IQ_CHECK(slots * H <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
   if (window >= Nk) window = 0;  // hides nothing
   const float c = scale * 1.44269504088896340736f;
   PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,

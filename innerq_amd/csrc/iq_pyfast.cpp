@@ -513,6 +513,13 @@ const at::Tensor* rows_of(PyObject* o, int64_t dims, at::ScalarType dt, int devi
     if (t->stride(i) % 8) return nullptr;
   return t;
 }
+// rows_of() to be written: no two rows in one place
+const at::Tensor* out_rows_of(PyObject* o, int64_t dims, at::ScalarType dt, int device, int64_t D) {
+  const at::Tensor* t = rows_of(o, dims, dt, device, D);
+  for (int64_t i = 0; t && i + 1 < dims; ++i)
+    if (t->size(i) > 1 && t->stride(i) == 0) return nullptr;
+  return t;
+}
 // a contiguous int32 vector of n values on the device
 const at::Tensor* ints_of(PyObject* o, int64_t n, int device) {
   const at::Tensor* t = tensor_of(o);
@@ -586,7 +593,7 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
     q = rows_of(a[11], 3, dt, dev, p.D);
     if (!q || q->size(0) != k->size(0) || q->size(1) < 1 || q->size(1) > 4096) Py_RETURN_NONE;
     if (a[12] != Py_None) {
-      const at::Tensor* o = rows_of(a[12], 3, dt, dev, p.D);
+      const at::Tensor* o = out_rows_of(a[12], 3, dt, dev, p.D);
       if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
       out = *o;
     }
@@ -663,7 +670,7 @@ PyObject* paged_attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
   at::Tensor out;
   if (a[9] != Py_None) {
-    const at::Tensor* o = rows_of(a[9], nd, dt, dev, p.D);
+    const at::Tensor* o = out_rows_of(a[9], nd, dt, dev, p.D);
     if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
     out = *o;
   }
@@ -713,7 +720,7 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
   at::Tensor out;
   if (a[8] != Py_None) {
-    const at::Tensor* o = rows_of(a[8], 3, dt, dev, D);
+    const at::Tensor* o = out_rows_of(a[8], 3, dt, dev, D);
     if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
     out = *o;
   }

@@ -12,6 +12,7 @@ import ctypes
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import IQ_MODE_ASYM, IQ_MODE_HYBRID, IQ_MODE_SYM, TOKEN_BLOCK, call
@@ -91,6 +92,19 @@ def on_device(device: torch.device):
 def rows_aligned(t: torch.Tensor) -> bool:
     """Whether every row over the last dim is contiguous and starts on a 16-byte boundary (16-bit types)."""
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in t.stride()[:-1])
+
+
+def autograd_follows(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether autograd, backward or forward mode, follows what is computed from any of the tensors."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
+
+
+def writable_rows(t: torch.Tensor) -> bool:
+    """rows_aligned(), and no two rows in one place (an expanded tensor's are)."""
+    return rows_aligned(t) and not any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
 
 
 def check_cu(cu: torch.Tensor, name: str, S: Optional[int], device: torch.device) -> torch.Tensor:
@@ -890,13 +904,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     keys, each row before it one less (a chunk of a prompt behind its earlier keys has more keys than rows); window:
     only the last ``window`` of the keys up to its own.  Rows that see no key are 0; rows outside the sequences are
     not written.  Inference only: tensors that autograd follows are refused."""
-    fast = _native(q)
+    fast = _native(q) if forward_ad._current_level < 0 else None
     if fast is not None:
         r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out)
         if r is not None:
             return r
     require_act(q, "q")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if autograd_follows(q, k, v):
         raise NotImplementedError("prompt_attention has no backward: call it under torch.no_grad()")
     if q.dim() != 3 or k.dim() != 3:
         _shape_error(f"q must be [N, Hq, D] and k [Nk, H, D], got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -926,7 +940,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     else:
         require_device(out, "out", q.dtype)
         check_out(out.shape, (N, Hq, D))
-        if out.device != dev or not rows_aligned(out):
+        if out.device != dev or not writable_rows(out):
             _shape_error("out needs a contiguous head_dim, rows on 16-byte boundaries and q's device")
     with on_device(dev):
         call("iq_prompt_attention", _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),

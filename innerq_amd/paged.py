@@ -26,6 +26,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from ._lib import call
@@ -36,7 +37,7 @@ MAX_NEW = 16  # new tokens per sequence of an attend()
 
 
 def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if ops.autograd_follows(*tensors):
         raise NotImplementedError("paged KV calls have no backward: call them under torch.no_grad()")
 
 
@@ -56,8 +57,8 @@ def _out_rows(t: torch.Tensor, name: str, shape: tuple, dtype, device) -> torch.
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the store on {device}")
     ops.check_out(t.shape, shape, name)
-    if not ops.rows_aligned(t):
-        raise ValueError(f"{name} needs a contiguous head_dim and rows on 16-byte boundaries")
+    if not ops.writable_rows(t):
+        raise ValueError(f"{name} needs a contiguous head_dim and rows of their own on 16-byte boundaries")
     return t
 
 
@@ -147,7 +148,7 @@ class PagedStore:
         token's row (pairs d, d + R/2).  Returns q [N, Hq, D] rotated, written to ``q_out`` (which may be q) or a new
         tensor; None without q.  Rows outside the sequences are neither appended nor written to q_out.  Sequences
         that append must not share the pages they append to."""
-        fast = ops._native(k)
+        fast = ops._native(k) if forward_ad._current_level < 0 else None
         if fast is not None:
             r = fast.paged_append(self.pages, self.D, self.dtype, self.status, table, lens, k, v, cu_seqlens, cos, sin, q,
                                   q_out)
@@ -221,7 +222,7 @@ class PagedStore:
         """softmax(q K^T * scale) V over each sequence's first lens[s] tokens, the new ones among them.  q [S, Hq, D]
         (one new token) or [S, m, Hq, D] (m <= 16: token j sees all but the m - 1 - j after it); window: only the last
         ``window`` tokens up to its own.  Rows that see no token are 0.  Returns a tensor of q's shape."""
-        fast = ops._native(q)
+        fast = ops._native(q) if forward_ad._current_level < 0 else None
         if fast is not None:
             r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out)
             if r is not None:

@@ -261,6 +261,34 @@ def test_attend_many_sequences():
     check_attend(st, table, cu, lens, normal(g, len(lens), 2, 64, outliers=False), 0.125)
 
 
+@pytest.mark.parametrize("S", [257, 700])
+def test_attend_more_sequences_than_one_chunk(S):
+    """Past the 256 sequences that a wave takes at a time; runs of empty ones, one long one near the end."""
+    g, rng = torch.Generator().manual_seed(S), random.Random(S)
+    lens = [rng.choice([0, 0, 0, 1, 3]) for _ in range(S)]
+    lens[0], lens[S - 2] = 70, 1300
+    st, table, cu, _, _ = filled(g, rng, lens, 1, 64, torch.float16, width=21)
+    check_attend(st, table, cu, lens, normal(g, S, 2, 64, outliers=False), 0.125)
+
+
+def test_lengths_past_the_table_are_told():
+    """A length that the table has no pages for, and a negative one: NaN and 0, told by check(); the others right."""
+    g, rng = torch.Generator().manual_seed(20), random.Random(20)
+    for width in (2, 30):  # a workgroup per sequence and head, and shares
+        st, table, cu, _, _ = filled(g, rng, [100, 128, 60], 1, 64, torch.float16, width=width)
+        q = normal(g, 3, 2, 64, outliers=False).to(DEV)
+        want = st.attend(q, table, i32([100, 128, 60]), 0.125)
+        st.check()
+        got = st.attend(q, table, i32([100, width * 64 + 1, 60]), 0.125)
+        assert torch.equal(got[::2], want[::2]) and bool(got[1].isnan().all())
+        with pytest.raises(RuntimeError, match="past"):
+            st.check()
+        got = st.attend(q, table, i32([100, -7, 60]), 0.125)
+        assert torch.equal(got[::2], want[::2]) and bool((got[1] == 0).all())
+        with pytest.raises(RuntimeError, match="negative"):
+            st.check()
+
+
 def test_attend_strides_and_out():
     g, rng = torch.Generator().manual_seed(7), random.Random(7)
     lens = [70, 300]
@@ -492,6 +520,10 @@ def test_refusals():
             st.attend(**{**ok, **kw})
     with torch.no_grad():
         st.attend(q.clone().requires_grad_(), table, lens, 1.0)
+    with pytest.raises(ValueError):  # rows in one place
+        st.attend(q, table, lens, 1.0, out=q[:, :1].expand(2, 4, 64))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        st.attend(torch.autograd.forward_ad.make_dual(q, q), table, lens, 1.0)
     for bad in (torch.zeros(4, 2, 100, dtype=torch.int32, device=DEV), torch.zeros(0, 2, 640, dtype=torch.int32, device=DEV),
                 torch.zeros(4, 2, 1280, dtype=torch.int32, device=DEV)[..., ::2]):
         with pytest.raises(ValueError):

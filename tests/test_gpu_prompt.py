@@ -92,6 +92,15 @@ def test_windows_past_every_length():
         check(q, k, v, lq, lk, 0.125, True, window)
 
 
+@pytest.mark.parametrize("S", [64, 65, 256, 257, 4097, 5000])
+def test_more_sequences_than_one_search_step(S):
+    rng = random.Random(S)
+    lens = [rng.choice([0, 0, 1, 2]) for _ in range(S)]
+    lens[S - 2] = 150
+    q, k, v = inputs(S, lens, lens, 2, 1, 64, torch.float16)
+    check(q, k, v, lens, lens, 0.125)
+
+
 def test_many_sequences():
     rng = random.Random(2)
     lens = [rng.choice([0, 1, 2, 7, 40]) for _ in range(200)]
@@ -231,6 +240,10 @@ def test_refusals():
                     (dict(v=v.clone().requires_grad_()), NotImplementedError)]:
         with pytest.raises(err):
             ops.prompt_attention(**{**ok, **kw})
+    with pytest.raises(ValueError):  # rows in one place
+        ops.prompt_attention(**ok, out=q[:, :1].expand(20, 4, 64))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        ops.prompt_attention(**{**ok, "k": torch.autograd.forward_ad.make_dual(k, k)})
     assert ops.prompt_attention(q[:0], k, v, cu, 1.0, cu_seqlens_k=cu).shape == (0, 4, 64)
     none = ops.prompt_attention(q, k[:0], v[:0], cu, 1.0, cu_seqlens_k=i32([0, 0]))
     assert bool((none == 0).all())
