@@ -76,11 +76,12 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   const int item = x * base + min(x, rest) + blockIdx.x / 8, slot = item % a.slots, kvh = item / a.slots;
 
   // The slot's sequence and tile of rows, a sequence's last tiles (the longest) first.
-  int s = 0, q0, q1, tile;
+  int s = 0, q0, q1, k0, k1, tile;
   if (a.S <= 256) {  // the sequences' tiles lie behind one another (128 prompts of 16 tokens: 18 us, with the search 20)
     uint64_t past;
     for (int before = 0;; s += 64) {
       rows_of(a.cu_q, min(s + lane, a.S - 1), a.N, q0, q1);
+      rows_of(a.cu_k, min(s + lane, a.S - 1), a.Nk, k0, k1);
       const int end = before + wave_scan(s + lane < a.S ? tiles_of(q1 - q0, a.nrep) : 0);
       past = __ballot(end > slot);
       if (past) {
@@ -88,6 +89,8 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
         s += l;
         q0 = __builtin_amdgcn_readlane(q0, l);
         q1 = __builtin_amdgcn_readlane(q1, l);
+        k0 = __builtin_amdgcn_readlane(k0, l);
+        k1 = __builtin_amdgcn_readlane(k1, l);
         tile = __builtin_amdgcn_readlane(end, l) - 1 - slot;
         break;
       }
@@ -105,6 +108,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
       s += at * step;
     }
     rows_of(a.cu_q, s, a.N, q0, q1);
+    rows_of(a.cu_k, s, a.Nk, k0, k1);
     tile = tiles_of(q1 - q0, a.nrep) - 1 - (slot - first_slot(s));
     if (tile < 0 || tile >= tiles_of(q1 - q0, a.nrep)) return;
   }
@@ -112,8 +116,6 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   q0 = __builtin_amdgcn_readfirstlane(q0);
   q1 = __builtin_amdgcn_readfirstlane(q1);
   tile = __builtin_amdgcn_readfirstlane(tile);
-  int k0, k1;
-  rows_of(a.cu_k, s, a.Nk, k0, k1);
   k0 = __builtin_amdgcn_readfirstlane(k0);
   k1 = __builtin_amdgcn_readfirstlane(k1);
   const int lq = q1 - q0, keys = k1 - k0, off = keys - lq, rows = lq * a.nrep;
@@ -131,8 +133,6 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     const uint16_t* p = a.q + int64_t(q0 + row) * a.sq_n + head * a.sq_h + 8 * hi;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[ks] = *reinterpret_cast<const u4_t*>(p + 16 * ks);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) q[ks] = (q[ks] & a.keep) ^ a.sign;
   }
   f16_t o[DB];
 #pragma unroll
@@ -352,6 +352,8 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   // does not cover them on all paths.
   auto arrived = [&] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
   if (count > 0) fetch(tile_at(0), lk0, lv0);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) q[ks] = (q[ks] & a.keep) ^ a.sign;  // (the queries arrive with the first tile)
   while (i < nw) {
     arrived();
     __syncthreads();  // the tile is there, and no wave reads the other buffer any more
@@ -390,15 +392,25 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(y[0]) + __uint_as_float(y[1]);
   }
-  if (vrow >= rows) return;
+  // Rows leave through LDS: 16 lanes write a whole row of 128 dims, where a lane's own dims are 8 bytes here and there.
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* out = a.out + int64_t(q0 + row) * a.so_n + head * a.so_h + 4 * hi;
+  __syncthreads();  // nobody reads tiles any more
+  u4_t* const lo = (wave < 2 ? lk0 : lk1) + (wave & 1) * 32 * CH;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<u2_t*>(out + 32 * b + 8 * i) = u2_t{pack2<BF>(o[b][4 * i] * inv, o[b][4 * i + 1] * inv),
-                                                            pack2<BF>(o[b][4 * i + 2] * inv, o[b][4 * i + 3] * inv)};
+      reinterpret_cast<u2_t*>(lo + chunk_at<D>(n, 4 * b + i))[hi] =
+          u2_t{pack2<BF>(o[b][4 * i] * inv, o[b][4 * i + 1] * inv), pack2<BF>(o[b][4 * i + 2] * inv, o[b][4 * i + 3] * inv)};
+  wave_lds_sync();
+  const int64_t at = int64_t(q0 + row) * a.so_n + head * a.so_h;
+  const int at0 = int(at), at1 = int(at >> 32);
+#pragma unroll
+  for (int j = 0; j < CH / 2; ++j) {
+    const int r = j * (64 / CH) + lane / CH, c = lane % CH;  // row and chunk
+    const int64_t to = int64_t(uint32_t(__shfl(at0, r, 64))) | int64_t(__shfl(at1, r, 64)) << 32;
+    if (tile * BM + wave * 32 + r < rows) *reinterpret_cast<u4_t*>(a.out + to + 8 * c) = lo[chunk_at<D>(r, c)];
+  }
 }
 
 }  // namespace
