@@ -230,9 +230,17 @@ __global__ __launch_bounds__(THREADS) void read_kernel(ReadArgs a, int heads_per
   }
 }
 
-// Heads that a block does for its tokens: 8 where the tokens alone fill the card (the look-up of a token, three or more
-// loads that wait for each other, then serves 8 heads), one where there are few.
-inline int heads_per_block(int tiles) { return tiles >= 256 ? 8 : 1; }
+// Heads that a block does for its tokens: one while there are few blocks; then as many as leave `blocks` blocks, up to
+// `most`, a power of two (finding a token, three or more loads that wait for each other, then serves all of them).
+//   append, 768 blocks, 16 heads at most (8 KV, 32 query heads, D = 128, bf16; us with 1, 2, 4, 8, 16 heads per block):
+//     256 tokens 4.9 5.1 6.1 8.5 13; 1024: 12 9.0 7.3 9.8 15; 2048: 24 17 13 12 17; 32768: 418 257 175 164 149
+//     (2 KV, 8 query heads, 4096 tokens: 12 9.1 7.4 8.6 9.8; 32 and 32, 256 tokens: 7.2 5.7 6.3 8.6 13)
+//   read, 256 blocks, 4 heads: 256 tokens 3.8 3.9 4.1 5.1 6.4; 1024: 5.2 4.7 4.6 5.5 6.8; 32768: 72 43 33 33 33
+inline int heads_per_block(int tiles, int heads, int blocks, int most) {
+  int n = 1;
+  while (2 * n <= most && int64_t(tiles) * heads >= int64_t(blocks) * 2 * n) n *= 2;
+  return n;
+}
 
 inline bool rows_ok(const void* p, int64_t s_n, int64_t s_h) { return aligned(p, 16) && s_n % 8 == 0 && s_h % 8 == 0; }
 
@@ -278,7 +286,7 @@ extern "C" int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, cons
                      sq_n, sq_h, (uint16_t*)q_out, so_n, so_h, cos, sin, n_pos, R};
   return by_format(p->D, p->mode, [&]<int D, bool BF>() {
     const int tiles = int(ceil_div(N, THREADS / (D / 8))), heads = 2 * p->H + (q ? Hq : 0);
-    const int hpb = heads_per_block(tiles);
+    const int hpb = heads_per_block(tiles, heads, 768, 16);
     append_kernel<D, BF><<<dim3(tiles, unsigned(ceil_div(heads, hpb))), THREADS, 0, (hipStream_t)stream>>>(a, hpb);
     return launch_status();
   });
@@ -293,7 +301,7 @@ extern "C" int iq_paged_read(const iq_paged* p, const int32_t* cu, int N, void* 
   if (N == 0) return IQ_OK;
   const ReadArgs a{*p, cu, N, (uint16_t*)k_out, (uint16_t*)v_out, sk_n, sk_h, sv_n, sv_h};
   return by_format(p->D, p->mode, [&]<int D, bool BF>() {
-    const int tiles = int(ceil_div(N, THREADS / (D / 8))), hpb = heads_per_block(tiles);
+    const int tiles = int(ceil_div(N, THREADS / (D / 8))), hpb = heads_per_block(tiles, 2 * p->H, 256, 4);
     read_kernel<D, BF><<<dim3(tiles, unsigned(ceil_div(2 * p->H, hpb))), THREADS, 0, (hipStream_t)stream>>>(a, hpb);
     return launch_status();
   });

@@ -619,15 +619,22 @@ __global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
 
 constexpr int GRID = 512;  // two workgroups per CU
 
-// tiles of (sequence, head) items; whether a workgroup takes a whole one: those of few pages
+// tiles of (sequence, head) items; whether workgroups share out the pages, or each takes a whole item
 struct Launch {
   int tiles, split, grid;
 };
+// Whole items, one launch and no list to go through, while tables are narrow: up to 8 pages per sequence, 16 with 64
+// items, 32 with 256.  us whole / shared out (8 KV heads, D = 128, fp16):
+//   sequences of 500 tokens (P = 8)  1: 8.7 / 10.4;  16: 9.0 / 13.4;  128: 24 / 28
+//   of 1000 (P = 16)                 1: 12.1 / 10.6;  8: 12.3 / 12.4;  32: 13.7 / 20.3;  128: 36 / 40
+//   of 1500 (P = 24)                 8: 15.8 / 14.7;  16: 16.1 / 17.0;  32: 17.6 / 23.9;  128: 46 / 52
+//   of 4032 (P = 63)                64: 61 / 63, but of 50 .. 4096 tokens 48 / 36
 inline Launch plan_of(int S, int P, int m, int nrep, int H) {
   Launch p;
   p.tiles = int(ceil_div(int64_t(m) * nrep, ROWS));
-  p.split = P > 2 * WAVES;
-  p.grid = p.split ? GRID : S * H * p.tiles;
+  const int64_t items = int64_t(S) * H * p.tiles;
+  p.split = P > (items >= 256 ? 32 : items >= 64 ? 16 : 8);
+  p.grid = p.split ? GRID : int(items);
   return p;
 }
 

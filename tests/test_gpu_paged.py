@@ -271,6 +271,46 @@ def test_attend_more_sequences_than_one_chunk(S):
     check_attend(st, table, cu, lens, normal(g, S, 2, 64, outliers=False), 0.125)
 
 
+@pytest.mark.parametrize("S,H,width", [(2, 1, 8), (2, 1, 9), (16, 4, 16), (16, 4, 17), (64, 4, 32), (64, 4, 33), (257, 1, 40),
+                                       (700, 1, 40)])
+def test_attend_table_widths(S, H, width):
+    """Both sides of the widths up to which a workgroup takes a whole sequence and head."""
+    g, rng = torch.Generator().manual_seed(width), random.Random(S)
+    lens = [rng.choice([0, 1, 64, 130]) for _ in range(S)]
+    lens[0], lens[S - 1] = width * 64, 200
+    st, table, cu, _, _ = filled(g, rng, lens, H, 64, torch.float16)
+    assert table.shape[1] == width
+    check_attend(st, table, cu, lens, normal(g, S, 2 * H, 64, outliers=False), 0.125)
+
+
+@pytest.mark.parametrize("H,Hq,D,N", [(8, 32, 128, 2100), (2, 8, 64, 9000), (32, 32, 64, 700)])
+def test_append_and_read_of_many_tokens(H, Hq, D, N):
+    """Enough tokens for blocks of several heads: as a few tokens at a time, which take one head per block."""
+    g, rng = torch.Generator().manual_seed(N), random.Random(N)
+    lens = [N // 2 + 3, 0, N - N // 2 - 3]
+    k, v, q = (normal(g, N, h, D).to(DEV) for h in (H, H, Hq))
+    cos, sin = (x.to(DEV) for x in angles(N, D // 2))
+    pool, table = tables(rng, lens)
+    one, few = (paged.PagedStore(pool, H, D, DEV) for _ in range(2))
+    for st in (one, few):
+        st.pages.zero_()
+    cu = i32([0, lens[0], lens[0], N])
+    turned = one.append(k, v, table, i32([0, 0, 0]), cu, cos, sin, q)
+    parts = torch.empty_like(q)
+    for s, a in ((0, 0), (2, lens[0])):
+        for i in range(0, lens[s], 60):
+            n = min(60, lens[s] - i)
+            row = slice(a + i, a + i + n)
+            few.append(k[row], v[row], table[s:s + 1], i32([i]), i32([0, n]), cos, sin, q[row], parts[row])
+    assert torch.equal(one.pages, few.pages) and torch.equal(turned, parts)
+    kk, vv = one.read(table, i32([0, 0, 0]), cu, N)
+    for i in range(0, lens[2], 61):
+        n = min(61, lens[2] - i)
+        a, b = few.read(table[2:], i32([i]), i32([0, n]), n)
+        assert torch.equal(a, kk[lens[0] + i:lens[0] + i + n]) and torch.equal(b, vv[lens[0] + i:lens[0] + i + n])
+    one.check(), few.check()
+
+
 def test_lengths_past_the_table_are_told():
     """A length that the table has no pages for, and a negative one: NaN and 0, told by check(); the others right."""
     g, rng = torch.Generator().manual_seed(20), random.Random(20)
