@@ -124,9 +124,10 @@ struct VRegs {
 };
 
 // A page is read through a buffer descriptor of its own (one page's bytes; none for a page outside the pool): lane
-// offsets stay in 32 bits and the offsets within a page in the instructions' immediates.  (Non-temporal loads were the
-// slower ones here: 48 sequences of 130 .. 16001 tokens 77.3 us against 75.8 in bf16, 62.7 against 61.1 in fp16.)
+// offsets stay in 32 bits and the offsets within a page in the instructions' immediates.  Each byte is read once:
+// the loads leave the caches to others.
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr int STREAM = 2;  // non-temporal
 
 template <int D>
 struct Lane {
@@ -142,7 +143,7 @@ struct Lane {
   }
 };
 __device__ __forceinline__ u4_t bload4(rsrc_t r, uint32_t off) {
-  return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+  return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, STREAM));
 }
 
 template <int D>
@@ -153,10 +154,10 @@ __device__ __forceinline__ void load_k(rsrc_t pg, const Lane<D>& at, KRegs& r) {
     if constexpr (D == 128) {
       r.c[t] = bload4(pg, c);
     } else {
-      const u2_t x = __builtin_bit_cast(u2_t, __builtin_amdgcn_raw_buffer_load_b64(pg, c, 0, 0));
+      const u2_t x = __builtin_bit_cast(u2_t, __builtin_amdgcn_raw_buffer_load_b64(pg, c, 0, STREAM));
       r.c[t] = u4_t{x.x, x.y, 0, 0};
     }
-    r.m[t] = __builtin_amdgcn_raw_buffer_load_b32(pg, at.km + t * 16 * (D / 32) * 4, 0, 0);
+    r.m[t] = __builtin_amdgcn_raw_buffer_load_b32(pg, at.km + t * 16 * (D / 32) * 4, 0, STREAM);
   }
 }
 template <int D>
