@@ -1,11 +1,17 @@
 // Attention over packed prompts (gfx950): iq_prompt_attention.
 //
 // Sequences of different lengths lie one behind the other; a workgroup takes 128 rows of one KV head of one sequence
-// (query rows times the heads that share the KV head; four waves of 32) and walks over the sequence's keys in tiles of 64, staged through LDS.  Both
-// products run transposed on v_mfma_f32_32x32x16: S^T = K Q^T leaves a query row per lane and its keys in the lane's
-// registers, where the running softmax needs one exchange (with the lane of the other half-wave) per tile, and the
-// exponentials, rounded to the activation dtype, are the B operand of O^T += V^T P^T as they are: V^T's A operand
-// reads LDS with ds_read_b64_tr_b16 in the same order of keys.
+// (query rows times the heads that share the KV head; four waves of 32) and walks over the sequence's keys in tiles of
+// 64, staged through LDS.  Both products run transposed on v_mfma_f32_32x32x16: S^T = K Q^T leaves a query row per lane
+// and its keys in the lane's registers, where the running softmax needs one exchange (with the lane of the other
+// half-wave) per tile, and the exponentials, rounded to the activation dtype, are the B operand of O^T += V^T P^T as
+// they are: V^T's A operand reads LDS with ds_read_b64_tr_b16 in the same order of keys.
+//
+// A tile holds the rows of all heads of a group, so short prompts fill tiles and stage their keys once (32 query heads
+// over 8, a tile per query head before: 128 prompts of 16 tokens 58 us, now 18; one of 77 11.8, now 8.0).
+// Bound: the matrix unit and the softmax's vector work, which two workgroups per CU overlap.  A prompt of 16384 tokens
+// (32 query, 8 KV heads, D = 128, bf16): 1.94 ms, 1130 TFLOP/s, where a 16384^3 bf16 library product reaches 1370; the
+// matrix unit is busy 58 % of the clocks, HBM moves 0.8 GB.  Short prompts wait for their first tile: 77 tokens 7.4 us.
 #include "iq_paged.h"
 
 using namespace iq;
@@ -77,7 +83,8 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
 
   // The slot's sequence and tile of rows, a sequence's last tiles (the longest) first.
   int s = 0, q0, q1, k0, k1, tile;
-  if (a.S <= 256) {  // the sequences' tiles lie behind one another (128 prompts of 16 tokens: 18 us, with the search 20)
+  // (prompts of 16 tokens, us here / with the search below: 64 9.4 / 12.5, 128 17 / 20, 256 32 / 32, 512 65 / 57)
+  if (a.S <= 256) {  // the sequences' tiles lie behind one another
     uint64_t past;
     for (int before = 0;; s += 64) {
       rows_of(a.cu_q, min(s + lane, a.S - 1), a.N, q0, q1);
@@ -143,7 +150,8 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
 
   // Tiles go from memory to LDS without registers, one tile ahead.  LDS is written in lane order, so the spreading of
   // chunk_at is in the source address: a thread's chunk of every pass of THREADS chunks has the same place in its row.
-  // Rows past the last key that the workgroup sees are past the descriptor's bound and read as zeros.
+  // Rows past the last key that the workgroup sees are past the descriptor's bound and read as zeros (the bound counts the
+  // scalar offset too, also where that alone is past it).
   const uint16_t *kp = a.k + int64_t(k0) * a.sk_n + kvh * a.sk_h, *vp = a.v + int64_t(k0) * a.sv_n + kvh * a.sv_h;
   const int sk = int(a.sk_n) * 2, sv = int(a.sv_n) * 2, fr = threadIdx.x / CH, fc = (chunk_at<D>(fr, threadIdx.x % CH) % CH) * 16;
   const int vk = fr * sk + fc, vv = fr * sv + fc;
@@ -433,11 +441,10 @@ extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, co
   const int64_t slots = rows / BM + S;  // first_slot(S) at most
   IQ_CHECK(slots * H <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
   if (window >= Nk) window = 0;  // hides nothing
-  const float c = scale * 1.44269504088896340736f;
+  const float c = scale * 1.44269504088896340736f, abs_c = c == 0 ? 1.f : c < 0 ? -c : c;
   PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
-               sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), c == 0 ? 1.f : c < 0 ? -c : c, c == 0 ? 8.f : 8.f / (c < 0 ? -c : c), c == 0 ? 0u : ~0u,
-               c < 0 ? 0x80008000u : 0u,
-               causal ? 1 : 0, window};
+               sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), abs_c, 8.f / abs_c, c == 0 ? 0u : ~0u,
+               c < 0 ? 0x80008000u : 0u, causal ? 1 : 0, window};
   auto launch = [&]<int D_, bool BF>() {
     prompt_kernel<D_, BF><<<unsigned(slots * H), THREADS, 0, (hipStream_t)stream>>>(a);
     return launch_status();
