@@ -105,7 +105,7 @@ class PagedStore:
 
     def check(self) -> None:
         """Raises RuntimeError if a call since the last check needed a page outside the pool or a token past the
-        table (reads the status word: waits for the device)."""
+        table (reads the status word on the current stream: waits for it, and for calls that it waits for)."""
         bad = int(self.status.item())
         if bad:
             self.status.zero_()
@@ -145,8 +145,8 @@ class PagedStore:
         """Appends k and v [N, H, D]: rows cu_seqlens[s] .. cu_seqlens[s+1] (int32 [S+1]; None: one row per sequence)
         become tokens lens[s], lens[s] + 1, ... of sequence s (lens: tokens held before the call, which it leaves as
         they are).  cos, sin: fp32 [positions, R/2]; the first R dims of each key and query are rotated by their
-        token's row (pairs d, d + R/2).  Returns q [N, Hq, D] rotated, written to ``q_out`` (which may be q) or a new
-        tensor; None without q.  Rows outside the sequences are neither appended nor written to q_out.  Sequences
+        token's row (pairs d, d + R/2).  Returns q [N, Hq, D] rotated, written to ``q_out`` (q itself, or memory that no
+        other argument uses) or a new tensor; None without q.  Rows outside the sequences are neither appended nor written to q_out.  Sequences
         that append must not share the pages they append to."""
         fast = ops._native(k) if forward_ad._current_level < 0 else None
         if fast is not None:
@@ -221,7 +221,8 @@ class PagedStore:
                window: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """softmax(q K^T * scale) V over each sequence's first lens[s] tokens, the new ones among them.  q [S, Hq, D]
         (one new token) or [S, m, Hq, D] (m <= 16: token j sees all but the m - 1 - j after it); window: only the last
-        ``window`` tokens up to its own.  Rows that see no token are 0.  Returns a tensor of q's shape."""
+        ``window`` tokens up to its own.  Rows that see no token are 0.  Returns ``out`` (q itself, or memory that no
+        other argument uses) or a new tensor of q's shape."""
         fast = ops._native(q) if forward_ad._current_level < 0 else None
         if fast is not None:
             r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out)

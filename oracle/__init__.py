@@ -18,6 +18,9 @@ attn_ref    dequantize-then-matmul references for the decode QK^T and attn.V
 cache_ref   restatement of the ``InnerqDynamicLayer`` state machine
             (sinks / recent window / flush / key normalization) over numpy
             arrays, producing the dense K/V that ``update()`` returns.
+serving_ref plain 64-bit definitions of the operators for many sequences: the
+            rotation, a page's codes and values (bit-exact), attention with
+            the error that the kernels' roundings allow.
 timing      the CPU baseline: the reference's torch CPU path
             (dequantize-then-matmul on int32 codes) timed on host cores.
 

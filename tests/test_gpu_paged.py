@@ -271,6 +271,19 @@ def test_attend_more_sequences_than_one_chunk(S):
     check_attend(st, table, cu, lens, normal(g, S, 2, 64, outliers=False), 0.125)
 
 
+@pytest.mark.parametrize("width", [5, 40])
+def test_attend_into_its_queries(width):
+    """Whole items, and items that several workgroups share."""
+    g, rng = torch.Generator().manual_seed(11), random.Random(11)
+    lens = [300, 0, 64 * width, 7]
+    st, table, cu, _, _ = filled(g, rng, lens, 2, 128, torch.bfloat16)
+    for m in (1, 5):
+        q = normal(g, 4, m, 8, 128, dtype=torch.bfloat16, outliers=False).to(DEV)
+        want = st.attend(q, table, i32(lens), 0.09)
+        got = st.attend(q, table, i32(lens), 0.09, out=q)
+        assert got is q and torch.equal(q, want)
+
+
 @pytest.mark.parametrize("S,H,width", [(2, 1, 8), (2, 1, 9), (16, 4, 16), (16, 4, 17), (64, 4, 32), (64, 4, 33), (257, 1, 40),
                                        (700, 1, 40)])
 def test_attend_table_widths(S, H, width):

@@ -224,6 +224,15 @@ def test_tiles_are_waited_for(D):
         assert torch.equal(ops.prompt_attention(a, b, c, cu, 0.09), want)
 
 
+@pytest.mark.parametrize("Hq,H", [(4, 1), (2, 2), (6, 2)])
+def test_into_its_queries(Hq, H):
+    lens = [300, 1, 0, 129]
+    q, k, v = (t.to(DEV) for t in inputs(17, lens, lens, Hq, H, 128, torch.bfloat16))
+    cu = i32(starts(lens))
+    want = ops.prompt_attention(q, k, v, cu, 0.09)
+    assert ops.prompt_attention(q, k, v, cu, 0.09, out=q) is q and torch.equal(q, want)
+
+
 def test_refusals():
     q, k, v = (t.to(DEV) for t in inputs(15, [20], [20], 4, 2, 64, torch.float16))
     cu = i32([0, 20])
