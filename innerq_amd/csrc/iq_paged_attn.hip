@@ -1,6 +1,6 @@
 // Attention of one or a few new tokens per sequence over 4-bit pages (gfx950): iq_paged_attention.
 //
-// Flash decoding over a ragged batch: the pages of all (sequence, KV head, tile of 16 query rows), each with PAD
+// Flash decoding over a ragged batch: the pages of all (sequence, KV head, tile of query rows), each with PAD
 // units before them, lie behind one another in one list, which the workgroups share out evenly (read from the
 // sequences' lengths on the device, so a captured call follows them); a workgroup's four waves take its pages in
 // turn, each with its own running maximum, sum and accumulators, merged over LDS at the end of each (sequence, head).
@@ -22,7 +22,7 @@ using namespace iq;
 
 namespace {
 
-constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 16;
+constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 16;  // rows of an MFMA operand: a tile has T times as many
 // What a (sequence, head, tile) costs beside its pages, in pages: its queries, its first page's latency and the
 // merge of the waves.  Counted where the workgroups share out the list; without it a workgroup whose share was many
 // short sequences came last (48 sequences of 130 .. 16001 tokens, bf16: 181 us against 82).
@@ -35,7 +35,7 @@ struct AttnArgs {
   int64_t sq_s, sq_m, sq_h;
   uint16_t* out;
   int64_t so_s, so_m, so_h;
-  int m, nrep, tiles;  // new tokens per sequence, query heads per KV head, tiles of 16 rows (row = token * nrep + head)
+  int m, nrep, tiles;  // new tokens per sequence, query heads per KV head, tiles of 16 T rows (row = token * nrep + head)
   float scale;         // times log2(e)
   int window;          // 0: none
   int grid;
@@ -117,8 +117,9 @@ struct Row {
   int token, head;
   bool real;
 };
+template <int T>
 __device__ __forceinline__ Row row_of(const AttnArgs& a, int tile, int r) {
-  const int i = tile * ROWS + r, token = i / a.nrep;
+  const int i = tile * (ROWS * T) + r, token = i / a.nrep;
   return {token, i - token * a.nrep, token < a.m};
 }
 
@@ -230,15 +231,21 @@ struct Acc {
   float m, l;
 };
 
-// the logits of a page's 64 tokens: s[t][i] of token 16 t + 4 (lane/16) + i for query row lane % 16
-template <int D, bool BF>
-__device__ __forceinline__ void logits(const KRegs& r, const u4_t (&q)[D / 32], float scale, f4_t (&s)[4]) {
+// the logits of a page's 64 tokens: s[g][t][i] of token 16 t + 4 (lane/16) + i for query row 16 g + lane % 16
+template <int D, bool BF, int T>
+__device__ __forceinline__ void logits(const KRegs& r, const u4_t (&q)[T][D / 32], float scale, f4_t (&s)[T][4]) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    s[t] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) s[t] = mma<BF>(k_values<BF>(r.c[t][j], r.m[t]), q[j], s[t]);
-    s[t] *= scale;
+    for (int g = 0; g < T; ++g) s[g][t] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const u4_t k = k_values<BF>(r.c[t][j], r.m[t]);
+#pragma unroll
+      for (int g = 0; g < T; ++g) s[g][t] = mma<BF>(k, q[g][j], s[g][t]);
+    }
+#pragma unroll
+    for (int g = 0; g < T; ++g) s[g][t] *= scale;
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -289,13 +296,13 @@ __device__ __forceinline__ bool odd_values(uint32_t s, uint32_t z) {
   return odd;
 }
 
-// Readies 32 tokens of a page that not every row sees all of (k0: the first token's number; the row sees [low, lim),
+// Readies 32 tokens of a page that not every row sees all of (k0: the first token's number; a row sees [low, lim),
 // no row sees tokens outside [lo, len)): tokens that no row sees, whose page rows may hold anything, get values 0.
 // A token whose values hold an infinity or NaN is taken by itself, into the rows that see it (the product would carry
 // it into every row, as 0 * inf), and then gets values 0 too.
-template <int D, bool BF>
-__device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t& z, u4_t p, Acc<D, BF>& acc, int k0, int lim,
-                                              int low, int lo, int len) {
+template <int D, bool BF, int T>
+__device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t& z, const u4_t (&p)[T], Acc<D, BF> (&acc)[T],
+                                              int k0, const int (&lim)[T], const int (&low)[T], int lo, int len) {
   const int quarter = (threadIdx.x & 63) >> 4;
   bool odd = false;
 #pragma unroll
@@ -315,24 +322,29 @@ __device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t&
   for (int t = 0; t < 32; ++t) {
     const int qd = t / 8, e = t % 8, k = k0 + e / 4 * 16 + qd * 4 + e % 4;
     const uint32_t half = quarter == qd ? (e & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
-    u4_t st, zt, pt;
+    u4_t st, zt;
     odd = false;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const uint32_t at = w == e / 2 ? half : 0u;
       st[w] = s[w] & at;
       zt[w] = z[w] & at;
-      pt[w] = p[w] & at;
       odd |= odd_values<BF>(st[w], zt[w]);
     }
     if (!__any(odd)) continue;
-    const bool sees = k < lim && k >= low;
     u4_t x[D / 16];
     v_operands<D, BF>(c, st, zt, x);
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      const f4_t y = mma<BF>(x[j], pt, acc.o[j]);
-      if (sees) acc.o[j] = y;
+    for (int g = 0; g < T; ++g) {
+      const bool sees = k < lim[g] && k >= low[g];
+      u4_t pt;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) pt[w] = p[g][w] & (w == e / 2 ? half : 0u);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const f4_t y = mma<BF>(x[j], pt, acc[g].o[j]);
+        if (sees) acc[g].o[j] = y;
+      }
     }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -343,30 +355,35 @@ __device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t&
   }
 }
 
-template <int D, bool BF>
-__device__ __forceinline__ void values(VRegs& r, const f4_t (&s)[4], Acc<D, BF>& acc, bool mask, int tok0, int lim, int low,
-                                       int lo, int len) {
+template <int D, bool BF, int T>
+__device__ __forceinline__ void values(VRegs& r, const f4_t (&s)[T][4], Acc<D, BF> (&acc)[T], bool mask, int tok0,
+                                       const int (&lim)[T], const int (&low)[T], int lo, int len) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const u4_t p = {pack2<BF>(s[2 * h][0], s[2 * h][1]), pack2<BF>(s[2 * h][2], s[2 * h][3]),
-                    pack2<BF>(s[2 * h + 1][0], s[2 * h + 1][1]), pack2<BF>(s[2 * h + 1][2], s[2 * h + 1][3])};
-    if (mask) unseen_values<D, BF>(r.c[h], r.s[h], r.z[h], p, acc, tok0 + h * 32, lim, low, lo, len);
+    u4_t p[T];
+#pragma unroll
+    for (int g = 0; g < T; ++g)
+      p[g] = u4_t{pack2<BF>(s[g][2 * h][0], s[g][2 * h][1]), pack2<BF>(s[g][2 * h][2], s[g][2 * h][3]),
+                  pack2<BF>(s[g][2 * h + 1][0], s[g][2 * h + 1][1]), pack2<BF>(s[g][2 * h + 1][2], s[g][2 * h + 1][3])};
+    if (mask) unseen_values<D, BF, T>(r.c[h], r.s[h], r.z[h], p, acc, tok0 + h * 32, lim, low, lo, len);
     u4_t x[D / 16];
     v_operands<D, BF>(r.c[h], r.s[h], r.z[h], x);
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) acc.o[j] = mma<BF>(x[j], p, acc.o[j]);
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int g = 0; g < T; ++g) acc[g].o[j] = mma<BF>(x[j], p[g], acc[g].o[j]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// a slot of the workspace: 16 rows of D sums, 16 maxima, 16 sums of weights
-template <int D>
-__device__ __forceinline__ float* slot_of(float* ws, int i) { return ws + int64_t(i) * (ROWS * D + 2 * ROWS); }
+// a slot of the workspace: R = 16 T rows of D sums, R maxima, R sums of weights
+template <int D, int R>
+__device__ __forceinline__ float* slot_of(float* ws, int i) { return ws + int64_t(i) * (R * D + 2 * R); }
 
-template <int D, bool BF>
+template <int D, bool BF, int T>
 __device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, int tile, int r, int d, const float (&v)[8],
                                           float inv) {
-  const Row w = row_of(a, tile, r);
+  const Row w = row_of<T>(a, tile, r);
   if (!w.real) return;
   u4_t x;
 #pragma unroll
@@ -374,11 +391,15 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, in
   *reinterpret_cast<u4_t*>(a.out + s * a.so_s + w.token * a.so_m + (int64_t(head) * a.nrep + w.head) * a.so_h + d) = x;
 }
 
-template <int D, bool BF>
-__global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
-  constexpr int J = D / 16;
-  __shared__ float so[WAVES][ROWS][D + 4];
-  __shared__ float sm[WAVES][ROWS], sl[WAVES][ROWS];
+// workgroups per CU (registers: D = 128 with T = 2 would spill 209 of them at two; D = 64 spills 6, 31 in bf16, in
+// paths that are rarely taken, and is faster so: 48 of 1500 tokens, bf16, 26 us against 30)
+constexpr int per_cu(int D, int T) { return T == 1 || D == 64 ? 2 : 1; }
+
+template <int D, bool BF, int T>
+__global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a) {
+  constexpr int J = D / 16, R = ROWS * T;
+  __shared__ float so[WAVES][R][D + 4];
+  __shared__ float sm[WAVES][R], sl[WAVES][R];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15,
             quarter = lane >> 4;
   const int H = a.p.H;
@@ -408,7 +429,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
     for (int i = threadIdx.x; i < nh * rows * (D / 8); i += THREADS) {
       const int d = i % (D / 8) * 8, r = i / (D / 8) % rows;
       const int h = a.split ? i / (D / 8) / rows : blockIdx.x / a.tiles % H;
-      store_row<D, BF>(a, e, h, r / ROWS, r % ROWS, d, zero, 0.f);
+      store_row<D, BF, T>(a, e, h, r / R, r % R, d, zero, 0.f);
     }
   }
   while (u < u1) {
@@ -423,11 +444,15 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
     if (cnt <= 0) continue;
     const int head = hr / a.tiles, tile = hr - head * a.tiles;
     const int len = __builtin_amdgcn_readfirstlane(min(a.p.lens[s], a.p.P * PAGE));
-    const Row row = row_of(a, tile, l);
-    const int lim = len - (a.m - 1 - row.token), low = a.window ? lim - a.window : 0;  // the row sees keys [low, lim)
-    // the query row of this lane, its octets in the order of k_values' pairs
-    u4_t q[D / 32];  // (rows past the last repeat it and are not stored)
-    {
+    // the query rows of this lane (16 g + l), their octets in the order of k_values' pairs
+    u4_t q[T][D / 32];  // (rows past the last repeat it and are not stored)
+    int lim[T], low[T];  // a row sees keys [low, lim)
+    Acc<D, BF> acc[T];
+#pragma unroll
+    for (int g = 0; g < T; ++g) {
+      const Row row = row_of<T>(a, tile, ROWS * g + l);
+      lim[g] = len - (a.m - 1 - row.token);
+      low[g] = a.window ? lim[g] - a.window : 0;
       const int token = min(row.token, a.m - 1), h = row.real ? row.head : a.nrep - 1;
       const uint16_t* x = a.q + s * a.sq_s + token * a.sq_m + (int64_t(head) * a.nrep + h) * a.sq_h + quarter * (D / 4);
       u4_t w[D / 32];
@@ -435,14 +460,14 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
       for (int j = 0; j < D / 32; ++j) w[j] = *reinterpret_cast<const u4_t*>(x + 8 * j);
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
-        q[j] = u4_t{__builtin_amdgcn_perm(w[j][2], w[j][0], 0x05040100u), __builtin_amdgcn_perm(w[j][2], w[j][0], 0x07060302u),
-                    __builtin_amdgcn_perm(w[j][3], w[j][1], 0x05040100u), __builtin_amdgcn_perm(w[j][3], w[j][1], 0x07060302u)};
-    }
-    Acc<D, BF> acc;
 #pragma unroll
-    for (int j = 0; j < J; ++j) acc.o[j] = f4_t{0.f, 0.f, 0.f, 0.f};
-    acc.m = NEG_INF;
-    acc.l = 0.f;
+        for (int e = 0; e < 4; ++e)
+          q[g][j][e] = __builtin_amdgcn_perm(w[j][2 + e / 2], w[j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[g].o[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+      acc[g].m = NEG_INF;
+      acc[g].l = 0.f;
+    }
     // (read as constants, by scalar loads: a vector load here would wait for the pages under way)
     typedef const __attribute__((address_space(4))) int32_t* consts_t;
     const consts_t table = (consts_t)(a.p.table + s * a.p.s_table + lo + p0);
@@ -481,48 +506,52 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
     for (int i = 0; i < mine; ++i) {
       const int tok0 = (lo + p0 + wave + i * WAVES) * PAGE;
       const bool mask = tok0 + PAGE > len - a.m + 1 || (a.window && tok0 < len - a.window);
-      f4_t w[4];
-      logits<D, BF>(kr, q, a.scale, w);
+      f4_t w[T][4];
+      logits<D, BF, T>(kr, q, a.scale, w);
       const rsrc_t next = page_of(id, i + 1 < mine);
       id = id_of(i + 2);
       load_k<D>(next, at, kr);
       if (mask) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int g = 0; g < T; ++g)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = tok0 + t * 16 + quarter * 4 + e;
-            if (k >= lim || k < low) w[t][e] = NEG_INF;
-          }
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int k = tok0 + t * 16 + quarter * 4 + e;
+              if (k >= lim[g] || k < low[g]) w[g][t][e] = NEG_INF;
+            }
       }
       __builtin_amdgcn_sched_barrier(0);
-      weights<D, BF>(w, acc);
+#pragma unroll
+      for (int g = 0; g < T; ++g) weights<D, BF>(w[g], acc[g]);
       __builtin_amdgcn_sched_barrier(0);
-      values<D, BF>(vr, w, acc, mask, tok0, lim, low, see0, len);
+      values<D, BF, T>(vr, w, acc, mask, tok0, lim, low, see0, len);
       load_v<D>(next, at, vr);
     }
-    if (bad) acc.l = __builtin_nanf("");
     // the waves' sums
-    {
-      auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc.l), __float_as_uint(acc.l), false, false);
-      acc.l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-      x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc.l), __float_as_uint(acc.l), false, false);
-      acc.l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-    }
-    if (quarter == 0) {
-      sm[wave][l] = acc.m;
-      sl[wave][l] = acc.l;
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int g = 0; g < T; ++g) {
+      float sum = bad ? __builtin_nanf("") : acc[g].l;
+      auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+      sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+      x = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+      sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+      if (quarter == 0) {
+        sm[wave][ROWS * g + l] = acc[g].m;
+        sl[wave][ROWS * g + l] = sum;
+      }
 #pragma unroll
-      for (int j = 0; j < J; j += 4)
-        *reinterpret_cast<f4_t*>(&so[wave][l][(quarter * 4 + i) * J + j]) =
-            f4_t{acc.o[j][i], acc.o[j + 1][i], acc.o[j + 2][i], acc.o[j + 3][i]};
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < J; j += 4)
+          *reinterpret_cast<f4_t*>(&so[wave][ROWS * g + l][(quarter * 4 + i) * J + j]) =
+              f4_t{acc[g].o[j][i], acc[g].o[j + 1][i], acc[g].o[j + 2][i], acc[g].o[j + 3][i]};
+    }
     __syncthreads();
     const bool whole = cnt == n;
-    float* slot = whole ? nullptr : slot_of<D>(a.ws, 2 * blockIdx.x + (p0 == 0 ? 1 : 0));
-    for (int i = threadIdx.x; i < ROWS * (D / 8); i += THREADS) {
+    float* slot = whole ? nullptr : slot_of<D, R>(a.ws, 2 * blockIdx.x + (p0 == 0 ? 1 : 0));
+    for (int i = threadIdx.x; i < R * (D / 8); i += THREADS) {
       const int rr = i / (D / 8), d = i % (D / 8) * 8;
       float mx = NEG_INF;
 #pragma unroll
@@ -537,13 +566,13 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
           for (int e = 0; e < 8; ++e) v[e] += f * so[w][rr][d + e];
       }
       if (whole) {
-        store_row<D, BF>(a, s, head, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+        store_row<D, BF, T>(a, s, head, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) slot[rr * D + d + e] = v[e];
         if (d == 0) {
-          slot[ROWS * D + rr] = mx;
-          slot[ROWS * D + ROWS + rr] = sum;
+          slot[R * D + rr] = mx;
+          slot[R * D + R + rr] = sum;
         }
       }
     }
@@ -556,8 +585,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_kernel(AttnArgs a) {
 }
 
 // one workgroup per (sequence, head, tile): merges the slots of those that several workgroups computed, in order
-template <int D, bool BF>
-__global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
+template <int D, bool BF, int T>
+__global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a) {
+  constexpr int R = ROWS * T;
   const int per_seq = a.p.H * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
   Part part = part_at(a, 0, 0);
   const int total = total_units(a, part), per = units_per_group(total, a.grid);
@@ -569,7 +599,7 @@ __global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
   const int u0 = end - units + hr * n, g0 = (u0 + PAD) / per, g1 = (u0 + n - 1) / per;
   if (g0 == g1) return;
   // lanes of D/8 take a row's dims, `parts` of them its slots in runs
-  const int tile = hr % a.tiles, rows = min(ROWS, a.m * a.nrep - tile * ROWS), parts = g1 - g0 < 4 ? 1 : ROWS / rows;
+  const int tile = hr % a.tiles, rows = min(R, a.m * a.nrep - tile * R), parts = g1 - g0 < 4 ? 1 : R / rows;
   const int grp = threadIdx.x / (D / 8), part_i = grp / rows, rr = grp - part_i * rows, d = threadIdx.x % (D / 8) * 8;
   const int run = (g1 - g0 + parts) / parts, ga = g0 + part_i * run, gz = part_i < parts ? min(ga + run - 1, g1) : -1;
   constexpr int B = 4;  // slots whose loads are under way together
@@ -580,9 +610,9 @@ __global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < B; ++i) {
       const int gi = min(g + i, gz);
-      const float* p = slot_of<D>(a.ws, 2 * gi + (gi == g0 ? 1 : 0));
-      m[i] = p[ROWS * D + rr];
-      l[i] = p[ROWS * D + ROWS + rr];
+      const float* p = slot_of<D, R>(a.ws, 2 * gi + (gi == g0 ? 1 : 0));
+      m[i] = p[R * D + rr];
+      l[i] = p[R * D + R + rr];
       x[i][0] = *reinterpret_cast<const f4_t*>(p + rr * D + d);
       x[i][1] = *reinterpret_cast<const f4_t*>(p + rr * D + d + 4);
     }
@@ -603,7 +633,7 @@ __global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
         for (int e = 0; e < 8; ++e) v[e] += f * x[i][e / 4][e % 4];
     }
   }
-  __shared__ float sv[ROWS][D], sm[ROWS], sl[ROWS];
+  __shared__ float sv[R][D], sm[R], sl[R];
   if (parts > 1) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) sv[grp][d + e] = v[e];
@@ -624,27 +654,33 @@ __global__ __launch_bounds__(ROWS * (D / 8)) void combine_kernel(AttnArgs a) {
     }
   }
   if (part_i > 0) return;
-  store_row<D, BF>(a, s, hr / a.tiles, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+  store_row<D, BF, T>(a, s, hr / a.tiles, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
 }
 
 constexpr int GRID = 512;  // two workgroups per CU
 
-// tiles of (sequence, head) items; whether workgroups share out the pages, or each takes a whole item
 struct Launch {
-  int tiles, split, grid;
+  int T, tiles, split, grid;  // split: workgroups share out the pages, or each takes a whole (sequence, head, tile)
 };
+// T: a tile of more than 16 rows takes two groups of 16 to each page, which is loaded and converted once for both.  With
+// D = 128 their accumulators leave room for one workgroup per CU, so the batch has to be large enough: 8192 pages of 16
+// rows.  us with one / two groups (8 KV heads, 8 new tokens on 32 query heads, D = 128; fp16, bf16):
+//   8 sequences of 16384 tokens  66 / 52, 79 / 56;  48 of 1500  39 / 42, 56 / 45;  64 of 500  24 / 23, 32 / 25
+//   16 of 1000 (4096 pages)  13 / 17;  16 new tokens, 48 of 1500  78 / 63, 101 / 68
 // Whole items, one launch and no list to go through, while tables are narrow: up to 8 pages per sequence, 16 with 64
 // items, 32 with 256.  us whole / shared out (8 KV heads, D = 128, fp16):
 //   sequences of 500 tokens (P = 8)  1: 8.7 / 10.4;  16: 9.0 / 13.4;  128: 24 / 28
 //   of 1000 (P = 16)                 1: 12.1 / 10.6;  8: 12.3 / 12.4;  32: 13.7 / 20.3;  128: 36 / 40
 //   of 1500 (P = 24)                 8: 15.8 / 14.7;  16: 16.1 / 17.0;  32: 17.6 / 23.9;  128: 46 / 52
 //   of 4032 (P = 63)                64: 61 / 63, but of 50 .. 4096 tokens 48 / 36
-inline Launch plan_of(int S, int P, int m, int nrep, int H) {
+inline Launch plan_of(int S, int P, int m, int nrep, int H, int D) {
+  const int64_t rows = int64_t(m) * nrep, pages = int64_t(S) * H * P * ceil_div(rows, ROWS);
   Launch p;
-  p.tiles = int(ceil_div(int64_t(m) * nrep, ROWS));
+  p.T = rows > ROWS && pages >= 8192 ? 2 : 1;
+  p.tiles = int(ceil_div(rows, ROWS * p.T));
   const int64_t items = int64_t(S) * H * p.tiles;
   p.split = P > (items >= 256 ? 32 : items >= 64 ? 16 : 8);
-  p.grid = p.split ? GRID : int(items);
+  p.grid = p.split ? GRID / 2 * per_cu(D, p.T) : int(items);
   return p;
 }
 
@@ -656,8 +692,8 @@ int check_paged(const iq_paged* p);
 
 extern "C" size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D) {
   if (S <= 0 || P <= 0 || m <= 0 || Hq <= 0 || H <= 0 || Hq % H || !d_ok(D)) return 0;
-  if (!plan_of(S, P, m, Hq / H, H).split) return 0;
-  return size_t(2 * GRID) * (ROWS * D + 2 * ROWS) * sizeof(float);
+  const Launch p = plan_of(S, P, m, Hq / H, H, D);
+  return p.split ? size_t(2 * GRID) * (ROWS * p.T) * (D + 2) * sizeof(float) : 0;
 }
 
 extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
@@ -669,23 +705,26 @@ extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s
   IQ_CHECK(aligned(q, 16) && aligned(out, 16) && sq_s % 8 == 0 && sq_m % 8 == 0 && sq_h % 8 == 0 && so_s % 8 == 0 &&
                so_m % 8 == 0 && so_h % 8 == 0, IQ_ERR_ALIGN);
   const int nrep = Hq / p->H;
-  const Launch pl = plan_of(p->S, p->P, m, nrep, p->H);
+  const Launch pl = plan_of(p->S, p->P, m, nrep, p->H, p->D);
   IQ_CHECK(int64_t(p->S) * (p->P + PAD) * p->H * pl.tiles <= INT32_MAX &&
-               int64_t(p->S) * p->H * pl.tiles <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
+               int64_t(p->S) * p->H * pl.tiles <= UINT32_MAX / 512, IQ_ERR_SHAPE);
   const size_t need = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
   IQ_CHECK(!need || (workspace && workspace_bytes >= need), IQ_ERR_WORKSPACE);
   IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   if (window >= p->P * PAGE) window = 0;  // hides nothing
   const AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, m, nrep, pl.tiles,
                    scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, p->S > 64 ? EACH : 1, pl.split};
-  auto launch = [&]<int D, bool BF>() {
-    attn_kernel<D, BF><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
+  auto launch = [&]<int D, bool BF, int T>() {
+    attn_kernel<D, BF, T><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
     if (const int st = launch_status()) return st;
     if (pl.split)
-      combine_kernel<D, BF><<<p->S * p->H * pl.tiles, ROWS * (D / 8), 0, (hipStream_t)stream>>>(a);
+      combine_kernel<D, BF, T><<<p->S * p->H * pl.tiles, ROWS * T * (D / 8), 0, (hipStream_t)stream>>>(a);
     return launch_status();
   };
+  auto with = [&]<int D, bool BF>() {
+    return pl.T == 2 ? launch.template operator()<D, BF, 2>() : launch.template operator()<D, BF, 1>();
+  };
   const bool bf = act_bf16(p->mode);
-  if (p->D == 128) return bf ? launch.operator()<128, true>() : launch.operator()<128, false>();
-  return bf ? launch.operator()<64, true>() : launch.operator()<64, false>();
+  if (p->D == 128) return bf ? with.operator()<128, true>() : with.operator()<128, false>();
+  return bf ? with.operator()<64, true>() : with.operator()<64, false>();
 }

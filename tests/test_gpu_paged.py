@@ -324,6 +324,64 @@ def test_append_and_read_of_many_tokens(H, Hq, D, N):
     one.check(), few.check()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("m,Hq", [(5, 8), (16, 4), (16, 16), (3, 22), (2, 32)])
+@pytest.mark.parametrize("window", [None, 1, 50, 200])
+def test_attend_rows_of_two_groups(dtype, D, m, Hq, window):
+    """Tables wide enough for tiles of 32 rows: 20, 32, 128, 33 and 32 rows per KV head."""
+    g, rng = torch.Generator().manual_seed(m), random.Random(m)
+    lens = [m, 3, 0, 64 + m - 1, 333, 1, 1600]
+    st, table, cu, _, _ = filled(g, rng, lens, 2, D, dtype, width=300)
+    check_attend(st, table, cu, lens, normal(g, len(lens), m, Hq, D, dtype=dtype, outliers=False), D ** -0.5, window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_rows_of_two_groups_whole(dtype, D):
+    """The same where a workgroup takes a whole sequence and head."""
+    S, H, m = 64, 4, 4
+    g, rng = torch.Generator().manual_seed(D), random.Random(D)
+    lens = [rng.choice([0, 1, 3, 64, 130]) for _ in range(S)]
+    lens[5], lens[S - 1] = 2048, 777
+    st, table, cu, _, _ = filled(g, rng, lens, H, D, dtype)
+    assert table.shape[1] == 32
+    check_attend(st, table, cu, lens, normal(g, S, m, 8 * H, D, dtype=dtype, outliers=False), D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_attend_infinities_in_rows_of_two_groups(dtype, D, bad):
+    """As below, for drafts in both groups of a tile; a bad page and a length past the table are told there too."""
+    g, rng = torch.Generator().manual_seed(18), random.Random(18)
+    lens, m, width = [130, 68, 5], 7, 1400
+    st, table, cu, k, v = filled(g, rng, lens, 1, D, dtype, width=width)
+    v = v.clone()
+    v[127, 0, 5] = bad            # sequence 0: seen by the drafts from 127 on
+    v[130 + 20, 0, 40] = bad      # sequence 1: outside the window of every row
+    v[130 + 66, 0, 3] = bad       # and its sixth draft's token
+    st.append(k.to(DEV), v.to(DEV), table, i32([0] * 3), cu)
+    q = normal(g, 3, m, 4, D, dtype=dtype, outliers=False)
+    kk, vv = held(st, table, cu, lens)
+    for window in (None, 40):
+        out = st.attend(q.to(DEV), table, i32(lens), D ** -0.5, window=window).cpu().double()
+        at = 0
+        for s, n in enumerate(lens):
+            want, bound = R.attention(q[s], kk[at:at + n], vv[at:at + n], D ** -0.5, window=window or 0)
+            at += n
+            fine = want.isfinite()
+            assert torch.equal(fine, out[s].isfinite()), (s, window)
+            assert bool(((out[s] - want).abs() <= bound)[fine].all()), (s, window)
+            assert torch.equal(want.isnan(), out[s].isnan())
+    st.check()
+    table[0, 1] = 12345
+    got = st.attend(q.to(DEV), table, i32([130, width * 64 + 1, 5]), D ** -0.5).cpu()
+    assert bool(got[:2].isnan().all()) and bool(torch.isfinite(got[2]).all())
+    with pytest.raises(RuntimeError, match="outside the pool.*past"):
+        st.check()
+
+
 def test_lengths_past_the_table_are_told():
     """A length that the table has no pages for, and a negative one: NaN and 0, told by check(); the others right."""
     g, rng = torch.Generator().manual_seed(20), random.Random(20)
