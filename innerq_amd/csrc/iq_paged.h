@@ -53,42 +53,40 @@ __device__ __forceinline__ float hi_half(uint32_t w) {
 }
 
 // ---- values of packed codes: RN(c s + z) in the activation dtype ---------------------------------------------
-// fp16: codes become fp16 integers by an exponent pattern or-ed over their bits (1024 + c, or 64 + c for a field at
-// bit 4), the pattern's value is subtracted (exact), and one packed fma rounds c s + z once.  bf16 has no packed
-// arithmetic on gfx950: fp32 (c s is exact there, the sum rounds to 24 bits first, as the reference's fp32
-// dequantization followed by a cast).
+// Codes leave their nibbles for bytes, and a byte 0 .. 15 is, as an OCP e4m3 number, exactly its code times 2^-9: one
+// conversion per two codes.  fp16: one packed fma rounds c s + z once.  bf16 has no packed arithmetic on gfx950: fp32
+// (c s is exact there, the sum rounds to 24 bits first, as the reference's fp32 dequantization followed by a cast).
 
-// the four pairs {code i of a, code i of b}, i = 0..3, of two 16-bit fields a (low half) and b (high half)
-__device__ __forceinline__ void pairs4(uint32_t x, h2_t (&c)[4]) {
-  const h2_t b0 = {_Float16(1024.f), _Float16(1024.f)}, b1 = {_Float16(64.f), _Float16(64.f)};
-  const uint32_t y = x >> 8;
-  c[0] = __builtin_bit_cast(h2_t, (x & 0x000f000fu) | 0x64006400u) - b0;
-  c[1] = __builtin_bit_cast(h2_t, (x & 0x00f000f0u) | 0x54005400u) - b1;
-  c[2] = __builtin_bit_cast(h2_t, (y & 0x000f000fu) | 0x64006400u) - b0;
-  c[3] = __builtin_bit_cast(h2_t, (y & 0x00f000f0u) | 0x54005400u) - b1;
-}
-// codes in bytes 0, 1 (HI: 2, 3) of x as floats: a byte 0 .. 15 is, as an OCP e4m3 number, exactly its code times 2^-9
+// codes in bytes 0, 1 (HI: 2, 3) of x
 template <bool HI>
 __device__ __forceinline__ fl2_t codes2(uint32_t x) { return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x, 512.f, HI); }
+template <bool HI>
+__device__ __forceinline__ h2_t codes2h(uint32_t x) {
+  return __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 512.f, HI));
+}
 
-// the values of one token's word w with meta {s, z}: dwords of the pairs (0,4), (1,5), (2,6), (3,7)
+// the values of four codes in the bytes of x: of the pair in bytes 0, 1 with scales s and zeros z (a pair of halves
+// each), of that in bytes 2, 3
+template <bool BF>
+__device__ __forceinline__ u2_t values4(uint32_t x, uint32_t s, uint32_t z) {
+  if constexpr (!BF) {
+    const h2_t sh = __builtin_bit_cast(h2_t, s), zh = __builtin_bit_cast(h2_t, z);
+    return u2_t{__builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes2h<false>(x), sh, zh)),
+                __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(codes2h<true>(x), sh, zh))};
+  } else {
+    const float s0 = lo_half<BF>(s), s1 = hi_half<BF>(s), z0 = lo_half<BF>(z), z1 = hi_half<BF>(z);
+    const fl2_t a = codes2<false>(x), b = codes2<true>(x);
+    return u2_t{pack2<true>(__builtin_fmaf(a.x, s0, z0), __builtin_fmaf(a.y, s1, z1)),
+                pack2<true>(__builtin_fmaf(b.x, s0, z0), __builtin_fmaf(b.y, s1, z1))};
+  }
+}
+
+// the values of one token's word w with meta {s, z}: dwords of the pairs (0,2), (4,6), (1,3), (5,7)
 template <bool BF>
 __device__ __forceinline__ u4_t k_values(uint32_t w, uint32_t meta) {
-  u4_t r;
-  if constexpr (!BF) {
-    const h2_t m = __builtin_bit_cast(h2_t, meta), s = {m.x, m.x}, z = {m.y, m.y};
-    h2_t c[4];
-    pairs4(w, c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[i], s, z));
-  } else {
-    const float s = __uint_as_float(meta << 16), z = __uint_as_float(meta & 0xffff0000u);
-    const uint32_t e = w & 0x0f0f0f0fu, o = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6 and 1 3 5 7
-    const fl2_t c02 = codes2<false>(e), c46 = codes2<true>(e), c13 = codes2<false>(o), c57 = codes2<true>(o);
-    auto two = [&](float a, float b) { return pack2<true>(__builtin_fmaf(a, s, z), __builtin_fmaf(b, s, z)); };
-    r = u4_t{two(c02.x, c46.x), two(c13.x, c57.x), two(c02.y, c46.y), two(c13.y, c57.y)};
-  }
-  return r;
+  const uint32_t s = __builtin_amdgcn_perm(meta, meta, 0x01000100u), z = __builtin_amdgcn_perm(meta, meta, 0x03020302u);
+  const u2_t e = values4<BF>(w & 0x0f0f0f0fu, s, z), o = values4<BF>((w >> 4) & 0x0f0f0f0fu, s, z);
+  return u4_t{e.x, e.y, o.x, o.y};
 }
 
 // inclusive sum over the wave's 64 lanes (of ints; every lane takes part): within rows of 16, then from row to row

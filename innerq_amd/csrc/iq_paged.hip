@@ -229,9 +229,9 @@ __global__ __launch_bounds__(THREADS) void read_kernel(ReadArgs a, int heads_per
       if (h >= h1) break;
       u4_t r = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // no such token: NaN
       if (!bad) {
-        const u4_t x = k_values<BF>(w[i], s16[i] | z16[i] << 16);  // pairs (0,4) (1,5) (2,6) (3,7) -> (0,1) (2,3) (4,5) (6,7)
-        r = u4_t{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
-                 __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+        const u4_t x = k_values<BF>(w[i], s16[i] | z16[i] << 16);  // pairs (0,2) (4,6) (1,3) (5,7) -> (0,1) (2,3) (4,5) (6,7)
+        r = u4_t{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
+                 __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
       }
       uint16_t* out = h >= H ? a.v + n * a.sv_n + (h - H) * a.sv_h : a.k + n * a.sk_n + h * a.sk_h;
       *reinterpret_cast<u4_t*>(out + 8 * o) = r;

@@ -12,10 +12,10 @@
 // rounded to the activation dtype, are the B operand of V^T P^T as they are (iq_paged.h's V blocks).  The codes go
 // from memory to registers, one page ahead; LDS only merges the waves.
 //
-// Bound (8 KV heads, 32 query heads, D = 128): long sequences in fp16 by HBM (8 of 32768 tokens: 336 MB in 68 us with
-// the merge, 4.9 TB/s, more than the 4.8 TB/s of a large copy); in bf16 by the conversion of the codes on the vector
-// unit (48 of 130 .. 16001 tokens: 79 us, in fp16 62 us); short ones by the loads that wait for each other, lengths,
-// table, page (one sequence of 1000 tokens: 10.6 us, 5 of them the merging launch).
+// Bound (8 KV heads, 32 query heads, D = 128): long sequences in fp16 by HBM and the vector unit alike (8 of 32768
+// tokens: 336 MB in 63 us with the merge, 5.3 TB/s, where a large copy reaches 4.8; a wave spends about 1.3 us on a
+// page); in bf16 by the conversion of the codes (48 of 130 .. 16001 tokens: 78 us, in fp16 60 us); short ones by the
+// loads that wait for each other, lengths, table, page (one sequence of 1000 tokens: 10.4 us, 3.5 the merging launch).
 #include "iq_paged.h"
 
 using namespace iq;
@@ -135,7 +135,7 @@ struct VRegs {
 // A page is read through a buffer descriptor of its own (one page's bytes; none for a page outside the pool): lane
 // offsets stay in 32 bits and the offsets within a page in the instructions' immediates.  Each byte is read once: the
 // loads leave the caches to others (8 sequences of 32768 tokens, caches full of other data before each call: 68 us
-// against 73, 48 of 130 .. 16001 tokens 79 against 84; a small cache called again and again is 2 % slower).
+// against 73 when measured, 48 of 130 .. 16001 tokens 79 against 84; a small cache called again and again is 2 % slower).
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 constexpr int STREAM = 2;  // non-temporal
 
@@ -200,27 +200,15 @@ __device__ __forceinline__ void v_operands(const u4_t (&c)[2], u4_t s, u4_t z, u
     const uint32_t sp = s[pr], zp = z[pr];  // (a bit_cast of a vector's element would take its first one)
 #pragma unroll
     for (int half = 0; half < D / 64; ++half) {
-      uint32_t f;  // 16-bit fields of the two tokens: 4 dims
-      if constexpr (D == 128) f = __builtin_amdgcn_perm(w1, w0, half ? 0x07060302u : 0x05040100u);
-      else f = __builtin_amdgcn_perm(w1, w0, lane & 1 ? 0x07060302u : 0x05040100u);
-      if constexpr (!BF) {
-        h2_t cc[4];
-        pairs4(f, cc);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[half * 4 + i][pr] = __builtin_bit_cast(
-              uint32_t, __builtin_elementwise_fma(cc[i], __builtin_bit_cast(h2_t, sp), __builtin_bit_cast(h2_t, zp)));
-      } else {
-        const float s0 = lo_half<BF>(sp), s1 = hi_half<BF>(sp);
-        const float z0 = lo_half<BF>(zp), z1 = hi_half<BF>(zp);
-        const uint32_t e = f & 0x0f0f0f0fu, o = (f >> 4) & 0x0f0f0f0fu;  // dims 0 2 (token 0), 0 2 (token 1); 1 3
-        const fl2_t e0 = codes2<false>(e), e1 = codes2<true>(e), o0 = codes2<false>(o), o1 = codes2<true>(o);
-        auto two = [&](float a, float b) { return pack2<true>(__builtin_fmaf(a, s0, z0), __builtin_fmaf(b, s1, z1)); };
-        x[half * 4][pr] = two(e0.x, e1.x);
-        x[half * 4 + 1][pr] = two(o0.x, o1.x);
-        x[half * 4 + 2][pr] = two(e0.y, e1.y);
-        x[half * 4 + 3][pr] = two(o0.y, o1.y);
-      }
+      uint32_t f;  // 4 dims of the two tokens, two dims of each token in turn in a byte
+      if constexpr (D == 128) f = __builtin_amdgcn_perm(w1, w0, half ? 0x07030602u : 0x05010400u);
+      else f = __builtin_amdgcn_perm(w1, w0, lane & 1 ? 0x07030602u : 0x05010400u);
+      const u2_t e = values4<BF>(f & 0x0f0f0f0fu, sp, zp), o = values4<BF>((f >> 4) & 0x0f0f0f0fu, sp, zp);
+      const uint32_t e0 = e.x, e1 = e.y, o0 = o.x, o1 = o.y;
+      x[half * 4][pr] = e0;
+      x[half * 4 + 1][pr] = o0;
+      x[half * 4 + 2][pr] = e1;
+      x[half * 4 + 3][pr] = o1;
     }
   }
 }
@@ -462,7 +450,7 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
       for (int j = 0; j < D / 32; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          q[g][j][e] = __builtin_amdgcn_perm(w[j][2 + e / 2], w[j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+          q[g][j][e] = __builtin_amdgcn_perm(w[j][e % 2 * 2 + 1], w[j][e % 2 * 2], e / 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
       for (int j = 0; j < J; ++j) acc[g].o[j] = f4_t{0.f, 0.f, 0.f, 0.f};
       acc[g].m = NEG_INF;
