@@ -11,7 +11,7 @@
 // over 8, a tile per query head before: 128 prompts of 16 tokens 58 us, now 18; one of 77 11.8, now 8.0).
 // Bound: the matrix unit and the softmax's vector work, which two workgroups per CU overlap.  A prompt of 16384 tokens
 // (32 query, 8 KV heads, D = 128, bf16): 1.94 ms, 1130 TFLOP/s, where a 16384^3 bf16 library product reaches 1370; the
-// matrix unit is busy 61 % of the clocks, HBM moves 0.8 GB.  Short prompts wait for their first tile: 77 tokens 7.4 us.
+// matrix unit is busy 60 % of the clocks, HBM moves 0.8 GB.  Short prompts wait for their first tile: 77 tokens 7.4 us.
 #include "iq_paged.h"
 
 using namespace iq;
