@@ -18,7 +18,7 @@
 
 namespace iq {
 
-constexpr int PAGE = 64, PGROUP = 32;
+constexpr int PAGE = 64;
 __host__ __device__ constexpr int page_km(int D) { return PAGE * (D / 8); }                 // K meta's first word
 __host__ __device__ constexpr int page_vc(int D) { return PAGE * (D / 8 + D / 32); }        // V codes'
 __host__ __device__ constexpr int page_vm(int D) { return page_vc(D) + PAGE * (D / 8); }    // V meta's
