@@ -584,9 +584,9 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
       Py_RETURN_NONE;
     n_pos = t->size(0);
     half = t->size(1);
+    if (n_pos < 1 || half < 1 || half > 128) Py_RETURN_NONE;  // (an empty table's pointer is null: no rotation)
     tab[i] = (const float*)t->data_ptr();
   }
-  if (half > 128) Py_RETURN_NONE;
   const at::Tensor* q = nullptr;
   at::Tensor out;
   if (a[11] != Py_None) {
