@@ -400,9 +400,9 @@ int iq_decode_attention_noalloc(const void* q, int64_t sq_b, int64_t sq_h, const
  *
  * table[s * s_table + i] is the page of sequence s's tokens [64 i, 64 i + 64), lens[s] its token count (see each
  * call), both read on the device: a captured call follows their values.  What they hold is checked there, before any
- * access: an entry that names no page of the pool, or a token past P * 64 (or past the rotation's rows, or of a
- * negative length), is not accessed, and the call ORs IQ_PAGED_BAD_* into *status, which nothing here clears.  Two
- * sequences may share pages that no call writes. */
+ * access: an entry that names no page of the pool, or a token past P * 64 or of a negative length, is not accessed, and
+ * the call ORs IQ_PAGED_BAD_* into *status, which nothing here clears; a token past the rotation's rows that has a page
+ * becomes NaN there and is told alike.  Two sequences may share pages that no call writes. */
 enum iq_paged_status {
   IQ_PAGED_BAD_PAGE = 1,  /* a table entry outside [0, n_pages) was needed */
   IQ_PAGED_BAD_TOKEN = 2  /* a token past the table's P * 64 or past the rotation's rows, or a negative length */
@@ -428,9 +428,9 @@ int iq_page_bytes(int H, int D, int64_t* bytes);
  * dims (R <= D, a multiple of 16) are rotated by row lens[s] + i before they are quantized,
  *     y[d] = x[d] cos[d] - x[d + R/2] sin[d],  y[d + R/2] = x[d + R/2] cos[d] + x[d] sin[d],  d < R/2,
  * in fp32 with each product rounded, then rounded to the activation dtype.  q [N, Hq, D] (or NULL) is written rotated
- * (unrotated without cos) to q_out, which may be q.  Strides in elements, multiples of 8; D contiguous, 16-byte
- * aligned.  A sequence's rows must not lie in a page that another sequence's rows of this call lie in.
- * At most 2^27 rows a call. */
+ * (unrotated without cos) to q_out, which may be q; NaN for a token that the checks above refuse.  Strides in elements,
+ * multiples of 8; D contiguous, 16-byte aligned.  A sequence's rows must not lie in a page that another sequence's rows
+ * of this call lie in.  At most 2^27 rows a call. */
 int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, const void* k, int64_t sk_n, int64_t sk_h,
                     const void* v, int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int64_t n_pos, int R,
                     const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* q_out, int64_t so_n, int64_t so_h,

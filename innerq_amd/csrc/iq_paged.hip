@@ -99,6 +99,33 @@ __device__ __forceinline__ void rotate8(float (&f)[8], const float (&p)[8], cons
   }
 }
 
+// A lane's share of token n, which cannot be appended: its queries are NaN, and so is its row of its page, where it has
+// one (a token past the rotation's rows), so that nothing computed from it passes for a result.
+template <int D>
+__device__ __forceinline__ void refuse(const AppendArgs& a, int n, int page, int row, int h0, int h1) {
+  constexpr int U = D / 8;
+  constexpr uint32_t nan2 = 0x7fff7fffu;  // of both activation dtypes
+  const int o = threadIdx.x % U, H = a.p.H, b = v_block(row), e = v_place(row);
+#pragma clang loop unroll(disable)
+  for (int h = h0; h < h1; ++h) {
+    if (h >= 2 * H) {
+      *reinterpret_cast<u4_t*>(a.qo + n * a.so_n + (h - 2 * H) * a.so_h + 8 * o) = u4_t{nan2, nan2, nan2, nan2};
+    } else if (page >= 0) {
+      uint32_t* pg = a.p.pages + (int64_t(page) * H + (h < H ? h : h - H)) * page_words(D);
+      if (h < H) {
+        pg[row * U + o] = 0;
+        if (o % 4 == 0) pg[page_km(D) + row * (D / 32) + o / 4] = nan2;
+      } else {
+        pg[page_vc(D) + (b * U + o) * 8 + e] = 0;
+        if (o % 4 == 0) {
+          uint16_t* m = reinterpret_cast<uint16_t*>(pg + page_vm(D)) + (b * (D / 32) + o / 4) * 16 + e;
+          m[0] = m[8] = uint16_t(nan2);
+        }
+      }
+    }
+  }
+}
+
 template <int D, bool BF>
 __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a, int heads_per_block) {
   constexpr int U = D / 8, TOK = THREADS / U;
@@ -109,16 +136,21 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a, int heads
   const int64_t at = int64_t(held) + i;
   const int H = a.p.H, heads = 2 * H + (a.q ? a.Hq : 0);
   int32_t bad = 0, page = -1;
-  if (held < 0 || at >= int64_t(a.p.P) * PAGE || (a.cos && at >= a.n_pos)) bad = PAGED_BAD_TOKEN;
+  if (held < 0 || at >= int64_t(a.p.P) * PAGE) bad = PAGED_BAD_TOKEN;
   else {
     page = a.p.table[s * a.p.s_table + at / PAGE];
-    if (page < 0 || page >= a.p.n_pages) bad = PAGED_BAD_PAGE;
-  }
-  if (bad) {  // the token is left out
-    if (o == 0 && blockIdx.y == 0) atomicOr(a.p.status, bad);
-    return;
+    if (page < 0 || page >= a.p.n_pages) {
+      bad = PAGED_BAD_PAGE;
+      page = -1;
+    }
+    if (a.cos && at >= a.n_pos) bad |= PAGED_BAD_TOKEN;
   }
   const int row = int(at % PAGE);
+  if (bad) {
+    if (o == 0 && blockIdx.y == 0) atomicOr(a.p.status, bad);
+    refuse<D>(a, n, page, row, blockIdx.y * heads_per_block, min(heads, int(blockIdx.y + 1) * heads_per_block));
+    return;
+  }
   const bool turn = a.cos && 8 * o < a.R, second = 16 * o >= a.R;
   float c[8], sn[8];
   if (turn) {

@@ -146,8 +146,10 @@ class PagedStore:
         become tokens lens[s], lens[s] + 1, ... of sequence s (lens: tokens held before the call, which it leaves as
         they are).  cos, sin: fp32 [positions, R/2]; the first R dims of each key and query are rotated by their
         token's row (pairs d, d + R/2).  Returns q [N, Hq, D] rotated, written to ``q_out`` (q itself, or memory that no
-        other argument uses) or a new tensor; None without q.  Rows outside the sequences are neither appended nor written to q_out.  Sequences
-        that append must not share the pages they append to."""
+        other argument uses) or a new tensor; None without q.  Rows outside the sequences are neither appended nor
+        written to q_out.  A token that cannot be appended (check()) has NaN queries, and one that only the rotation has
+        no row for NaN in its page, so that read() and attend() give NaN.  Sequences that append must not share the
+        pages they append to."""
         fast = ops._native(k) if forward_ad._current_level < 0 else None
         if fast is not None:
             r = fast.paged_append(self.pages, self.D, self.dtype, self.status, table, lens, k, v, cu_seqlens, cos, sin, q,

@@ -40,3 +40,55 @@ def test_empty_rotation_tables_are_refused(front, shape):
     with pytest.raises(ValueError, match="rotation"):
         st.append(k, k, i32([[0], [1]]), i32([3, 4]), cos=empty, sin=empty, q=q)
     assert torch.equal(st.pages, before)
+
+
+def angles(n, half):
+    a = torch.arange(n)[:, None] * 10000.0 ** (-torch.arange(half) / half)
+    return a.cos().float().to(DEV), a.sin().float().to(DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,H,Hq,each", [(64, 2, 4, 5), (128, 1, 3, 70), (128, 8, 32, 500)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_tokens_that_append_refuses_are_nan(front, dtype, D, H, Hq, each, in_place):
+    """Sequence 0 fits; 1 runs past the rotation's rows, 2 past the table too, 3 needs a page outside the pool, 4 has a
+    negative length: their tokens' queries are NaN, and so is what read and attend give for the rows that have pages."""
+    g = torch.Generator().manual_seed(D + each)
+    S, P, n_pos = 5, -(-(each + 40) // 64) + 1, each + 30
+    held = [2, n_pos - each // 3, P * 64 - 2, 0, -2]
+    cos, sin = angles(P * 64, D // 2)
+    N = S * each
+    k, v, q = randn(g, N, H, D, dtype=dtype), randn(g, N, H, D, dtype=dtype), randn(g, N, Hq, D, dtype=dtype)
+    cu = i32([each * s for s in range(S + 1)])
+    table = torch.arange(S * P, dtype=torch.int32, device=DEV).view(S, P).clone()
+    st, want = (paged.PagedStore(S * P, H, D, DEV, dtype) for _ in range(2))
+    for x in (st, want):
+        x.pages.fill_(0x3C003C00)  # finite values: a row that is left as it was would pass for a token
+    turned = want.append(k, v, table, i32([2, held[1], 0, 0, 0]), cu, cos, sin, q)
+    table[3] = S * P
+    fine = torch.zeros(N, dtype=torch.bool)
+    for s in (0, 1, 2):
+        most = [n_pos, n_pos, P * 64][s]
+        fine[s * each:(s + 1) * each] = torch.arange(each) + held[s] < min(most, n_pos, P * 64)
+    assert bool(fine[:each].all()) and 0 < int(fine[each:2 * each].sum()) < each and not bool(fine[2 * each:].any())
+    q_out = q.clone() if in_place else None
+    got = st.append(k, v, table, i32(held), cu, cos[:n_pos], sin[:n_pos], q_out if in_place else q, q_out)
+    assert int(st.status) == 3
+    assert torch.equal(got[fine], turned[fine]) and bool(got[~fine].isnan().all())
+    # the pages: sequence 0's as they should be, sequence 1's with NaN from the first refused token on
+    kk, vv = st.read(table[:2], i32(held[:2]), cu[:3], 2 * each)
+    wk, wv = want.read(table[:2], i32(held[:2]), cu[:3], 2 * each)
+    for a, b in ((kk, wk), (vv, wv)):
+        assert torch.equal(a[fine[:2 * each]], b[fine[:2 * each]]) and bool(a[~fine[:2 * each]].isnan().all())
+    # nothing else is touched: rows of sequence 1 outside its tokens, and the pages of 3 and 4
+    rest = (torch.arange(P * 64, device=DEV) < held[1]) | (torch.arange(P * 64, device=DEV) >= held[1] + each)
+    whole = torch.arange(2, dtype=torch.int32, device=DEV) * P * 64
+    a, b = st.read(table[1:2], i32([0]), whole, P * 64), want.read(table[1:2], i32([0]), whole, P * 64)
+    assert torch.equal(a[0][rest], b[0][rest]) and torch.equal(a[1][rest], b[1][rest])
+    assert bool((st.pages[3 * P:] == 0x3C003C00).all())
+    st.status.zero_()
+    x = randn(g, 2, Hq, D, dtype=dtype)
+    out = st.attend(x, table[:2], i32([held[0] + each, held[1] + each]), 0.1)
+    assert torch.equal(out[0], want.attend(x, table[:2], i32([held[0] + each, held[1] + each]), 0.1)[0])
+    assert bool(out[1].isnan().all())
+    assert bool(st.attend(x, table[:2], i32([held[0] + each, n_pos]), 0.1).isfinite().all())
