@@ -94,6 +94,12 @@ def rows_aligned(t: torch.Tensor) -> bool:
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in t.stride()[:-1])
 
 
+def readable_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy of it, with rows_aligned().  (contiguous() would return ``t`` where only its memory's first byte
+    or the stride of a dim of size 1 is in the way.)"""
+    return t if rows_aligned(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def autograd_follows(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether autograd, backward or forward mode, follows what is computed from any of the tensors."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
@@ -926,7 +932,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         check_out(t.shape, shape, name)
         if t.device != dev:
             _shape_error(f"{name} is on {t.device}, q on {dev}")
-        rows.append(t if rows_aligned(t) and t.stride(0) < 2 ** 23 else t.contiguous())
+        rows.append(readable_rows(t if t.stride(0) < 2 ** 23 else t.clone(memory_format=torch.contiguous_format)))
     q, k, v = rows
     cu_q = check_cu(cu_seqlens, "cu_seqlens", None, dev)
     S = cu_q.shape[0] - 1

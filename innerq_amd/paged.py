@@ -47,9 +47,7 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, device) -> torch.Tens
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the store on {device}")
     ops.check_out(t.shape, shape, name)
-    if not ops.rows_aligned(t):
-        t = t.contiguous()
-    return t
+    return ops.readable_rows(t)
 
 
 def _out_rows(t: torch.Tensor, name: str, shape: tuple, dtype, device) -> torch.Tensor:

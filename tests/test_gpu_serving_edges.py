@@ -92,3 +92,35 @@ def test_tokens_that_append_refuses_are_nan(front, dtype, D, H, Hq, each, in_pla
     assert torch.equal(out[0], want.attend(x, table[:2], i32([held[0] + each, held[1] + each]), 0.1)[0])
     assert bool(out[1].isnan().all())
     assert bool(st.attend(x, table[:2], i32([held[0] + each, n_pos]), 0.1).isfinite().all())
+
+
+def off_grid(x):
+    """The values of x [n, h, d] in memory that the kernels cannot read as it is, two ways: rows of an odd width, and a
+    contiguous block that starts between 16-byte boundaries."""
+    n, h, d = x.shape
+    wide = torch.empty(n, h * d + 4, dtype=x.dtype, device=DEV)[:, :h * d].view(n, h, d)
+    flat = torch.empty(4 + n * h * d, dtype=x.dtype, device=DEV)[4:].view(n, h, d)
+    return [wide.copy_(x), flat.copy_(x)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [1, 2, 5])
+def test_inputs_off_the_16_byte_grid(front, dtype, N):
+    """Copied, as documented, for one row as for many."""
+    g = torch.Generator().manual_seed(N)
+    H, Hq, D = 2, 4, 64
+    k, v, q = randn(g, N, H, D, dtype=dtype), randn(g, N, H, D, dtype=dtype), randn(g, N, Hq, D, dtype=dtype)
+    table, lens, cu = torch.arange(N, dtype=torch.int32, device=DEV)[:, None], i32([3] * N), i32([0, N])
+    cos, sin = angles(10, D // 2)
+    stores = [paged.PagedStore(N, H, D, DEV, dtype) for _ in range(3)]
+    for st in stores:
+        st.pages.zero_()
+    want = stores[0].append(k, v, table, lens, None, cos, sin, q)
+    out = stores[0].attend(want, table, lens + 1, 0.1)
+    prompt = ops.prompt_attention(q, k, v, cu, 0.1)
+    for st, kk, vv, qq, ww in zip(stores[1:], off_grid(k), off_grid(v), off_grid(q), off_grid(want)):
+        assert torch.equal(st.append(kk, vv, table, lens, None, cos, sin, qq), want)
+        assert torch.equal(st.pages, stores[0].pages)
+        assert torch.equal(st.attend(ww, table, lens + 1, 0.1), out)
+        for a in ((qq, k, v), (q, kk, v), (q, k, vv), (qq, kk, vv)):
+            assert torch.equal(ops.prompt_attention(*a, cu, 0.1), prompt)
