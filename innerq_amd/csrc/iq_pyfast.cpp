@@ -21,6 +21,9 @@
 // the C ABI's function addresses, handed in by bind().
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <utility>
+
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
@@ -513,11 +516,20 @@ const at::Tensor* rows_of(PyObject* o, int64_t dims, at::ScalarType dt, int devi
     if (t->stride(i) % 8) return nullptr;
   return t;
 }
-// rows_of() to be written: no two rows in one place
+// rows_of() to be written (3 or 4 dims): no two rows share memory (ops.writable_rows)
 const at::Tensor* out_rows_of(PyObject* o, int64_t dims, at::ScalarType dt, int device, int64_t D) {
   const at::Tensor* t = rows_of(o, dims, dt, device, D);
-  for (int64_t i = 0; t && i + 1 < dims; ++i)
-    if (t->size(i) > 1 && t->stride(i) == 0) return nullptr;
+  if (!t) return nullptr;
+  std::pair<int64_t, int64_t> d[3];  // (stride, size), by stride
+  int n = 0;
+  for (int64_t i = 0; i + 1 < dims; ++i)
+    if (t->size(i) > 1) d[n++] = {t->stride(i), t->size(i)};
+  std::sort(d, d + n);
+  int64_t end = D;  // each dim's stride is past all that the dims of smaller strides cover
+  for (int i = 0; i < n; ++i) {
+    if (d[i].first < end) return nullptr;
+    end += d[i].first * (d[i].second - 1);
+  }
   return t;
 }
 // a contiguous int32 vector of n values on the device

@@ -109,8 +109,16 @@ def autograd_follows(*tensors: Optional[torch.Tensor]) -> bool:
 
 
 def writable_rows(t: torch.Tensor) -> bool:
-    """rows_aligned(), and no two rows in one place (an expanded tensor's are)."""
-    return rows_aligned(t) and not any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+    """rows_aligned(), and no two rows share memory (an expanded or a sliding view's do): each dim's stride is past all
+    that the dims of smaller strides cover."""
+    if not rows_aligned(t):
+        return False
+    end = t.shape[-1]
+    for s, n in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        if s < end:
+            return False
+        end += s * (n - 1)
+    return True
 
 
 def check_cu(cu: torch.Tensor, name: str, S: Optional[int], device: torch.device) -> torch.Tensor:

@@ -124,3 +124,26 @@ def test_inputs_off_the_16_byte_grid(front, dtype, N):
         assert torch.equal(st.attend(ww, table, lens + 1, 0.1), out)
         for a in ((qq, k, v), (q, kk, v), (q, k, vv), (qq, kk, vv)):
             assert torch.equal(ops.prompt_attention(*a, cu, 0.1), prompt)
+
+
+def test_outputs_whose_rows_share_memory_are_refused(front):
+    g = torch.Generator().manual_seed(2)
+    S, H, Hq, D = 4, 2, 8, 64
+    k, q = randn(g, S, H, D), randn(g, S, Hq, D)
+    st = paged.PagedStore(S, H, D, DEV)
+    table, lens, cu = i32([[0], [1], [2], [3]]), i32([1] * S), i32([0, S])
+    st.append(k, k, table, i32([0] * S))
+    memory = torch.full((4 * S * Hq * D,), 5.0, dtype=torch.float16, device=DEV)
+    for size, stride in (((S, Hq, D), (8, D, 1)), ((S, Hq, D), (Hq * D - 8, D, 1)), ((S, Hq, D), (Hq * D, D - 8, 1)),
+                         ((S, Hq, D), (0, D, 1))):
+        out = memory.as_strided(size, stride)
+        for call in (lambda: st.attend(q, table, lens, 0.1, out=out),
+                     lambda: st.attend(q[:, None].expand(S, 2, Hq, D), table, lens, 0.1, out=out[:, None].expand(S, 2, Hq, D)),
+                     lambda: st.append(k, k, table, lens, q=q, q_out=out),
+                     lambda: st.read(table, i32([0] * S), None, S, k_out=out[:, :H], v_out=k.clone()),
+                     lambda: ops.prompt_attention(q, k, k, cu, 0.1, out=out)):
+            with pytest.raises(ValueError, match="rows"):
+                call()
+    assert bool((memory == 5).all())
+    out = memory.as_strided((S, Hq, D), (D, S * D, 1))  # heads outermost: rows of their own
+    assert torch.equal(st.attend(q, table, lens, 0.1, out=out), st.attend(q, table, lens, 0.1))

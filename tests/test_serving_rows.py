@@ -28,3 +28,17 @@ def test_rows_are_readable(dtype):
 
 def test_no_rows():
     assert ops.readable_rows(torch.zeros(0, 4, 64)).shape == (0, 4, 64)
+
+
+def test_rows_of_their_own():
+    x = torch.zeros(6, 8, 128, dtype=torch.float16)
+    for t in (x, x[1:], x[:, 2:6], x[::2], x.transpose(0, 1), x[:1], x[:, :1], x[:, :1].expand(6, 1, 128), x[:0],
+              x.view(2, 3, 8, 128), x.view(2, 3, 8, 128).permute(2, 0, 1, 3), x[..., :64],
+              x.as_strided((2, 2, 2, 64), (256, 64, 1024, 1)), x.as_strided((1, 4, 128), (8, 128, 1))):
+        assert ops.writable_rows(t), t.stride()
+    for size, stride in (((4, 8, 128), (8, 128, 1)),      # rows that slide over one another by 8 elements
+                         ((4, 8, 128), (1016, 128, 1)),   # a row's last head is the next row's first, but for 8
+                         ((4, 8, 128), (128, 128, 1)), ((4, 8, 128), (1024, 120, 1)), ((4, 8, 128), (0, 128, 1)),
+                         ((4, 8, 128), (1024, 0, 1)), ((2, 3, 4, 64), (128, 64, 256, 1)), ((4, 2, 128), (64, 512, 1))):
+        assert not ops.writable_rows(x.as_strided(size, stride)), stride
+    assert not ops.writable_rows(x[..., 4:68]) and not ops.writable_rows(x[..., ::2])
