@@ -140,10 +140,14 @@ def test_outputs_whose_rows_share_memory_are_refused(front):
         for call in (lambda: st.attend(q, table, lens, 0.1, out=out),
                      lambda: st.attend(q[:, None].expand(S, 2, Hq, D), table, lens, 0.1, out=out[:, None].expand(S, 2, Hq, D)),
                      lambda: st.append(k, k, table, lens, q=q, q_out=out),
-                     lambda: st.read(table, i32([0] * S), None, S, k_out=out[:, :H], v_out=k.clone()),
                      lambda: ops.prompt_attention(q, k, k, cu, 0.1, out=out)):
             with pytest.raises(ValueError, match="rows"):
                 call()
+    for stride in ((8, D, 1), (H * D - 8, D, 1), (H * D, D - 8, 1), (H * D, 0, 1)):
+        out = memory.as_strided((S, H, D), stride)
+        for kw in (dict(k_out=out), dict(v_out=out)):
+            with pytest.raises(ValueError, match="rows"):
+                st.read(table, i32([0] * S), None, S, **kw)
     assert bool((memory == 5).all())
     out = memory.as_strided((S, Hq, D), (D, S * D, 1))  # heads outermost: rows of their own
     assert torch.equal(st.attend(q, table, lens, 0.1, out=out), st.attend(q, table, lens, 0.1))
