@@ -108,17 +108,30 @@ def autograd_follows(*tensors: Optional[torch.Tensor]) -> bool:
                                                   for t in tensors)
 
 
-def writable_rows(t: torch.Tensor) -> bool:
-    """rows_aligned(), and no two rows share memory (an expanded or a sliding view's do): each dim's stride is past all
-    that the dims of smaller strides cover."""
-    if not rows_aligned(t):
-        return False
-    end = t.shape[-1]
-    for s, n in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+def _nested(dims, end: int) -> bool:
+    """Whether each (stride, size)'s stride is past all that the ones of smaller strides cover, of blocks of ``end``."""
+    for s, n in sorted((s, n) for s, n in dims if n > 1):
         if s < end:
             return False
         end += s * (n - 1)
     return True
+
+
+def writable_rows(t: torch.Tensor) -> bool:
+    """rows_aligned(), and no two rows share memory (an expanded or a sliding view's do)."""
+    return rows_aligned(t) and _nested(zip(t.stride()[:-1], t.shape[:-1]), t.shape[-1])
+
+
+def apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two outputs of one shape and dtype, each with writable_rows(), share no memory: one lies behind the other,
+    or they take turns (halves of one tensor)."""
+    if not a.numel():
+        return True
+    size = a.element_size()
+    (p, s), (q, t) = ((x.data_ptr(), size * (1 + sum(s * (n - 1) for s, n in zip(x.stride(), x.shape)))) for x in (a, b))
+    if p + s <= q or q + t <= p:
+        return True
+    return a.stride() == b.stride() and _nested([*zip(a.stride()[:-1], a.shape[:-1]), (abs(p - q) // size, 2)], a.shape[-1])
 
 
 def check_cu(cu: torch.Tensor, name: str, S: Optional[int], device: torch.device) -> torch.Tensor:

@@ -198,7 +198,8 @@ class PagedStore:
     def read(self, table: torch.Tensor, lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor], n: int,
              k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
         """K and V [n, H, D] of tokens lens[s] + i of every sequence, at rows cu_seqlens[s] + i (as ``append`` takes
-        them; n rows in all).  Rows outside the sequences are not written."""
+        them; n rows in all), in ``k_out`` and ``v_out`` (memory of their own) or new tensors.  Rows outside the
+        sequences are not written."""
         fast = ops._native(self.pages)
         if fast is not None and k_out is None and v_out is None:
             r = fast.paged_read(self.pages, self.D, self.dtype, self.status, table, lens, cu_seqlens, n)
@@ -212,6 +213,8 @@ class PagedStore:
             outs.append(torch.empty(want, dtype=self.dtype, device=self.device) if t is None else
                         _out_rows(t, name, want, self.dtype, self.device))
         k, v = outs
+        if not ops.apart(k, v):
+            raise ValueError("read: k_out and v_out share memory")
         with ops.on_device(self.device):
             call("iq_paged_read", ctypes.byref(p), ops._p(cu), n, ops._p(k), k.stride(0), k.stride(1), ops._p(v),
                  v.stride(0), v.stride(1), ops._stream(self.device))

@@ -151,3 +151,19 @@ def test_outputs_whose_rows_share_memory_are_refused(front):
     assert bool((memory == 5).all())
     out = memory.as_strided((S, Hq, D), (D, S * D, 1))  # heads outermost: rows of their own
     assert torch.equal(st.attend(q, table, lens, 0.1, out=out), st.attend(q, table, lens, 0.1))
+
+
+def test_read_into_one_memory_is_refused():
+    g = torch.Generator().manual_seed(3)
+    st = paged.PagedStore(2, 2, 64, DEV)
+    k, v = randn(g, 20, 2, 64), randn(g, 20, 2, 64)
+    table, cu = i32([[0], [1]]), i32([0, 8, 20])
+    st.append(k, v, table, i32([0, 0]), cu)
+    wide = torch.full((20, 5, 64), 5.0, dtype=torch.float16, device=DEV)
+    for a, b in ((wide[:, :2], wide[:, :2]), (wide[:, :2], wide[:, 1:3]), (wide[:, 1:3], wide[:, :2])):
+        with pytest.raises(ValueError, match="share memory"):
+            st.read(table, i32([0, 0]), cu, 20, k_out=a, v_out=b)
+    assert bool((wide == 5).all())
+    want = st.read(table, i32([0, 0]), cu, 20)
+    got = st.read(table, i32([0, 0]), cu, 20, k_out=wide[:, 3:], v_out=wide[:, :2])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and bool((wide[:, 2] == 5).all())

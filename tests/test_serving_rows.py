@@ -42,3 +42,14 @@ def test_rows_of_their_own():
                          ((4, 8, 128), (1024, 0, 1)), ((2, 3, 4, 64), (128, 64, 256, 1)), ((4, 2, 128), (64, 512, 1))):
         assert not ops.writable_rows(x.as_strided(size, stride)), stride
     assert not ops.writable_rows(x[..., 4:68]) and not ops.writable_rows(x[..., ::2])
+
+
+def test_outputs_apart():
+    x = torch.zeros(6, 8, 128, dtype=torch.float16)
+    y = torch.zeros(6, 2, 8, 64, dtype=torch.float16)
+    for a, b in ((x, torch.zeros_like(x)), (x[:3], x[3:]), (x[:, :4], x[:, 4:]), (x[:, 4:], x[:, :4]), (x[::2], x[1::2]),
+                 (x[..., :64], x[..., 64:]), (y[:, 0], y[:, 1]), (x[:0], x[:0]), (x[:, ::2], x[:, 1::2])):
+        assert ops.writable_rows(a) and ops.writable_rows(b) and ops.apart(a, b) and ops.apart(b, a)
+    for a, b in ((x, x), (x[:3], x[2:5]), (x[:, :4], x[:, 3:7]), (x[..., :64], x[..., 8:72]), (x[:, :4], x[:, :4]),
+                 (x[:4, :4], x.view(-1)[64:].as_strided((4, 4, 128), (512, 128, 1)))):
+        assert not ops.apart(a, b) and not ops.apart(b, a)
