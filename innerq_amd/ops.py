@@ -930,14 +930,15 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     values) of q and, by cu_seqlens_k (default: the same), of k and v.  causal: a sequence's last row sees all its
     keys, each row before it one less (a chunk of a prompt behind its earlier keys has more keys than rows); window:
     only the last ``window`` of the keys up to its own.  Rows that see no key are 0; rows outside the sequences are
-    not written.  ``out`` may be q, or memory that no other argument uses.  Inference only: tensors that autograd follows are refused."""
+    not written.  ``out`` may be q, or memory that no other argument uses.  Inference only: tensors that autograd
+    follows are refused, ``out`` too."""
     fast = _native(q) if forward_ad._current_level < 0 else None
     if fast is not None:
         r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out)
         if r is not None:
             return r
     require_act(q, "q")
-    if autograd_follows(q, k, v):
+    if autograd_follows(q, k, v, out):
         raise NotImplementedError("prompt_attention has no backward: call it under torch.no_grad()")
     if q.dim() != 3 or k.dim() != 3:
         _shape_error(f"q must be [N, Hq, D] and k [Nk, H, D], got {tuple(q.shape)} and {tuple(k.shape)}")

@@ -18,7 +18,7 @@ A prompt attends with ops.prompt_attention over its dense K and V; a later chunk
     q = store.append(k, v, table, lens, cos=cos, sin=sin, q=q)                # a step: one token per sequence
     out = store.attend(q, table, lens + 1, scale)
 
-Inference only: tensors that autograd follows are refused.  Device tensors only; there is no CPU path.
+Inference only: tensors that autograd follows are refused, outputs too.  Device tensors only; there is no CPU path.
 """
 from __future__ import annotations
 
@@ -154,7 +154,7 @@ class PagedStore:
                                   q_out)
             if r is not None:
                 return r[0]
-        _no_grad(k, v, q, cos, sin)
+        _no_grad(k, v, q, cos, sin, q_out)
         p = self._args(table, lens)
         if k.dim() != 3:
             raise ValueError(f"append: k must be [N, H, D], got {tuple(k.shape)}")
@@ -180,7 +180,6 @@ class PagedStore:
             if q.dim() != 3 or q.shape[1] == 0:
                 raise ValueError(f"append: q must be [N, Hq, D], got {tuple(q.shape)}")
             Hq = q.shape[1]
-            given = q
             q = _rows(q, "q", (N, Hq, self.D), self.dtype, self.device)
             if q_out is None:
                 q_out = torch.empty(N, Hq, self.D, dtype=self.dtype, device=self.device)
@@ -205,6 +204,7 @@ class PagedStore:
             r = fast.paged_read(self.pages, self.D, self.dtype, self.status, table, lens, cu_seqlens, n)
             if r is not None:
                 return r
+        _no_grad(k_out, v_out)
         p = self._args(table, lens)
         cu = self._cu(cu_seqlens, p.S, n)
         want = (n, self.H, self.D)
@@ -231,7 +231,7 @@ class PagedStore:
             r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out)
             if r is not None:
                 return r
-        _no_grad(q)
+        _no_grad(q, out)
         p = self._args(table, lens)
         if q.dim() not in (3, 4) or q.shape[0] != p.S:
             raise ValueError(f"attend: q must be [S, Hq, D] or [S, m, Hq, D] with S = {p.S}, got {tuple(q.shape)}")

@@ -167,3 +167,35 @@ def test_read_into_one_memory_is_refused():
     want = st.read(table, i32([0, 0]), cu, 20)
     got = st.read(table, i32([0, 0]), cu, 20, k_out=wide[:, 3:], v_out=wide[:, :2])
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and bool((wide[:, 2] == 5).all())
+
+
+def test_outputs_that_autograd_follows_are_refused(front):
+    """A leaf, what was computed from one, a dual tensor; under no_grad the first two are memory as any other."""
+    g = torch.Generator().manual_seed(4)
+    S, H, Hq, D = 3, 2, 4, 64
+    k, q = randn(g, S, H, D), randn(g, S, Hq, D)
+    st = paged.PagedStore(S, H, D, DEV)
+    table, lens, cu = i32([[0], [1], [2]]), i32([1] * S), i32([0, S])
+    st.append(k, k, table, i32([0] * S))
+    want, turned = st.attend(q, table, lens, 0.1), ops.prompt_attention(q, k, k, cu, 0.1)
+    leaf = torch.full((S, Hq, D), 5.0, dtype=torch.float16, device=DEV, requires_grad=True)
+
+    def calls(out):
+        return [lambda: st.attend(q, table, lens, 0.1, out=out), lambda: ops.prompt_attention(q, k, k, cu, 0.1, out=out),
+                lambda: st.append(k, k, table, lens, q=q, q_out=out), lambda: st.read(table, i32([0] * S), None, S, k_out=out[:, :H]),
+                lambda: st.read(table, i32([0] * S), None, S, v_out=out[:, :H])]
+
+    for out in (leaf, leaf * 1):
+        for call in calls(out):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert bool((out == 5).all())
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(leaf.detach(), q)
+        for call in calls(dual):
+            with pytest.raises(NotImplementedError):
+                call()
+    assert bool((leaf == 5).all())
+    with torch.no_grad():
+        for out in (leaf, leaf * 1):
+            assert torch.equal(calls(out)[0](), want) and torch.equal(calls(out)[1](), turned)
