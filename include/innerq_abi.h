@@ -401,8 +401,8 @@ int iq_decode_attention_noalloc(const void* q, int64_t sq_b, int64_t sq_h, const
  * table[s * s_table + i] is the page of sequence s's tokens [64 i, 64 i + 64), lens[s] its token count (see each
  * call), both read on the device: a captured call follows their values.  What they hold is checked there, before any
  * access: an entry that names no page of the pool, or a token past P * 64 or of a negative length, is not accessed, and
- * the call ORs IQ_PAGED_BAD_* into *status, which nothing here clears; a token past the rotation's rows that has a page
- * becomes NaN there and is told alike.  Two sequences may share pages that no call writes. */
+ * the call ORs IQ_PAGED_BAD_* into *status, which only iq_paged_take_status clears; a token past the rotation's rows that
+ * has a page becomes NaN there and is told alike.  Two sequences may share pages that no call writes. */
 enum iq_paged_status {
   IQ_PAGED_BAD_PAGE = 1,  /* a table entry outside [0, n_pages) was needed */
   IQ_PAGED_BAD_TOKEN = 2  /* a token past the table's P * 64 or past the rotation's rows, or a negative length */
@@ -421,6 +421,10 @@ typedef struct iq_paged {
 
 /* Bytes of one page (H heads). */
 int iq_page_bytes(int H, int D, int64_t* bytes);
+
+/* *taken = *status and *status = 0 at once (both on the device): a bit that a call on another stream sets is in this
+ * *taken or in the next. */
+int iq_paged_take_status(int32_t* status, int32_t* taken, void* stream);
 
 /* Appends N new tokens: those of sequence s are rows [cu[s], cu[s+1]) of k and v [N, H, D] (cu int32 [S+1] on the
  * device, non-decreasing; NULL: one token per sequence, N = S) and become its tokens lens[s] + i (lens: tokens held

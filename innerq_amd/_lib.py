@@ -115,6 +115,7 @@ SIGNATURES = {
                                             I, I, I, I, I, F, P, S, ctypes.POINTER(iq_split_plan), P]),
     "iq_decode_attention_combine_live": (I, [ctypes.POINTER(iq_split_plan), I, I, I, I, P, L, L, P, S, P]),
     "iq_page_bytes": (I, [I, I, ctypes.POINTER(L)]),
+    "iq_paged_take_status": (I, [P, P, P]),
     "iq_paged_append": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P, P, L, I, P, L, L, I, P, L, L, P]),
     "iq_paged_read": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P]),
     "iq_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I]),

@@ -1,4 +1,4 @@
-// Appending to and reading 4-bit pages (gfx950): iq_paged_append, iq_paged_read.
+// Appending to and reading 4-bit pages (gfx950): iq_paged_append, iq_paged_read; their status word: iq_paged_take_status.
 //
 // append: U = D/8 lanes hold one token of one head, 8 values each.  A lane that rotates reads its own 8 values and
 // the 8 of its partner half (the second read hits L1), so neither the rotation nor a q rotated in place needs LDS;
@@ -271,6 +271,8 @@ __global__ __launch_bounds__(THREADS) void read_kernel(ReadArgs a, int heads_per
   }
 }
 
+__global__ void take_status_kernel(int32_t* status, int32_t* taken) { *taken = atomicExch(status, 0); }
+
 // Heads that a block does for its tokens: one while there are few blocks; then as many as leave `blocks` blocks, up to
 // `most`, a power of two (finding a token, three or more loads that wait for each other, then serves all of them).
 //   append, 768 blocks, 16 heads at most (8 KV, 32 query heads, D = 128, bf16; us with 1, 2, 4, 8, 16 heads per block):
@@ -309,6 +311,13 @@ extern "C" int iq_page_bytes(int H, int D, int64_t* bytes) {
   IQ_CHECK(d_ok(D) && H > 0 && H <= 4096, IQ_ERR_SHAPE);
   *bytes = int64_t(H) * page_words(D) * 4;
   return IQ_OK;
+}
+
+extern "C" int iq_paged_take_status(int32_t* status, int32_t* taken, void* stream) {
+  IQ_CHECK(status && taken, IQ_ERR_NULL);
+  IQ_CHECK(aligned(status, 4) && aligned(taken, 4), IQ_ERR_ALIGN);
+  take_status_kernel<<<1, 1, 0, (hipStream_t)stream>>>(status, taken);
+  return launch_status();
 }
 
 extern "C" int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, const void* k, int64_t sk_n, int64_t sk_h,

@@ -103,10 +103,13 @@ class PagedStore:
 
     def check(self) -> None:
         """Raises RuntimeError if a call since the last check needed a page outside the pool or a token past the
-        table (reads the status word on the current stream: waits for it, and for calls that it waits for)."""
-        bad = int(self.status.item())
+        table (takes the status word on the current stream: waits for it, and for calls that it waits for; what a call
+        on another stream tells meanwhile is kept for the next check)."""
+        with ops.on_device(self.device):
+            taken = torch.empty(1, dtype=torch.int32, device=self.device)
+            call("iq_paged_take_status", ops._p(self.status), ops._p(taken), ops._stream(self.device))
+        bad = int(taken.item())
         if bad:
-            self.status.zero_()
             why = [w for b, w in ((1, "a table entry outside the pool"),
                                   (2, "a token past the table's pages or the rotation's rows, or a negative length"))
                    if bad & b]

@@ -199,3 +199,28 @@ def test_outputs_that_autograd_follows_are_refused(front):
     with torch.no_grad():
         for out in (leaf, leaf * 1):
             assert torch.equal(calls(out)[0](), want) and torch.equal(calls(out)[1](), turned)
+
+
+def test_check_keeps_what_is_told_while_it_reads(monkeypatch):
+    """A call that meets a bad length after check() has taken the status word, and before check() returns, is told by the
+    next check()."""
+    g = torch.Generator().manual_seed(5)
+    st = paged.PagedStore(2, 2, 64, DEV)
+    k, table = randn(g, 2, 2, 64), i32([[0], [1]])
+    st.append(k, k, i32([[9], [1]]), i32([0, 0]))
+    item, other = torch.Tensor.item, torch.cuda.Stream()
+
+    def late(t):
+        word = item(t)
+        monkeypatch.setattr(torch.Tensor, "item", item)
+        with torch.cuda.stream(other):
+            st.append(k, k, table, i32([-1, 0]))
+        other.synchronize()
+        return word
+
+    monkeypatch.setattr(torch.Tensor, "item", late)
+    with pytest.raises(RuntimeError, match="outside the pool$"):
+        st.check()
+    with pytest.raises(RuntimeError, match="met a token past"):
+        st.check()
+    st.check()
