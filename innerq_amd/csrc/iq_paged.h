@@ -100,6 +100,19 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+// ---- shares --------------------------------------------------------------------------------------------------
+// A list of `total` units (up to 2^31 - 1) shared out evenly over `grid` workgroups: workgroup g's are the units from
+// share_begin(g) to share_begin(g + 1), unit u's workgroup is u / per.  A page per wave (of four) at least.
+constexpr int SHARE_LEAST = 4;
+__host__ __device__ inline int units_per_group(int total, int grid) {
+  const int n = total / grid + (total % grid ? 1 : 0);
+  return n < SHARE_LEAST ? SHARE_LEAST : n;
+}
+__host__ __device__ inline int share_begin(int g, int per, int total) {
+  const int64_t u = int64_t(g) * per;
+  return int(u < total ? u : total);
+}
+
 // ---- sequences -----------------------------------------------------------------------------------------------
 // token n of a flat list belongs to sequence s at place i (cu null: one token each); false: to none
 __device__ __forceinline__ bool sequence_of(const int32_t* cu, int S, int n, int& s, int& i) {

@@ -22,7 +22,7 @@ using namespace iq;
 
 namespace {
 
-constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 16;  // rows of an MFMA operand: a tile has T times as many
+constexpr int WAVES = SHARE_LEAST, THREADS = 64 * WAVES, ROWS = 16;  // rows of an MFMA operand: a tile has T times as many
 // What a (sequence, head, tile) costs beside its pages, in pages: its queries, its first page's latency and the
 // merge of the waves.  Counted where the workgroups share out the list; without it a workgroup whose share was many
 // short sequences came last (48 sequences of 130 .. 16001 tokens, bf16: 181 us against 82).
@@ -108,10 +108,6 @@ __device__ __forceinline__ void find_unit(const AttnArgs& a, Part p, int u, int&
     p = part_at(a, s0, __builtin_amdgcn_readlane(p.end, 63));
   }
 }
-__device__ __forceinline__ int units_per_group(int total, int grid) {
-  return max((total + grid - 1) / grid, WAVES);  // a page per wave at least
-}
-
 // row r of tile t of sequence s: its query head offset (head in the group, token)
 struct Row {
   int token, head;
@@ -395,8 +391,8 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
   if (a.split) {
     const Part part = part_at(a, 0, 0);
     const int total = total_units(a, part), per = units_per_group(total, a.grid);
-    u = min(int64_t(blockIdx.x) * per, int64_t(total));
-    u1 = min(u + per, total);
+    u = share_begin(blockIdx.x, per, total);
+    u1 = share_begin(blockIdx.x + 1, per, total);
     if (u < u1) find_unit(a, part, u, s, first);
   } else {
     s = blockIdx.x / (H * a.tiles);
