@@ -124,7 +124,7 @@ class PagedStore:
         S, P = table.shape
         if lens.shape[0] != S or not S or not P:
             raise ValueError(f"table [S, P] and lens [S] do not fit: {tuple(table.shape)}, {tuple(lens.shape)}")
-        if table.stride(1) != 1 or lens.stride(0) != 1:
+        if (P > 1 and table.stride(1) != 1) or not lens.is_contiguous():
             raise ValueError("table rows and lens must be contiguous")
         p = _lib.iq_paged()
         p.pages, p.n_pages = self.pages.data_ptr(), self.n_pages

@@ -224,3 +224,25 @@ def test_check_keeps_what_is_told_while_it_reads(monkeypatch):
     with pytest.raises(RuntimeError, match="met a token past"):
         st.check()
     st.check()
+
+
+def test_strides_of_one_length_and_of_one_page(front):
+    """A stride that is never used refuses nothing: the length of one sequence, a table of one page, taken from wider
+    tensors."""
+    g = torch.Generator().manual_seed(6)
+    H, Hq, D = 2, 4, 64
+    st = paged.PagedStore(3, H, D, DEV)
+    for S in (1, 3):
+        k, q = randn(g, S, H, D), randn(g, S, Hq, D)
+        table, lens = i32([[0], [1], [2]])[:S], i32([2, 2, 2])[:S]
+        odd_table = table.clone().as_strided((S, 1), (1, 7))
+        odd_lens = i32([[2, 9]])[:, 0] if S == 1 else lens
+        st.pages.zero_()
+        want = st.append(k, k, table, lens, q=q), st.pages.clone(), st.attend(q, table, lens + 1, 0.1), *st.read(table, lens, None, S)
+        st.pages.zero_()
+        got = st.append(k, k, odd_table, odd_lens, q=q), st.pages, st.attend(q, odd_table, lens + 1, 0.1), *st.read(odd_table, odd_lens, None, S)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(ValueError, match="contiguous"):
+        st.attend(q, i32([[0, 1, 2], [0, 1, 2]]).t()[:, :2], lens, 0.1)
+    with pytest.raises(ValueError, match="contiguous"):
+        st.attend(q, table, i32([[2, 9], [2, 9], [2, 9]])[:, 0], 0.1)
