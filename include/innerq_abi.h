@@ -449,9 +449,9 @@ int iq_paged_read(const iq_paged* p, const int32_t* cu, int N, void* k_out, int6
 /* softmax(q K^T scale) V over the pages for m (1 .. 16) new tokens per sequence: q [S, m, Hq, D], lens[s] the tokens
  * held with the new ones, so token j of the m sees keys below lens[s] - (m - 1 - j), with window > 0 only the last
  * `window` of them.  Logits, softmax statistics and sums in fp32, the weights rounded to the activation dtype for
- * their product with V.  A row that sees no key is 0; a sequence that needs a page outside the pool, or holds more
- * than P * 64 tokens, gives NaN.  Any Hq that H divides.  out may be q.  workspace:
- * iq_paged_attention_workspace_bytes (0: none needed), 16-byte aligned, of this call alone while it runs. */
+ * their product with V.  A row that sees no key, or only keys whose logits are minus infinity, is 0; a sequence that
+ * needs a page outside the pool, or holds more than P * 64 tokens, gives NaN.  Any Hq that H divides.  out may be q.
+ * workspace: iq_paged_attention_workspace_bytes (0: none needed), 16-byte aligned, of this call alone while it runs. */
 size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D);
 int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
                        float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h, void* workspace,
@@ -462,9 +462,9 @@ int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t s
  * cu_q[s+1]) attend to keys [cu_k[s], cu_k[s+1]) (int32 [S+1] on the device, non-decreasing; bounds outside [0, N] or
  * [0, Nk] are moved to them).  causal: the last row sees all keys, row i of lq all but the lq - 1 - i last of lk;
  * window > 0 (causal only): only the last `window` of those.  Logits, softmax statistics and sums in fp32, the weights
- * rounded to the activation dtype for their product with V.  A row that sees no key is 0; rows of q outside
- * [cu_q[0], cu_q[S]) are not written.  k and v may be NULL with Nk = 0.  Key strides below 2^23.  Any Hq that H
- * divides.  out may be q.  No workspace. */
+ * rounded to the activation dtype for their product with V.  A row that sees no key, or only keys whose logits are
+ * minus infinity, is 0; rows of q outside [cu_q[0], cu_q[S]) are not written.  k and v may be NULL with Nk = 0.  Key
+ * strides below 2^23.  Any Hq that H divides.  out may be q.  No workspace. */
 int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
                         const void* v, int64_t sv_n, int64_t sv_h, const int32_t* cu_q, const int32_t* cu_k, int S, int N,
                         int Nk, int Hq, int H, int D, int mode, float scale, int causal, int window, void* out,

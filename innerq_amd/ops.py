@@ -929,9 +929,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu_seqlens[s] .. cu_seqlens[s+1] (int32 [S+1] on the device, read by the kernel: a captured call follows its
     values) of q and, by cu_seqlens_k (default: the same), of k and v.  causal: a sequence's last row sees all its
     keys, each row before it one less (a chunk of a prompt behind its earlier keys has more keys than rows); window:
-    only the last ``window`` of the keys up to its own.  Rows that see no key are 0; rows outside the sequences are
-    not written.  ``out`` may be q, or memory that no other argument uses.  Inference only: tensors that autograd
-    follows are refused, ``out`` too."""
+    only the last ``window`` of the keys up to its own.  Rows that see no key, or only keys whose logits are minus
+    infinity, are 0; rows outside the sequences are not written.  ``out`` may be q, or memory that no other argument
+    uses.  Inference only: tensors that autograd follows are refused, ``out`` too."""
     fast = _native(q) if forward_ad._current_level < 0 else None
     if fast is not None:
         r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out)

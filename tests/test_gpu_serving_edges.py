@@ -246,3 +246,91 @@ def test_strides_of_one_length_and_of_one_page(front):
         st.attend(q, i32([[0, 1, 2], [0, 1, 2]]).t()[:, :2], lens, 0.1)
     with pytest.raises(ValueError, match="contiguous"):
         st.attend(q, table, i32([[2, 9], [2, 9], [2, 9]])[:, 0], 0.1)
+
+
+# ---- logits of minus infinity, and large finite ones -------------------------------------------------------------
+def check_rows(out, q, k, v, ends, low, scale, window=0):
+    """Row i of ``out`` [n, Hq, D] against attention in 64 bits over the keys below ends[i] (the last ``window`` of them)
+    that are not ``low``: those have weights of exactly 0, and where all are, the row is 0."""
+    got, low = out.cpu().double(), low.cpu()
+    q, k, v = q.cpu(), k.cpu(), v.cpu()
+    zeros = 0
+    for i, end in enumerate(ends):
+        keys = torch.arange(max(0, end - window) if window else 0, max(0, end))
+        keys = keys[~low[keys]]
+        if not len(keys):
+            assert bool((got[i] == 0).all()), i
+            zeros += 1
+            continue
+        want, bound = R.attention(q[i:i + 1], k[keys], v[keys], scale, causal=False)
+        assert bool(((got[i] - want[0]).abs() <= bound[0]).all()), i
+    return zeros
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [None, 3, 70])
+def test_prompt_keys_of_minus_infinity(dtype, D, window):
+    g = torch.Generator().manual_seed(D)
+    n = 200
+    q, k, v = randn(g, n, 2, D, dtype=dtype), randn(g, n, 1, D, dtype=dtype), randn(g, n, 1, D, dtype=dtype)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    low = torch.zeros(n, dtype=torch.bool)
+    low[:5] = low[40:50] = low[128:192] = True  # the first rows see nothing else; a whole tile of keys
+    k[low.to(DEV), 0, 3] = float("-inf")
+    out = ops.prompt_attention(q, k, v, i32([0, n]), 0.125, window=window)
+    assert check_rows(out, q, k, v, range(1, n + 1), low, 0.125, window or 0) >= 5
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("width", [2, 30])
+@pytest.mark.parametrize("window", [None, 2])
+def test_attend_logits_that_overflow_to_minus_infinity(D, width, window):
+    """(bf16: a page's finite keys and finite queries whose products pass fp32's range.)  Whole sequences and shares."""
+    g = torch.Generator().manual_seed(D + width)
+    lens, m, big = [5, 128, 70, 3], 3, 3e38
+    N, starts = sum(lens), [0, 5, 133, 203]
+    low = torch.zeros(N, dtype=torch.bool)
+    low[:3] = low[5:15] = low[5 + 64:5 + 128] = low[203:206] = True  # (sequence 3: every key; 0: all that its first row sees)
+    k, v = randn(g, N, 1, D, dtype=torch.bfloat16), randn(g, N, 1, D, dtype=torch.bfloat16)
+    q = randn(g, 4, m, 2, D, dtype=torch.bfloat16)
+    k[..., :32] = 0
+    k[low.to(DEV), :, :32] = big
+    q[..., :32] = -big
+    st = paged.PagedStore(4 * width, 1, D, DEV, torch.bfloat16)
+    table = torch.arange(4 * width, dtype=torch.int32, device=DEV).view(4, width)
+    st.append(k, v, table, i32([0] * 4), i32(starts + [N]))
+    kk, vv = st.read(table, i32([0] * 4), i32(starts + [N]), N)
+    assert torch.equal(kk[..., :32], k[..., :32])
+    out = st.attend(q, table, i32(lens), 0.125, window=window)
+    zeros = 0
+    for s, (a, n) in enumerate(zip(starts, lens)):
+        zeros += check_rows(out[s], q[s], kk[a:a + n], vv[a:a + n], [n - 2, n - 1, n], low[a:a + n], 0.125, window or 0)
+    assert zeros >= 4
+    st.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("width", [5, 30])
+def test_attend_large_finite_logits(dtype, D, width):
+    """Over pages that every row sees whole: one weight is 1, the rest 0."""
+    g = torch.Generator().manual_seed(D + width)
+    n, m, Hq = 300, 16, 4
+    k, v = randn(g, n, 1, D, dtype=dtype) * 300, randn(g, n, 1, D, dtype=dtype)
+    q = randn(g, 1, m, Hq, D, dtype=dtype) * 300
+    st = paged.PagedStore(width, 1, D, DEV, dtype)
+    table = torch.arange(width, dtype=torch.int32, device=DEV)[None]
+    st.append(k, v, table, i32([0]), i32([0, n]))
+    kk, vv = (x.cpu().double()[:, 0] for x in st.read(table, i32([0]), i32([0, n]), n))
+    out = st.attend(q, table, i32([n]), 1.0).cpu()[0]
+    assert bool(out.isfinite().all())
+    seen = torch.arange(n)[None] < n - (m - 1) + torch.arange(m)[:, None]
+    qq = q[0].cpu().double()
+    s = torch.matmul(qq, kk.T).masked_fill(~seen[:, None], -1e300)
+    size = torch.matmul(qq.abs(), kk.abs().T).amax(-1)
+    top = s.topk(2, -1).values
+    # a logit's sum of D products is off by at most (D + 8) 2^-24 of their absolute sum, on both sides; e^-100 is no weight
+    sure = top[..., 0] - top[..., 1] > 100 + 2 * (D + 8) * 2.0 ** -24 * size
+    assert int(sure.sum()) > 50
+    assert torch.equal(out[sure].double(), vv[s.argmax(-1)[sure]])
