@@ -2,7 +2,7 @@
 //
 // A page holds 64 tokens of every KV head, K and V both in 4-bit asym groups of 32 along head_dim, so a token is
 // whole in its page as soon as it is appended: sequences of any lengths append one token or many without an fp16
-// window, and no two tokens share a word.  One (page, head) is one run of 32-bit words (U = D/8, G = D/32):
+// window, and no two tokens share a word of codes.  One (page, head) is one run of 32-bit words (U = D/8, G = D/32):
 //
 //   K codes  [64 tokens][U]            a token's row: one 16-byte load per lane is one group (D = 128)
 //   K meta   [64 tokens][G]            {scale, zero} halves

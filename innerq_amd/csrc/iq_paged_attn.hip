@@ -14,8 +14,12 @@
 //
 // Bound (8 KV heads, 32 query heads, D = 128): long sequences in fp16 by HBM and the vector unit alike (8 of 32768
 // tokens: 336 MB in 63 us with the merge, 5.3 TB/s, where a large copy reaches 4.8; a wave spends about 1.3 us on a
-// page); in bf16 by the conversion of the codes (48 of 130 .. 16001 tokens: 78 us, in fp16 60 us); short ones by the
+// page); in bf16 by the conversion of the codes (48 of 130 .. 16001 tokens: 78 us, in fp16 62 us); short ones by the
 // loads that wait for each other, lengths, table, page (one sequence of 1000 tokens: 10.4 us, 3.5 the merging launch).
+//
+// The exponentials are rounded because the matrix unit's two operands have one type, that of V's values: each weight
+// moves by half a step at most, and its sum takes it unrounded (outputs' error 1.1 - 1.4 times that of fp32 weights,
+// against 64 bits).
 #include "iq_paged.h"
 
 using namespace iq;
@@ -375,8 +379,9 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, in
   *reinterpret_cast<u4_t*>(a.out + s * a.so_s + w.token * a.so_m + (int64_t(head) * a.nrep + w.head) * a.so_h + d) = x;
 }
 
-// workgroups per CU (registers: D = 128 with T = 2 would spill 209 of them at two; D = 64 spills 6, 31 in bf16, in
-// paths that are rarely taken, and is faster so: 48 of 1500 tokens, bf16, 26 us against 30)
+// workgroups per CU (registers: D = 128 with T = 2 would spill 209 of them at two.  Spilled as it is: D = 64 with T = 2 6
+// registers, 31 in bf16, and D = 128 with T = 1 in bf16 22, in the masked path and where a (sequence, head) begins and
+// ends; D = 64 is faster so: 48 of 1500 tokens, bf16, 26 us against 30)
 constexpr int per_cu(int D, int T) { return T == 1 || D == 64 ? 2 : 1; }
 
 template <int D, bool BF, int T>
@@ -657,6 +662,8 @@ struct Launch {
 //   of 1000 (P = 16)                 1: 12.1 / 10.6;  8: 12.3 / 12.4;  32: 13.7 / 20.3;  128: 36 / 40
 //   of 1500 (P = 24)                 8: 15.8 / 14.7;  16: 16.1 / 17.0;  32: 17.6 / 23.9;  128: 46 / 52
 //   of 4032 (P = 63)                64: 61 / 63, but of 50 .. 4096 tokens 48 / 36
+// The lengths are on the device, so the table's width P stands for them: a caller whose tables are wider than any sequence
+// passes the columns that are needed (16 sequences of 500 tokens: P = 8 8.2 us, P = 512 13.2; bf16 10.8, 16.7).
 inline Launch plan_of(int S, int P, int m, int nrep, int H, int D) {
   const int64_t rows = int64_t(m) * nrep, pages = int64_t(S) * H * P * ceil_div(rows, ROWS);
   Launch p;

@@ -5,13 +5,17 @@
 // 64, staged through LDS.  Both products run transposed on v_mfma_f32_32x32x16: S^T = K Q^T leaves a query row per lane
 // and its keys in the lane's registers, where the running softmax needs one exchange (with the lane of the other
 // half-wave) per tile, and the exponentials, rounded to the activation dtype, are the B operand of O^T += V^T P^T as
-// they are: V^T's A operand reads LDS with ds_read_b64_tr_b16 in the same order of keys.
+// they are: V^T's A operand reads LDS with ds_read_b64_tr_b16 in the same order of keys.  (Rounded, because the matrix
+// unit's two operands have one type, V's; a weight moves by half a step at most, and its sum takes it unrounded: outputs'
+// error 1.1 - 1.4 times that of fp32 weights, against 64 bits.)
 //
 // A tile holds the rows of all heads of a group, so short prompts fill tiles and stage their keys once (32 query heads
 // over 8, a tile per query head before: 128 prompts of 16 tokens 58 us, now 18; one of 77 11.8, now 8.0).
 // Bound: the matrix unit and the softmax's vector work, which two workgroups per CU overlap.  A prompt of 16384 tokens
 // (32 query, 8 KV heads, D = 128, bf16): 1.94 ms, 1130 TFLOP/s, where a 16384^3 bf16 library product reaches 1370; the
-// matrix unit is busy 60 % of the clocks, HBM moves 0.8 GB.  Short prompts wait for their first tile: 77 tokens 7.4 us.
+// matrix unit is busy 60 % of the clocks, HBM moves 0.8 GB.  With D = 64 there are half the products per exponential: the
+// vector unit is busy 79 % of the clocks, the matrix unit 50 % (1.11 - 1.18 ms, 930 - 990 TFLOP/s).  Short prompts wait for
+// their first tile: 77 tokens 7.4 us.
 #include "iq_paged.h"
 
 using namespace iq;

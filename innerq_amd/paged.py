@@ -227,8 +227,10 @@ class PagedStore:
                window: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """softmax(q K^T * scale) V over each sequence's first lens[s] tokens, the new ones among them.  q [S, Hq, D]
         (one new token) or [S, m, Hq, D] (m <= 16: token j sees all but the m - 1 - j after it); window: only the last
-        ``window`` tokens up to its own.  Rows that see no token, or only tokens whose logits are minus infinity, are 0.
-        Returns ``out`` (q itself, or memory that no other argument uses) or a new tensor of q's shape."""
+        ``window`` tokens up to its own.  The table's width plans the work: pass ``table[:, :pages that the longest
+        sequence needs]`` where tables are wider than any sequence.  Rows that see no token, or only tokens whose logits
+        are minus infinity, are 0.  Returns ``out`` (q itself, or memory that no other argument uses) or a new tensor of
+        q's shape."""
         fast = ops._native(q) if forward_ad._current_level < 0 else None
         if fast is not None:
             r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out)
