@@ -101,11 +101,12 @@ def readable_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def autograd_follows(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether autograd, backward or forward mode, follows what is computed from any of the tensors."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    """Whether autograd, backward or forward mode, follows what is computed from any of the tensors (what is none is for
+    the call's own checks to refuse)."""
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         return True
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                                  for t in tensors)
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _nested(dims, end: int) -> bool:

@@ -334,3 +334,12 @@ def test_attend_large_finite_logits(dtype, D, width):
     sure = top[..., 0] - top[..., 1] > 100 + 2 * (D + 8) * 2.0 ** -24 * size
     assert int(sure.sum()) > 50
     assert torch.equal(out[sure].double(), vv[s.argmax(-1)[sure]])
+
+
+def test_outputs_that_are_no_tensors_are_refused(front):
+    st = paged.PagedStore(2, 2, 64, DEV)
+    k, table, lens = torch.zeros(2, 2, 64, dtype=torch.float16, device=DEV), i32([[0], [1]]), i32([0, 0])
+    for call in (lambda: st.append(k, k, table, lens, q=k, q_out=5), lambda: st.attend(k, table, lens, 1.0, out=[k]),
+                 lambda: st.read(table, lens, None, 2, v_out=5), lambda: ops.prompt_attention(k, k, k, i32([0, 2]), 1.0, out=5)):
+        with pytest.raises(TypeError):
+            call()

@@ -53,3 +53,10 @@ def test_outputs_apart():
     for a, b in ((x, x), (x[:3], x[2:5]), (x[:, :4], x[:, 3:7]), (x[..., :64], x[..., 8:72]), (x[:, :4], x[:, :4]),
                  (x[:4, :4], x.view(-1)[64:].as_strided((4, 4, 128), (512, 128, 1)))):
         assert not ops.apart(a, b) and not ops.apart(b, a)
+
+
+def test_autograd_follows_tensors_only():
+    x = torch.zeros(3)
+    assert not ops.autograd_follows(None, x, 5, [x]) and ops.autograd_follows(None, 5, x.clone().requires_grad_())
+    with torch.no_grad():
+        assert not ops.autograd_follows(x.clone().requires_grad_())
