@@ -343,3 +343,32 @@ def test_outputs_that_are_no_tensors_are_refused(front):
                  lambda: st.read(table, lens, None, 2, v_out=5), lambda: ops.prompt_attention(k, k, k, i32([0, 2]), 1.0, out=5)):
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_queries_of_nan_stay_in_their_rows(dtype, D, bad):
+    """One head's query of one row: its output is NaN, the other rows' (of the same tiles) are right."""
+    g = torch.Generator().manual_seed(D)
+    Hq, n, m = 4, 150, 5
+    k, v = randn(g, n, 1, D, dtype=dtype), randn(g, n, 1, D, dtype=dtype)
+    q = randn(g, n, Hq, D, dtype=dtype)
+    q[3, 1, 0] = q[100, 2, D - 1] = bad
+    for causal, window in ((True, None), (True, 20), (False, None)):
+        out = ops.prompt_attention(q, k, v, i32([0, n]), 0.1, causal=causal, window=window).cpu().double()
+        want, bound = R.attention(q.cpu(), k.cpu(), v.cpu(), 0.1, causal, window or 0)
+        assert torch.equal(out.isnan().all(-1).nonzero(), torch.tensor([[3, 1], [100, 2]]))
+        fine = ~out.isnan()
+        assert int((~fine).sum()) == 2 * D and bool(((out - want).abs() <= bound)[fine].all())
+    for width in (3, 30):
+        st = paged.PagedStore(width, 1, D, DEV, dtype)
+        st.pages.fill_(-1)
+        table = torch.arange(width, dtype=torch.int32, device=DEV)[None]
+        st.append(k, v, table, i32([0]), i32([0, n]))
+        kk, vv = (x.cpu() for x in st.read(table, i32([0]), i32([0, n]), n))
+        out = st.attend(q[None, :m], table, i32([n]), 0.1).cpu().double()[0]
+        want, bound = R.attention(q[:m].cpu(), kk, vv, 0.1)
+        assert torch.equal(out.isnan().all(-1).nonzero(), torch.tensor([[3, 1]]))
+        fine = ~out.isnan()
+        assert int((~fine).sum()) == D and bool(((out - want).abs() <= bound)[fine].all())
