@@ -440,6 +440,28 @@ int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, const void* k, 
                     const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* q_out, int64_t so_n, int64_t so_h,
                     void* stream);
 
+/* iq_paged_append for sequences that have dropped tokens (iq_paged_evict): row lens[s] + i + evicted[s] of the rotation
+ * (int32 [S] on the device; NULL: 0) is token lens[s] + i's, where the checks above are of that row. */
+int iq_paged_append_at(const iq_paged* p, const int32_t* cu, int N, const void* k, int64_t sk_n, int64_t sk_h,
+                       const void* v, int64_t sv_n, int64_t sv_h, const float* cos, const float* sin, int64_t n_pos, int R,
+                       const int32_t* evicted, const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* q_out,
+                       int64_t so_n, int64_t so_h, void* stream);
+
+/* Sequences of more than `keep` tokens drop the others: every run of `shared` heads (H a multiple; heads of one run
+ * keep the same tokens, by the sum of their weights) keeps its last `recent` tokens, its first `sinks` ones and, of the
+ * others, those of most weight (equal ones: the first; NaN counts as most), keep in all.  With B = keep - recent: a kept
+ * token below B stays where it is, the places below B of dropped tokens are filled, in order, by the kept ones of
+ * [B, lens[s] - recent), and the last ones become tokens B .. keep - 1 in their order.  K, V and weights move together;
+ * rows from keep on are left as they are.  weights, weights_out: fp32 [S][H][T], T >= P * 64, contiguous in T; they may
+ * be one (with the same strides), or share no memory.  weights_out of a sequence that drops tokens is 0 from `keep` on,
+ * of another one weights as they are.  lens_out [S] (may be lens): keep, or lens[s] as it was.  A sequence that drops
+ * tokens must share none of its pages with another of the call.  A row that has to move from a page outside the pool
+ * becomes NaN.  workspace: iq_paged_evict_workspace_bytes, of this call alone while it runs. */
+size_t iq_paged_evict_workspace_bytes(int S, int P, int H, int keep, int recent, int shared);
+int iq_paged_evict(const iq_paged* p, const float* weights, int64_t sw_s, int64_t sw_h, float* weights_out, int64_t so_s,
+                   int64_t so_h, int64_t T, int keep, int recent, int sinks, int shared, int32_t* lens_out,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* The values of tokens lens[s] + i of every sequence (i < cu[s+1] - cu[s], as iq_paged_append), written to rows
  * cu[s] + i of k_out and v_out [N, H, D]; NaN for a token that the checks above refuse; rows outside [cu[0], cu[S])
  * are not written. */

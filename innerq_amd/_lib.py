@@ -117,6 +117,9 @@ SIGNATURES = {
     "iq_page_bytes": (I, [I, I, ctypes.POINTER(L)]),
     "iq_paged_take_status": (I, [P, P, P]),
     "iq_paged_append": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P, P, L, I, P, L, L, I, P, L, L, P]),
+    "iq_paged_append_at": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P, P, L, I, P, P, L, L, I, P, L, L, P]),
+    "iq_paged_evict_workspace_bytes": (S, [I, I, I, I, I, I]),
+    "iq_paged_evict": (I, [ctypes.POINTER(iq_paged), P, L, L, P, L, L, L, I, I, I, I, P, P, S, P]),
     "iq_paged_read": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P]),
     "iq_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I]),
     "iq_paged_attention": (I, [ctypes.POINTER(iq_paged), P, L, L, L, I, I, F, I, P, L, L, L, P, S, P]),

@@ -1,0 +1,335 @@
+// Dropping tokens from 4-bit pages by the attention weight that they have gathered (gfx950): iq_paged_evict.
+//
+// Of a sequence of n > keep tokens each KV head (or run of `shared` heads) keeps its last `recent` tokens and, of the
+// others, the `sinks` first ones and those of most weight.  Attention does not ask for the order of a cache's rows, so
+// only the rows that have to move do: with B = keep - recent, a kept token below B stays; the places below B that a
+// dropped token leaves are filled, in order, by the kept ones from B on; the last `recent` tokens move down to B .. keep.
+// A step that drops a page of 64 tokens from 2048 moves some 60 rows and the recent ones, where keeping the order would
+// move all of them.
+//
+// Three launches, one behind the other (each reads what the next one writes over):
+//   select  one workgroup per (sequence, run of heads): the B-th largest weight by three passes over the bits of the
+//           weights (11, 11, 10 from the top), then the lists of free places and of the rows that come; moves the weights.
+//   fill    rows into the free places: sources from B on, destinations below B, in any order.
+//   shift   the last `recent` rows, which may overlap their destinations: one workgroup per (sequence, head), in order,
+//           each batch read whole before it is written.
+#include "iq_paged.h"
+
+using namespace iq;
+
+namespace {
+
+constexpr int SELECT = 1024, FILL = 256, SHIFT = 1024;
+constexpr int BATCH = 4;                        // rows (or weights) of a lane that are under way together
+constexpr int BITS[3] = {11, 11, 10}, BINS = 1 << 11;
+
+struct EvictArgs {
+  iq_paged p;
+  const float* w;
+  int64_t sw_s, sw_h;
+  float* wo;
+  int64_t so_s, so_h, T;
+  int keep, recent, sinks, shared, most;  // most: rows that can come, at most
+  int32_t* lens_out;
+  int32_t* ws;
+  int chunks;  // of FILL rows per (sequence, head)
+};
+
+// a (sequence, run of heads)'s part of the workspace: its tokens if it drops any (else 0), the rows that come, the free
+// places, the rows
+__device__ __forceinline__ int32_t* plan_of(const EvictArgs& a, int64_t run) { return a.ws + run * (2 + 2 * int64_t(a.most)); }
+
+// inclusive sum over the workgroup; `total` the whole sum
+__device__ __forceinline__ int group_scan(int v, int& total) {
+  __shared__ int part[SELECT / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int x = wave_scan(v);
+  __syncthreads();  // (nobody reads the last call's sums any more)
+  if (lane == 63) part[wave] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < SELECT / 64; ++i) {
+    const int y = part[i];
+    if (i < wave) before += y;
+    total += y;
+  }
+  return before + x;
+}
+
+// every thread of the workgroup has what it has read in registers: what it read may be written over
+__device__ __forceinline__ void all_read() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
+  __shared__ int hist[BINS];
+  __shared__ int found[3];  // the digit, how many of its keys are wanted, how many there are
+  const int runs = a.p.H / a.shared, s = blockIdx.x / runs, h0 = (blockIdx.x - s * runs) * a.shared, tid = threadIdx.x;
+  const float* w = a.w + s * a.sw_s + h0 * a.sw_h;
+  float* wo = a.wo + s * a.so_s + h0 * a.so_h;
+  int32_t* plan = plan_of(a, blockIdx.x);
+  const int n = a.p.lens[s];
+  const bool there = n >= 0 && n <= int64_t(a.p.P) * PAGE;
+  if (!there && tid == 0) atomicOr(a.p.status, PAGED_BAD_TOKEN);
+  if (!there || n <= a.keep) {
+    if (tid == 0) plan[0] = plan[1] = 0;
+    if (a.wo != a.w)
+      for (int h = 0; h < a.shared; ++h)
+        for (int64_t i = tid; i < a.T; i += SELECT) wo[h * a.so_h + i] = w[h * a.sw_h + i];
+    return;
+  }
+  const int old = n - a.recent, B = a.keep - a.recent;  // B of the first `old` tokens stay
+  // Weights as whole numbers of the same order: NaN above all, -0 as 0.  The sinks are above all too, and come first.
+  auto key_of = [&](int i) {
+    float x = w[i] + 0.f;
+    for (int h = 1; h < a.shared; ++h) x += w[h * a.sw_h + i];
+    const uint32_t b = __float_as_uint(x);
+    return i < a.sinks || x != x ? ~0u : b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+  };
+  uint32_t least = 0;  // the B-th largest key
+  int cut = old;       // of the keys equal to it, those of tokens below `cut` stay
+  if (B > 0) {
+    uint32_t mask = 0;
+    int want = B;
+    for (int pass = 0, low = 32; pass < 3; ++pass) {
+      const int bits = BITS[pass];
+      low -= bits;
+      for (int i = tid; i < BINS; i += SELECT) hist[i] = 0;
+      __syncthreads();
+      for (int i0 = tid; i0 < old; i0 += SELECT * BATCH) {
+        uint32_t k[BATCH];
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) k[e] = key_of(min(i0 + e * SELECT, old - 1));
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e)
+          if (i0 + e * SELECT < old && (k[e] & mask) == least) atomicAdd(&hist[k[e] >> low & ((1u << bits) - 1)], 1);
+      }
+      __syncthreads();
+      const int hi = BINS - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1];
+      int total;
+      const int end = group_scan(c0 + c1, total), before = end - c0 - c1;
+      if (before < want && want <= end) {
+        const bool second = before + c0 < want;
+        found[0] = second ? hi - 1 : hi;
+        found[1] = second ? want - before - c0 : want - before;
+        found[2] = second ? c1 : c0;
+      }
+      __syncthreads();
+      least |= uint32_t(found[0]) << low;
+      mask |= ((1u << bits) - 1) << low;
+      want = found[1];
+    }
+    if (want < found[2]) {  // ties: the first ones stay
+      __syncthreads();
+      for (int i0 = 0, seen = 0; i0 < old && seen < want; i0 += SELECT) {
+        const int i = i0 + tid, tie = i < old && key_of(i) == least;
+        int total;
+        const int rank = seen + group_scan(tie, total);
+        if (tie && rank == want) found[0] = i + 1;
+        seen += total;
+      }
+      __syncthreads();
+      cut = found[0];
+    }
+  }
+  auto stays = [&](int i) {
+    const uint32_t k = key_of(i);
+    return B > 0 && (k > least || (k == least && i < cut));
+  };
+  // the places below B that become free, and the tokens from B on that stay: as many
+  int count = 0;
+  for (int list = 0; list < 2; ++list) {
+    const int begin = list ? B : 0, end = list ? old : B;
+    int32_t* to = plan + 2 + list * int64_t(a.most);
+    count = 0;
+    for (int i0 = begin; i0 < end; i0 += SELECT * BATCH) {
+      const int first = i0 + tid * BATCH;
+      bool in[BATCH];
+      int mine = 0;
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        in[e] = first + e < end && stays(min(first + e, end - 1)) == (list == 1);
+        mine += in[e];
+      }
+      int total, at = count + group_scan(mine, total) - mine;
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e)
+        if (in[e]) to[at++] = first + e;
+      count += total;
+    }
+  }
+  if (tid == 0) {
+    plan[0] = n;
+    plan[1] = count;
+  }
+  // the weights go where their rows go
+  for (int h = 0; h < a.shared; ++h) {
+    const float* x = w + h * a.sw_h;
+    float* y = wo + h * a.so_h;
+    if (a.wo != a.w)
+      for (int i = tid; i < B; i += SELECT) y[i] = x[i];
+    __syncthreads();
+    for (int i = tid; i < count; i += SELECT) y[plan[2 + i]] = x[plan[2 + int64_t(a.most) + i]];
+    for (int i0 = 0; i0 < a.recent; i0 += SELECT) {
+      const int i = i0 + tid;
+      const float v = i < a.recent ? x[old + i] : 0.f;
+      all_read();  // (wo may be w)
+      if (i < a.recent) y[B + i] = v;
+    }
+    all_read();
+    for (int64_t i = a.keep + tid; i < a.T; i += SELECT) y[i] = 0.f;
+  }
+}
+
+// A lane's share of one token's row of one head: word o of K and V, and for o % 4 == 0 their group's scales and zeros.
+struct Piece {
+  uint32_t k, v, km;
+  uint16_t vs, vz;
+};
+template <int D>
+__device__ __forceinline__ Piece load_piece(const uint32_t* pg, int row, int o) {
+  constexpr int U = D / 8, G = D / 32;
+  const int b = v_block(row), e = v_place(row);
+  Piece x{pg[row * U + o], pg[page_vc(D) + (b * U + o) * 8 + e], 0, 0, 0};
+  if (o % 4 == 0) {
+    const uint16_t* m = reinterpret_cast<const uint16_t*>(pg + page_vm(D)) + (b * G + o / 4) * 16 + e;
+    x.km = pg[page_km(D) + row * G + o / 4];
+    x.vs = m[0];
+    x.vz = m[8];
+  }
+  return x;
+}
+template <int D>
+__device__ __forceinline__ void store_piece(uint32_t* pg, int row, int o, const Piece& x) {
+  constexpr int U = D / 8, G = D / 32;
+  const int b = v_block(row), e = v_place(row);
+  pg[row * U + o] = x.k;
+  pg[page_vc(D) + (b * U + o) * 8 + e] = x.v;
+  if (o % 4 == 0) {
+    uint16_t* m = reinterpret_cast<uint16_t*>(pg + page_vm(D)) + (b * G + o / 4) * 16 + e;
+    pg[page_km(D) + row * G + o / 4] = x.km;
+    m[0] = x.vs;
+    m[8] = x.vz;
+  }
+}
+
+// token t's page of head h, null if the table names none of the pool
+template <int D>
+__device__ __forceinline__ uint32_t* page_of(const EvictArgs& a, int s, int h, int t) {
+  const int id = a.p.table[s * a.p.s_table + t / PAGE];
+  return id < 0 || id >= a.p.n_pages ? nullptr : a.p.pages + (int64_t(id) * a.p.H + h) * page_words(D);
+}
+
+// BATCH rows of a lane from tokens `from` to `to` (from < 0: none): reads all, calls `between`, writes all.  A row whose
+// page is missing is not read and becomes NaN; one whose place has no page is not written.
+template <int D, typename F>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int s, int h, int o, const int (&from)[BATCH],
+                                          const int (&to)[BATCH], F&& between) {
+  constexpr uint16_t nan = 0x7fff;  // of both activation dtypes
+  const uint32_t* src[BATCH];
+  uint32_t* dst[BATCH];
+  Piece x[BATCH];
+#pragma unroll
+  for (int e = 0; e < BATCH; ++e) {
+    src[e] = from[e] < 0 ? nullptr : page_of<D>(a, s, h, from[e]);
+    dst[e] = from[e] < 0 ? nullptr : page_of<D>(a, s, h, to[e]);
+    if (from[e] >= 0 && (!src[e] || !dst[e]) && o == 0) atomicOr(a.p.status, PAGED_BAD_PAGE);
+  }
+#pragma unroll
+  for (int e = 0; e < BATCH; ++e)
+    x[e] = src[e] ? load_piece<D>(src[e], from[e] % PAGE, o) : Piece{0, 0, nan | uint32_t(nan) << 16, nan, nan};
+  between();
+#pragma unroll
+  for (int e = 0; e < BATCH; ++e)
+    if (dst[e]) store_piece<D>(dst[e], to[e] % PAGE, o, x[e]);
+}
+
+template <int D>
+__global__ __launch_bounds__(FILL) void fill_kernel(EvictArgs a) {
+  constexpr int U = D / 8, ROWS = FILL / U * BATCH;  // rows of a workgroup's turn
+  const int sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.p.H, h = sh - s * a.p.H;
+  const int32_t* plan = plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared);
+  const int o = threadIdx.x % U, count = plan[1];
+  if (h == 0 && chunk == 0 && threadIdx.x == 0) a.lens_out[s] = plan[0] ? a.keep : a.p.lens[s];
+  for (int r0 = chunk * ROWS + threadIdx.x / U; r0 < count; r0 += a.chunks * ROWS) {
+    int from[BATCH], to[BATCH];
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) {
+      const int r = r0 + e * (FILL / U);
+      to[e] = plan[2 + min(r, count - 1)];
+      from[e] = r < count ? plan[2 + int64_t(a.most) + r] : -1;
+    }
+    move_rows<D>(a, s, h, o, from, to, [] {});
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(SHIFT) void shift_kernel(EvictArgs a) {
+  constexpr int U = D / 8, ROWS = SHIFT / U * BATCH;
+  const int s = blockIdx.x / a.p.H, h = blockIdx.x - s * a.p.H, o = threadIdx.x % U;
+  const int n = plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared)[0];
+  if (!n) return;
+  for (int r0 = 0; r0 < a.recent; r0 += ROWS) {
+    int from[BATCH], to[BATCH];
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) {
+      const int r = r0 + e * (SHIFT / U) + threadIdx.x / U;
+      from[e] = r < a.recent ? n - a.recent + r : -1;
+      to[e] = a.keep - a.recent + min(r, a.recent - 1);
+    }
+    move_rows<D>(a, s, h, o, from, to, [] { all_read(); });
+  }
+}
+
+inline int64_t rows_that_come(int P, int keep, int recent) {
+  const int64_t past = int64_t(P) * PAGE - keep;
+  return past <= 0 ? 0 : past < keep - recent ? past : keep - recent;
+}
+
+}  // namespace
+
+namespace iq {
+int check_paged(const iq_paged* p);
+}
+
+extern "C" size_t iq_paged_evict_workspace_bytes(int S, int P, int H, int keep, int recent, int shared) {
+  if (S <= 0 || P <= 0 || H <= 0 || keep <= 0 || recent < 0 || recent > keep || shared <= 0 || H % shared) return 0;
+  return size_t(S) * (H / shared) * size_t(2 + 2 * rows_that_come(P, keep, recent)) * sizeof(int32_t);
+}
+
+extern "C" int iq_paged_evict(const iq_paged* p, const float* weights, int64_t sw_s, int64_t sw_h, float* weights_out,
+                              int64_t so_s, int64_t so_h, int64_t T, int keep, int recent, int sinks, int shared,
+                              int32_t* lens_out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int st = iq::check_paged(p)) return st;
+  IQ_CHECK(weights && weights_out && lens_out, IQ_ERR_NULL);
+  IQ_CHECK(keep > 0 && recent >= 0 && sinks >= 0 && int64_t(recent) + sinks <= keep, IQ_ERR_SHAPE);
+  IQ_CHECK(shared > 0 && p->H % shared == 0 && T >= int64_t(p->P) * PAGE, IQ_ERR_SHAPE);
+  IQ_CHECK(sw_s >= 0 && sw_h >= 0 && so_s >= 0 && so_h >= 0, IQ_ERR_SHAPE);
+  IQ_CHECK(weights != weights_out || (sw_s == so_s && sw_h == so_h), IQ_ERR_SHAPE);
+  IQ_CHECK(int64_t(p->S) * p->H <= INT32_MAX / SHIFT && p->P < INT32_MAX / PAGE - SELECT, IQ_ERR_SHAPE);
+  IQ_CHECK(aligned(weights, 4) && aligned(weights_out, 4) && aligned(lens_out, 4), IQ_ERR_ALIGN);
+  const size_t need = iq_paged_evict_workspace_bytes(p->S, p->P, p->H, keep, recent, shared);
+  IQ_CHECK(workspace && workspace_bytes >= need, IQ_ERR_WORKSPACE);
+  IQ_CHECK(aligned(workspace, 4), IQ_ERR_ALIGN);
+  const int64_t most = rows_that_come(p->P, keep, recent);
+  // at most 8192 workgroups fill: a longer list is taken in turns
+  const int64_t sh = int64_t(p->S) * p->H, rows = FILL / (p->D / 8) * BATCH, turns = sh < 8192 ? 8192 / sh : 1;
+  int64_t chunks = ceil_div(most, rows);
+  chunks = chunks < 1 ? 1 : chunks < turns ? chunks : turns;
+  const EvictArgs a{*p, weights, sw_s, sw_h, weights_out, so_s, so_h, T, keep, recent, sinks, shared, int(most), lens_out,
+                    (int32_t*)workspace, int(chunks)};
+  const hipStream_t q = (hipStream_t)stream;
+  select_kernel<<<p->S * (p->H / shared), SELECT, 0, q>>>(a);
+  if (const int st = launch_status()) return st;
+  auto rest = [&]<int D>() {
+    fill_kernel<D><<<unsigned(sh * chunks), FILL, 0, q>>>(a);
+    if (const int st = launch_status()) return st;
+    if (!recent || int64_t(p->P) * PAGE <= keep) return int(IQ_OK);
+    shift_kernel<D><<<unsigned(sh), SHIFT, 0, q>>>(a);
+    return launch_status();
+  };
+  return p->D == 128 ? rest.operator()<128>() : rest.operator()<64>();
+}

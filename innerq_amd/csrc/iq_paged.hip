@@ -26,6 +26,7 @@ struct AppendArgs {
   const float *cos, *sin;
   int64_t n_pos;
   int R;
+  const int32_t* evicted;  // tokens that each sequence has dropped (null: none): what its places are behind its positions
 };
 
 template <bool BF>
@@ -135,6 +136,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a, int heads
   const int held = a.p.lens[s];
   const int64_t at = int64_t(held) + i;
   const int H = a.p.H, heads = 2 * H + (a.q ? a.Hq : 0);
+  const int64_t pos = at + (a.evicted ? a.evicted[s] : 0);
   int32_t bad = 0, page = -1;
   if (held < 0 || at >= int64_t(a.p.P) * PAGE) bad = PAGED_BAD_TOKEN;
   else {
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a, int heads
       bad = PAGED_BAD_PAGE;
       page = -1;
     }
-    if (a.cos && at >= a.n_pos) bad |= PAGED_BAD_TOKEN;
+    if (a.cos && (pos < 0 || pos >= a.n_pos)) bad |= PAGED_BAD_TOKEN;
   }
   const int row = int(at % PAGE);
   if (bad) {
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a, int heads
   const bool turn = a.cos && 8 * o < a.R, second = 16 * o >= a.R;
   float c[8], sn[8];
   if (turn) {
-    const int64_t d = at * (a.R / 2) + 8 * o - (second ? a.R / 2 : 0);
+    const int64_t d = pos * (a.R / 2) + 8 * o - (second ? a.R / 2 : 0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const f4_t x = *reinterpret_cast<const f4_t*>(a.cos + d + 4 * j), y = *reinterpret_cast<const f4_t*>(a.sin + d + 4 * j);
@@ -324,6 +326,14 @@ extern "C" int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, cons
                                const void* v, int64_t sv_n, int64_t sv_h, const float* cos, const float* sin,
                                int64_t n_pos, int R, const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* q_out,
                                int64_t so_n, int64_t so_h, void* stream) {
+  return iq_paged_append_at(p, cu, N, k, sk_n, sk_h, v, sv_n, sv_h, cos, sin, n_pos, R, nullptr, q, sq_n, sq_h, Hq, q_out, so_n,
+                            so_h, stream);
+}
+
+extern "C" int iq_paged_append_at(const iq_paged* p, const int32_t* cu, int N, const void* k, int64_t sk_n, int64_t sk_h,
+                                  const void* v, int64_t sv_n, int64_t sv_h, const float* cos, const float* sin,
+                                  int64_t n_pos, int R, const int32_t* evicted, const void* q, int64_t sq_n, int64_t sq_h,
+                                  int Hq, void* q_out, int64_t so_n, int64_t so_h, void* stream) {
   if (const int st = iq::check_paged(p)) return st;
   IQ_CHECK((N == 0 || (k && v && (!q || q_out))) && (!cos == !sin), IQ_ERR_NULL);
   IQ_CHECK(N >= 0 && N <= MOST_TOKENS && (cu || N == p->S), IQ_ERR_SHAPE);
@@ -331,9 +341,10 @@ extern "C" int iq_paged_append(const iq_paged* p, const int32_t* cu, int N, cons
   IQ_CHECK(!cos || (R > 0 && R <= p->D && R % 16 == 0 && n_pos > 0), IQ_ERR_SHAPE);
   IQ_CHECK(rows_ok(k, sk_n, sk_h) && rows_ok(v, sv_n, sv_h) && aligned(cos, 16) && aligned(sin, 16), IQ_ERR_ALIGN);
   IQ_CHECK(!q || (rows_ok(q, sq_n, sq_h) && rows_ok(q_out, so_n, so_h)), IQ_ERR_ALIGN);
+  IQ_CHECK(aligned(evicted, 4), IQ_ERR_ALIGN);
   if (N == 0) return IQ_OK;
   const AppendArgs a{*p, cu, N, Hq, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)q, sk_n, sk_h, sv_n, sv_h,
-                     sq_n, sq_h, (uint16_t*)q_out, so_n, so_h, cos, sin, n_pos, R};
+                     sq_n, sq_h, (uint16_t*)q_out, so_n, so_h, cos, sin, n_pos, R, evicted};
   return by_format(p->D, p->mode, [&]<int D, bool BF>() {
     const int tiles = int(ceil_div(N, THREADS / (D / 8))), heads = 2 * p->H + (q ? Hq : 0);
     const int hpb = heads_per_block(tiles, heads, 768, 16);

@@ -139,19 +139,27 @@ class PagedStore:
             return None
         return ops.check_cu(cu, "cu_seqlens", S, self.device)
 
+    def _ints(self, t: torch.Tensor, name: str, S: int) -> torch.Tensor:
+        ops.require_device(t, name, torch.int32)
+        if t.dim() != 1 or t.shape[0] != S or t.device != self.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 [{S}] tensor on {self.device}, got {tuple(t.shape)} on "
+                             f"{t.device}")
+        return t
+
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
                cu_seqlens: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
                sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
-               q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+               q_out: Optional[torch.Tensor] = None, evicted: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """Appends k and v [N, H, D]: rows cu_seqlens[s] .. cu_seqlens[s+1] (int32 [S+1]; None: one row per sequence)
         become tokens lens[s], lens[s] + 1, ... of sequence s (lens: tokens held before the call, which it leaves as
         they are).  cos, sin: fp32 [positions, R/2]; the first R dims of each key and query are rotated by their
-        token's row (pairs d, d + R/2).  Returns q [N, Hq, D] rotated, written to ``q_out`` (q itself, or memory that no
+        token's row (pairs d, d + R/2): row lens[s] + i, or lens[s] + i + evicted[s] (int32 [S] on the device) in sequences
+        that have dropped tokens (evict()).  Returns q [N, Hq, D] rotated, written to ``q_out`` (q itself, or memory that no
         other argument uses) or a new tensor; None without q.  Rows outside the sequences are neither appended nor
         written to q_out.  A token that cannot be appended (check()) has NaN queries, and one that only the rotation has
         no row for NaN in its page, so that read() and attend() give NaN.  Sequences that append must not share the
         pages they append to."""
-        fast = ops._native(k) if forward_ad._current_level < 0 else None
+        fast = ops._native(k) if forward_ad._current_level < 0 and evicted is None else None
         if fast is not None:
             r = fast.paged_append(self.pages, self.D, self.dtype, self.status, table, lens, k, v, cu_seqlens, cos, sin, q,
                                   q_out)
@@ -178,6 +186,10 @@ class PagedStore:
             if R % 16 or not 0 < R <= self.D or not n_pos:
                 raise ValueError(f"append: the rotation covers R dims, a multiple of 16 up to {self.D}, got {R} "
                                  f"({n_pos} positions)")
+        if evicted is not None:
+            if cos is None:
+                raise ValueError("append: evicted without a rotation")
+            self._ints(evicted, "evicted", p.S)
         Hq, qs, qos = 0, (0, 0), (0, 0)
         if q is not None:
             if q.dim() != 3 or q.shape[1] == 0:
@@ -192,8 +204,8 @@ class PagedStore:
         elif q_out is not None:
             raise ValueError("append: q_out without q")
         with ops.on_device(self.device):
-            call("iq_paged_append", ctypes.byref(p), ops._p(cu), N, ops._p(k), k.stride(0), k.stride(1), ops._p(v),
-                 v.stride(0), v.stride(1), ops._p(cos), ops._p(sin), n_pos, R, ops._p(q), qs[0], qs[1], Hq,
+            call("iq_paged_append_at", ctypes.byref(p), ops._p(cu), N, ops._p(k), k.stride(0), k.stride(1), ops._p(v),
+                 v.stride(0), v.stride(1), ops._p(cos), ops._p(sin), n_pos, R, ops._p(evicted), ops._p(q), qs[0], qs[1], Hq,
                  ops._p(q_out), qos[0], qos[1], ops._stream(self.device))
         return q_out
 
@@ -261,3 +273,49 @@ class PagedStore:
             call("iq_paged_attention", ctypes.byref(p), ops._p(q), qs[0], qs[1], qs[2], m, Hq, float(scale), window or 0,
                  ops._p(out), os[0], os[1], os[2], ops._p(ws), nbytes, ops._stream(self.device))
         return out
+
+    def evict(self, table: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor, keep: int, recent: int = 0,
+              sinks: int = 0, shared: int = 1, out: Optional[torch.Tensor] = None,
+              lens_out: Optional[torch.Tensor] = None):
+        """Cuts sequences of more than ``keep`` tokens down to ``keep``, by the attention weight that their tokens have
+        gathered: weights [S, H, T], fp32, T at least the table's P * 64, as ``attend`` and ops.prompt_attention add it
+        up.  Each KV head keeps the sequence's last ``recent`` tokens and, of the others, the first ``sinks`` and those of
+        most weight (of equal ones the first; NaN counts as most); with shared > 1, every run of ``shared`` heads keeps the
+        same tokens, by the sum of their weights (2: the two maps of diff_attend()).
+
+        The kept tokens become the sequence's first ``keep``: the last ones its last, in their order, and of the others
+        those below keep - recent stay where they are, while the rest fill, in order, the places that dropped ones leave.
+        Pages from ceil(keep / 64) on are free then; their rows are left as they are.  A sequence that drops tokens must
+        share none of its pages with another one.
+
+        Returns (lens, weights) of what is kept: lens_out (lens itself, memory of its own, or a new tensor) and ``out``
+        (weights itself, memory that no other argument uses, or a new tensor), 0 from ``keep`` on where tokens were
+        dropped.  A sequence of a bad length is left as it is, a row that has to move from a page outside the pool becomes
+        NaN (check())."""
+        _no_grad(weights, out)
+        p = self._args(table, lens)
+        keep, recent, sinks, shared = (int(x) for x in (keep, recent, sinks, shared))
+        if not 0 < keep < 2 ** 31 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError(f"evict: keep > 0 tokens, the recent ones and the sinks among them, got keep={keep}, "
+                             f"recent={recent}, sinks={sinks}")
+        if shared <= 0 or self.H % shared:
+            raise ValueError(f"evict: {self.H} heads are no runs of {shared}")
+        ops.check_weights(weights, "weights", p.S, self.H, p.P * PAGE_TOKENS, self.device)
+        if out is None:
+            out = torch.empty(weights.shape, dtype=torch.float32, device=self.device)
+        else:
+            ops.check_weights(out, "out", p.S, self.H, p.P * PAGE_TOKENS, self.device, written=True)
+            ops.check_out(out.shape, weights.shape)
+            if (out.data_ptr() != weights.data_ptr() or out.stride() != weights.stride()) and not ops.apart(out, weights):
+                raise ValueError("evict: out is weights itself or shares no memory with it")
+        if lens_out is None:
+            lens_out = torch.empty_like(lens)
+        elif self._ints(lens_out, "lens_out", p.S).data_ptr() != lens.data_ptr() and not ops.apart(lens_out, lens):
+            raise ValueError("evict: lens_out is lens itself or shares no memory with it")
+        nbytes = _lib.lib().iq_paged_evict_workspace_bytes(p.S, p.P, p.H, keep, recent, shared)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        with ops.on_device(self.device):
+            call("iq_paged_evict", ctypes.byref(p), ops._p(weights), weights.stride(0), weights.stride(1), ops._p(out),
+                 out.stride(0), out.stride(1), weights.shape[2], keep, recent, sinks, shared, ops._p(lens_out), ops._p(ws),
+                 nbytes, ops._stream(self.device))
+        return lens_out, out
