@@ -479,6 +479,17 @@ int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t s
                        float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* iq_paged_attention of one new token per sequence (q, out [S, Hq, D]) that also adds each token's softmax weights, summed
+ * over the query heads of its KV head, to weights, fp32 [S][H][T], T >= P * 64, contiguous in T: weights[s][h][j] grows by
+ * the fp32 weights of token j.  Tokens that the row does not see, and places behind the sequence's end, are left as they
+ * are; a row whose output is NaN gives NaN to all it might have seen, one that is 0 (no key that counts) gives 0.  Rows are
+ * added in a fixed order.  The workspace holds the logits: 4 bytes per query head and place of the table, beside
+ * iq_paged_attention's. */
+size_t iq_paged_attention_weights_workspace_bytes(int S, int P, int Hq, int H, int D);
+int iq_paged_attention_weights(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_h, int Hq, float scale, int window,
+                               void* out, int64_t so_s, int64_t so_h, float* weights, int64_t sw_s, int64_t sw_h, int64_t T,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 /* softmax(q K^T scale) V of S prompts that lie one behind the other: q, out [N, Hq, D], k, v [Nk, H, D] (fp16, or
  * bf16 with mode IQ_MODE_BF16; strides in elements, multiples of 8; D contiguous, 16-byte aligned).  Rows [cu_q[s],
  * cu_q[s+1]) attend to keys [cu_k[s], cu_k[s+1]) (int32 [S+1] on the device, non-decreasing; bounds outside [0, N] or

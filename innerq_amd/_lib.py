@@ -123,6 +123,8 @@ SIGNATURES = {
     "iq_paged_read": (I, [ctypes.POINTER(iq_paged), P, I, P, L, L, P, L, L, P]),
     "iq_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I]),
     "iq_paged_attention": (I, [ctypes.POINTER(iq_paged), P, L, L, L, I, I, F, I, P, L, L, L, P, S, P]),
+    "iq_paged_attention_weights_workspace_bytes": (S, [I, I, I, I, I]),
+    "iq_paged_attention_weights": (I, [ctypes.POINTER(iq_paged), P, L, L, I, F, I, P, L, L, P, L, L, L, P, S, P]),
     "iq_prompt_attention": (I, [P, L, L, P, L, L, P, L, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P]),
     "iq_decode_noalloc_max_bytes": (S, []),
     "iq_decode_attention_noalloc": (I, [P, L, L, P, ctypes.POINTER(iq_segment), ctypes.POINTER(iq_segment),

@@ -46,6 +46,12 @@ struct AttnArgs {
   float* ws;
   int each;            // sequences per lane where a wave adds up their pages (Part)
   int split;           // 0: a workgroup takes a whole (sequence, head, tile)
+  // where the keys' weights are wanted (m = 1): the logits [S][H][P][nrep][64], {maximum, 1 / sum} of each row
+  // [S][H][nrep], and the weights to add to, fp32 [S][H][>= 64 P]
+  float* logits;
+  float2* stats;
+  float* weights;
+  int64_t sw_s, sw_h;
 };
 
 // pages that sequence s reads: [lo, lo + n)
@@ -384,7 +390,14 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, in
 // ends; D = 64 is faster so: 48 of 1500 tokens, bf16, 26 us against 30)
 constexpr int per_cu(int D, int T) { return T == 1 || D == 64 ? 2 : 1; }
 
-template <int D, bool BF, int T>
+// a row's softmax, for the keys' weights: {maximum, 1 / sum}; a row without a sum gives weights of 0
+__device__ __forceinline__ void store_stats(const AttnArgs& a, int s, int head, int r, float mx, float sum) {
+  if (r < a.nrep)
+    a.stats[(int64_t(s) * a.p.H + head) * a.nrep + r] = float2{mx == NEG_INF ? 0.f : mx, sum == 0.f ? 0.f : 1.f / sum};
+}
+
+// W: the logits and the rows' sums are kept, for weights_kernel
+template <int D, bool BF, int T, bool W>
 __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a) {
   constexpr int J = D / 16, R = ROWS * T;
   __shared__ float so[WAVES][R][D + 4];
@@ -511,6 +524,16 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
               if (k >= lim[g] || k < low[g]) w[g][t][e] = NEG_INF;
             }
       }
+      if constexpr (W) {
+#pragma unroll
+        for (int g = 0; g < T; ++g) {
+          const int r = tile * R + ROWS * g + l;
+          float* to = a.logits + (((int64_t(s) * H + head) * a.p.P + tok0 / PAGE) * a.nrep + r) * PAGE + quarter * 4;
+          if (r < a.nrep)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) *reinterpret_cast<f4_t*>(to + t * 16) = w[g][t];
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < T; ++g) weights<D, BF>(w[g], acc[g]);
@@ -556,6 +579,8 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
       }
       if (whole) {
         store_row<D, BF, T>(a, s, head, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+        if constexpr (W)
+          if (d == 0) store_stats(a, s, head, tile * R + rr, mx, sum);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) slot[rr * D + d + e] = v[e];
@@ -574,7 +599,7 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
 }
 
 // one workgroup per (sequence, head, tile): merges the slots of those that several workgroups computed, in order
-template <int D, bool BF, int T>
+template <int D, bool BF, int T, bool W>
 __global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a) {
   constexpr int R = ROWS * T;
   const int per_seq = a.p.H * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
@@ -644,6 +669,32 @@ __global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a)
   }
   if (part_i > 0) return;
   store_row<D, BF, T>(a, s, hr / a.tiles, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+  if constexpr (W)
+    if (d == 0) store_stats(a, s, hr / a.tiles, tile * R + rr, mx, sum);
+}
+
+// Adds each key's softmax weights, over a KV head's query rows, to what it has gathered: from the logits that attn_kernel
+// has kept, a wave a page, a lane a key.  Rows are added in their order.
+constexpr int WEIGH_PAGES = 4;  // of a wave
+__global__ __launch_bounds__(THREADS) void weights_kernel(AttnArgs a, int chunks) {
+  const int sh = blockIdx.x / chunks, s = sh / a.p.H, head = sh - s * a.p.H, lane = threadIdx.x & 63;
+  const int len = min(a.p.lens[s], a.p.P * PAGE);
+  int lo;
+  const int n = pages_of(a, s, lo);
+  const float2* st = a.stats + int64_t(sh) * a.nrep;
+  const int first = lo + (blockIdx.x - sh * chunks) * (WAVES * WEIGH_PAGES) + (threadIdx.x >> 6);
+#pragma unroll
+  for (int i = 0; i < WEIGH_PAGES; ++i) {
+    const int page = first + i * WAVES, t = page * PAGE + lane;
+    if (page >= lo + n || t >= len) break;
+    const float* x = a.logits + (int64_t(sh) * a.p.P + page) * a.nrep * PAGE + lane;
+    float sum = 0.f;
+    for (int r = 0; r < a.nrep; ++r) {
+      const float2 y = st[r];
+      sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x[r * PAGE] - y.x), y.y, sum);
+    }
+    a.weights[s * a.sw_s + head * a.sw_h + t] += sum;
+  }
 }
 
 constexpr int GRID = 512;  // two workgroups per CU
@@ -675,6 +726,8 @@ inline Launch plan_of(int S, int P, int m, int nrep, int H, int D) {
   return p;
 }
 
+inline size_t stats_bytes(int S, int Hq) { return (size_t(S) * Hq * sizeof(float2) + 15) / 16 * 16; }
+
 }  // namespace
 
 namespace iq {
@@ -687,10 +740,15 @@ extern "C" size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq
   return p.split ? size_t(2 * GRID) * (ROWS * p.T) * (D + 2) * sizeof(float) : 0;
 }
 
-extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
-                                  float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
-  if (const int st = iq::check_paged(p)) return st;
+extern "C" size_t iq_paged_attention_weights_workspace_bytes(int S, int P, int Hq, int H, int D) {
+  if (S <= 0 || P <= 0 || Hq <= 0 || H <= 0 || Hq % H || !d_ok(D)) return 0;
+  return iq_paged_attention_workspace_bytes(S, P, 1, Hq, H, D) + stats_bytes(S, Hq) + size_t(S) * Hq * P * PAGE * sizeof(float);
+}
+
+namespace {
+int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq, float scale,
+              int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h, float* weights, int64_t sw_s, int64_t sw_h,
+              void* workspace, size_t workspace_bytes, void* stream) {
   IQ_CHECK(q && out, IQ_ERR_NULL);
   IQ_CHECK(m > 0 && m <= 16 && Hq > 0 && Hq % p->H == 0 && Hq <= 4096 && window >= 0, IQ_ERR_SHAPE);
   IQ_CHECK(aligned(q, 16) && aligned(out, 16) && sq_s % 8 == 0 && sq_m % 8 == 0 && sq_h % 8 == 0 && so_s % 8 == 0 &&
@@ -699,23 +757,55 @@ extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s
   const Launch pl = plan_of(p->S, p->P, m, nrep, p->H, p->D);
   IQ_CHECK(int64_t(p->S) * (p->P + PAD) * p->H * pl.tiles <= INT32_MAX &&
                int64_t(p->S) * p->H * pl.tiles <= UINT32_MAX / 512, IQ_ERR_SHAPE);
-  const size_t need = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
+  const size_t slots = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
+  const size_t need = weights ? iq_paged_attention_weights_workspace_bytes(p->S, p->P, Hq, p->H, p->D) : slots;
   IQ_CHECK(!need || (workspace && workspace_bytes >= need), IQ_ERR_WORKSPACE);
   IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   if (window >= p->P * PAGE) window = 0;  // hides nothing
+  const int64_t chunks = ceil_div(p->P, WAVES * WEIGH_PAGES);  // of weights_kernel, per (sequence, head)
+  IQ_CHECK(!weights || int64_t(p->S) * p->H * chunks <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
+  char* const ws = (char*)workspace;
   const AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, m, nrep, pl.tiles,
-                   scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, p->S > 64 ? EACH : 1, pl.split};
-  auto launch = [&]<int D, bool BF, int T>() {
-    attn_kernel<D, BF, T><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
+                   scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, p->S > 64 ? EACH : 1, pl.split,
+                   weights ? (float*)(ws + slots + stats_bytes(p->S, Hq)) : nullptr,
+                   weights ? (float2*)(ws + slots) : nullptr, weights, sw_s, sw_h};
+  auto launch = [&]<int D, bool BF, int T, bool W>() {
+    attn_kernel<D, BF, T, W><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
     if (const int st = launch_status()) return st;
     if (pl.split)
-      combine_kernel<D, BF, T><<<p->S * p->H * pl.tiles, ROWS * T * (D / 8), 0, (hipStream_t)stream>>>(a);
-    return launch_status();
+      combine_kernel<D, BF, T, W><<<p->S * p->H * pl.tiles, ROWS * T * (D / 8), 0, (hipStream_t)stream>>>(a);
+    if (const int st = launch_status()) return st;
+    if constexpr (W) {
+      weights_kernel<<<unsigned(int64_t(p->S) * p->H * chunks), THREADS, 0, (hipStream_t)stream>>>(a, int(chunks));
+      return launch_status();
+    }
+    return int(IQ_OK);
   };
   auto with = [&]<int D, bool BF>() {
-    return pl.T == 2 ? launch.template operator()<D, BF, 2>() : launch.template operator()<D, BF, 1>();
+    if (weights) return pl.T == 2 ? launch.template operator()<D, BF, 2, true>() : launch.template operator()<D, BF, 1, true>();
+    return pl.T == 2 ? launch.template operator()<D, BF, 2, false>() : launch.template operator()<D, BF, 1, false>();
   };
   const bool bf = act_bf16(p->mode);
   if (p->D == 128) return bf ? with.operator()<128, true>() : with.operator()<128, false>();
   return bf ? with.operator()<64, true>() : with.operator()<64, false>();
+}
+}  // namespace
+
+extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
+                                  float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int st = iq::check_paged(p)) return st;
+  return attention(p, q, sq_s, sq_m, sq_h, m, Hq, scale, window, out, so_s, so_m, so_h, nullptr, 0, 0, workspace,
+                   workspace_bytes, stream);
+}
+
+extern "C" int iq_paged_attention_weights(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_h, int Hq, float scale,
+                                          int window, void* out, int64_t so_s, int64_t so_h, float* weights, int64_t sw_s,
+                                          int64_t sw_h, int64_t T, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int st = iq::check_paged(p)) return st;
+  IQ_CHECK(weights, IQ_ERR_NULL);
+  IQ_CHECK(T >= int64_t(p->P) * PAGE && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
+  IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
+  return attention(p, q, sq_s, 0, sq_h, 1, Hq, scale, window, out, so_s, 0, so_h, weights, sw_s, sw_h, workspace,
+                   workspace_bytes, stream);
 }

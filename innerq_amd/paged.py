@@ -236,19 +236,25 @@ class PagedStore:
         return k, v
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float,
-               window: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               window: Optional[int] = None, out: Optional[torch.Tensor] = None,
+               weights: Optional[torch.Tensor] = None) -> torch.Tensor:
         """softmax(q K^T * scale) V over each sequence's first lens[s] tokens, the new ones among them.  q [S, Hq, D]
         (one new token) or [S, m, Hq, D] (m <= 16: token j sees all but the m - 1 - j after it); window: only the last
         ``window`` tokens up to its own.  The table's width plans the work: pass ``table[:, :pages that the longest
         sequence needs]`` where tables are wider than any sequence.  Rows that see no token, or only tokens whose logits
         are minus infinity, are 0.  Returns ``out`` (q itself, or memory that no other argument uses) or a new tensor of
-        q's shape."""
-        fast = ops._native(q) if forward_ad._current_level < 0 else None
+        q's shape.
+
+        weights: fp32 [S, H, T], T at least the table's P * 64, memory that no other argument uses: weights[s, h, j] grows
+        by the softmax weights of token j, summed over the query heads of KV head h (evict() goes by what they add up
+        to).  With one new token per sequence only (a drafted token's weights could not be taken back).  The call then
+        takes 4 bytes of memory per query head and place of the table."""
+        fast = ops._native(q) if forward_ad._current_level < 0 and weights is None else None
         if fast is not None:
             r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out)
             if r is not None:
                 return r
-        _no_grad(q, out)
+        _no_grad(q, out, weights)
         p = self._args(table, lens)
         if q.dim() not in (3, 4) or q.shape[0] != p.S:
             raise ValueError(f"attend: q must be [S, Hq, D] or [S, m, Hq, D] with S = {p.S}, got {tuple(q.shape)}")
@@ -267,6 +273,17 @@ class PagedStore:
         else:
             _out_rows(out, "out", tuple(q.shape), self.dtype, self.device)
         qs, os = (t.stride() if m > 1 or t.dim() == 4 else (t.stride(0), 0, t.stride(1)) for t in (q, out))
+        if weights is not None:
+            if m > 1:
+                raise ValueError(f"attend: weights are added up for one new token per sequence, got {m}")
+            ops.check_weights(weights, "weights", p.S, self.H, p.P * PAGE_TOKENS, self.device, written=True)
+            nbytes = _lib.lib().iq_paged_attention_weights_workspace_bytes(p.S, p.P, Hq, self.H, self.D)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            with ops.on_device(self.device):
+                call("iq_paged_attention_weights", ctypes.byref(p), ops._p(q), qs[0], qs[2], Hq, float(scale), window or 0,
+                     ops._p(out), os[0], os[2], ops._p(weights), weights.stride(0), weights.stride(1), weights.shape[2],
+                     ops._p(ws), nbytes, ops._stream(self.device))
+            return out
         nbytes = _lib.lib().iq_paged_attention_workspace_bytes(p.S, p.P, m, Hq, self.H, self.D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         with ops.on_device(self.device):

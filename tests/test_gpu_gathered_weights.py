@@ -1,0 +1,209 @@
+"""The attention weights that keys gather (attend(weights=), prompt_attention(weights=)) on the GPU against 64 bits
+(oracle/evict_ref.py); the output is that of the call without them."""
+import random
+
+import pytest
+import torch
+
+from innerq_amd import ops, paged
+from oracle import evict_ref as E
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def filled(seed, lens, H, D, dtype, width=None):
+    """A store whose sequences hold random tokens (NaN behind their ends), and K as the store holds it."""
+    g, rng = torch.Generator().manual_seed(seed), random.Random(seed)
+    P = width or max(1, max(-(-n // 64) for n in lens))
+    pool = sum(-(-n // 64) for n in lens) + 2
+    ids = rng.sample(range(pool), pool)
+    table = [[-1] * P for _ in lens]
+    for s, n in enumerate(lens):
+        for i in range(-(-n // 64)):
+            table[s][i] = ids.pop()
+    table = i32(table)
+    st = paged.PagedStore(pool, H, D, DEV, dtype)
+    st.pages.fill_(-1)
+    N, cu = sum(lens), [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    k = torch.randn(max(N, 1), H, D, generator=g)
+    k[..., :3] *= 6
+    v = torch.randn(max(N, 1), H, D, generator=g)
+    if N:
+        st.append(k.to(dtype).to(DEV), v.to(dtype).to(DEV), table, i32([0] * len(lens)), i32(cu))
+        k = st.read(table, i32([0] * len(lens)), i32(cu), N)[0].cpu()
+    return st, table, cu, k, g
+
+
+def held(g, S, H, T):
+    """What the keys have gathered before: NaN nowhere, marks behind the ends."""
+    return torch.rand(S, H, T, generator=g).to(DEV)
+
+
+def check(got, before, want, bound, what):
+    """got = before + want, the sum rounded once."""
+    b = before.double()
+    worst = ((got.double() - b - want).abs() - bound - 2.0 ** -24 * (b + want).abs()).max()
+    assert worst <= 0, (what, float(worst))
+
+
+def check_attend(st, table, cu, k, lens, q, w, scale, window=None):
+    before = w.cpu().clone()
+    want_out = st.attend(q, table, i32(lens), scale, window=window)
+    out = st.attend(q, table, i32(lens), scale, window=window, weights=w)
+    st.check()
+    assert torch.equal(out, want_out)
+    got = w.cpu()
+    for s, n in enumerate(lens):
+        assert torch.equal(got[s, :, n:], before[s, :, n:]), s
+        if n:
+            want, bound = E.weights(q[s].cpu().view(1, -1, st.D), k[cu[s]:cu[s + 1]], scale, window=window or 0)
+            check(got[s, :, :n], before[s, :, :n], want, bound, s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,H,Hq", [(128, 2, 8), (64, 2, 2), (128, 1, 3), (64, 1, 32), (128, 3, 3), (64, 1, 40)])
+@pytest.mark.parametrize("lens", [[1], [2, 63, 64, 65], [0, 5, 0, 300], [1000, 17, 128, 511], [700, 1, 2100]])
+def test_attend_lengths(dtype, D, H, Hq, lens):
+    st, table, cu, k, g = filled(sum(lens) + H, lens, H, D, dtype)
+    w = held(g, len(lens), H, table.shape[1] * 64)
+    q = torch.randn(len(lens), Hq, D, generator=g).to(dtype).to(DEV)
+    check_attend(st, table, cu, k, lens, q, w, D ** -0.5)
+    check_attend(st, table, cu, k, lens, q, w, D ** -0.5)  # on top of the first
+
+
+@pytest.mark.parametrize("window", [1, 50, 64, 65, 700, 2 ** 31 - 1])
+@pytest.mark.parametrize("width", [None, 60])
+def test_attend_windows(window, width):
+    lens = [1, 64, 65, 900, 0, 129]
+    st, table, cu, k, g = filled(3, lens, 2, 128, torch.float16, width)
+    w = held(g, 6, 2, table.shape[1] * 64 + 3)
+    q = torch.randn(6, 4, 128, generator=g).half().to(DEV)
+    check_attend(st, table, cu, k, lens, q, w, 0.1, window)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_attend_scales(scale):
+    lens = [300, 1, 64, 1200]
+    st, table, cu, k, g = filled(4, lens, 2, 64, torch.bfloat16)
+    w = held(g, 4, 2, table.shape[1] * 64)
+    q = torch.randn(4, 4, 64, generator=g).bfloat16().to(DEV)
+    check_attend(st, table, cu, k, lens, q, w, scale)
+
+
+@pytest.mark.parametrize("S,H,width", [(2, 1, 8), (2, 1, 9), (16, 4, 17), (64, 4, 32), (64, 4, 33), (300, 1, 40)])
+def test_attend_table_widths(S, H, width):
+    """Both sides of the widths up to which a workgroup takes a whole sequence and head."""
+    rng = random.Random(S)
+    lens = [rng.choice([0, 1, 64, 130]) for _ in range(S)]
+    lens[0], lens[S - 1] = width * 64, 200
+    st, table, cu, k, g = filled(width, lens, H, 64, torch.float16, width)
+    w = held(g, S, H, width * 64)
+    q = torch.randn(S, 2 * H, 64, generator=g).half().to(DEV)
+    check_attend(st, table, cu, k, lens, q, w, 0.125)
+
+
+def test_attend_two_groups_of_rows():
+    """More than 16 query heads per KV head, over enough pages for two groups of rows at a time."""
+    lens = [40, 600, 0] + [64] * 125
+    st, table, cu, k, g = filled(5, lens, 4, 64, torch.float16, 10)
+    w = held(g, 128, 4, 640)
+    q = torch.randn(128, 4 * 20, 64, generator=g).half().to(DEV)
+    check_attend(st, table, cu, k, lens, q, w, 0.125)
+
+
+@pytest.mark.parametrize("width", [8, 40])
+def test_attend_special_rows(width):
+    """Infinite and NaN queries, keys and pages: NaN stays with its sequence and head, and within the tokens it saw."""
+    lens = [200, 100, 130, 64]
+    st, table, cu, k, g = filled(6, lens, 2, 64, torch.float16, width)
+    q = torch.randn(4, 4, 64, generator=g).half().to(DEV)
+    clean = held(g, 4, 2, width * 64)
+    want = clean.clone()
+    st.attend(q, table, i32(lens), 0.1, weights=want)
+    w = clean.clone()
+    bad = q.clone()
+    bad[0, 0, 3] = float("nan")  # of KV head 0
+    st.attend(bad, table, i32(lens), 0.1, weights=w)
+    assert bool(w[0, 0, :200].isnan().all()) and torch.equal(w[0, 1], want[0, 1]) and torch.equal(w[1:], want[1:])
+    assert torch.equal(w[0, 0, 200:], clean[0, 0, 200:])
+    # a page outside the pool, and a sequence longer than its table
+    w = clean.clone()
+    bad_table = table.clone()
+    bad_table[1, 0] = 10 ** 6
+    st.attend(q, bad_table, i32([200, 100, width * 64 + 1, 64]), 0.1, weights=w)
+    with pytest.raises(RuntimeError, match="outside the pool and a token past"):
+        st.check()
+    assert bool(w[1, :, :100].isnan().all()) and torch.equal(w[1, :, 100:], clean[1, :, 100:])
+    assert bool(w[2].isnan().all()) and torch.equal(w[0], want[0]) and torch.equal(w[3], want[3])
+    # all logits minus infinity: a row of 0, and no weights
+    keys = torch.full((64, 2, 64), -1.0)
+    keys[..., 0] = float("-inf")
+    one = paged.PagedStore(1, 2, 64, DEV)
+    one.pages.zero_()
+    half = one.pages.view(torch.int16)  # K: code 0 with zero point -inf in group 0
+    half[:, :, 2 * 64 * 8 + 1:2 * 64 * 8 + 2 * 64 * 2:4] = torch.tensor([-1024], dtype=torch.int16, device=DEV)
+    x = torch.zeros(1, 2, 64, dtype=torch.float16, device=DEV)
+    x[..., :32] = 1.0
+    w = clean[:1, :, :64].clone()
+    out = one.attend(x, i32([[0]]), i32([50]), 1.0, weights=w)
+    assert bool((out == 0).all()) and torch.equal(w, clean[:1, :, :64])
+
+
+def test_attend_strides_streams_and_graphs():
+    lens = [700, 30, 400]
+    st, table, cu, k, g = filled(7, lens, 2, 128, torch.bfloat16, 40)
+    ll = i32(lens)
+    q = torch.randn(3, 4, 128, generator=g).bfloat16().to(DEV)
+    clean = held(g, 3, 2, 2560)
+    want = clean.clone()
+    out = st.attend(q, table, ll, 0.1, weights=want)
+    wide = torch.zeros(2, 3, 2601, device=DEV).transpose(0, 1)
+    w = wide[..., 41:]
+    w.copy_(clean)
+    assert torch.equal(st.attend(q[:, None], table, ll, 0.1, weights=w)[:, 0], out) and torch.equal(w, want)
+    assert not wide[..., :41].any()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    w = clean.clone()
+    with torch.cuda.stream(side):
+        st.attend(q, table, ll, 0.1, weights=w)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        o = st.attend(q, table, ll, 0.1, weights=w)
+    for n in ([700, 30, 400], [5, 2560, 0]):
+        ll.copy_(i32(n))
+        table.clamp_(min=0)
+        w.copy_(clean)
+        graph.replay()
+        torch.cuda.synchronize()
+        x = clean.clone()
+        y = st.attend(q, table, ll, 0.1, weights=x)
+        assert torch.equal(o, y) or bool(y.isnan().any())
+        assert torch.equal(w.nan_to_num(7.0), x.nan_to_num(7.0))
+
+
+def test_attend_refusals():
+    lens = [100, 30]
+    st, table, cu, k, g = filled(8, lens, 2, 64, torch.float16)
+    q = torch.randn(2, 4, 64, generator=g).half().to(DEV)
+    w = held(g, 2, 2, 128)
+    with pytest.raises(ValueError, match="one new token"):
+        st.attend(q[:, None].expand(2, 2, 4, 64), table, i32(lens), 0.1, weights=w)
+    for bad in (w[:1], w[:, :1], w[..., :127], w.transpose(1, 2), w[0], w[:1].expand(2, 2, 128), w[:, :1].expand(2, 2, 128)):
+        with pytest.raises(ValueError):
+            st.attend(q, table, i32(lens), 0.1, weights=bad)
+    for bad in (w.half(), w.cpu()):
+        with pytest.raises(TypeError):
+            st.attend(q, table, i32(lens), 0.1, weights=bad)
+    with pytest.raises(NotImplementedError):
+        st.attend(q, table, i32(lens), 0.1, weights=w.clone().requires_grad_())
