@@ -16,18 +16,13 @@
 // matrix unit is busy 60 % of the clocks, HBM moves 0.8 GB.  With D = 64 there are half the products per exponential: the
 // vector unit is busy 79 % of the clocks, the matrix unit 50 % (1.11 - 1.18 ms, 930 - 990 TFLOP/s).  Short prompts wait for
 // their first tile: 77 tokens 7.4 us.
-#include "iq_paged.h"
+#include "iq_prompt.h"
 
 using namespace iq;
 
 namespace {
 
-typedef float f16_t __attribute__((ext_vector_type(16)));
-typedef short s4_t __attribute__((ext_vector_type(4)));
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
-
 constexpr int WAVES = 4, THREADS = 64 * WAVES, BM = 32 * WAVES, BN = 64;
-constexpr float NEG_INF = -__builtin_inff();
 
 struct PromptArgs {
   const uint16_t *q, *k, *v;
@@ -35,41 +30,15 @@ struct PromptArgs {
   int64_t sq_n, sq_h, sk_n, sk_h, sv_n, sv_h, so_n, so_h;
   const int32_t *cu_q, *cu_k;
   int S, N, Nk, Hq, nrep, slots;
-  float c;              // |scale| log2(e); 1 for a scale of 0
+  float c;              // Scale
   float slack;          // 8 / c
-  uint32_t keep, sign;  // and-ed, xor-ed into the queries: a scale of 0 clears them, a negative one flips their signs
+  uint32_t keep, sign;  // Scale
   int causal, window;
+  float2* stats;        // [N][Hq] {base, 1 / sum of weights} of each row, or null
 };
-
-// rows [r0, r1) of sequence s in a packed tensor of n rows (whatever cu holds)
-__device__ __forceinline__ void rows_of(const int32_t* cu, int s, int n, int& r0, int& r1) {
-  r0 = min(max(cu[s], 0), n);
-  r1 = min(max(cu[s + 1], r0), n);
-}
 
 // tiles of BM rows that a KV head's share of a sequence of lq query rows makes
 __device__ __forceinline__ int tiles_of(int lq, int nrep) { return int((int64_t(lq) * nrep + BM - 1) / BM); }
-
-template <bool BF>
-__device__ __forceinline__ f16_t mma32(u4_t a, u4_t b, f16_t c) {
-  if constexpr (BF)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
-}
-
-__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
-  typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2_t, a), __builtin_bit_cast(us2_t, b)));
-}
-
-// 16-byte chunk c of row r in an LDS tile: spread so that neither K's reads (one chunk of 16 rows) nor V's transposed
-// ones (four chunks of 4 rows) meet in a bank
-template <int D>
-__device__ __forceinline__ int chunk_at(int r, int c) {
-  if constexpr (D == 128) return r * 16 + (c ^ ((r & 3) << 2 | (r >> 2 & 3)));
-  else return r * 8 + (c ^ ((r >> 1 & 1) << 2 | (r >> 2 & 3)));
-}
 
 template <int D, bool BF>
 __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
@@ -411,6 +380,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   }
   // Rows leave through LDS: 16 lanes write a whole row of 128 dims, where a lane's own dims are 8 bytes here and there.
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (a.stats && hi == 0 && vrow < rows) a.stats[int64_t(q0 + row) * a.Hq + head] = float2{base_of(m), inv};
   __syncthreads();  // nobody reads tiles any more
   u4_t* const lo = (wave < 2 ? lk0 : lk1) + (wave & 1) * 32 * CH;
 #pragma unroll
@@ -430,12 +400,10 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   }
 }
 
-}  // namespace
-
-extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
-                                   const void* v, int64_t sv_n, int64_t sv_h, const int32_t* cu_q, const int32_t* cu_k,
-                                   int S, int N, int Nk, int Hq, int H, int D, int mode, float scale, int causal, int window,
-                                   void* out, int64_t so_n, int64_t so_h, void* stream) {
+int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h, const void* v, int64_t sv_n,
+              int64_t sv_h, const int32_t* cu_q, const int32_t* cu_k, int S, int N, int Nk, int Hq, int H, int D, int mode,
+              float scale, int causal, int window, void* out, int64_t so_n, int64_t so_h, float* weights, int64_t sw_s,
+              int64_t sw_h, int64_t T, void* workspace, size_t workspace_bytes, void* stream) {
   IQ_CHECK(cu_q && cu_k && (N == 0 || (q && out)) && (Nk == 0 || (k && v)), IQ_ERR_NULL);
   IQ_CHECK(base_mode(mode) == 0, IQ_ERR_MODE);
   IQ_CHECK(d_ok(D) && H > 0 && Hq > 0 && Hq % H == 0 && Hq <= 4096 && S > 0 && N >= 0 && Nk >= 0 && window >= 0, IQ_ERR_SHAPE);
@@ -444,21 +412,59 @@ extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, co
   for (const int64_t s : {sq_n, sq_h, sk_n, sk_h, sv_n, sv_h, so_n, so_h}) IQ_CHECK(s % 8 == 0, IQ_ERR_ALIGN);
   IQ_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, 4) && aligned(cu_k, 4),
            IQ_ERR_ALIGN);
+  if (weights) {
+    // a tile's rows of q in 32 bits
+    IQ_CHECK(sq_n >= 0 && sq_n < (1 << 23) && sq_h >= 0 && sq_h < (1 << 29) / (Hq / H), IQ_ERR_SHAPE);
+    IQ_CHECK(T >= 0 && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
+    IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
+  }
   if (N == 0) return IQ_OK;
   const int64_t rows = int64_t(N) * (Hq / H);
   IQ_CHECK(rows <= INT32_MAX - BM && int64_t(N) + Nk <= INT32_MAX, IQ_ERR_SHAPE);
   const int64_t slots = rows / BM + S;  // first_slot(S) at most
   IQ_CHECK(slots * H <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
+  if (weights) {
+    IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(N, Hq), IQ_ERR_WORKSPACE);
+    IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
+  }
   if (window >= Nk) window = 0;  // hides nothing
-  const float c = scale * 1.44269504088896340736f, abs_c = c == 0 ? 1.f : c < 0 ? -c : c;
+  const Scale sc = scale_of(scale);
   PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
-               sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), abs_c, 8.f / abs_c, c == 0 ? 0u : ~0u,
-               c < 0 ? 0x80008000u : 0u, causal ? 1 : 0, window};
+               sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), sc.c, 8.f / sc.c, sc.keep, sc.sign,
+               causal ? 1 : 0, window, weights ? (float2*)workspace : nullptr};
   auto launch = [&]<int D_, bool BF>() {
     prompt_kernel<D_, BF><<<unsigned(slots * H), THREADS, 0, (hipStream_t)stream>>>(a);
     return launch_status();
   };
   const bool bf = act_bf16(mode);
-  if (D == 128) return bf ? launch.operator()<128, true>() : launch.operator()<128, false>();
-  return bf ? launch.operator()<64, true>() : launch.operator()<64, false>();
+  const int st = D == 128 ? (bf ? launch.operator()<128, true>() : launch.operator()<128, false>())
+                          : (bf ? launch.operator()<64, true>() : launch.operator()<64, false>());
+  if (st || !weights || !Nk) return st;
+  return launch_prompt_weights({a.q, a.k, sq_n, sq_h, sk_n, sk_h, a.stats, weights, sw_s, sw_h, T, cu_q, cu_k, S, N, Nk, Hq,
+                                Hq / H, 0, sc, causal ? 1 : 0, window}, D, bf, (hipStream_t)stream);
+}
+
+}  // namespace
+
+extern "C" size_t iq_prompt_weights_workspace_bytes(int N, int Hq) {
+  return N <= 0 || Hq <= 0 ? 0 : size_t(N) * Hq * sizeof(float2);
+}
+
+extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
+                                   const void* v, int64_t sv_n, int64_t sv_h, const int32_t* cu_q, const int32_t* cu_k,
+                                   int S, int N, int Nk, int Hq, int H, int D, int mode, float scale, int causal, int window,
+                                   void* out, int64_t so_n, int64_t so_h, void* stream) {
+  return attention(q, sq_n, sq_h, k, sk_n, sk_h, v, sv_n, sv_h, cu_q, cu_k, S, N, Nk, Hq, H, D, mode, scale, causal, window,
+                   out, so_n, so_h, nullptr, 0, 0, 0, nullptr, 0, stream);
+}
+
+extern "C" int iq_prompt_attention_weights(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n,
+                                           int64_t sk_h, const void* v, int64_t sv_n, int64_t sv_h, const int32_t* cu_q,
+                                           const int32_t* cu_k, int S, int N, int Nk, int Hq, int H, int D, int mode,
+                                           float scale, int causal, int window, void* out, int64_t so_n, int64_t so_h,
+                                           float* weights, int64_t sw_s, int64_t sw_h, int64_t T, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  IQ_CHECK(weights, IQ_ERR_NULL);
+  return attention(q, sq_n, sq_h, k, sk_n, sk_h, v, sv_n, sv_h, cu_q, cu_k, S, N, Nk, Hq, H, D, mode, scale, causal, window,
+                   out, so_n, so_h, weights, sw_s, sw_h, T, workspace, workspace_bytes, stream);
 }

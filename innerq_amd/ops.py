@@ -934,7 +934,7 @@ def decode_attention_combine_live(plan, B: int, Hq: int, T: int, D: int, device,
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float,
                      cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = True, window: Optional[int] = None,
-                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(q K^T * scale) V of prompts of different lengths that lie one behind the other.
 
     q [N, Hq, D]; k, v [Nk, H, D] of q's dtype (fp16 or bf16), Hq a multiple of H, D 64 or 128.  Sequence s is rows
@@ -943,14 +943,19 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     keys, each row before it one less (a chunk of a prompt behind its earlier keys has more keys than rows); window:
     only the last ``window`` of the keys up to its own.  Rows that see no key, or only keys whose logits are minus
     infinity, are 0; rows outside the sequences are not written.  ``out`` may be q, or memory that no other argument
-    uses.  Inference only: tensors that autograd follows are refused, ``out`` too."""
-    fast = _native(q) if forward_ad._current_level < 0 else None
+    uses.  Inference only: tensors that autograd follows are refused, ``out`` too.
+
+    weights: fp32 [S, H, T], memory that no other argument uses: weights[s, h, j] grows by the softmax weights of key j of
+    sequence s (of those below T), summed over its rows and the query heads of KV head h, as PagedStore.evict goes by.
+    The rows may be a prompt's last ones, behind all its keys.  The call then takes 8 bytes of memory per row and query
+    head."""
+    fast = _native(q) if forward_ad._current_level < 0 and weights is None else None
     if fast is not None:
         r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out)
         if r is not None:
             return r
     require_act(q, "q")
-    if autograd_follows(q, k, v, out):
+    if autograd_follows(q, k, v, out, weights):
         raise NotImplementedError("prompt_attention has no backward: call it under torch.no_grad()")
     if q.dim() != 3 or k.dim() != 3:
         _shape_error(f"q must be [N, Hq, D] and k [Nk, H, D], got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -968,6 +973,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             _shape_error(f"{name} is on {t.device}, q on {dev}")
         rows.append(readable_rows(t if t.stride(0) < 2 ** 23 else t.clone(memory_format=torch.contiguous_format)))
     q, k, v = rows
+    if weights is not None and q.stride(1) * (Hq // H) >= 2 ** 29:
+        q = q.clone(memory_format=torch.contiguous_format)
     cu_q = check_cu(cu_seqlens, "cu_seqlens", None, dev)
     S = cu_q.shape[0] - 1
     cu_k = cu_q if cu_seqlens_k is None else check_cu(cu_seqlens_k, "cu_seqlens_k", S, dev)
@@ -982,10 +989,19 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         check_out(out.shape, (N, Hq, D))
         if out.device != dev or not writable_rows(out):
             _shape_error("out needs a contiguous head_dim, rows on 16-byte boundaries and q's device")
+    args = (_p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1), _p(cu_q),
+            _p(cu_k), S, N, Nk, Hq, H, D, act_flag(q.dtype), float(scale), 1 if causal else 0, window or 0, _p(out),
+            out.stride(0), out.stride(1))
     with on_device(dev):
-        call("iq_prompt_attention", _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
-             v.stride(1), _p(cu_q), _p(cu_k), S, N, Nk, Hq, H, D, act_flag(q.dtype), float(scale), 1 if causal else 0,
-             window or 0, _p(out), out.stride(0), out.stride(1), _stream(dev))
+        if weights is not None:
+            check_weights(weights, "weights", S, H, 0, dev, written=True)
+        if weights is None or not weights.numel():
+            call("iq_prompt_attention", *args, _stream(dev))
+            return out
+        nbytes = _lib.lib().iq_prompt_weights_workspace_bytes(N, Hq)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        call("iq_prompt_attention_weights", *args, _p(weights), weights.stride(0), weights.stride(1), weights.shape[2], _p(ws),
+             nbytes, _stream(dev))
     return out
 
 

@@ -207,3 +207,167 @@ def test_attend_refusals():
             st.attend(q, table, i32(lens), 0.1, weights=bad)
     with pytest.raises(NotImplementedError):
         st.attend(q, table, i32(lens), 0.1, weights=w.clone().requires_grad_())
+
+
+# ---- prompts ---------------------------------------------------------------------------------------------------
+def prompts(seed, lens, past, H, Hq, D, dtype):
+    g = torch.Generator().manual_seed(seed)
+    past = past if isinstance(past, list) else [past] * len(lens)
+    N, Nk = sum(lens), sum(max(a + b, 0) for a, b in zip(lens, past))
+    q, k, v = torch.randn(N, Hq, D, generator=g), torch.randn(Nk, H, D, generator=g), torch.randn(Nk, H, D, generator=g)
+    k[..., :3] *= 4
+    cu, cu_k = [0], [0]
+    for a, b in zip(lens, past):
+        cu.append(cu[-1] + a)
+        cu_k.append(cu_k[-1] + max(a + b, 0))
+    return g, *(x.to(dtype).to(DEV) for x in (q, k, v)), cu, cu_k
+
+
+def check_prompts(g, q, k, v, cu, cu_k, scale, T=None, **kw):
+    S, H = len(cu) - 1, k.shape[1]
+    longest = max(b - a for a, b in zip(cu_k, cu_k[1:]))
+    T = longest + 3 if T is None else T
+    w = held(g, S, H, T)
+    before = w.cpu().clone()
+    want_out = ops.prompt_attention(q, k, v, i32(cu), scale, i32(cu_k), **kw)
+    out = ops.prompt_attention(q, k, v, i32(cu), scale, i32(cu_k), weights=w, **kw)
+    assert torch.equal(out, want_out)
+    got, qc, kc = w.cpu(), q.cpu(), k.cpu()
+    for s in range(S):
+        n = min(cu_k[s + 1] - cu_k[s], T)
+        assert torch.equal(got[s, :, n:], before[s, :, n:]), s
+        if n and cu[s + 1] > cu[s]:
+            want, bound = E.weights(qc[cu[s]:cu[s + 1]], kc[cu_k[s]:cu_k[s + 1]], scale, kw.get("causal", True),
+                                    kw.get("window") or 0)
+            check(got[s, :, :n], before[s, :, :n], want[:, :n], bound[:, :n], s)
+        else:
+            assert torch.equal(got[s], before[s])
+    return w
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,H,Hq", [(128, 2, 8), (64, 2, 2), (128, 1, 3), (64, 1, 5)])
+@pytest.mark.parametrize("lens", [[1], [63, 0, 64, 65, 1], [300, 17], [128, 129, 127]])
+@pytest.mark.parametrize("past", [0, 1, 200])
+def test_prompt_lengths(dtype, D, H, Hq, lens, past):
+    check_prompts(*prompts(sum(lens) + past, lens, past, H, Hq, D, dtype), D ** -0.5)
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 130, 400, 2 ** 31 - 1])
+@pytest.mark.parametrize("past", [0, 150])
+@pytest.mark.parametrize("Hq", [2, 6])
+def test_prompt_windows(window, past, Hq):
+    check_prompts(*prompts(window % 1000, [200, 1, 90, 257], past, 2, Hq, 64, torch.float16), 0.125, window=window)
+
+
+@pytest.mark.parametrize("past", [[0, 70, -20], [-39, 300, -89], [5, 0, 0]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_fewer_and_more_keys(past, causal):
+    """More rows than keys (the first see none), more keys than rows, and every row all keys."""
+    check_prompts(*prompts(9, [40, 100, 90], past, 2, 4, 128, torch.bfloat16), 0.09, causal=causal)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0, 50.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompt_scales(scale, dtype):
+    check_prompts(*prompts(10, [150, 40], 0, 2, 4, 64, dtype), scale)
+
+
+@pytest.mark.parametrize("T", [0, 1, 100, 128, 129, 200])
+def test_prompt_keys_past_the_weights(T):
+    check_prompts(*prompts(11, [260, 40], 0, 1, 2, 64, torch.float16), 0.125, T=T)
+
+
+def test_prompt_many_sequences():
+    rng = random.Random(12)
+    lens = [rng.choice([0, 0, 1, 3, 40]) for _ in range(400)]
+    lens[7] = 300
+    check_prompts(*prompts(12, lens, [rng.choice([0, 0, 5, 130]) for _ in lens], 1, 2, 64, torch.float16), 0.125)
+
+
+def test_prompt_long():
+    check_prompts(*prompts(13, [1500], 700, 2, 4, 128, torch.bfloat16), 0.09)
+
+
+def test_prompt_special_rows():
+    """NaN stays with the keys that its row and head see; rows of minus infinity give nothing."""
+    g, q, k, v, cu, cu_k = prompts(14, [200, 100], 0, 2, 4, 64, torch.float16)
+    clean = held(g, 2, 2, 200)
+    want = clean.clone()
+    ops.prompt_attention(q, k, v, i32(cu), 0.1, weights=want)
+    bad = q.clone()
+    bad[150, 0, 3] = float("nan")  # of KV head 0, sees keys 0 .. 150
+    w = clean.clone()
+    ops.prompt_attention(bad, k, v, i32(cu), 0.1, weights=w)
+    assert bool(w[0, 0, :151].isnan().all()) and torch.equal(w[0, 0, 151:], want[0, 0, 151:])
+    assert torch.equal(w[0, 1], want[0, 1]) and torch.equal(w[1], want[1])
+    bad = k.clone()
+    bad[120, 1, 3] = float("nan")  # rows from 120 on are NaN for KV head 1, and with them all keys they see
+    w = clean.clone()
+    ops.prompt_attention(q, bad, v, i32(cu), 0.1, weights=w)
+    assert bool(w[0, 1].isnan().all()) and torch.equal(w[0, 0], want[0, 0]) and torch.equal(w[1], want[1])
+    x = torch.ones_like(q)
+    bad = k.clone()
+    bad[:200, 0] = 0
+    bad[:200, 0, 0] = float("-inf")
+    bad[100, 0] = 0  # the only key that counts
+    w = clean.clone()
+    out = ops.prompt_attention(x, bad, v, i32(cu), 0.1, weights=w)
+    got = w[0, 0] - clean[0, 0]
+    assert torch.equal(out[:100, :2], torch.zeros_like(out[:100, :2])) and bool((got[:100] == 0).all())
+    assert bool((got[101:] == 0).all()) and abs(float(got[100]) - 200) < 1e-3
+    w = clean.clone()
+    ops.prompt_attention(q * 1e4, k, v, i32(cu), 1e3, weights=w)  # logits past 65536, no infinity of their own
+    assert bool(w.isfinite().all())
+    assert abs(float((w - clean)[0].double().sum()) - 200 * 4) < 1.0
+
+
+def test_prompt_strides_and_graphs():
+    g, q, k, v, cu, cu_k = prompts(15, [300, 40, 7], 0, 2, 4, 128, torch.bfloat16)
+    clean = held(g, 3, 2, 300)
+    want = clean.clone()
+    ops.prompt_attention(q, k, v, i32(cu), 0.1, weights=want)
+    wide = torch.zeros(347 + 40, 13, 128, dtype=q.dtype, device=DEV)
+    wide[:347, 1:5], wide[:347, 5:7] = q, k
+    w = clean.transpose(0, 1).contiguous().transpose(0, 1)
+    qt = q.transpose(0, 1).contiguous().transpose(0, 1)
+    for qq in (wide[:347, 1:5], qt, torch.cat([q, q], 2)[..., 128:]):
+        x = w.clone()
+        ops.prompt_attention(qq, wide[:347, 5:7], v, i32(cu), 0.1, weights=x)
+        assert torch.equal(x, want)
+    ints, w = i32(cu), clean.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.prompt_attention(q, k, v, ints, 0.1, weights=w)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.prompt_attention(q, k, v, ints, 0.1, weights=w)
+    for c in (cu, [0, 0, 300, 347], [40, 41, 60, 300]):
+        ints.copy_(i32(c))
+        w.copy_(clean)
+        graph.replay()
+        torch.cuda.synchronize()
+        x = clean.clone()
+        ops.prompt_attention(q, k, v, ints, 0.1, weights=x)
+        assert torch.equal(w, x)
+
+
+def test_prompt_refusals():
+    g, q, k, v, cu, cu_k = prompts(16, [60, 40], 0, 2, 4, 64, torch.float16)
+    w = held(g, 2, 2, 60)
+    for bad in (w[:1], w[:, :1], w.transpose(1, 2), w[0], w[:1].expand(2, 2, 60), w[:, :1].expand(2, 2, 60)):
+        with pytest.raises(ValueError):
+            ops.prompt_attention(q, k, v, i32(cu), 0.1, weights=bad)
+    for bad in (w.half(), w.cpu(), 5):
+        with pytest.raises(TypeError):
+            ops.prompt_attention(q, k, v, i32(cu), 0.1, weights=bad)
+    with pytest.raises(NotImplementedError):
+        ops.prompt_attention(q, k, v, i32(cu), 0.1, weights=w.clone().requires_grad_())
+    before = w.clone()
+    none = torch.empty(0, 4, 64, dtype=torch.float16, device=DEV)
+    assert ops.prompt_attention(none, k, v, i32([0, 0, 0]), 0.1, i32(cu), weights=w).shape == (0, 4, 64)
+    ops.prompt_attention(q, k[:0], v[:0], i32(cu), 0.1, i32([0, 0, 0]), weights=w)
+    assert torch.equal(w, before)
