@@ -515,6 +515,17 @@ int iq_prompt_attention_weights(const void* q, int64_t sq_n, int64_t sq_h, const
                                 int64_t so_n, int64_t so_h, float* weights, int64_t sw_s, int64_t sw_h, int64_t T,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* Differential attention of S prompts: q [N, Hq, D], k [Nk, H, D], v [Nk, H/2, 2 D], out [N, Hq/2, 2 D], H even, Hq a
+ * multiple of H.  Output head j (of group g = j / (Hq / H)) is
+ *     (softmax(q_2j k_2g^T scale) - lam[j * s_lam] softmax(q_(2j+1) k_(2g+1)^T scale)) v_g,
+ * each map over the keys that its row sees, everything else as iq_prompt_attention: a map that sees no key, or only keys
+ * whose logits are minus infinity, counts as 0.  lam: fp32 [Hq/2] on the device.  The difference is taken in fp32.  out must
+ * not be q. */
+int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
+                             const void* v, int64_t sv_n, int64_t sv_h, const float* lam, int64_t s_lam, const int32_t* cu_q,
+                             const int32_t* cu_k, int S, int N, int Nk, int Hq, int H, int D, int mode, float scale,
+                             int causal, int window, void* out, int64_t so_n, int64_t so_h, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

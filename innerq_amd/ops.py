@@ -145,6 +145,19 @@ def check_cu(cu: torch.Tensor, name: str, S: Optional[int], device: torch.device
     return cu
 
 
+def check_diff_heads(Hq: int, H: int) -> None:
+    """Heads of differential attention: pairs of neighbouring ones, H KV heads and a multiple of them."""
+    if H <= 0 or H % 2 or Hq <= 0 or Hq % H:
+        _shape_error(f"differential attention takes an even number of KV heads and a multiple of query heads, got {H} and {Hq}")
+
+
+def check_lam(lam: torch.Tensor, n: int, device: torch.device) -> None:
+    """The second map's factor: fp32 [n] on ``device``, one number per output head (of any stride, 0 too)."""
+    require_device(lam, "lam", torch.float32)
+    if lam.dim() != 1 or lam.shape[0] != n or lam.device != device:
+        _shape_error(f"lam must be an fp32 [{n}] tensor on {device}, got {tuple(lam.shape)} on {lam.device}")
+
+
 def check_weights(w: torch.Tensor, name: str, S: int, H: int, T: int, device: torch.device, written: bool = False) -> None:
     """Attention weights that tokens have gathered: fp32 [S, H, T or more] on ``device``, T contiguous; where they are
     ``written``, rows of their own."""
@@ -1002,6 +1015,59 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         call("iq_prompt_attention_weights", *args, _p(weights), weights.stride(0), weights.stride(1), weights.shape[2], _p(ws),
              nbytes, _stream(dev))
+    return out
+
+
+def diff_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, lam: torch.Tensor,
+                          scale: float, cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = True,
+                          window: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Differential attention of prompts that lie one behind the other: output head j is
+
+        (softmax(q[2j] K[2g]^T * scale) - lam[j] * softmax(q[2j+1] K[2g+1]^T * scale)) V[g],    g = j // (Hq // H).
+
+    q [N, Hq, D]; k [Nk, H, D]; v [Nk, H/2, 2 D] of q's dtype; lam fp32 [Hq/2] on the device (learned: a model's own number per
+    output head); returns [N, Hq/2, 2 D], ``out`` or a new tensor.  H is even, Hq a multiple of H, D 64 or 128.  Lengths,
+    ``causal`` and ``window`` as in prompt_attention, for both maps.  A map that sees no key, or only keys whose logits
+    are minus infinity, counts as 0; rows outside the sequences are not written.  ``out`` takes memory that no argument
+    uses.  Inference only: tensors that autograd follows are refused, ``out`` too.
+
+    The steps behind such a prompt are PagedStore.diff_attend's: store.append(k, v.view(Nk, H, D), ...)."""
+    require_act(q, "q")
+    if autograd_follows(q, k, v, lam, out):
+        raise NotImplementedError("diff_prompt_attention has no backward: call it under torch.no_grad()")
+    if q.dim() != 3 or k.dim() != 3:
+        _shape_error(f"q must be [N, Hq, D] and k [Nk, H, D], got {tuple(q.shape)} and {tuple(k.shape)}")
+    (N, Hq, D), (Nk, H), dev = q.shape, k.shape[:2], q.device
+    if D not in (64, 128):
+        _shape_error(f"diff_prompt_attention takes head_dim 64 or 128, got {D}")
+    check_diff_heads(Hq, H)
+    rows = []
+    for t, name, shape in ((q, "q", (N, Hq, D)), (k, "k", (Nk, H, D)), (v, "v", (Nk, H // 2, 2 * D))):
+        require_device(t, name, q.dtype)
+        check_out(t.shape, shape, name)
+        if t.device != dev:
+            _shape_error(f"{name} is on {t.device}, q on {dev}")
+        rows.append(readable_rows(t if t.stride(0) < 2 ** 23 else t.clone(memory_format=torch.contiguous_format)))
+    q, k, v = rows
+    check_lam(lam, Hq // 2, dev)
+    cu_q = check_cu(cu_seqlens, "cu_seqlens", None, dev)
+    S = cu_q.shape[0] - 1
+    cu_k = cu_q if cu_seqlens_k is None else check_cu(cu_seqlens_k, "cu_seqlens_k", S, dev)
+    if cu_seqlens_k is None and Nk != N:
+        _shape_error(f"{N} rows of q and {Nk} of k need a cu_seqlens_k of their own")
+    if window is not None and (not causal or not 0 < window < 2 ** 31):
+        raise ValueError(f"a window is positive and causal, got window={window}, causal={causal}")
+    if out is None:
+        out = torch.empty(N, Hq // 2, 2 * D, dtype=q.dtype, device=dev)
+    else:
+        require_device(out, "out", q.dtype)
+        check_out(out.shape, (N, Hq // 2, 2 * D))
+        if out.device != dev or not writable_rows(out):
+            _shape_error("out needs a contiguous head_dim, rows on 16-byte boundaries and q's device")
+    with on_device(dev):
+        call("iq_diff_prompt_attention", _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
+             v.stride(1), _p(lam), lam.stride(0), _p(cu_q), _p(cu_k), S, N, Nk, Hq, H, D, act_flag(q.dtype), float(scale),
+             1 if causal else 0, window or 0, _p(out), out.stride(0), out.stride(1), _stream(dev))
     return out
 
 
