@@ -520,11 +520,24 @@ int iq_prompt_attention_weights(const void* q, int64_t sq_n, int64_t sq_h, const
  *     (softmax(q_2j k_2g^T scale) - lam[j * s_lam] softmax(q_(2j+1) k_(2g+1)^T scale)) v_g,
  * each map over the keys that its row sees, everything else as iq_prompt_attention: a map that sees no key, or only keys
  * whose logits are minus infinity, counts as 0.  lam: fp32 [Hq/2] on the device.  The difference is taken in fp32.  out must
- * not be q. */
+ * not be q.  weights (NULL: none): as iq_prompt_attention_weights', [S][H][T], each KV head gathering its own map's weights,
+ * whatever lam; workspace as there (unused without weights). */
 int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
                              const void* v, int64_t sv_n, int64_t sv_h, const float* lam, int64_t s_lam, const int32_t* cu_q,
                              const int32_t* cu_k, int S, int N, int Nk, int Hq, int H, int D, int mode, float scale,
-                             int causal, int window, void* out, int64_t so_n, int64_t so_h, void* stream);
+                             int causal, int window, void* out, int64_t so_n, int64_t so_h, float* weights, int64_t sw_s,
+                             int64_t sw_h, int64_t T, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Differential attention over pages: q [S, m, Hq, D], out [S, m, Hq/2, 2 D], maps and lam as iq_diff_prompt_attention's over
+ * the pages' H KV heads (even), V's head g of 2 D being the pages' V heads 2g and 2g + 1; everything else as
+ * iq_paged_attention.  out must not be q.  weights (NULL: none; m = 1 only): as iq_paged_attention_weights', each KV head
+ * gathering its own map's weights, whatever lam.  workspace: iq_diff_paged_attention_workspace_bytes (weights: whether there
+ * are any; 0: none needed), 16-byte aligned, of this call alone while it runs. */
+size_t iq_diff_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D, int weights);
+int iq_diff_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
+                            const float* lam, int64_t s_lam, float scale, int window, void* out, int64_t so_s, int64_t so_m,
+                            int64_t so_h, float* weights, int64_t sw_s, int64_t sw_h, int64_t T, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

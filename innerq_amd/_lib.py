@@ -129,7 +129,10 @@ SIGNATURES = {
     "iq_prompt_weights_workspace_bytes": (S, [I, I]),
     "iq_prompt_attention_weights": (I, [P, L, L, P, L, L, P, L, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P, L, L, L, P, S,
                                         P]),
-    "iq_diff_prompt_attention": (I, [P, L, L, P, L, L, P, L, L, P, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P]),
+    "iq_diff_prompt_attention": (I, [P, L, L, P, L, L, P, L, L, P, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P, L, L, L,
+                                     P, S, P]),
+    "iq_diff_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I, I]),
+    "iq_diff_paged_attention": (I, [ctypes.POINTER(iq_paged), P, L, L, L, I, I, P, L, F, I, P, L, L, L, P, L, L, L, P, S, P]),
     "iq_decode_noalloc_max_bytes": (S, []),
     "iq_decode_attention_noalloc": (I, [P, L, L, P, ctypes.POINTER(iq_segment), ctypes.POINTER(iq_segment),
                                         I, I, I, I, I, F, P, L, L, P]),

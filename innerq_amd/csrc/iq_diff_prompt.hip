@@ -19,7 +19,8 @@ struct DiffArgs {
   const int32_t *cu_q, *cu_k;
   const float* lam;  // of each output head
   int64_t s_lam;
-  int S, N, Nk, nrep, slots;  // nrep: output heads per pair of KV heads
+  float2* stats;  // [N][Hq] {base, 1 / sum of weights} of each row of each map, or null
+  int S, N, Nk, Hq, nrep, slots;  // nrep: output heads per pair of KV heads
   Scale scale;
   float slack;  // 8 / c
   int causal, window;
@@ -331,6 +332,7 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
   // The difference, 128 dims at a time: the second map's waves hand theirs to the first map's (the same rows and dims are in
   // the same lanes and registers), which store them through LDS, whole rows at a time.
   float inv = l == 0.f ? 0.f : 1.f / l;
+  if (a.stats && hi == 0 && vrow < rows) a.stats[int64_t(q0 + row) * a.Hq + 2 * head + map] = float2{base_of(m), inv};
   if (map) inv *= a.lam[head * a.s_lam];
   static_assert(X::MAP_WAVES * 64 * 64 * 4 <= 2 * TILE * 16, "a part of the difference fits the two tiles");
   const int64_t at = int64_t(q0 + row) * a.so_n + head * a.so_h;
@@ -377,7 +379,8 @@ extern "C" int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_
                                         const void* v, int64_t sv_n, int64_t sv_h, const float* lam, int64_t s_lam,
                                         const int32_t* cu_q, const int32_t* cu_k, int S, int N, int Nk, int Hq, int H, int D,
                                         int mode, float scale, int causal, int window, void* out, int64_t so_n, int64_t so_h,
-                                        void* stream) {
+                                        float* weights, int64_t sw_s, int64_t sw_h, int64_t T, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
   IQ_CHECK(cu_q && cu_k && lam && (N == 0 || (q && out)) && (Nk == 0 || (k && v)), IQ_ERR_NULL);
   IQ_CHECK(base_mode(mode) == 0, IQ_ERR_MODE);
   IQ_CHECK(d_ok(D) && H > 0 && H % 2 == 0 && Hq > 0 && Hq % H == 0 && Hq <= 4096 && S > 0 && N >= 0 && Nk >= 0 && window >= 0,
@@ -388,7 +391,18 @@ extern "C" int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_
   for (const int64_t s : {sq_n, sq_h, sk_n, sk_h, sv_n, sv_h, so_n, so_h}) IQ_CHECK(s % 8 == 0, IQ_ERR_ALIGN);
   IQ_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, 4) && aligned(cu_k, 4) &&
                aligned(lam, 4), IQ_ERR_ALIGN);
+  if (weights) {
+    // a tile's rows of q in 32 bits
+    IQ_CHECK(sq_n >= 0 && sq_n < (1 << 23) && sq_h >= 0 && sq_h < (1 << 29) / (Hq / H), IQ_ERR_SHAPE);
+    IQ_CHECK(T >= 0 && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
+    IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
+  }
   if (N == 0) return IQ_OK;
+  if (weights) {
+    IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(N, Hq), IQ_ERR_WORKSPACE);
+    IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
+  }
+  float2* const stats = weights ? (float2*)workspace : nullptr;
   const int G = H / 2, nrep = Hq / H;
   if (window >= Nk) window = 0;  // hides nothing
   const Scale sc = scale_of(scale);
@@ -397,12 +411,15 @@ extern "C" int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_
     const int64_t rows = int64_t(N) * nrep, slots = rows / X::BM + S;  // first_slot(S) at most
     IQ_CHECK(rows <= INT32_MAX - X::BM && int64_t(N) + Nk <= INT32_MAX && slots * G <= UINT32_MAX / X::THREADS, IQ_ERR_SHAPE);
     const DiffArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
-                     sv_h, so_n, so_h, cu_q, cu_k, lam, s_lam, S, N, Nk, nrep, int(slots), sc, 8.f / sc.c, causal ? 1 : 0,
+                     sv_h, so_n, so_h, cu_q, cu_k, lam, s_lam, stats, S, N, Nk, Hq, nrep, int(slots), sc, 8.f / sc.c, causal ? 1 : 0,
                      window};
     diff_kernel<D_, BF><<<unsigned(slots * G), X::THREADS, 0, (hipStream_t)stream>>>(a);
     return launch_status();
   };
   const bool bf = act_bf16(mode);
-  if (D == 128) return bf ? launch.operator()<128, true>() : launch.operator()<128, false>();
-  return bf ? launch.operator()<64, true>() : launch.operator()<64, false>();
+  const int st = D == 128 ? (bf ? launch.operator()<128, true>() : launch.operator()<128, false>())
+                          : (bf ? launch.operator()<64, true>() : launch.operator()<64, false>());
+  if (st || !weights || !Nk) return st;
+  return launch_prompt_weights({(const uint16_t*)q, (const uint16_t*)k, sq_n, sq_h, sk_n, sk_h, stats, weights, sw_s, sw_h, T,
+                                cu_q, cu_k, S, N, Nk, Hq, nrep, 0, sc, causal ? 1 : 0, window, 2}, D, bf, (hipStream_t)stream);
 }

@@ -39,13 +39,16 @@ struct AttnArgs {
   int64_t sq_s, sq_m, sq_h;
   uint16_t* out;
   int64_t so_s, so_m, so_h;
-  int m, nrep, tiles;  // new tokens per sequence, query heads per KV head, tiles of 16 T rows (row = token * nrep + head)
+  int heads;           // KV heads, or pairs of them (MAPS = 2)
+  int m, nrep, tiles;  // new tokens per sequence, (output) heads per KV head or pair, tiles of rows (row = token * nrep + head)
   float scale;         // times log2(e)
   int window;          // 0: none
   int grid;
   float* ws;
   int each;            // sequences per lane where a wave adds up their pages (Part)
   int split;           // 0: a workgroup takes a whole (sequence, head, tile)
+  const float* lam;    // of each output head (MAPS = 2)
+  int64_t s_lam;
   // where the keys' weights are wanted (m = 1): the logits [S][H][P][nrep][64], {maximum, 1 / sum} of each row
   // [S][H][nrep], and the weights to add to, fp32 [S][H][>= 64 P]
   float* logits;
@@ -78,7 +81,7 @@ __device__ __forceinline__ Part part_at(const AttnArgs& a, int s0, int base) {
     if (i >= a.each) continue;
     int lo;
     const int s = s0 + int(threadIdx.x & 63) * a.each + i, pages = pages_of(a, min(s, a.p.S - 1), lo);
-    p.n[i] = s < a.p.S && pages > 0 ? (pages + PAD) * a.p.H * a.tiles : 0;
+    p.n[i] = s < a.p.S && pages > 0 ? (pages + PAD) * a.heads * a.tiles : 0;
     sum += p.n[i];
   }
   p.end = base + wave_scan(sum);
@@ -118,14 +121,18 @@ __device__ __forceinline__ void find_unit(const AttnArgs& a, Part p, int u, int&
     p = part_at(a, s0, __builtin_amdgcn_readlane(p.end, 63));
   }
 }
+// Rows.  A tile has R rows of MAPS maps: T groups of 16 columns of the matrix unit's operand, column c being row c % R of
+// map c / R.  (Differential attention: up to 8 rows of both maps share a group, more have a group for each map.)
+template <int T, int MAPS>
+constexpr int tile_rows() { return ROWS * T / MAPS; }
 // row r of tile t of sequence s: its query head offset (head in the group, token)
 struct Row {
   int token, head;
   bool real;
 };
-template <int T>
+template <int R>
 __device__ __forceinline__ Row row_of(const AttnArgs& a, int tile, int r) {
-  const int i = tile * (ROWS * T) + r, token = i / a.nrep;
+  const int i = tile * R + r, token = i / a.nrep;
   return {token, i - token * a.nrep, token < a.m};
 }
 
@@ -219,25 +226,34 @@ __device__ __forceinline__ void v_operands(const u4_t (&c)[2], u4_t s, u4_t z, u
   }
 }
 
-template <int D, bool BF>
+template <int D, bool BF, int MAPS>
 struct Acc {
-  f4_t o[D / 16];  // dims row * D/16 + j of query row lane % 16, row = lane/16 * 4 + i
+  f4_t o[MAPS * D / 16];  // of V head h: o[h D/16 + j], dims row * D/16 + j of column lane % 16, row = lane/16 * 4 + i
   float m, l;
 };
 
-// the logits of a page's 64 tokens: s[g][t][i] of token 16 t + 4 (lane/16) + i for query row 16 g + lane % 16
-template <int D, bool BF, int T>
-__device__ __forceinline__ void logits(const KRegs& r, const u4_t (&q)[T][D / 32], float scale, f4_t (&s)[T][4]) {
+// the logits of a page's 64 tokens: s[g][t][i] of token 16 t + 4 (lane/16) + i for column 16 g + lane % 16
+template <int D, bool BF, int T, int MAPS, int NQ>
+__device__ __forceinline__ void logits(const KRegs (&r)[MAPS], const u4_t (&q)[NQ][D / 32], float scale, f4_t (&s)[T][4]) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
+    f4_t x[NQ];
 #pragma unroll
-    for (int g = 0; g < T; ++g) s[g][t] = f4_t{0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < NQ; ++g) x[g] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const u4_t k = k_values<BF>(r.c[t][j], r.m[t]);
+    for (int h = 0; h < MAPS; ++h)
 #pragma unroll
-      for (int g = 0; g < T; ++g) s[g][t] = mma<BF>(k, q[g][j], s[g][t]);
-    }
+      for (int j = 0; j < D / 32; ++j) {
+        const u4_t k = k_values<BF>(r[h].c[t][j], r[h].m[t]);
+#pragma unroll
+        for (int g = 0; g < NQ; ++g)
+          if (MAPS == 1 || g == h) x[g] = mma<BF>(k, q[g][j], x[g]);
+      }
+    // (two maps in one group of columns: each had all columns, so that no value of one's keys meets the other's)
+    if constexpr (MAPS == 2 && T == 1) s[0][t] = (threadIdx.x & 15) < 8 ? x[0] : x[1];
+    else
+#pragma unroll
+      for (int g = 0; g < T; ++g) s[g][t] = x[g];
 #pragma unroll
     for (int g = 0; g < T; ++g) s[g][t] *= scale;
     __builtin_amdgcn_sched_barrier(0);
@@ -245,8 +261,8 @@ __device__ __forceinline__ void logits(const KRegs& r, const u4_t (&q)[T][D / 32
 }
 
 // the running softmax over 64 more logits; s becomes the weights
-template <int D, bool BF>
-__device__ __forceinline__ void weights(f4_t (&s)[4], Acc<D, BF>& acc) {
+template <int D, bool BF, int MAPS>
+__device__ __forceinline__ void weights(f4_t (&s)[4], Acc<D, BF, MAPS>& acc) {
   float mx = acc.m;
 #pragma unroll
   for (int t = 0; t < 4; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
@@ -261,7 +277,7 @@ __device__ __forceinline__ void weights(f4_t (&s)[4], Acc<D, BF>& acc) {
     const float f = __builtin_amdgcn_exp2f(acc.m - base);
     acc.l *= f;
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) acc.o[j] *= f;
+    for (int j = 0; j < MAPS * D / 16; ++j) acc.o[j] *= f;
     acc.m = mx;
   }
   float sum = 0.f;
@@ -294,9 +310,9 @@ __device__ __forceinline__ bool odd_values(uint32_t s, uint32_t z) {
 // no row sees tokens outside [lo, len)): tokens that no row sees, whose page rows may hold anything, get values 0.
 // A token whose values hold an infinity or NaN is taken by itself, into the rows that see it (the product would carry
 // it into every row, as 0 * inf), and then gets values 0 too.
-template <int D, bool BF, int T>
-__device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t& z, const u4_t (&p)[T], Acc<D, BF> (&acc)[T],
-                                              int k0, const int (&lim)[T], const int (&low)[T], int lo, int len) {
+template <int D, bool BF, int T, int MAPS>
+__device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t& z, const u4_t (&p)[T],
+                                              Acc<D, BF, MAPS> (&acc)[T], int o0, int k0, const int (&lim)[T], const int (&low)[T], int lo, int len) {
   const int quarter = (threadIdx.x & 63) >> 4;
   bool odd = false;
 #pragma unroll
@@ -336,8 +352,8 @@ __device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t&
       for (int w = 0; w < 4; ++w) pt[w] = p[g][w] & (w == e / 2 ? half : 0u);
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
-        const f4_t y = mma<BF>(x[j], pt, acc[g].o[j]);
-        if (sees) acc[g].o[j] = y;
+        const f4_t y = mma<BF>(x[j], pt, acc[g].o[o0 + j]);
+        if (sees) acc[g].o[o0 + j] = y;
       }
     }
 #pragma unroll
@@ -349,8 +365,9 @@ __device__ __forceinline__ void unseen_values(const u4_t (&c)[2], u4_t& s, u4_t&
   }
 }
 
-template <int D, bool BF, int T>
-__device__ __forceinline__ void values(VRegs& r, const f4_t (&s)[T][4], Acc<D, BF> (&acc)[T], bool mask, int tok0,
+// o0: the V head's first accumulator
+template <int D, bool BF, int T, int MAPS>
+__device__ __forceinline__ void values(VRegs& r, const f4_t (&s)[T][4], Acc<D, BF, MAPS> (&acc)[T], int o0, bool mask, int tok0,
                                        const int (&lim)[T], const int (&low)[T], int lo, int len) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -359,25 +376,26 @@ __device__ __forceinline__ void values(VRegs& r, const f4_t (&s)[T][4], Acc<D, B
     for (int g = 0; g < T; ++g)
       p[g] = u4_t{pack2<BF>(s[g][2 * h][0], s[g][2 * h][1]), pack2<BF>(s[g][2 * h][2], s[g][2 * h][3]),
                   pack2<BF>(s[g][2 * h + 1][0], s[g][2 * h + 1][1]), pack2<BF>(s[g][2 * h + 1][2], s[g][2 * h + 1][3])};
-    if (mask) unseen_values<D, BF, T>(r.c[h], r.s[h], r.z[h], p, acc, tok0 + h * 32, lim, low, lo, len);
+    if (mask) unseen_values<D, BF, T, MAPS>(r.c[h], r.s[h], r.z[h], p, acc, o0, tok0 + h * 32, lim, low, lo, len);
     u4_t x[D / 16];
     v_operands<D, BF>(r.c[h], r.s[h], r.z[h], x);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-      for (int g = 0; g < T; ++g) acc[g].o[j] = mma<BF>(x[j], p[g], acc[g].o[j]);
+      for (int g = 0; g < T; ++g) acc[g].o[o0 + j] = mma<BF>(x[j], p[g], acc[g].o[o0 + j]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// a slot of the workspace: R = 16 T rows of D sums, R maxima, R sums of weights
-template <int D, int R>
-__device__ __forceinline__ float* slot_of(float* ws, int i) { return ws + int64_t(i) * (R * D + 2 * R); }
+// a slot of the workspace: C = 16 T columns of W = MAPS D sums, C maxima, C sums of weights
+template <int W, int C>
+__device__ __forceinline__ float* slot_of(float* ws, int i) { return ws + int64_t(i) * (C * W + 2 * C); }
 
-template <int D, bool BF, int T>
+// R: rows of a tile
+template <int D, bool BF, int R>
 __device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, int tile, int r, int d, const float (&v)[8],
                                           float inv) {
-  const Row w = row_of<T>(a, tile, r);
+  const Row w = row_of<R>(a, tile, r);
   if (!w.real) return;
   u4_t x;
 #pragma unroll
@@ -390,21 +408,29 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, in
 // ends; D = 64 is faster so: 48 of 1500 tokens, bf16, 26 us against 30)
 constexpr int per_cu(int D, int T) { return T == 1 || D == 64 ? 2 : 1; }
 
+// the second map's factor of row r of a tile, negated
+template <int R>
+__device__ __forceinline__ float minus_lam(const AttnArgs& a, int head, int tile, int r) {
+  const Row w = row_of<R>(a, tile, r);
+  return w.real ? -a.lam[(int64_t(head) * a.nrep + w.head) * a.s_lam] : 0.f;
+}
+
 // a row's softmax, for the keys' weights: {maximum, 1 / sum}; a row without a sum gives weights of 0
 __device__ __forceinline__ void store_stats(const AttnArgs& a, int s, int head, int r, float mx, float sum) {
-  if (r < a.nrep)
+  if (r < a.nrep)  // (head: of the store)
     a.stats[(int64_t(s) * a.p.H + head) * a.nrep + r] = float2{mx == NEG_INF ? 0.f : mx, sum == 0.f ? 0.f : 1.f / sum};
 }
 
-// W: the logits and the rows' sums are kept, for weights_kernel
-template <int D, bool BF, int T, bool W>
+// W: the logits and the rows' sums are kept, for weights_kernel.  MAPS = 2: differential attention (see the end of the
+// file): KV heads in pairs, whose keys are the two maps' and whose V heads are the halves of one of 2 D dims.
+template <int D, bool BF, int T, bool W, int MAPS>
 __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a) {
-  constexpr int J = D / 16, R = ROWS * T;
-  __shared__ float so[WAVES][R][D + 4];
-  __shared__ float sm[WAVES][R], sl[WAVES][R];
+  constexpr int J = D / 16, C = ROWS * T, R = tile_rows<T, MAPS>(), DV = MAPS * D, NQ = MAPS == 1 ? T : MAPS;
+  __shared__ float so[WAVES][C][DV + 4];
+  __shared__ float sm[WAVES][C], sl[WAVES][C];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15,
             quarter = lane >> 4;
-  const int H = a.p.H;
+  const int H = a.heads;
   int u, u1, s = 0, first = 0;
   if (a.split) {
     const Part part = part_at(a, 0, 0);
@@ -428,10 +454,10 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
     if (a.p.lens[e] < 0 && threadIdx.x == 0) atomicOr(a.p.status, PAGED_BAD_TOKEN);
     const float zero[8] = {};
     const int rows = a.m * a.nrep, nh = a.split ? H : 1;
-    for (int i = threadIdx.x; i < nh * rows * (D / 8); i += THREADS) {
-      const int d = i % (D / 8) * 8, r = i / (D / 8) % rows;
-      const int h = a.split ? i / (D / 8) / rows : blockIdx.x / a.tiles % H;
-      store_row<D, BF, T>(a, e, h, r / R, r % R, d, zero, 0.f);
+    for (int i = threadIdx.x; i < nh * rows * (DV / 8); i += THREADS) {
+      const int d = i % (DV / 8) * 8, r = i / (DV / 8) % rows;
+      const int h = a.split ? i / (DV / 8) / rows : blockIdx.x / a.tiles % H;
+      store_row<D, BF, R>(a, e, h, r / R, r % R, d, zero, 0.f);
     }
   }
   while (u < u1) {
@@ -446,17 +472,16 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
     if (cnt <= 0) continue;
     const int head = hr / a.tiles, tile = hr - head * a.tiles;
     const int len = __builtin_amdgcn_readfirstlane(min(a.p.lens[s], a.p.P * PAGE));
-    // the query rows of this lane (16 g + l), their octets in the order of k_values' pairs
-    u4_t q[T][D / 32];  // (rows past the last repeat it and are not stored)
-    int lim[T], low[T];  // a row sees keys [low, lim)
-    Acc<D, BF> acc[T];
+    // the query rows of this lane's columns (16 g + l), their octets in the order of k_values' pairs
+    u4_t q[NQ][D / 32];  // (rows past the last repeat it and are not stored)
+    int lim[T], low[T];  // a column's row sees keys [low, lim)
+    Acc<D, BF, MAPS> acc[T];
 #pragma unroll
-    for (int g = 0; g < T; ++g) {
-      const Row row = row_of<T>(a, tile, ROWS * g + l);
-      lim[g] = len - (a.m - 1 - row.token);
-      low[g] = a.window ? lim[g] - a.window : 0;
+    for (int g = 0; g < NQ; ++g) {
+      const Row row = row_of<R>(a, tile, MAPS == 1 ? ROWS * g + l : l % R);
       const int token = min(row.token, a.m - 1), h = row.real ? row.head : a.nrep - 1;
-      const uint16_t* x = a.q + s * a.sq_s + token * a.sq_m + (int64_t(head) * a.nrep + h) * a.sq_h + quarter * (D / 4);
+      const uint16_t* x = a.q + s * a.sq_s + token * a.sq_m +
+                          ((int64_t(head) * a.nrep + h) * MAPS + (MAPS == 1 ? 0 : g)) * a.sq_h + quarter * (D / 4);
       u4_t w[D / 32];
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) w[j] = *reinterpret_cast<const u4_t*>(x + 8 * j);
@@ -465,8 +490,14 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           q[g][j][e] = __builtin_amdgcn_perm(w[j][e % 2 * 2 + 1], w[j][e % 2 * 2], e / 2 ? 0x07060302u : 0x05040100u);
+    }
 #pragma unroll
-      for (int j = 0; j < J; ++j) acc[g].o[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < T; ++g) {
+      const Row row = row_of<R>(a, tile, (ROWS * g + l) % R);
+      lim[g] = len - (a.m - 1 - row.token);
+      low[g] = a.window ? lim[g] - a.window : 0;
+#pragma unroll
+      for (int j = 0; j < MAPS * J; ++j) acc[g].o[j] = f4_t{0.f, 0.f, 0.f, 0.f};
       acc[g].m = NEG_INF;
       acc[g].l = 0.f;
     }
@@ -474,8 +505,8 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
     typedef const __attribute__((address_space(4))) int32_t* consts_t;
     const consts_t table = (consts_t)(a.p.table + s * a.p.s_table + lo + p0);
     const int mine = wave < cnt ? (cnt - wave + WAVES - 1) / WAVES : 0;  // this wave's pages: wave, wave + WAVES, ...
-    const uint32_t* pages = a.p.pages + int64_t(head) * page_words(D);
-    const int64_t stride = int64_t(H) * page_words(D);
+    const uint32_t* pages = a.p.pages + int64_t(head) * MAPS * page_words(D);
+    const int64_t stride = int64_t(a.p.H) * page_words(D);
     // the page of the wave's turn i: one outside the pool is not read and counts as NaN
     bool bad = false;
     if (a.p.lens[s] > a.p.P * PAGE) {  // more tokens than the table has pages for: NaN too
@@ -485,23 +516,32 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
     // past its last page a wave loads from a descriptor of no bytes: the loop has no branch that a load depends on,
     // which the wait counts would have to allow for
     auto id_of = [&](int i) { return i < mine ? table[wave + i * WAVES] : 0; };
+    struct Page {
+      rsrc_t head[MAPS];
+    };
     auto page_of = [&](int id, bool there) {
       const bool b = id < 0 || id >= a.p.n_pages;
       if (b && there) {
         bad = true;
         if (lane == 0) atomicOr(a.p.status, PAGED_BAD_PAGE);
       }
-      return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(pages + (b ? 0 : id) * stride), 0,
-                                               b || !there ? 0 : page_words(D) * 4, 0x00020000);
+      Page pg;
+#pragma unroll
+      for (int h = 0; h < MAPS; ++h)
+        pg.head[h] = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(pages + (b ? 0 : id) * stride + h * page_words(D)),
+                                                       0, b || !there ? 0 : page_words(D) * 4, 0x00020000);
+      return pg;
     };
     // K of the next page is on its way from the moment this page's logits are done, V from its product's end
     const Lane<D> at;
-    KRegs kr;
-    VRegs vr;
+    KRegs kr[MAPS];
+    VRegs vr[MAPS];
     {
-      const rsrc_t pg = page_of(id_of(0), mine > 0);
-      load_k<D>(pg, at, kr);
-      load_v<D>(pg, at, vr);
+      const Page pg = page_of(id_of(0), mine > 0);
+#pragma unroll
+      for (int h = 0; h < MAPS; ++h) load_k<D>(pg.head[h], at, kr[h]);
+#pragma unroll
+      for (int h = 0; h < MAPS; ++h) load_v<D>(pg.head[h], at, vr[h]);
     }
     const int see0 = a.window ? max(0, len - a.m + 1 - a.window) : 0;  // the first key that any row sees
     int id = id_of(1);
@@ -509,10 +549,11 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
       const int tok0 = (lo + p0 + wave + i * WAVES) * PAGE;
       const bool mask = tok0 + PAGE > len - a.m + 1 || (a.window && tok0 < len - a.window);
       f4_t w[T][4];
-      logits<D, BF, T>(kr, q, a.scale, w);
-      const rsrc_t next = page_of(id, i + 1 < mine);
+      logits<D, BF, T, MAPS, NQ>(kr, q, a.scale, w);
+      const Page next = page_of(id, i + 1 < mine);
       id = id_of(i + 2);
-      load_k<D>(next, at, kr);
+#pragma unroll
+      for (int h = 0; h < MAPS; ++h) load_k<D>(next.head[h], at, kr[h]);
       if (mask) {
 #pragma unroll
         for (int g = 0; g < T; ++g)
@@ -527,8 +568,8 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
       if constexpr (W) {
 #pragma unroll
         for (int g = 0; g < T; ++g) {
-          const int r = tile * R + ROWS * g + l;
-          float* to = a.logits + (((int64_t(s) * H + head) * a.p.P + tok0 / PAGE) * a.nrep + r) * PAGE + quarter * 4;
+          const int r = tile * R + (ROWS * g + l) % R, h = head * MAPS + (ROWS * g + l) / R;
+          float* to = a.logits + (((int64_t(s) * a.p.H + h) * a.p.P + tok0 / PAGE) * a.nrep + r) * PAGE + quarter * 4;
           if (r < a.nrep)
 #pragma unroll
             for (int t = 0; t < 4; ++t) *reinterpret_cast<f4_t*>(to + t * 16) = w[g][t];
@@ -536,10 +577,13 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int g = 0; g < T; ++g) weights<D, BF>(w[g], acc[g]);
+      for (int g = 0; g < T; ++g) weights<D, BF, MAPS>(w[g], acc[g]);
       __builtin_amdgcn_sched_barrier(0);
-      values<D, BF, T>(vr, w, acc, mask, tok0, lim, low, see0, len);
-      load_v<D>(next, at, vr);
+#pragma unroll
+      for (int h = 0; h < MAPS; ++h) {
+        values<D, BF, T, MAPS>(vr[h], w, acc, h * J, mask, tok0, lim, low, see0, len);
+        load_v<D>(next.head[h], at, vr[h]);
+      }
     }
     // the waves' sums
 #pragma unroll
@@ -554,39 +598,59 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
         sl[wave][ROWS * g + l] = sum;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int h = 0; h < MAPS; ++h)
 #pragma unroll
-        for (int j = 0; j < J; j += 4)
-          *reinterpret_cast<f4_t*>(&so[wave][ROWS * g + l][(quarter * 4 + i) * J + j]) =
-              f4_t{acc[g].o[j][i], acc[g].o[j + 1][i], acc[g].o[j + 2][i], acc[g].o[j + 3][i]};
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < J; j += 4)
+            *reinterpret_cast<f4_t*>(&so[wave][ROWS * g + l][h * D + (quarter * 4 + i) * J + j]) =
+                f4_t{acc[g].o[h * J + j][i], acc[g].o[h * J + j + 1][i], acc[g].o[h * J + j + 2][i], acc[g].o[h * J + j + 3][i]};
     }
     __syncthreads();
     const bool whole = cnt == n;
-    float* slot = whole ? nullptr : slot_of<D, R>(a.ws, 2 * blockIdx.x + (p0 == 0 ? 1 : 0));
-    for (int i = threadIdx.x; i < R * (D / 8); i += THREADS) {
-      const int rr = i / (D / 8), d = i % (D / 8) * 8;
-      float mx = NEG_INF;
+    float* slot = whole ? nullptr : slot_of<DV, C>(a.ws, 2 * blockIdx.x + (p0 == 0 ? 1 : 0));
+    // 8 dims of a column over the waves
+    auto merge = [&](int c, int d, float& mx, float& sum, float (&v)[8]) {
+      mx = NEG_INF;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, sm[w][rr]);
-      float sum = 0.f, v[8] = {};
+      for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, sm[w][c]);
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
-        const float f = sm[w][rr] == NEG_INF ? 0.f : exp2f(sm[w][rr] - mx);
-        sum += sl[w][rr] == 0.f ? 0.f : sl[w][rr] * (sl[w][rr] != sl[w][rr] ? 1.f : f);
+        const float f = sm[w][c] == NEG_INF ? 0.f : exp2f(sm[w][c] - mx);
+        sum += sl[w][c] == 0.f ? 0.f : sl[w][c] * (sl[w][c] != sl[w][c] ? 1.f : f);
         if (f != 0.f)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += f * so[w][rr][d + e];
+          for (int e = 0; e < 8; ++e) v[e] += f * so[w][c][d + e];
       }
+    };
+    for (int i = threadIdx.x; i < (MAPS == 2 && whole ? R : C) * (DV / 8); i += THREADS) {
+      const int rr = i / (DV / 8), d = i % (DV / 8) * 8;
+      float mx, sum, v[8];
+      merge(rr, d, mx, sum, v);
       if (whole) {
-        store_row<D, BF, T>(a, s, head, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
         if constexpr (W)
-          if (d == 0) store_stats(a, s, head, tile * R + rr, mx, sum);
+          if (d == 0) store_stats(a, s, head * MAPS, tile * R + rr, mx, sum);
+        float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if constexpr (MAPS == 2) {
+          float mx2, sum2, v2[8];
+          merge(R + rr, d, mx2, sum2, v2);
+          if constexpr (W)
+            if (d == 0) store_stats(a, s, head * MAPS + 1, tile * R + rr, mx2, sum2);
+          const float f = minus_lam<R>(a, head, tile, rr) * (sum2 == 0.f ? 0.f : 1.f / sum2);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = v[e] * inv + f * v2[e];
+          inv = 1.f;
+        }
+        store_row<D, BF, R>(a, s, head, tile, rr, d, v, inv);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) slot[rr * D + d + e] = v[e];
+        for (int e = 0; e < 8; ++e) slot[rr * DV + d + e] = v[e];
         if (d == 0) {
-          slot[R * D + rr] = mx;
-          slot[R * D + R + rr] = sum;
+          slot[C * DV + rr] = mx;
+          slot[C * DV + C + rr] = sum;
         }
       }
     }
@@ -599,10 +663,10 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
 }
 
 // one workgroup per (sequence, head, tile): merges the slots of those that several workgroups computed, in order
-template <int D, bool BF, int T, bool W>
-__global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a) {
-  constexpr int R = ROWS * T;
-  const int per_seq = a.p.H * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
+template <int D, bool BF, int T, bool W, int MAPS>
+__global__ __launch_bounds__(ROWS * T * (MAPS * D / 8)) void combine_kernel(AttnArgs a) {
+  constexpr int C = ROWS * T, R = tile_rows<T, MAPS>(), DV = MAPS * D;
+  const int per_seq = a.heads * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
   Part part = part_at(a, 0, 0);
   const int total = total_units(a, part), per = units_per_group(total, a.grid);
   for (int s0 = 64 * a.each; s0 <= s; s0 += 64 * a.each) part = part_at(a, s0, __builtin_amdgcn_readlane(part.end, 63));
@@ -612,9 +676,11 @@ __global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a)
   if (n <= 0) return;
   const int u0 = end - units + hr * n, g0 = (u0 + PAD) / per, g1 = (u0 + n - 1) / per;
   if (g0 == g1) return;
-  // lanes of D/8 take a row's dims, `parts` of them its slots in runs
-  const int tile = hr % a.tiles, rows = min(R, a.m * a.nrep - tile * R), parts = g1 - g0 < 4 ? 1 : R / rows;
-  const int grp = threadIdx.x / (D / 8), part_i = grp / rows, rr = grp - part_i * rows, d = threadIdx.x % (D / 8) * 8;
+  // lanes of DV/8 take a column's dims, `parts` of them its slots in runs
+  const int tile = hr % a.tiles, per_map = min(R, a.m * a.nrep - tile * R), rows = MAPS * per_map;
+  const int parts = g1 - g0 < 4 ? 1 : C / rows;
+  const int grp = threadIdx.x / (DV / 8), part_i = grp / rows, ri = grp - part_i * rows, d = threadIdx.x % (DV / 8) * 8;
+  const int map = MAPS == 1 ? 0 : ri / per_map, r = ri - map * per_map, rr = map * R + r;
   const int run = (g1 - g0 + parts) / parts, ga = g0 + part_i * run, gz = part_i < parts ? min(ga + run - 1, g1) : -1;
   constexpr int B = 4;  // slots whose loads are under way together
   float mx = NEG_INF, sum = 0.f, v[8] = {};
@@ -624,11 +690,11 @@ __global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a)
 #pragma unroll
     for (int i = 0; i < B; ++i) {
       const int gi = min(g + i, gz);
-      const float* p = slot_of<D, R>(a.ws, 2 * gi + (gi == g0 ? 1 : 0));
-      m[i] = p[R * D + rr];
-      l[i] = p[R * D + R + rr];
-      x[i][0] = *reinterpret_cast<const f4_t*>(p + rr * D + d);
-      x[i][1] = *reinterpret_cast<const f4_t*>(p + rr * D + d + 4);
+      const float* p = slot_of<DV, C>(a.ws, 2 * gi + (gi == g0 ? 1 : 0));
+      m[i] = p[C * DV + rr];
+      l[i] = p[C * DV + C + rr];
+      x[i][0] = *reinterpret_cast<const f4_t*>(p + rr * DV + d);
+      x[i][1] = *reinterpret_cast<const f4_t*>(p + rr * DV + d + 4);
     }
     const float was = mx;
 #pragma unroll
@@ -647,7 +713,7 @@ __global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a)
         for (int e = 0; e < 8; ++e) v[e] += f * x[i][e / 4][e % 4];
     }
   }
-  __shared__ float sv[R][D], sm[R], sl[R];
+  __shared__ float sv[C][DV], sm[C], sl[C];
   if (parts > 1) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) sv[grp][d + e] = v[e];
@@ -656,9 +722,8 @@ __global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a)
       sl[grp] = sum;
     }
     __syncthreads();
-    if (part_i > 0) return;
-    for (int i = 1; i < parts; ++i) {
-      const int o = i * rows + rr;
+    for (int i = 1; i < (part_i > 0 ? 1 : parts); ++i) {
+      const int o = i * rows + ri;
       const float was = mx;
       mx = fmaxf(mx, sm[o]);
       const float keep = was == NEG_INF ? 0.f : exp2f(was - mx), f = sm[o] == NEG_INF ? 0.f : exp2f(sm[o] - mx);
@@ -667,10 +732,25 @@ __global__ __launch_bounds__(ROWS * T * (D / 8)) void combine_kernel(AttnArgs a)
       for (int e = 0; e < 8; ++e) v[e] = keep * v[e] + (f != 0.f ? f * sv[o][d + e] : 0.f);
     }
   }
-  if (part_i > 0) return;
-  store_row<D, BF, T>(a, s, hr / a.tiles, tile, rr, d, v, sum == 0.f ? 0.f : 1.f / sum);
+  const int head = hr / a.tiles;
+  float inv = sum == 0.f ? 0.f : 1.f / sum;
   if constexpr (W)
-    if (d == 0) store_stats(a, s, hr / a.tiles, tile * R + rr, mx, sum);
+    if (part_i == 0 && d == 0) store_stats(a, s, head * MAPS + map, tile * R + r, mx, sum);
+  if constexpr (MAPS == 2) {
+    if (parts > 1) __syncthreads();  // nobody reads the parts any more
+    if (part_i == 0 && map == 1) {
+      const float f = minus_lam<R>(a, head, tile, r) * inv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sv[r][d + e] = f * v[e];
+    }
+    __syncthreads();
+    if (map == 0)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * inv + sv[r][d + e];
+    inv = 1.f;
+  }
+  if (part_i > 0 || map > 0) return;
+  store_row<D, BF, R>(a, s, head, tile, r, d, v, inv);
 }
 
 // Adds each key's softmax weights, over a KV head's query rows, to what it has gathered: from the logits that attn_kernel
@@ -715,17 +795,21 @@ struct Launch {
 //   of 4032 (P = 63)                64: 61 / 63, but of 50 .. 4096 tokens 48 / 36
 // The lengths are on the device, so the table's width P stands for them: a caller whose tables are wider than any sequence
 // passes the columns that are needed (16 sequences of 500 tokens: P = 8 8.2 us, P = 512 13.2; bf16 10.8, 16.7).
-inline Launch plan_of(int S, int P, int m, int nrep, int H, int D) {
-  const int64_t rows = int64_t(m) * nrep, pages = int64_t(S) * H * P * ceil_div(rows, ROWS);
+// Two maps: a group for each where there are more than 8 rows (a tile of 8 would read its pages again for the others).
+inline Launch plan_of(int S, int P, int m, int nrep, int heads, int D, int maps) {
+  const int64_t rows = int64_t(m) * nrep, pages = int64_t(S) * heads * P * ceil_div(rows, ROWS);
   Launch p;
-  p.T = rows > ROWS && pages >= 8192 ? 2 : 1;
-  p.tiles = int(ceil_div(rows, ROWS * p.T));
-  const int64_t items = int64_t(S) * H * p.tiles;
+  p.T = maps == 2 ? (rows > ROWS / 2 ? 2 : 1) : rows > ROWS && pages >= 8192 ? 2 : 1;
+  p.tiles = int(ceil_div(rows, ROWS * p.T / maps));
+  const int64_t items = int64_t(S) * heads * p.tiles;
   p.split = P > (items >= 256 ? 32 : items >= 64 ? 16 : 8);
   p.grid = p.split ? GRID / 2 * per_cu(D, p.T) : int(items);
   return p;
 }
 
+inline size_t slots_bytes(const Launch& p, int D, int maps) {
+  return p.split ? size_t(2 * GRID) * (ROWS * p.T) * (maps * D + 2) * sizeof(float) : 0;
+}
 inline size_t stats_bytes(int S, int Hq) { return (size_t(S) * Hq * sizeof(float2) + 15) / 16 * 16; }
 
 }  // namespace
@@ -734,46 +818,52 @@ namespace iq {
 int check_paged(const iq_paged* p);
 }
 
-extern "C" size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D) {
-  if (S <= 0 || P <= 0 || m <= 0 || Hq <= 0 || H <= 0 || Hq % H || !d_ok(D)) return 0;
-  const Launch p = plan_of(S, P, m, Hq / H, H, D);
-  return p.split ? size_t(2 * GRID) * (ROWS * p.T) * (D + 2) * sizeof(float) : 0;
-}
-
-extern "C" size_t iq_paged_attention_weights_workspace_bytes(int S, int P, int Hq, int H, int D) {
-  if (S <= 0 || P <= 0 || Hq <= 0 || H <= 0 || Hq % H || !d_ok(D)) return 0;
-  return iq_paged_attention_workspace_bytes(S, P, 1, Hq, H, D) + stats_bytes(S, Hq) + size_t(S) * Hq * P * PAGE * sizeof(float);
-}
-
 namespace {
-int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq, float scale,
-              int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h, float* weights, int64_t sw_s, int64_t sw_h,
-              void* workspace, size_t workspace_bytes, void* stream) {
-  IQ_CHECK(q && out, IQ_ERR_NULL);
-  IQ_CHECK(m > 0 && m <= 16 && Hq > 0 && Hq % p->H == 0 && Hq <= 4096 && window >= 0, IQ_ERR_SHAPE);
+// slots, then for the keys' weights the rows' statistics and the logits
+size_t workspace_bytes_of(int S, int P, int m, int Hq, int H, int D, int maps, bool weights) {
+  if (S <= 0 || P <= 0 || m <= 0 || Hq <= 0 || H <= 0 || Hq % H || H % maps || !d_ok(D)) return 0;
+  const size_t slots = slots_bytes(plan_of(S, P, m, Hq / H, H / maps, D, maps), D, maps);
+  return weights ? slots + stats_bytes(S, Hq) + size_t(S) * Hq * P * PAGE * sizeof(float) : slots;
+}
+
+template <int MAPS>
+int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq, const float* lam,
+              int64_t s_lam, float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h, float* weights,
+              int64_t sw_s, int64_t sw_h, int64_t Tw, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int st = iq::check_paged(p)) return st;
+  IQ_CHECK(q && out && (MAPS == 1 || lam), IQ_ERR_NULL);
+  IQ_CHECK(m > 0 && m <= 16 && Hq > 0 && Hq % p->H == 0 && p->H % MAPS == 0 && Hq <= 4096 && window >= 0 && s_lam >= 0,
+           IQ_ERR_SHAPE);
   IQ_CHECK(aligned(q, 16) && aligned(out, 16) && sq_s % 8 == 0 && sq_m % 8 == 0 && sq_h % 8 == 0 && so_s % 8 == 0 &&
-               so_m % 8 == 0 && so_h % 8 == 0, IQ_ERR_ALIGN);
-  const int nrep = Hq / p->H;
-  const Launch pl = plan_of(p->S, p->P, m, nrep, p->H, p->D);
-  IQ_CHECK(int64_t(p->S) * (p->P + PAD) * p->H * pl.tiles <= INT32_MAX &&
-               int64_t(p->S) * p->H * pl.tiles <= UINT32_MAX / 512, IQ_ERR_SHAPE);
-  const size_t slots = iq_paged_attention_workspace_bytes(p->S, p->P, m, Hq, p->H, p->D);
-  const size_t need = weights ? iq_paged_attention_weights_workspace_bytes(p->S, p->P, Hq, p->H, p->D) : slots;
+               so_m % 8 == 0 && so_h % 8 == 0 && aligned(lam, 4), IQ_ERR_ALIGN);
+  const int nrep = Hq / p->H, heads = p->H / MAPS;
+  const Launch pl = plan_of(p->S, p->P, m, nrep, heads, p->D, MAPS);
+  IQ_CHECK(int64_t(p->S) * (p->P + PAD) * heads * pl.tiles <= INT32_MAX &&
+               int64_t(p->S) * heads * pl.tiles <= UINT32_MAX / (ROWS * 2 * MAPS * 16), IQ_ERR_SHAPE);
+  const int64_t chunks = ceil_div(p->P, WAVES * WEIGH_PAGES);  // of weights_kernel, per (sequence, head)
+  if (weights) {
+    IQ_CHECK(m == 1 && Tw >= int64_t(p->P) * PAGE && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
+    IQ_CHECK(int64_t(p->S) * p->H * chunks <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
+    IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
+  }
+  const size_t need = workspace_bytes_of(p->S, p->P, m, Hq, p->H, p->D, MAPS, weights != nullptr);
   IQ_CHECK(!need || (workspace && workspace_bytes >= need), IQ_ERR_WORKSPACE);
   IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   if (window >= p->P * PAGE) window = 0;  // hides nothing
-  const int64_t chunks = ceil_div(p->P, WAVES * WEIGH_PAGES);  // of weights_kernel, per (sequence, head)
-  IQ_CHECK(!weights || int64_t(p->S) * p->H * chunks <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
-  char* const ws = (char*)workspace;
-  const AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, m, nrep, pl.tiles,
-                   scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, p->S > 64 ? EACH : 1, pl.split,
-                   weights ? (float*)(ws + slots + stats_bytes(p->S, Hq)) : nullptr,
-                   weights ? (float2*)(ws + slots) : nullptr, weights, sw_s, sw_h};
+  AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, heads, m, nrep, pl.tiles,
+             scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, p->S > 64 ? EACH : 1, pl.split, lam, s_lam,
+             nullptr, nullptr, weights, sw_s, sw_h};
+  if (weights) {
+    char* const ws = (char*)workspace + slots_bytes(pl, p->D, MAPS);
+    a.stats = (float2*)ws;
+    a.logits = (float*)(ws + stats_bytes(p->S, Hq));
+  }
   auto launch = [&]<int D, bool BF, int T, bool W>() {
-    attn_kernel<D, BF, T, W><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
+    attn_kernel<D, BF, T, W, MAPS><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
     if (const int st = launch_status()) return st;
     if (pl.split)
-      combine_kernel<D, BF, T, W><<<p->S * p->H * pl.tiles, ROWS * T * (D / 8), 0, (hipStream_t)stream>>>(a);
+      combine_kernel<D, BF, T, W, MAPS>
+          <<<p->S * heads * pl.tiles, ROWS * T * (MAPS * D / 8), 0, (hipStream_t)stream>>>(a);
     if (const int st = launch_status()) return st;
     if constexpr (W) {
       weights_kernel<<<unsigned(int64_t(p->S) * p->H * chunks), THREADS, 0, (hipStream_t)stream>>>(a, int(chunks));
@@ -786,26 +876,46 @@ int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int6
     return pl.T == 2 ? launch.template operator()<D, BF, 2, false>() : launch.template operator()<D, BF, 1, false>();
   };
   const bool bf = act_bf16(p->mode);
-  if (p->D == 128) return bf ? with.operator()<128, true>() : with.operator()<128, false>();
-  return bf ? with.operator()<64, true>() : with.operator()<64, false>();
+  if (p->D == 128) return bf ? with.template operator()<128, true>() : with.template operator()<128, false>();
+  return bf ? with.template operator()<64, true>() : with.template operator()<64, false>();
 }
 }  // namespace
+
+extern "C" size_t iq_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D) {
+  return workspace_bytes_of(S, P, m, Hq, H, D, 1, false);
+}
 
 extern "C" int iq_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
                                   float scale, int window, void* out, int64_t so_s, int64_t so_m, int64_t so_h,
                                   void* workspace, size_t workspace_bytes, void* stream) {
-  if (const int st = iq::check_paged(p)) return st;
-  return attention(p, q, sq_s, sq_m, sq_h, m, Hq, scale, window, out, so_s, so_m, so_h, nullptr, 0, 0, workspace,
-                   workspace_bytes, stream);
+  return attention<1>(p, q, sq_s, sq_m, sq_h, m, Hq, nullptr, 0, scale, window, out, so_s, so_m, so_h, nullptr, 0, 0, 0,
+                      workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t iq_paged_attention_weights_workspace_bytes(int S, int P, int Hq, int H, int D) {
+  return workspace_bytes_of(S, P, 1, Hq, H, D, 1, true);
 }
 
 extern "C" int iq_paged_attention_weights(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_h, int Hq, float scale,
                                           int window, void* out, int64_t so_s, int64_t so_h, float* weights, int64_t sw_s,
                                           int64_t sw_h, int64_t T, void* workspace, size_t workspace_bytes, void* stream) {
-  if (const int st = iq::check_paged(p)) return st;
   IQ_CHECK(weights, IQ_ERR_NULL);
-  IQ_CHECK(T >= int64_t(p->P) * PAGE && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
-  IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
-  return attention(p, q, sq_s, 0, sq_h, 1, Hq, scale, window, out, so_s, 0, so_h, weights, sw_s, sw_h, workspace,
-                   workspace_bytes, stream);
+  return attention<1>(p, q, sq_s, 0, sq_h, 1, Hq, nullptr, 0, scale, window, out, so_s, 0, so_h, weights, sw_s, sw_h, T,
+                      workspace, workspace_bytes, stream);
+}
+
+// Differential attention (MAPS = 2).  KV heads 2g, 2g + 1 of a page are the keys of the two maps and the two halves of V; a
+// workgroup takes a pair, so each page is read once for both maps.  Up to 8 rows of both maps share the 16 columns of a group
+// (one softmax, one product with V for both), more take a group for each map.  Their sums stay apart until the waves, or the
+// workgroups, are merged: then out = first / sum - lam second / sum in fp32.
+extern "C" size_t iq_diff_paged_attention_workspace_bytes(int S, int P, int m, int Hq, int H, int D, int weights) {
+  return workspace_bytes_of(S, P, m, Hq, H, D, 2, weights != 0);
+}
+
+extern "C" int iq_diff_paged_attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int64_t sq_h, int m, int Hq,
+                                       const float* lam, int64_t s_lam, float scale, int window, void* out, int64_t so_s,
+                                       int64_t so_m, int64_t so_h, float* weights, int64_t sw_s, int64_t sw_h, int64_t T,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  return attention<2>(p, q, sq_s, sq_m, sq_h, m, Hq, lam, s_lam, scale, window, out, so_s, so_m, so_h, weights, sw_s, sw_h, T,
+                      workspace, workspace_bytes, stream);
 }

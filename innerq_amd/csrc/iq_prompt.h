@@ -60,6 +60,7 @@ struct WeighArgs {
   int S, N, Nk, Hq, nrep, slots;
   Scale scale;
   int causal, window;
+  int maps;  // 2: differential attention, KV head 2g + i's rows are those of query heads 2j + i, j in its group
 };
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream);
 

@@ -24,6 +24,7 @@ __global__ __launch_bounds__(THREADS, 2) void weigh_kernel(WeighArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
   const int kw = wave & 1, rw = wave >> 1;
   const int H = gridDim.x / a.slots, kvh = blockIdx.x % H, slot = blockIdx.x / H;
+  const int head0 = kvh / a.maps * a.nrep * a.maps + kvh % a.maps;  // its query heads: head0 + i * maps
   // sequence s has the slots from first_slot(s) to first_slot(s + 1), at least as many as it has tiles of keys
   auto first_slot = [&](int i) { return min(max(a.cu_k[i], 0), a.Nk) / BK + i; };
   int s = 0;
@@ -63,11 +64,11 @@ __global__ __launch_bounds__(THREADS, 2) void weigh_kernel(WeighArgs a) {
   auto fetch = [&](int t, u4_t* lds) {
     const int first = (v0 + t * BR) / a.nrep;  // the descriptor begins at the tile's first row
     const rsrc_t d = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint16_t*>(a.q + int64_t(q0 + first) * a.sq_n + kvh * a.nrep * a.sq_h), 0, -1, 0x00020000);
+        const_cast<uint16_t*>(a.q + int64_t(q0 + first) * a.sq_n + head0 * a.sq_h), 0, -1, 0x00020000);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int v = min(v0 + t * BR + i * (THREADS / CH) + fr, v1 - 1), row = v / a.nrep, head = v - row * a.nrep;
-      const uint32_t at = uint32_t(row - first) * uint32_t(a.sq_n) * 2 + uint32_t(head) * uint32_t(a.sq_h) * 2 + fc;
+      const uint32_t at = uint32_t(row - first) * uint32_t(a.sq_n) * 2 + uint32_t(head * a.maps) * uint32_t(a.sq_h) * 2 + fc;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)(lds + i * THREADS + wave * 64), 16,
                                                at, 0, 0, 0);
     }
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(THREADS, 2) void weigh_kernel(WeighArgs a) {
   };
   auto row_of = [&](int t) {
     const int v = v0 + t * BR + rw * 32 + n, w = min(v, v1 - 1), row = w / a.nrep;
-    return Row{row, v < v1, a.stats[int64_t(q0 + row) * a.Hq + kvh * a.nrep + w - row * a.nrep]};
+    return Row{row, v < v1, a.stats[int64_t(q0 + row) * a.Hq + head0 + (w - row * a.nrep) * a.maps]};
   };
   auto add_tile = [&](int t, const u4_t* lds, const Row& r) {
     u4_t x[KS];

@@ -1020,7 +1020,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
 def diff_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, lam: torch.Tensor,
                           scale: float, cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = True,
-                          window: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                          window: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                          weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Differential attention of prompts that lie one behind the other: output head j is
 
         (softmax(q[2j] K[2g]^T * scale) - lam[j] * softmax(q[2j+1] K[2g+1]^T * scale)) V[g],    g = j // (Hq // H).
@@ -1029,11 +1030,13 @@ def diff_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
     output head); returns [N, Hq/2, 2 D], ``out`` or a new tensor.  H is even, Hq a multiple of H, D 64 or 128.  Lengths,
     ``causal`` and ``window`` as in prompt_attention, for both maps.  A map that sees no key, or only keys whose logits
     are minus infinity, counts as 0; rows outside the sequences are not written.  ``out`` takes memory that no argument
-    uses.  Inference only: tensors that autograd follows are refused, ``out`` too.
+    uses.  weights: as prompt_attention's, fp32 [S, H, T]: each KV head's keys gather the weights of its own map, whatever
+    lam (PagedStore.evict(shared=2) keeps the same tokens for both).  Inference only: tensors that autograd follows are
+    refused, ``out`` too.
 
     The steps behind such a prompt are PagedStore.diff_attend's: store.append(k, v.view(Nk, H, D), ...)."""
     require_act(q, "q")
-    if autograd_follows(q, k, v, lam, out):
+    if autograd_follows(q, k, v, lam, out, weights):
         raise NotImplementedError("diff_prompt_attention has no backward: call it under torch.no_grad()")
     if q.dim() != 3 or k.dim() != 3:
         _shape_error(f"q must be [N, Hq, D] and k [Nk, H, D], got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -1064,10 +1067,19 @@ def diff_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
         check_out(out.shape, (N, Hq // 2, 2 * D))
         if out.device != dev or not writable_rows(out):
             _shape_error("out needs a contiguous head_dim, rows on 16-byte boundaries and q's device")
+    if weights is not None:
+        check_weights(weights, "weights", S, H, 0, dev, written=True)
+        if q.stride(1) * (Hq // H) >= 2 ** 29:
+            q = q.clone(memory_format=torch.contiguous_format)
+    kept = weights is not None and weights.numel() > 0
+    nbytes = _lib.lib().iq_prompt_weights_workspace_bytes(N, Hq) if kept else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if kept else None
     with on_device(dev):
         call("iq_diff_prompt_attention", _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
              v.stride(1), _p(lam), lam.stride(0), _p(cu_q), _p(cu_k), S, N, Nk, Hq, H, D, act_flag(q.dtype), float(scale),
-             1 if causal else 0, window or 0, _p(out), out.stride(0), out.stride(1), _stream(dev))
+             1 if causal else 0, window or 0, _p(out), out.stride(0), out.stride(1),
+             *((_p(weights), weights.stride(0), weights.stride(1), weights.shape[2]) if kept else (None, 0, 0, 0)), _p(ws), nbytes,
+             _stream(dev))
     return out
 
 

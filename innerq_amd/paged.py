@@ -291,6 +291,54 @@ class PagedStore:
                  ops._p(out), os[0], os[1], os[2], ops._p(ws), nbytes, ops._stream(self.device))
         return out
 
+    def diff_attend(self, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, lam: torch.Tensor, scale: float,
+                    window: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                    weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Differential attention over each sequence's first lens[s] tokens, for a store of an even number of heads: output
+        head j is
+
+            (softmax(q[2j] K[2g]^T * scale) - lam[j] * softmax(q[2j+1] K[2g+1]^T * scale)) [V[2g] | V[2g+1]],
+
+        g = j // (Hq // H), where ``append`` took V [N, H/2, 2 D] as [N, H, D].  q [S, Hq, D] or [S, m, Hq, D], Hq a multiple
+        of H; lam fp32 [Hq/2] on the device (learned: a model's own number per output head); returns [S, Hq/2, 2 D] or
+        [S, m, Hq/2, 2 D], ``out`` (memory that no argument uses) or a new tensor.  Everything else as attend(), for both
+        maps: a map that sees no token, or only tokens whose logits are minus infinity, counts as 0.
+
+        weights: as attend()'s, fp32 [S, H, T]: each KV head's tokens gather the weights of its own map, whatever lam
+        (evict(shared=2) keeps the same tokens for both)."""
+        _no_grad(q, out, lam, weights)
+        p = self._args(table, lens)
+        if q.dim() not in (3, 4) or q.shape[0] != p.S:
+            raise ValueError(f"diff_attend: q must be [S, Hq, D] or [S, m, Hq, D] with S = {p.S}, got {tuple(q.shape)}")
+        m, Hq = (1, q.shape[1]) if q.dim() == 3 else (q.shape[1], q.shape[2])
+        if not 0 < m <= MAX_NEW:
+            raise ValueError(f"diff_attend: 1 to {MAX_NEW} new tokens per sequence, got {m} (more: read() and "
+                             "ops.diff_prompt_attention)")
+        ops.check_diff_heads(Hq, self.H)
+        if window is not None and not 0 < window < 2 ** 31:
+            raise ValueError(f"diff_attend: window must be positive, got {window}")
+        ops.check_lam(lam, Hq // 2, self.device)
+        q = _rows(q, "q", (*q.shape[:-1], self.D), self.dtype, self.device)
+        want = (*q.shape[:-2], Hq // 2, 2 * self.D)
+        if out is None:
+            out = torch.empty(want, dtype=self.dtype, device=self.device)
+        else:
+            _out_rows(out, "out", want, self.dtype, self.device)
+        if weights is not None:
+            if m > 1:
+                raise ValueError(f"diff_attend: weights are added up for one new token per sequence, got {m}")
+            ops.check_weights(weights, "weights", p.S, self.H, p.P * PAGE_TOKENS, self.device, written=True)
+        qs, os = (t.stride() if t.dim() == 4 else (t.stride(0), 0, t.stride(1)) for t in (q, out))
+        nbytes = _lib.lib().iq_diff_paged_attention_workspace_bytes(p.S, p.P, m, Hq, self.H, self.D, weights is not None)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        with ops.on_device(self.device):
+            call("iq_diff_paged_attention", ctypes.byref(p), ops._p(q), qs[0], qs[1], qs[2], m, Hq, ops._p(lam), lam.stride(0),
+                 float(scale), window or 0, ops._p(out), os[0], os[1], os[2],
+                 *((None, 0, 0, 0) if weights is None else
+                   (ops._p(weights), weights.stride(0), weights.stride(1), weights.shape[2])),
+                 ops._p(ws), nbytes, ops._stream(self.device))
+        return out
+
     def evict(self, table: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor, keep: int, recent: int = 0,
               sinks: int = 0, shared: int = 1, out: Optional[torch.Tensor] = None,
               lens_out: Optional[torch.Tensor] = None):
