@@ -21,6 +21,11 @@ inline Scale scale_of(float scale) {
   return {c == 0 ? 1.f : c < 0 ? -c : c, c == 0 ? 0u : ~0u, c < 0 ? 0x80008000u : 0u};
 }
 
+// 16 bytes per lane from the descriptor's byte `at` (per lane) to LDS, lane by lane from `lds` on, without registers
+__device__ __forceinline__ void load_to_lds(rsrc_t d, u4_t* lds, uint32_t at) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)lds, 16, at, 0, 0, 0);
+}
+
 // rows [r0, r1) of sequence s in a packed tensor of n rows (whatever cu holds)
 __device__ __forceinline__ void rows_of(const int32_t* cu, int s, int n, int& r0, int& r1) {
   r0 = min(max(cu[s], 0), n);
@@ -61,7 +66,12 @@ struct WeighArgs {
   Scale scale;
   int causal, window;
   int maps;  // 2: differential attention, KV head 2g + i's rows are those of query heads 2j + i, j in its group
+  // set by launch_prompt_weights: rows (times heads) of a workgroup, and where several share a key, their sums [..][H][Nk]
+  int chunk;
+  float* part;
 };
+// its workspace: the stats, then the sums
+size_t prompt_weights_bytes(int N, int Nk, int Hq, int H);
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream);
 
 }  // namespace iq

@@ -424,7 +424,7 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
   const int64_t slots = rows / BM + S;  // first_slot(S) at most
   IQ_CHECK(slots * H <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
   if (weights) {
-    IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(N, Hq), IQ_ERR_WORKSPACE);
+    IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(N, Nk, Hq, H), IQ_ERR_WORKSPACE);
     IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   }
   if (window >= Nk) window = 0;  // hides nothing
@@ -441,13 +441,13 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
                           : (bf ? launch.operator()<64, true>() : launch.operator()<64, false>());
   if (st || !weights || !Nk) return st;
   return launch_prompt_weights({a.q, a.k, sq_n, sq_h, sk_n, sk_h, a.stats, weights, sw_s, sw_h, T, cu_q, cu_k, S, N, Nk, Hq,
-                                Hq / H, 0, sc, causal ? 1 : 0, window, 1}, D, bf, (hipStream_t)stream);
+                                Hq / H, 0, sc, causal ? 1 : 0, window, 1, 0, nullptr}, D, bf, (hipStream_t)stream);
 }
 
 }  // namespace
 
-extern "C" size_t iq_prompt_weights_workspace_bytes(int N, int Hq) {
-  return N <= 0 || Hq <= 0 ? 0 : size_t(N) * Hq * sizeof(float2);
+extern "C" size_t iq_prompt_weights_workspace_bytes(int N, int Nk, int Hq, int H) {
+  return N <= 0 || Nk < 0 || Hq <= 0 || H <= 0 || Hq % H ? 0 : iq::prompt_weights_bytes(N, Nk, Hq, H);
 }
 
 extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
