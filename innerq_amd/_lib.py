@@ -126,7 +126,7 @@ SIGNATURES = {
     "iq_paged_attention_weights_workspace_bytes": (S, [I, I, I, I, I]),
     "iq_paged_attention_weights": (I, [ctypes.POINTER(iq_paged), P, L, L, I, F, I, P, L, L, P, L, L, L, P, S, P]),
     "iq_prompt_attention": (I, [P, L, L, P, L, L, P, L, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P]),
-    "iq_prompt_weights_workspace_bytes": (S, [I, I, I, I]),
+    "iq_prompt_weights_workspace_bytes": (S, [I, I, I, I, I, I]),
     "iq_prompt_attention_weights": (I, [P, L, L, P, L, L, P, L, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P, L, L, L, P, S,
                                         P]),
     "iq_diff_prompt_attention": (I, [P, L, L, P, L, L, P, L, L, P, L, P, P, I, I, I, I, I, I, I, F, I, I, P, L, L, P, L, L, L,

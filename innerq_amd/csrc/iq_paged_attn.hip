@@ -49,8 +49,8 @@ struct AttnArgs {
   int split;           // 0: a workgroup takes a whole (sequence, head, tile)
   const float* lam;    // of each output head (MAPS = 2)
   int64_t s_lam;
-  // where the keys' weights are wanted (m = 1): the logits [S][H][P][nrep][64], {maximum, 1 / sum} of each row
-  // [S][H][nrep], and the weights to add to, fp32 [S][H][>= 64 P]
+  // where the keys' weights are wanted (m = 1): the logits [S][H][P][16][nrep][4 tokens], {maximum, 1 / sum} of each
+  // row [S][H][nrep], and the weights to add to, fp32 [S][H][>= 64 P]
   float* logits;
   float2* stats;
   float* weights;
@@ -543,6 +543,14 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
 #pragma unroll
       for (int h = 0; h < MAPS; ++h) load_v<D>(pg.head[h], at, vr[h]);
     }
+    uint32_t keep_at[T];  // where the columns' logits go, in bytes from the page's; past the descriptor's end: nowhere
+    if constexpr (W)
+#pragma unroll
+      for (int g = 0; g < T; ++g) {
+        const int c = ROWS * g + l, r = tile * R + c % R;
+        keep_at[g] = r < a.nrep ? uint32_t(c / R) * uint32_t(a.p.P) * a.nrep * (PAGE * 4) + (quarter * a.nrep + r) * 16 : 1u << 31;
+      }
+    const int keep_bytes = ((C / R - 1) * a.p.P + 1) * a.nrep * (PAGE * 4);  // to the end of the last column's map's page
     const int see0 = a.window ? max(0, len - a.m + 1 - a.window) : 0;  // the first key that any row sees
     int id = id_of(1);
     for (int i = 0; i < mine; ++i) {
@@ -565,15 +573,14 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
               if (k >= lim[g] || k < low[g]) w[g][t][e] = NEG_INF;
             }
       }
-      if constexpr (W) {
+      if constexpr (W) {  // (whole lines: the rows of 4 tokens lie side by side; no branch, as with the loads)
+        const int64_t first = ((int64_t(s) * a.p.H + head * MAPS) * a.p.P + tok0 / PAGE) * a.nrep * PAGE;
+        const rsrc_t d = __builtin_amdgcn_make_buffer_rsrc(a.logits + first, 0, keep_bytes, 0x00020000);
 #pragma unroll
-        for (int g = 0; g < T; ++g) {
-          const int r = tile * R + (ROWS * g + l) % R, h = head * MAPS + (ROWS * g + l) / R;
-          float* to = a.logits + (((int64_t(s) * a.p.H + h) * a.p.P + tok0 / PAGE) * a.nrep + r) * PAGE + quarter * 4;
-          if (r < a.nrep)
+        for (int g = 0; g < T; ++g)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) *reinterpret_cast<f4_t*>(to + t * 16) = w[g][t];
-        }
+          for (int t = 0; t < 4; ++t)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, w[g][t]), d, keep_at[g], t * 64 * a.nrep, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -767,11 +774,11 @@ __global__ __launch_bounds__(THREADS) void weights_kernel(AttnArgs a, int chunks
   for (int i = 0; i < WEIGH_PAGES; ++i) {
     const int page = first + i * WAVES, t = page * PAGE + lane;
     if (page >= lo + n || t >= len) break;
-    const float* x = a.logits + (int64_t(sh) * a.p.P + page) * a.nrep * PAGE + lane;
+    const float* x = a.logits + ((int64_t(sh) * a.p.P + page) * PAGE + lane / 4 * 4) * a.nrep + lane % 4;
     float sum = 0.f;
     for (int r = 0; r < a.nrep; ++r) {
       const float2 y = st[r];
-      sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x[r * PAGE] - y.x), y.y, sum);
+      sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x[r * 4] - y.x), y.y, sum);
     }
     a.weights[s * a.sw_s + head * a.sw_h + t] += sum;
   }
@@ -844,6 +851,7 @@ int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int6
   if (weights) {
     IQ_CHECK(m == 1 && Tw >= int64_t(p->P) * PAGE && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
     IQ_CHECK(int64_t(p->S) * p->H * chunks <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
+    IQ_CHECK((int64_t(p->P) + 1) * nrep < INT32_MAX / (PAGE * 4), IQ_ERR_SHAPE);  // a map's logits in 32 bits
     IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
   }
   const size_t need = workspace_bytes_of(p->S, p->P, m, Hq, p->H, p->D, MAPS, weights != nullptr);

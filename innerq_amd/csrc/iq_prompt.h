@@ -71,7 +71,7 @@ struct WeighArgs {
   float* part;
 };
 // its workspace: the stats, then the sums
-size_t prompt_weights_bytes(int N, int Nk, int Hq, int H);
+size_t prompt_weights_bytes(int N, int Nk, int Hq, int H);  // (a multiple of 16)
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream);
 
 }  // namespace iq

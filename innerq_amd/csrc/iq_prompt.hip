@@ -35,32 +35,25 @@ struct PromptArgs {
   uint32_t keep, sign;  // Scale
   int causal, window;
   float2* stats;        // [N][Hq] {base, 1 / sum of weights} of each row, or null
+  int splits;           // workgroups that share a tile of rows
+  float* part;          // their sums
 };
 
 // tiles of BM rows that a KV head's share of a sequence of lq query rows makes
 __device__ __forceinline__ int tiles_of(int lq, int nrep) { return int((int64_t(lq) * nrep + BM - 1) / BM); }
 
-template <int D, bool BF>
-__global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
-#pragma clang fp contract(off)  // logits times c and the maximum times c round alike
-  constexpr int CH = D / 8, KS = D / 16, DB = D / 32;  // chunks per row, k steps of S, blocks of 32 dims
-  constexpr int LOADS = BN * CH / THREADS;             // chunks per thread and tile
-  __shared__ u4_t lk0[BN * CH], lk1[BN * CH], lv0[BN * CH], lv1[BN * CH];
-  __shared__ int lodd[2][WAVES];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
-
-  // This workgroup's KV head and slot.  Blocks go round robin over the 8 XCDs: with the heads innermost, an XCD keeps to
-  // one or a few heads' keys, and where XCDs share a head each has its share of long and short tiles (a run of slots per
-  // XCD: a prompt of 8192 tokens, 8 query heads over one KV head 274 us, now 168; 32 over 4 652, now 497).
-  const int H = gridDim.x / a.slots, kvh = blockIdx.x % H, slot = blockIdx.x / H;
-
-  // The slot's sequence and tile of rows, a sequence's last tiles (the longest) first.
+// A slot's sequence and tile of rows, a sequence's last tiles (the longest) first.
+struct Slot {
+  int s, q0, q1, k0, k1, tile;
+};
+__device__ __forceinline__ bool slot_of(const PromptArgs& a, int slot, Slot& x) {
+  const int lane = threadIdx.x & 63;
   int s = 0, q0, q1, k0, k1, tile;
   if (a.S == 1) {
     rows_of(a.cu_q, 0, a.N, q0, q1);
     rows_of(a.cu_k, 0, a.Nk, k0, k1);
     tile = tiles_of(q1 - q0, a.nrep) - 1 - slot;
-    if (tile < 0) return;
+    if (tile < 0) return false;
     // (prompts of 16 tokens, us here / with the search below: 64 9.4 / 12.5, 128 17 / 20, 256 32 / 32, 512 65 / 57)
   } else if (a.S <= 256) {  // the sequences' tiles lie behind one another
     uint64_t past;
@@ -79,7 +72,7 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
         tile = __builtin_amdgcn_readlane(end, l) - 1 - slot;
         break;
       }
-      if (s + 64 >= a.S) return;
+      if (s + 64 >= a.S) return false;
       before = __builtin_amdgcn_readlane(end, 63);
     }
   } else {
@@ -95,15 +88,63 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     rows_of(a.cu_q, s, a.N, q0, q1);
     rows_of(a.cu_k, s, a.Nk, k0, k1);
     tile = tiles_of(q1 - q0, a.nrep) - 1 - (slot - first_slot(s));
-    if (tile < 0 || tile >= tiles_of(q1 - q0, a.nrep)) return;
+    if (tile < 0 || tile >= tiles_of(q1 - q0, a.nrep)) return false;
   }
-  s = __builtin_amdgcn_readfirstlane(s);  // (uniform, which the compiler does not see: it would loop over lanes at each load)
-  q0 = __builtin_amdgcn_readfirstlane(q0);
-  q1 = __builtin_amdgcn_readfirstlane(q1);
-  tile = __builtin_amdgcn_readfirstlane(tile);
-  k0 = __builtin_amdgcn_readfirstlane(k0);
-  k1 = __builtin_amdgcn_readfirstlane(k1);
-  const int lq = q1 - q0, keys = k1 - k0, off = keys - lq, rows = lq * a.nrep;
+  // (uniform, which the compiler does not see: it would loop over lanes at each load)
+  x = {__builtin_amdgcn_readfirstlane(s), __builtin_amdgcn_readfirstlane(q0), __builtin_amdgcn_readfirstlane(q1),
+       __builtin_amdgcn_readfirstlane(k0), __builtin_amdgcn_readfirstlane(k1), __builtin_amdgcn_readfirstlane(tile)};
+  return true;
+}
+
+// A wave's rows (of n's sums o, times inv) to `at`, the first `real` of them, through its part of LDS: 16 lanes write a whole
+// row of 128 dims, where a lane's own dims are 8 bytes here and there.
+template <int D, bool BF>
+__device__ __forceinline__ void store_rows(const PromptArgs& a, u4_t* lo, const f16_t (&o)[D / 32], float inv, int64_t at,
+                                           int real) {
+  constexpr int CH = D / 8;
+  const int lane = threadIdx.x & 63, n = lane & 31, hi = lane >> 5;
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<u2_t*>(lo + chunk_at<D>(n, 4 * b + i))[hi] =
+          u2_t{pack2<BF>(o[b][4 * i] * inv, o[b][4 * i + 1] * inv), pack2<BF>(o[b][4 * i + 2] * inv, o[b][4 * i + 3] * inv)};
+  wave_lds_sync();
+  const int at0 = int(at), at1 = int(at >> 32);
+#pragma unroll
+  for (int j = 0; j < CH / 2; ++j) {
+    const int r = j * (64 / CH) + lane / CH, c = lane % CH;  // row and chunk
+    const int64_t to = int64_t(uint32_t(__shfl(at0, r, 64))) | int64_t(__shfl(at1, r, 64)) << 32;
+    if (r < real) *reinterpret_cast<u4_t*>(a.out + to + 8 * c) = lo[chunk_at<D>(r, c)];
+  }
+}
+
+// A wave's sums of a split: 32 D of them in the order of its registers and lanes, then its rows' {base, sum of weights}.
+template <int D>
+__device__ __forceinline__ float* part_of(const PromptArgs& a, int group, int split, int wave) {
+  return a.part + ((int64_t(group) * a.splits + split) * WAVES + wave) * (32 * D + 64);
+}
+
+// SPLIT: the tiles of keys that a workgroup would walk over are shared out over the workgroups of a column of the grid; their
+// sums go to the workspace (few rows, many keys: a prompt's last rows over all of it).
+template <int D, bool BF, bool SPLIT>
+__global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
+#pragma clang fp contract(off)  // logits times c and the maximum times c round alike
+  constexpr int CH = D / 8, KS = D / 16, DB = D / 32;  // chunks per row, k steps of S, blocks of 32 dims
+  constexpr int LOADS = BN * CH / THREADS;             // chunks per thread and tile
+  __shared__ u4_t lk0[BN * CH], lk1[BN * CH], lv0[BN * CH], lv1[BN * CH];
+  __shared__ int lodd[2][WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
+
+  // This workgroup's KV head and slot.  Blocks go round robin over the 8 XCDs: with the heads innermost, an XCD keeps to
+  // one or a few heads' keys, and where XCDs share a head each has its share of long and short tiles (a run of slots per
+  // XCD: a prompt of 8192 tokens, 8 query heads over one KV head 274 us, now 168; 32 over 4 652, now 497).
+  const int H = gridDim.x / a.slots, kvh = blockIdx.x % H, slot = blockIdx.x / H;
+
+  Slot x;
+  if (!slot_of(a, slot, x)) return;
+  const int q0 = x.q0, k0 = x.k0, tile = x.tile;
+  const int lq = x.q1 - q0, keys = x.k1 - k0, off = keys - lq, rows = lq * a.nrep;
   // this lane's row of the KV head's rows, which are its query rows' heads one behind the other: row * nrep + head
   const int vrow = tile * BM + wave * 32 + n, row = min(vrow, rows - 1) / a.nrep, head = kvh * a.nrep + min(vrow, rows - 1) % a.nrep;
   // key j is seen iff first <= j < last
@@ -111,7 +152,12 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   // the tiles of keys that any row of the workgroup sees
   const int row_a = tile * BM / a.nrep, row_z = (min(tile * BM + BM, rows) - 1) / a.nrep;
   const int j_end = a.causal ? min(row_z + off + 1, keys) : keys, j_begin = a.window ? max(row_a + off + 1 - a.window, 0) : 0;
-  const int t_begin = j_begin / BN, t_end = j_end > j_begin ? (j_end + BN - 1) / BN : t_begin;
+  int t_begin = j_begin / BN, t_end = j_end > j_begin ? (j_end + BN - 1) / BN : t_begin;
+  if constexpr (SPLIT) {
+    const int per = (t_end - t_begin + a.splits - 1) / a.splits;
+    t_begin = min(t_begin + int(blockIdx.y) * per, t_end);
+    t_end = min(t_begin + per, t_end);
+  }
 
   u4_t q[KS];  // B operand: row n, dims 16 ks + 8 hi + e (rows past the end repeat the last one and are not stored)
   {
@@ -323,6 +369,10 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
   // buffer i % 2, and every wave passes the same barriers.
   int whole_a = a.window ? (max(row_z + off + 1 - a.window, 0) + BN - 1) / BN : 0;
   int whole_z = (a.causal ? min(row_a + off + 1, keys) : keys) / BN;
+  if constexpr (SPLIT) {
+    whole_a = max(whole_a, t_begin);
+    whole_z = min(whole_z, t_end);
+  }
   if (whole_a >= whole_z || t_begin >= t_end) whole_a = whole_z = t_begin;
   const int nw = whole_z - whole_a, tail = t_end - whole_z, count = t_end - t_begin;
   auto tile_at = [&](int i) { return i < nw ? whole_a + i : i < nw + tail ? whole_z + i - nw : t_begin + i - nw - tail; };
@@ -378,26 +428,70 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(y[0]) + __uint_as_float(y[1]);
   }
-  // Rows leave through LDS: 16 lanes write a whole row of 128 dims, where a lane's own dims are 8 bytes here and there.
+  if constexpr (SPLIT) {
+    float* part = part_of<D>(a, blockIdx.x, blockIdx.y, wave);
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<f4_t*>(part)[(b * 4 + i) * 64 + lane] = f4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
+    if (hi == 0) reinterpret_cast<float2*>(part + 32 * D)[n] = float2{base_of(m), l};
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (a.stats && hi == 0 && vrow < rows) a.stats[int64_t(q0 + row) * a.Hq + head] = float2{base_of(m), inv};
   __syncthreads();  // nobody reads tiles any more
-  u4_t* const lo = (wave < 2 ? lk0 : lk1) + (wave & 1) * 32 * CH;
-#pragma unroll
-  for (int b = 0; b < DB; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      reinterpret_cast<u2_t*>(lo + chunk_at<D>(n, 4 * b + i))[hi] =
-          u2_t{pack2<BF>(o[b][4 * i] * inv, o[b][4 * i + 1] * inv), pack2<BF>(o[b][4 * i + 2] * inv, o[b][4 * i + 3] * inv)};
-  wave_lds_sync();
-  const int64_t at = int64_t(q0 + row) * a.so_n + head * a.so_h;
-  const int at0 = int(at), at1 = int(at >> 32);
-#pragma unroll
-  for (int j = 0; j < CH / 2; ++j) {
-    const int r = j * (64 / CH) + lane / CH, c = lane % CH;  // row and chunk
-    const int64_t to = int64_t(uint32_t(__shfl(at0, r, 64))) | int64_t(__shfl(at1, r, 64)) << 32;
-    if (tile * BM + wave * 32 + r < rows) *reinterpret_cast<u4_t*>(a.out + to + 8 * c) = lo[chunk_at<D>(r, c)];
+  store_rows<D, BF>(a, (wave < 2 ? lk0 : lk1) + (wave & 1) * 32 * CH, o, inv, int64_t(q0 + row) * a.so_n + head * a.so_h,
+                    rows - tile * BM - wave * 32);
+}
+
+// Merges the sums of a tile's splits, in their order: 32 dims (a row of the grid) of its rows, in the lanes and registers
+// that they left.
+template <int D, bool BF>
+__global__ __launch_bounds__(THREADS) void merge_kernel(PromptArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
+  const int H = gridDim.x / a.slots, kvh = blockIdx.x % H, b = blockIdx.y;
+  Slot x;
+  if (!slot_of(a, blockIdx.x / H, x)) return;
+  const int rows = (x.q1 - x.q0) * a.nrep, v = x.tile * BM + wave * 32 + n, row = v / a.nrep, head = kvh * a.nrep + v % a.nrep;
+  if (v >= rows) return;
+  auto stats_of = [&](int z) { return reinterpret_cast<const float2*>(part_of<D>(a, blockIdx.x, z, wave) + 32 * D)[n]; };
+  float base = NEG_INF, l = 0.f, o[16];
+#pragma unroll 4
+  for (int z = 0; z < a.splits; ++z) {
+    const float2 st = stats_of(z);
+    base = st.y == 0.f ? base : fmaxf(base, st.x);  // (0: no key that counts)
   }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < a.splits; ++z) {
+    const float2 st = stats_of(z);
+    const f4_t* part = reinterpret_cast<const f4_t*>(part_of<D>(a, blockIdx.x, z, wave)) + b * 4 * 64 + lane;
+    f4_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = part[i * 64];
+    if (st.y == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(st.x - base);
+    l += st.y * f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] += y[i / 4][i % 4] * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (hi == 0 && b == 0) a.stats[int64_t(x.q0 + row) * a.Hq + head] = float2{base == NEG_INF ? 0.f : base, inv};
+  uint16_t* to = a.out + int64_t(x.q0 + row) * a.so_n + head * a.so_h + 32 * b + 4 * hi;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<u2_t*>(to + 8 * i) =
+        u2_t{pack2<BF>(o[4 * i] * inv, o[4 * i + 1] * inv), pack2<BF>(o[4 * i + 2] * inv, o[4 * i + 3] * inv)};
+}
+
+// Workgroups that share a tile of rows: as many as make 768 of the slots (two thirds of which hold a tile where sequences are
+// short of one), while each has 512 keys, by the mean of the sequences.  Only where there is a workspace.
+inline int splits_of(int S, int N, int Nk, int Hq, int H) {
+  const int64_t slots = int64_t(N) * (Hq / H) / BM + S, most = 768 / (slots * H), keys = int64_t(Nk) / S / 512;
+  const int64_t n = most < keys ? most : keys;
+  return n < 2 ? 1 : n > 16 ? 16 : int(n);
 }
 
 int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h, const void* v, int64_t sv_n,
@@ -424,16 +518,25 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
   const int64_t slots = rows / BM + S;  // first_slot(S) at most
   IQ_CHECK(slots * H <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
   if (weights) {
-    IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(N, Nk, Hq, H), IQ_ERR_WORKSPACE);
+    IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(S, N, Nk, Hq, H, D), IQ_ERR_WORKSPACE);
     IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   }
   if (window >= Nk) window = 0;  // hides nothing
   const Scale sc = scale_of(scale);
   PromptArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, sq_n, sq_h, sk_n, sk_h, sv_n,
                sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), sc.c, 8.f / sc.c, sc.keep, sc.sign,
-               causal ? 1 : 0, window, weights ? (float2*)workspace : nullptr};
+               causal ? 1 : 0, window, weights ? (float2*)workspace : nullptr, weights ? splits_of(S, N, Nk, Hq, H) : 1,
+               nullptr};
+  if (a.splits > 1) a.part = (float*)((char*)workspace + iq::prompt_weights_bytes(N, Nk, Hq, H));
   auto launch = [&]<int D_, bool BF>() {
-    prompt_kernel<D_, BF><<<unsigned(slots * H), THREADS, 0, (hipStream_t)stream>>>(a);
+    const dim3 grid(unsigned(slots * H), unsigned(a.splits));
+    if (a.splits == 1) {
+      prompt_kernel<D_, BF, false><<<grid, THREADS, 0, (hipStream_t)stream>>>(a);
+      return launch_status();
+    }
+    prompt_kernel<D_, BF, true><<<grid, THREADS, 0, (hipStream_t)stream>>>(a);
+    if (const int st = launch_status()) return st;
+    merge_kernel<D_, BF><<<dim3(grid.x, D_ / 32), THREADS, 0, (hipStream_t)stream>>>(a);
     return launch_status();
   };
   const bool bf = act_bf16(mode);
@@ -446,8 +549,11 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
 
 }  // namespace
 
-extern "C" size_t iq_prompt_weights_workspace_bytes(int N, int Nk, int Hq, int H) {
-  return N <= 0 || Nk < 0 || Hq <= 0 || H <= 0 || Hq % H ? 0 : iq::prompt_weights_bytes(N, Nk, Hq, H);
+extern "C" size_t iq_prompt_weights_workspace_bytes(int S, int N, int Nk, int Hq, int H, int D) {
+  if (S <= 0 || N <= 0 || Nk < 0 || Hq <= 0 || H <= 0 || Hq % H || !d_ok(D)) return 0;
+  const size_t slots = size_t(N) * (Hq / H) / BM + S, splits = splits_of(S, N, Nk, Hq, H);
+  return iq::prompt_weights_bytes(N, Nk, Hq, H) +
+         (splits > 1 ? slots * H * splits * WAVES * (32 * D + 64) * sizeof(float) : 0);
 }
 
 extern "C" int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,

@@ -265,7 +265,7 @@ namespace iq {
 size_t prompt_weights_bytes(int N, int Nk, int Hq, int H) {
   const int64_t rows = int64_t(N) * (Hq / H), chunks = ceil_div(rows, chunk_of(rows));
   const size_t stats = (size_t(N) * Hq * sizeof(float2) + 15) / 16 * 16;
-  return chunks > 1 ? stats + size_t(chunks) * H * Nk * sizeof(float) : stats;
+  return chunks > 1 ? stats + (size_t(chunks) * H * Nk * sizeof(float) + 15) / 16 * 16 : stats;
 }
 
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream) {

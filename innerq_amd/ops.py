@@ -1011,7 +1011,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if weights is None or not weights.numel():
             call("iq_prompt_attention", *args, _stream(dev))
             return out
-        nbytes = _lib.lib().iq_prompt_weights_workspace_bytes(N, Nk, Hq, H)
+        nbytes = _lib.lib().iq_prompt_weights_workspace_bytes(S, N, Nk, Hq, H, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         call("iq_prompt_attention_weights", *args, _p(weights), weights.stride(0), weights.stride(1), weights.shape[2], _p(ws),
              nbytes, _stream(dev))
@@ -1072,7 +1072,7 @@ def diff_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
         if q.stride(1) * (Hq // H) >= 2 ** 29:
             q = q.clone(memory_format=torch.contiguous_format)
     kept = weights is not None and weights.numel() > 0
-    nbytes = _lib.lib().iq_prompt_weights_workspace_bytes(N, Nk, Hq, H) if kept else 0
+    nbytes = _lib.lib().iq_prompt_weights_workspace_bytes(S, N, Nk, Hq, H, D) if kept else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if kept else None
     with on_device(dev):
         call("iq_diff_prompt_attention", _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
