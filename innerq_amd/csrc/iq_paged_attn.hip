@@ -55,6 +55,7 @@ struct AttnArgs {
   float2* stats;
   float* weights;
   int64_t sw_s, sw_h;
+  int items, weigh_each;  // workgroups of the second launch that merge; pages of one that weighs
 };
 
 // pages that sequence s reads: [lo, lo + n)
@@ -416,12 +417,14 @@ __device__ __forceinline__ float minus_lam(const AttnArgs& a, int head, int tile
 }
 
 // a row's softmax, for the keys' weights: {maximum, 1 / sum}; a row without a sum gives weights of 0
+__device__ __forceinline__ float2 row_stats(float mx, float sum) {
+  return {mx == NEG_INF ? 0.f : mx, sum == 0.f ? 0.f : 1.f / sum};
+}
 __device__ __forceinline__ void store_stats(const AttnArgs& a, int s, int head, int r, float mx, float sum) {
-  if (r < a.nrep)  // (head: of the store)
-    a.stats[(int64_t(s) * a.p.H + head) * a.nrep + r] = float2{mx == NEG_INF ? 0.f : mx, sum == 0.f ? 0.f : 1.f / sum};
+  if (r < a.nrep) a.stats[(int64_t(s) * a.p.H + head) * a.nrep + r] = row_stats(mx, sum);  // (head: of the store)
 }
 
-// W: the logits and the rows' sums are kept, for weights_kernel.  MAPS = 2: differential attention (see the end of the
+// W: the logits and the rows' sums are kept, for weigh_pages.  MAPS = 2: differential attention (see the end of the
 // file): KV heads in pairs, whose keys are the two maps' and whose V heads are the halves of one of 2 D dims.
 template <int D, bool BF, int T, bool W, int MAPS>
 __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a) {
@@ -669,10 +672,92 @@ __global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a)
   }
 }
 
-// one workgroup per (sequence, head, tile): merges the slots of those that several workgroups computed, in order
+// Adds each key's softmax weights, over a KV head's query rows, to what it has gathered: from the logits that attn_kernel
+// has kept, a wave a page, a lane a key.  Rows are added in their order, WEIGH_ROWS of WEIGH_PAGES pages under way together.
+// The rows' statistics are attn_kernel's, or, where several workgroups computed them, merged here as they are beside it.
+constexpr int WEIGH_PAGES = 4, WEIGH_ROWS = 4;
+template <int T, int MAPS, int DV>
+__device__ __forceinline__ void weigh_pages(const AttnArgs& a, int block) {
+  constexpr int C = ROWS * T, R = tile_rows<T, MAPS>();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x / 64;
+  const int chunk = block / (a.p.S * a.p.H), sh = block - chunk * (a.p.S * a.p.H), s = sh / a.p.H, h = sh - s * a.p.H, head = h / MAPS, map = h - head * MAPS;
+  int lo;
+  const int n = pages_of(a, s, lo), first = lo + chunk * a.weigh_each, len = min(a.p.lens[s], a.p.P * PAGE);
+  if (n <= 0 || first >= lo + n) return;
+  int units = 0, end = 0, per = 1;
+  if (a.split) {
+    Part part = part_at(a, 0, 0);
+    per = units_per_group(total_units(a, part), a.grid);
+    for (int s0 = 64 * a.each; s0 <= s; s0 += 64 * a.each) part = part_at(a, s0, __builtin_amdgcn_readlane(part.end, 63));
+    units_of(a, part, s, units, end);
+  }
+  for (int p0 = first + wave; p0 < min(first + a.weigh_each, lo + n); p0 += waves * WEIGH_PAGES) {
+    const float* x[WEIGH_PAGES];
+    float* to[WEIGH_PAGES];
+    bool there[WEIGH_PAGES];
+    float old[WEIGH_PAGES], sum[WEIGH_PAGES];
+#pragma unroll
+    for (int i = 0; i < WEIGH_PAGES; ++i) {
+      const int page = min(p0 + i * waves, lo + n - 1), t = page * PAGE + lane;
+      there[i] = p0 + i * waves < min(first + a.weigh_each, lo + n) && t < len;
+      x[i] = a.logits + ((int64_t(sh) * a.p.P + page) * PAGE + lane / 4 * 4) * a.nrep + lane % 4;
+      to[i] = a.weights + s * a.sw_s + h * a.sw_h + min(t, len - 1);
+      old[i] = *to[i];
+      sum[i] = 0.f;
+    }
+    for (int r0 = 0; r0 < a.nrep; r0 += 64) {
+      // a lane's row: its statistics
+      const int r = min(r0 + lane, a.nrep - 1), tile = r / R, c = map * R + r - tile * R;
+      float2 st = {NEG_INF, 0.f};
+      int g0 = 0, g1 = 0;
+      if (a.split) {
+        const int each = units / (a.heads * a.tiles), u0 = end - units + (head * a.tiles + tile) * each;
+        g0 = (u0 + PAD) / per;
+        g1 = (u0 + each - 1) / per;
+      }
+      if (g0 == g1) {
+        st = a.stats[int64_t(sh) * a.nrep + r];
+      } else {
+#pragma unroll 4
+        for (int g = g0; g <= g1; ++g) {
+          const float* p = slot_of<DV, C>(a.ws, 2 * g + (g == g0 ? 1 : 0)) + C * DV + c;
+          const float m = p[0], l = p[C], mx = fmaxf(st.x, m);
+          const float keep = st.x == NEG_INF ? 0.f : exp2f(st.x - mx), f = m == NEG_INF ? 0.f : exp2f(m - mx);
+          st.y = (st.x == NEG_INF ? st.y : st.y * keep) + (l != l ? l : f * l);
+          st.x = mx;
+        }
+        st = row_stats(st.x, st.y);
+      }
+      for (int rb = 0; rb < min(64, a.nrep - r0); rb += WEIGH_ROWS) {
+        float y[WEIGH_ROWS][WEIGH_PAGES];
+#pragma unroll
+        for (int e = 0; e < WEIGH_ROWS; ++e)
+#pragma unroll
+          for (int i = 0; i < WEIGH_PAGES; ++i) y[e][i] = x[i][min(r0 + rb + e, a.nrep - 1) * 4];
+#pragma unroll
+        for (int e = 0; e < WEIGH_ROWS; ++e) {
+          if (r0 + rb + e >= a.nrep) break;
+          const float mx = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(st.x), rb + e));
+          const float inv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(st.y), rb + e));
+#pragma unroll
+          for (int i = 0; i < WEIGH_PAGES; ++i)
+            sum[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(y[e][i] - mx), inv, sum[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < WEIGH_PAGES; ++i)
+      if (there[i]) *to[i] = old[i] + sum[i];
+  }
+}
+
+// One workgroup per (sequence, head, tile): merges the slots of those that several workgroups computed, in order.  W: behind
+// these (where there are any), the workgroups that weigh the keys.
 template <int D, bool BF, int T, bool W, int MAPS>
 __global__ __launch_bounds__(ROWS * T * (MAPS * D / 8)) void combine_kernel(AttnArgs a) {
   constexpr int C = ROWS * T, R = tile_rows<T, MAPS>(), DV = MAPS * D;
+  if constexpr (W)
+    if (blockIdx.x >= unsigned(a.items)) return weigh_pages<T, MAPS, DV>(a, blockIdx.x - a.items);
   const int per_seq = a.heads * a.tiles, s = blockIdx.x / per_seq, hr = blockIdx.x - s * per_seq;
   Part part = part_at(a, 0, 0);
   const int total = total_units(a, part), per = units_per_group(total, a.grid);
@@ -741,8 +826,6 @@ __global__ __launch_bounds__(ROWS * T * (MAPS * D / 8)) void combine_kernel(Attn
   }
   const int head = hr / a.tiles;
   float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if constexpr (W)
-    if (part_i == 0 && d == 0) store_stats(a, s, head * MAPS + map, tile * R + r, mx, sum);
   if constexpr (MAPS == 2) {
     if (parts > 1) __syncthreads();  // nobody reads the parts any more
     if (part_i == 0 && map == 1) {
@@ -758,30 +841,6 @@ __global__ __launch_bounds__(ROWS * T * (MAPS * D / 8)) void combine_kernel(Attn
   }
   if (part_i > 0 || map > 0) return;
   store_row<D, BF, R>(a, s, head, tile, r, d, v, inv);
-}
-
-// Adds each key's softmax weights, over a KV head's query rows, to what it has gathered: from the logits that attn_kernel
-// has kept, a wave a page, a lane a key.  Rows are added in their order.
-constexpr int WEIGH_PAGES = 4;  // of a wave
-__global__ __launch_bounds__(THREADS) void weights_kernel(AttnArgs a, int chunks) {
-  const int sh = blockIdx.x / chunks, s = sh / a.p.H, head = sh - s * a.p.H, lane = threadIdx.x & 63;
-  const int len = min(a.p.lens[s], a.p.P * PAGE);
-  int lo;
-  const int n = pages_of(a, s, lo);
-  const float2* st = a.stats + int64_t(sh) * a.nrep;
-  const int first = lo + (blockIdx.x - sh * chunks) * (WAVES * WEIGH_PAGES) + (threadIdx.x >> 6);
-#pragma unroll
-  for (int i = 0; i < WEIGH_PAGES; ++i) {
-    const int page = first + i * WAVES, t = page * PAGE + lane;
-    if (page >= lo + n || t >= len) break;
-    const float* x = a.logits + ((int64_t(sh) * a.p.P + page) * PAGE + lane / 4 * 4) * a.nrep + lane % 4;
-    float sum = 0.f;
-    for (int r = 0; r < a.nrep; ++r) {
-      const float2 y = st[r];
-      sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x[r * 4] - y.x), y.y, sum);
-    }
-    a.weights[s * a.sw_s + head * a.sw_h + t] += sum;
-  }
 }
 
 constexpr int GRID = 512;  // two workgroups per CU
@@ -847,10 +906,8 @@ int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int6
   const Launch pl = plan_of(p->S, p->P, m, nrep, heads, p->D, MAPS);
   IQ_CHECK(int64_t(p->S) * (p->P + PAD) * heads * pl.tiles <= INT32_MAX &&
                int64_t(p->S) * heads * pl.tiles <= UINT32_MAX / (ROWS * 2 * MAPS * 16), IQ_ERR_SHAPE);
-  const int64_t chunks = ceil_div(p->P, WAVES * WEIGH_PAGES);  // of weights_kernel, per (sequence, head)
   if (weights) {
     IQ_CHECK(m == 1 && Tw >= int64_t(p->P) * PAGE && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
-    IQ_CHECK(int64_t(p->S) * p->H * chunks <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
     IQ_CHECK((int64_t(p->P) + 1) * nrep < INT32_MAX / (PAGE * 4), IQ_ERR_SHAPE);  // a map's logits in 32 bits
     IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
   }
@@ -860,24 +917,24 @@ int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int6
   if (window >= p->P * PAGE) window = 0;  // hides nothing
   AttnArgs a{*p, (const uint16_t*)q, sq_s, sq_m, sq_h, (uint16_t*)out, so_s, so_m, so_h, heads, m, nrep, pl.tiles,
              scale * 1.44269504088896340736f, window, pl.grid, (float*)workspace, p->S > 64 ? EACH : 1, pl.split, lam, s_lam,
-             nullptr, nullptr, weights, sw_s, sw_h};
+             nullptr, nullptr, weights, sw_s, sw_h, pl.split ? p->S * heads * pl.tiles : 0, 0};
   if (weights) {
     char* const ws = (char*)workspace + slots_bytes(pl, p->D, MAPS);
     a.stats = (float2*)ws;
     a.logits = (float*)(ws + stats_bytes(p->S, Hq));
   }
-  auto launch = [&]<int D, bool BF, int T, bool W>() {
+  auto launch = [&]<int D, bool BF, int T, bool W>() -> int {
+    constexpr int threads = ROWS * T * (MAPS * D / 8);
+    int64_t groups = a.items;  // of the second launch
+    if constexpr (W) {
+      a.weigh_each = threads / 64 * WEIGH_PAGES;
+      groups += int64_t(p->S) * p->H * ceil_div(p->P, a.weigh_each);
+      IQ_CHECK(groups <= INT32_MAX / threads, IQ_ERR_SHAPE);
+    }
     attn_kernel<D, BF, T, W, MAPS><<<pl.grid, THREADS, 0, (hipStream_t)stream>>>(a);
     if (const int st = launch_status()) return st;
-    if (pl.split)
-      combine_kernel<D, BF, T, W, MAPS>
-          <<<p->S * heads * pl.tiles, ROWS * T * (MAPS * D / 8), 0, (hipStream_t)stream>>>(a);
-    if (const int st = launch_status()) return st;
-    if constexpr (W) {
-      weights_kernel<<<unsigned(int64_t(p->S) * p->H * chunks), THREADS, 0, (hipStream_t)stream>>>(a, int(chunks));
-      return launch_status();
-    }
-    return int(IQ_OK);
+    if (groups) combine_kernel<D, BF, T, W, MAPS><<<unsigned(groups), threads, 0, (hipStream_t)stream>>>(a);
+    return launch_status();
   };
   auto with = [&]<int D, bool BF>() {
     if (weights) return pl.T == 2 ? launch.template operator()<D, BF, 2, true>() : launch.template operator()<D, BF, 1, true>();
