@@ -9,10 +9,10 @@
 //
 // Three launches, one behind the other (each reads what the next one writes over):
 //   select  one workgroup per (sequence, run of heads): the B-th largest weight by three passes over the bits of the
-//           weights (11, 11, 10 from the top), then the lists of free places and of the rows that come; moves the weights.
-//   fill    rows into the free places: sources from B on, destinations below B, in any order.
-//   shift   the last `recent` rows, which may overlap their destinations: one workgroup per (sequence, head), in order,
-//           each batch read whole before it is written.
+//           weights (11, 11, 10 from the top), then the lists of free places and of the rows that come.
+//   fill    rows and their weights into the free places: sources from B on, destinations below B, in any order.
+//   shift   the last `recent` rows: where they overlap their destinations one workgroup per (sequence, head), in order,
+//           each batch read whole before it is written.  Weights from `keep` on become 0.
 #include "iq_paged.h"
 
 using namespace iq;
@@ -20,8 +20,12 @@ using namespace iq;
 namespace {
 
 constexpr int SELECT = 1024, FILL = 256, SHIFT = 1024;
-constexpr int BATCH = 4;                        // rows (or weights) of a lane that are under way together
+constexpr int BATCH = 4;                        // rows of a lane that are under way together
 constexpr int BITS[3] = {11, 11, 10}, BINS = 1 << 11;
+constexpr int WAVES = SELECT / 64;
+constexpr int KEYS = 32, ROUND = KEYS * SELECT, READS = 4;  // weights of a thread, of a workgroup; under way together from LDS
+
+typedef float f4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 
 struct EvictArgs {
   iq_paged p;
@@ -32,7 +36,7 @@ struct EvictArgs {
   int keep, recent, sinks, shared, most;  // most: rows that can come, at most
   int32_t* lens_out;
   int32_t* ws;
-  int chunks;  // of FILL rows per (sequence, head)
+  int chunks;  // workgroups per (sequence, head)
 };
 
 // a (sequence, run of heads)'s part of the workspace: its tokens if it drops any (else 0), the rows that come, the free
@@ -41,7 +45,7 @@ __device__ __forceinline__ int32_t* plan_of(const EvictArgs& a, int64_t run) { r
 
 // inclusive sum over the workgroup; `total` the whole sum
 __device__ __forceinline__ int group_scan(int v, int& total) {
-  __shared__ int part[SELECT / 64];
+  __shared__ int part[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int x = wave_scan(v);
   __syncthreads();  // (nobody reads the last call's sums any more)
@@ -50,7 +54,7 @@ __device__ __forceinline__ int group_scan(int v, int& total) {
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int i = 0; i < SELECT / 64; ++i) {
+  for (int i = 0; i < WAVES; ++i) {
     const int y = part[i];
     if (i < wave) before += y;
     total += y;
@@ -66,7 +70,8 @@ __device__ __forceinline__ void all_read() {
 
 __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
   __shared__ int hist[BINS];
-  __shared__ int found[3];  // the digit, how many of its keys are wanted, how many there are
+  __shared__ int found[2];  // the digit, and how many of its keys are wanted
+  __shared__ uint32_t keys[ROUND + ROUND / 32];
   const int runs = a.p.H / a.shared, s = blockIdx.x / runs, h0 = (blockIdx.x - s * runs) * a.shared, tid = threadIdx.x;
   const float* w = a.w + s * a.sw_s + h0 * a.sw_h;
   float* wo = a.wo + s * a.so_s + h0 * a.so_h;
@@ -76,36 +81,77 @@ __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
   if (!there && tid == 0) atomicOr(a.p.status, PAGED_BAD_TOKEN);
   if (!there || n <= a.keep) {
     if (tid == 0) plan[0] = plan[1] = 0;
-    if (a.wo != a.w)
-      for (int h = 0; h < a.shared; ++h)
-        for (int64_t i = tid; i < a.T; i += SELECT) wo[h * a.so_h + i] = w[h * a.sw_h + i];
     return;
   }
   const int old = n - a.recent, B = a.keep - a.recent;  // B of the first `old` tokens stay
-  // Weights as whole numbers of the same order: NaN above all, -0 as 0.  The sinks are above all too, and come first.
-  auto key_of = [&](int i) {
-    float x = w[i] + 0.f;
-    for (int h = 1; h < a.shared; ++h) x += w[h * a.sw_h + i];
-    const uint32_t b = __float_as_uint(x);
-    return i < a.sinks || x != x ? ~0u : b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+  if (a.wo != a.w)  // the weights below B (those of free places are written over by the next launch)
+    for (int h = 0; h < a.shared; ++h)
+      for (int i = tid; i < B; i += SELECT) wo[h * a.so_h + i] = w[h * a.sw_h + i];
+  // Weights as whole numbers of the same order: NaN above all, -0 as 0.  The sinks are above all too, and come first.  A
+  // round's keys lie in LDS, a thread's being those of `per` neighbouring tokens, 0 (less than any weight's) past the end.
+  // (Loops over them stay loops: unrolled, with the keys in registers, the code alone took 25 us to fetch.)
+  const bool one = old <= ROUND;
+  const int per = one ? (old + 4 * SELECT - 1) / (4 * SELECT) * 4 : KEYS;
+  auto key_at = [&](int j) -> uint32_t& { return keys[j + j / 32]; };  // (a thread's, 32 apart, in different banks)
+  auto load = [&](int round, bool count) {  // count: the first pass's digits too
+    auto four = [&](const float* p, int i) {  // weights i .. i + 3, which may be the row's last
+      if (i + 4 <= a.T) return f4_t(*reinterpret_cast<const f4_any_t*>(p + i));
+      f4_t x = {0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 4; ++e)
+        if (i + e < a.T) x[e] = p[i + e];
+      return x;
+    };
+    f4_t x[KEYS / 4];
+#pragma unroll
+    for (int v = 0; v < KEYS / 4; ++v) {
+      const int i = round + (v * SELECT + tid) * 4;
+      x[v] = i < old ? four(w, i) : f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    __syncthreads();  // nobody reads the last round's keys any more
+#pragma clang loop unroll(disable)
+    for (int v = 0; v < (per + 3) / 4; ++v) {
+      f4_t y;
+#pragma unroll
+      for (int u = 0; u < KEYS / 4; ++u)
+        if (u == v) y = x[u];
+      const int j = (v * SELECT + tid) * 4, i = round + j;
+      y += 0.f;
+      if (i < old)
+        for (int h = 1; h < a.shared; ++h) y += four(w + h * a.sw_h, i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t b = __float_as_uint(y[e]);
+        const uint32_t k = i + e < a.sinks || y[e] != y[e] ? ~0u : b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+        key_at(j + e) = i + e < old ? k : 0u;
+        if (count && i + e < old) atomicAdd(&hist[k >> (32 - BITS[0])], 1);
+      }
+    }
+    __syncthreads();
   };
+  for (int i = tid; i < BINS; i += SELECT) hist[i] = 0;
+  if (one) load(0, B > 0);
   uint32_t least = 0;  // the B-th largest key
-  int cut = old;       // of the keys equal to it, those of tokens below `cut` stay
+  int ties = 0;        // of the tokens whose key it is, the first `ties` stay
   if (B > 0) {
     uint32_t mask = 0;
     int want = B;
     for (int pass = 0, low = 32; pass < 3; ++pass) {
       const int bits = BITS[pass];
       low -= bits;
-      for (int i = tid; i < BINS; i += SELECT) hist[i] = 0;
+      if (pass > 0)
+        for (int i = tid; i < BINS; i += SELECT) hist[i] = 0;
       __syncthreads();
-      for (int i0 = tid; i0 < old; i0 += SELECT * BATCH) {
-        uint32_t k[BATCH];
+      for (int round = 0; round < old; round += ROUND) {
+        if (!one) load(round, false);
+        else if (pass == 0) break;
+        for (int e0 = 0; e0 < per; e0 += READS) {
+          uint32_t k[READS];
 #pragma unroll
-        for (int e = 0; e < BATCH; ++e) k[e] = key_of(min(i0 + e * SELECT, old - 1));
+          for (int e = 0; e < READS; ++e) k[e] = key_at(min(e0 + e, per - 1) * SELECT + tid);
 #pragma unroll
-        for (int e = 0; e < BATCH; ++e)
-          if (i0 + e * SELECT < old && (k[e] & mask) == least) atomicAdd(&hist[k[e] >> low & ((1u << bits) - 1)], 1);
+          for (int e = 0; e < READS; ++e)
+            if (e0 + e < per && k[e] && (k[e] & mask) == least) atomicAdd(&hist[k[e] >> low & ((1u << bits) - 1)], 1);
+        }
       }
       __syncthreads();
       const int hi = BINS - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1];
@@ -115,72 +161,53 @@ __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
         const bool second = before + c0 < want;
         found[0] = second ? hi - 1 : hi;
         found[1] = second ? want - before - c0 : want - before;
-        found[2] = second ? c1 : c0;
       }
       __syncthreads();
       least |= uint32_t(found[0]) << low;
       mask |= ((1u << bits) - 1) << low;
       want = found[1];
     }
-    if (want < found[2]) {  // ties: the first ones stay
-      __syncthreads();
-      for (int i0 = 0, seen = 0; i0 < old && seen < want; i0 += SELECT) {
-        const int i = i0 + tid, tie = i < old && key_of(i) == least;
-        int total;
-        const int rank = seen + group_scan(tie, total);
-        if (tie && rank == want) found[0] = i + 1;
-        seen += total;
-      }
-      __syncthreads();
-      cut = found[0];
-    }
+    ties = want;
   }
-  auto stays = [&](int i) {
-    const uint32_t k = key_of(i);
-    return B > 0 && (k > least || (k == least && i < cut));
-  };
-  // the places below B that become free, and the tokens from B on that stay: as many
-  int count = 0;
-  for (int list = 0; list < 2; ++list) {
-    const int begin = list ? B : 0, end = list ? old : B;
-    int32_t* to = plan + 2 + list * int64_t(a.most);
-    count = 0;
-    for (int i0 = begin; i0 < end; i0 += SELECT * BATCH) {
-      const int first = i0 + tid * BATCH;
-      bool in[BATCH];
-      int mine = 0;
+  // the places below B that become free, and the tokens from B on that stay (as many), each in order
+  int count[2] = {0, 0}, tied = 0;
+  for (int round = 0; round < old; round += ROUND) {
+    if (!one) load(round, false);
+    const int first = round + tid * per;
+    uint32_t stay = 0, same = 0;  // a bit of each of the thread's tokens
+    for (int e0 = 0; e0 < per; e0 += READS) {
+      uint32_t k[READS];
 #pragma unroll
-      for (int e = 0; e < BATCH; ++e) {
-        in[e] = first + e < end && stays(min(first + e, end - 1)) == (list == 1);
-        mine += in[e];
+      for (int e = 0; e < READS; ++e) k[e] = key_at(tid * per + min(e0 + e, per - 1));
+#pragma unroll
+      for (int e = 0; e < READS; ++e) {
+        stay |= uint32_t(k[e] > least && e0 + e < per) << (e0 + e);
+        same |= uint32_t(k[e] == least && e0 + e < per) << (e0 + e);
       }
-      int total, at = count + group_scan(mine, total) - mine;
+    }
+    // (the thread's tokens below B, and below the end)
+    auto up_to = [&](int end) { return end <= first ? 0u : end - first >= 32 ? ~0u : (1u << (end - first)) - 1; };
+    const uint32_t all = per == 32 ? ~0u : (1u << per) - 1, low = up_to(B) & all, real = up_to(old) & all;
+    same &= real;
+    if (B > 0) {
+      int total, rank = tied + group_scan(__builtin_popcount(same), total) - __builtin_popcount(same);
+      tied += total;
+      for (uint32_t left = same; left && rank < ties; left &= left - 1, ++rank) stay |= left & -left;
+    } else {
+      stay = 0;
+    }
+    const uint32_t in[2] = {real & low & ~stay, real & ~low & stay};
 #pragma unroll
-      for (int e = 0; e < BATCH; ++e)
-        if (in[e]) to[at++] = first + e;
-      count += total;
+    for (int list = 0; list < 2; ++list) {
+      int total, at = count[list] + group_scan(__builtin_popcount(in[list]), total) - __builtin_popcount(in[list]);
+      count[list] += total;
+      int32_t* to = plan + 2 + list * int64_t(a.most);
+      for (uint32_t left = in[list]; left; left &= left - 1) to[at++] = first + __builtin_ctz(left);
     }
   }
   if (tid == 0) {
     plan[0] = n;
-    plan[1] = count;
-  }
-  // the weights go where their rows go
-  for (int h = 0; h < a.shared; ++h) {
-    const float* x = w + h * a.sw_h;
-    float* y = wo + h * a.so_h;
-    if (a.wo != a.w)
-      for (int i = tid; i < B; i += SELECT) y[i] = x[i];
-    __syncthreads();
-    for (int i = tid; i < count; i += SELECT) y[plan[2 + i]] = x[plan[2 + int64_t(a.most) + i]];
-    for (int i0 = 0; i0 < a.recent; i0 += SELECT) {
-      const int i = i0 + tid;
-      const float v = i < a.recent ? x[old + i] : 0.f;
-      all_read();  // (wo may be w)
-      if (i < a.recent) y[B + i] = v;
-    }
-    all_read();
-    for (int64_t i = a.keep + tid; i < a.T; i += SELECT) y[i] = 0.f;
+    plan[1] = count[0];
   }
 }
 
@@ -223,8 +250,8 @@ __device__ __forceinline__ uint32_t* page_of(const EvictArgs& a, int s, int h, i
   return id < 0 || id >= a.p.n_pages ? nullptr : a.p.pages + (int64_t(id) * a.p.H + h) * page_words(D);
 }
 
-// BATCH rows of a lane from tokens `from` to `to` (from < 0: none): reads all, calls `between`, writes all.  A row whose
-// page is missing is not read and becomes NaN; one whose place has no page is not written.
+// BATCH rows of a lane, and their tokens' weights, from tokens `from` to `to` (from < 0: none): reads all, calls `between`,
+// writes all.  A row whose page is missing is not read and becomes NaN; one whose place has no page is not written.
 template <int D, typename F>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, int s, int h, int o, const int (&from)[BATCH],
                                           const int (&to)[BATCH], F&& between) {
@@ -232,6 +259,9 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int s, int h, int 
   const uint32_t* src[BATCH];
   uint32_t* dst[BATCH];
   Piece x[BATCH];
+  float weight[BATCH];
+  const float* w = a.w + s * a.sw_s + h * a.sw_h;
+  float* wo = a.wo + s * a.so_s + h * a.so_h;
 #pragma unroll
   for (int e = 0; e < BATCH; ++e) {
     src[e] = from[e] < 0 ? nullptr : page_of<D>(a, s, h, from[e]);
@@ -241,10 +271,14 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int s, int h, int 
 #pragma unroll
   for (int e = 0; e < BATCH; ++e)
     x[e] = src[e] ? load_piece<D>(src[e], from[e] % PAGE, o) : Piece{0, 0, nan | uint32_t(nan) << 16, nan, nan};
+#pragma unroll
+  for (int e = 0; e < BATCH; ++e) weight[e] = o == 1 && from[e] >= 0 ? w[from[e]] : 0.f;
   between();
 #pragma unroll
-  for (int e = 0; e < BATCH; ++e)
+  for (int e = 0; e < BATCH; ++e) {
     if (dst[e]) store_piece<D>(dst[e], to[e] % PAGE, o, x[e]);
+    if (o == 1 && from[e] >= 0) wo[to[e]] = weight[e];
+  }
 }
 
 template <int D>
@@ -269,18 +303,37 @@ __global__ __launch_bounds__(FILL) void fill_kernel(EvictArgs a) {
 template <int D>
 __global__ __launch_bounds__(SHIFT) void shift_kernel(EvictArgs a) {
   constexpr int U = D / 8, ROWS = SHIFT / U * BATCH;
-  const int s = blockIdx.x / a.p.H, h = blockIdx.x - s * a.p.H, o = threadIdx.x % U;
-  const int n = plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared)[0];
-  if (!n) return;
-  for (int r0 = 0; r0 < a.recent; r0 += ROWS) {
-    int from[BATCH], to[BATCH];
+  const int sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.p.H, h = sh - s * a.p.H;
+  const int o = threadIdx.x % U, n = plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared)[0];
+  float* wo = a.wo + s * a.so_s + h * a.so_h;
+  const int64_t first = chunk * int64_t(SHIFT) + threadIdx.x, step = int64_t(a.chunks) * SHIFT;
+  if (!n) {  // a sequence that drops nothing
+    if (a.wo != a.w)
+      for (int64_t i = first; i < a.T; i += step) wo[i] = a.w[s * a.sw_s + h * a.sw_h + i];
+    return;
+  }
+  const int src = n - a.recent;
+  const bool apart = n - a.keep >= a.recent;  // the rows and their places: they move in any order
+  if (apart || chunk == 0)
+    for (int r0 = chunk * ROWS; r0 < a.recent; r0 += (apart ? a.chunks : 1) * ROWS) {
+      int from[BATCH], to[BATCH];
 #pragma unroll
-    for (int e = 0; e < BATCH; ++e) {
-      const int r = r0 + e * (SHIFT / U) + threadIdx.x / U;
-      from[e] = r < a.recent ? n - a.recent + r : -1;
-      to[e] = a.keep - a.recent + min(r, a.recent - 1);
+      for (int e = 0; e < BATCH; ++e) {
+        const int r = r0 + e * (SHIFT / U) + threadIdx.x / U;
+        from[e] = r < a.recent ? src + r : -1;
+        to[e] = a.keep - a.recent + min(r, a.recent - 1);
+      }
+      move_rows<D>(a, s, h, o, from, to, [] { all_read(); });
+      // no weight is left where its token was: this batch's, or (they overlap) all from `keep` on, at the end
+      if (apart)
+        for (int i = threadIdx.x; i < min(ROWS, a.recent - r0); i += SHIFT) wo[src + r0 + i] = 0.f;
     }
-    move_rows<D>(a, s, h, o, from, to, [] { all_read(); });
+  // nor behind, nor, of the others, before them
+  for (int64_t i = a.keep + first; i < src; i += step) wo[i] = 0.f;
+  for (int64_t i = n + first; i < a.T; i += step) wo[i] = 0.f;
+  if (!apart && chunk == 0) {
+    all_read();
+    for (int i = max(a.keep, src) + threadIdx.x; i < n; i += SHIFT) wo[i] = 0.f;
   }
 }
 
@@ -314,21 +367,26 @@ extern "C" int iq_paged_evict(const iq_paged* p, const float* weights, int64_t s
   const size_t need = iq_paged_evict_workspace_bytes(p->S, p->P, p->H, keep, recent, shared);
   IQ_CHECK(workspace && workspace_bytes >= need, IQ_ERR_WORKSPACE);
   IQ_CHECK(aligned(workspace, 4), IQ_ERR_ALIGN);
-  const int64_t most = rows_that_come(p->P, keep, recent);
-  // at most 8192 workgroups fill: a longer list is taken in turns
-  const int64_t sh = int64_t(p->S) * p->H, rows = FILL / (p->D / 8) * BATCH, turns = sh < 8192 ? 8192 / sh : 1;
-  int64_t chunks = ceil_div(most, rows);
-  chunks = chunks < 1 ? 1 : chunks < turns ? chunks : turns;
-  const EvictArgs a{*p, weights, sw_s, sw_h, weights_out, so_s, so_h, T, keep, recent, sinks, shared, int(most), lens_out,
-                    (int32_t*)workspace, int(chunks)};
+  const int64_t most = rows_that_come(p->P, keep, recent), sh = int64_t(p->S) * p->H;
+  // workgroups per (sequence, head) for `n` rows in turns of `rows`: at most 8192 in all, the longer lists in turns
+  auto chunks_of = [&](int64_t n, int64_t rows) {
+    const int64_t turns = sh < 8192 ? 8192 / sh : 1, c = ceil_div(n, rows);
+    return int(c < 1 ? 1 : c < turns ? c : turns);
+  };
+  const int lanes = p->D / 8;
+  EvictArgs a{*p, weights, sw_s, sw_h, weights_out, so_s, so_h, T, keep, recent, sinks, shared, int(most), lens_out,
+              (int32_t*)workspace, chunks_of(most, FILL / lanes * BATCH)};
   const hipStream_t q = (hipStream_t)stream;
   select_kernel<<<p->S * (p->H / shared), SELECT, 0, q>>>(a);
   if (const int st = launch_status()) return st;
-  auto rest = [&]<int D>() {
-    fill_kernel<D><<<unsigned(sh * chunks), FILL, 0, q>>>(a);
+  auto rest = [&]<int D>() -> int {
+    fill_kernel<D><<<unsigned(sh * a.chunks), FILL, 0, q>>>(a);
     if (const int st = launch_status()) return st;
-    if (!recent || int64_t(p->P) * PAGE <= keep) return int(IQ_OK);
-    shift_kernel<D><<<unsigned(sh), SHIFT, 0, q>>>(a);
+    // a workgroup's turn: SHIFT / lanes * BATCH of the recent rows, and 8 weights per thread
+    const int64_t rows = ceil_div(recent < p->P * int64_t(PAGE) ? recent : p->P * int64_t(PAGE), SHIFT / lanes * BATCH);
+    const int64_t zeros = ceil_div(T, SHIFT * 8);
+    a.chunks = chunks_of(rows > zeros ? rows : zeros, 1);
+    shift_kernel<D><<<unsigned(sh * a.chunks), SHIFT, 0, q>>>(a);
     return launch_status();
   };
   return p->D == 128 ? rest.operator()<128>() : rest.operator()<64>();
