@@ -407,7 +407,9 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int s, int head, in
 // workgroups per CU (registers: D = 128 with T = 2 would spill 209 of them at two.  Spilled as it is: D = 64 with T = 2 6
 // registers, 31 in bf16, and D = 128 with T = 1 in bf16 22, in the masked path and where a (sequence, head) begins and
 // ends; D = 64 is faster so: 48 of 1500 tokens, bf16, 26 us against 30)
-constexpr int per_cu(int D, int T) { return T == 1 || D == 64 ? 2 : 1; }
+// Two maps: one, so that none spills (8 sequences of 16384 tokens, D = 128, at two / one: fp16 85 / 49 us, bf16 117 / 55; 3 new
+// tokens on 24 of 60 .. 6001, D = 64: 53 / 29; 8 of 32768, D = 64: 51 / 49).
+constexpr int per_cu(int D, int T, int maps) { return maps == 1 && (T == 1 || D == 64) ? 2 : 1; }
 
 // the second map's factor of row r of a tile, negated
 template <int R>
@@ -427,7 +429,7 @@ __device__ __forceinline__ void store_stats(const AttnArgs& a, int s, int head, 
 // W: the logits and the rows' sums are kept, for weigh_pages.  MAPS = 2: differential attention (see the end of the
 // file): KV heads in pairs, whose keys are the two maps' and whose V heads are the halves of one of 2 D dims.
 template <int D, bool BF, int T, bool W, int MAPS>
-__global__ __launch_bounds__(THREADS, per_cu(D, T)) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(THREADS, per_cu(D, T, MAPS)) void attn_kernel(AttnArgs a) {
   constexpr int J = D / 16, C = ROWS * T, R = tile_rows<T, MAPS>(), DV = MAPS * D, NQ = MAPS == 1 ? T : MAPS;
   __shared__ float so[WAVES][C][DV + 4];
   __shared__ float sm[WAVES][C], sl[WAVES][C];
@@ -869,7 +871,7 @@ inline Launch plan_of(int S, int P, int m, int nrep, int heads, int D, int maps)
   p.tiles = int(ceil_div(rows, ROWS * p.T / maps));
   const int64_t items = int64_t(S) * heads * p.tiles;
   p.split = P > (items >= 256 ? 32 : items >= 64 ? 16 : 8);
-  p.grid = p.split ? GRID / 2 * per_cu(D, p.T) : int(items);
+  p.grid = p.split ? GRID / 2 * per_cu(D, p.T, maps) : int(items);
   return p;
 }
 
