@@ -399,6 +399,7 @@ extern "C" int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_
   }
   if (N == 0) return IQ_OK;
   if (weights) {
+    IQ_CHECK(iq::prompt_weights_fit(S, N, Nk, Hq, H), IQ_ERR_SHAPE);
     IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(S, N, Nk, Hq, H, D), IQ_ERR_WORKSPACE);
     IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   }

@@ -72,6 +72,7 @@ struct WeighArgs {
 };
 // its workspace: the stats, then the sums
 size_t prompt_weights_bytes(int N, int Nk, int Hq, int H);  // (a multiple of 16)
+bool prompt_weights_fit(int S, int N, int Nk, int Hq, int H);  // a launch's limits
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream);
 
 }  // namespace iq

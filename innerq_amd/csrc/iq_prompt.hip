@@ -518,6 +518,7 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
   const int64_t slots = rows / BM + S;  // first_slot(S) at most
   IQ_CHECK(slots * H <= UINT32_MAX / THREADS, IQ_ERR_SHAPE);
   if (weights) {
+    IQ_CHECK(iq::prompt_weights_fit(S, N, Nk, Hq, H), IQ_ERR_SHAPE);
     IQ_CHECK(workspace && workspace_bytes >= iq_prompt_weights_workspace_bytes(S, N, Nk, Hq, H, D), IQ_ERR_WORKSPACE);
     IQ_CHECK(aligned(workspace, 16), IQ_ERR_ALIGN);
   }

@@ -268,11 +268,15 @@ size_t prompt_weights_bytes(int N, int Nk, int Hq, int H) {
   return chunks > 1 ? stats + (size_t(chunks) * H * Nk * sizeof(float) + 15) / 16 * 16 : stats;
 }
 
+bool prompt_weights_fit(int S, int N, int Nk, int Hq, int H) {
+  const int64_t rows = int64_t(N) * (Hq / H), chunk = chunk_of(rows), chunks = ceil_div(rows, chunk);
+  return (int64_t(Nk) / BK + S) * H <= UINT32_MAX / THREADS / chunks && chunk * chunks <= INT32_MAX;
+}
+
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream) {
   const int64_t slots = int64_t(a.Nk) / BK + a.S;  // first_slot(S) at most
   const int64_t rows = int64_t(a.N) * a.nrep, chunk = chunk_of(rows), chunks = ceil_div(rows, chunk);
   const int H = a.Hq / a.nrep;
-  IQ_CHECK(slots * H * chunks <= UINT32_MAX / THREADS && chunk * chunks <= INT32_MAX, IQ_ERR_SHAPE);
   a.slots = int(slots);
   a.chunk = int(chunk);
   a.part = chunks > 1 ? (float*)((char*)a.stats + (size_t(a.N) * a.Hq * sizeof(float2) + 15) / 16 * 16) : nullptr;

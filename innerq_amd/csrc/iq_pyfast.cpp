@@ -494,12 +494,35 @@ typedef int (*paged_attend_t)(const iq_paged*, const void*, int64_t, int64_t, in
 typedef int (*prompt_t)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, const void*, int64_t, int64_t,
                         const int32_t*, const int32_t*, int, int, int, int, int, int, int, float, int, int, void*, int64_t,
                         int64_t, void*);
+typedef size_t (*weigh_ws_t)(int, int, int, int, int);
+typedef int (*weigh_attend_t)(const iq_paged*, const void*, int64_t, int64_t, int, float, int, void*, int64_t, int64_t, float*,
+                              int64_t, int64_t, int64_t, void*, size_t, void*);
+typedef int (*weigh_prompt_t)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, const void*, int64_t, int64_t,
+                              const int32_t*, const int32_t*, int, int, int, int, int, int, int, float, int, int, void*,
+                              int64_t, int64_t, float*, int64_t, int64_t, int64_t, void*, size_t, void*);
+typedef size_t (*diff_ws_t)(int, int, int, int, int, int, int);
+typedef int (*diff_attend_t)(const iq_paged*, const void*, int64_t, int64_t, int64_t, int, int, const float*, int64_t, float, int,
+                             void*, int64_t, int64_t, int64_t, float*, int64_t, int64_t, int64_t, void*, size_t, void*);
+typedef int (*diff_prompt_t)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, const void*, int64_t, int64_t,
+                             const float*, int64_t, const int32_t*, const int32_t*, int, int, int, int, int, int, int, float,
+                             int, int, void*, int64_t, int64_t, float*, int64_t, int64_t, int64_t, void*, size_t, void*);
+typedef int (*evict_t)(const iq_paged*, const float*, int64_t, int64_t, float*, int64_t, int64_t, int64_t, int, int, int, int,
+                       int32_t*, void*, size_t, void*);
 struct Serving {
   paged_append_t append;
   paged_read_t read;
   paged_ws_t ws;
   paged_attend_t attend;
   prompt_t prompt;
+  weigh_ws_t weigh_ws;
+  weigh_attend_t weigh_attend;
+  paged_ws_t prompt_ws;
+  weigh_prompt_t weigh_prompt;
+  diff_ws_t diff_ws;
+  diff_attend_t diff_attend;
+  diff_prompt_t diff_prompt;
+  paged_ws_t evict_ws;
+  evict_t evict;
 } sv{};
 
 // whether a call on `device` may launch as things are: it is the current device
@@ -559,6 +582,30 @@ bool paged_of(PyObject* const* a, iq_paged* p, at::ScalarType* dt, int* dev) {
   p->H = int(pages->size(1)); p->D = int(PyLong_AsLong(a[1]));
   p->mode = act_flag(*dt);
   return true;
+}
+// gathered weights to add to: fp32 [S, H, >= T], T contiguous, rows of their own (ops.check_weights)
+const at::Tensor* weights_of(PyObject* o, int64_t S, int64_t H, int64_t T, int device) {
+  const at::Tensor* t = tensor_of(o);
+  if (!t || t->dim() != 3 || t->scalar_type() != at::kFloat || t->get_device() != device || t->size(0) != S || t->size(1) != H ||
+      t->size(2) < T || t->size(2) < 1 || t->stride(2) != 1 || followed(*t))
+    return nullptr;
+  std::pair<int64_t, int64_t> d[2];  // (stride, size), by stride
+  int n = 0;
+  for (int i = 0; i < 2; ++i)
+    if (t->size(i) > 1) d[n++] = {t->stride(i), t->size(i)};
+  std::sort(d, d + n);
+  int64_t end = t->size(2);
+  for (int i = 0; i < n; ++i) {
+    if (d[i].first < end) return nullptr;
+    end += d[i].first * (d[i].second - 1);
+  }
+  return t;
+}
+// the second map's factors: fp32 [n]
+const at::Tensor* lam_of(PyObject* o, int64_t n, int device) {
+  const at::Tensor* t = tensor_of(o);
+  return t && t->dim() == 1 && t->scalar_type() == at::kFloat && t->get_device() == device && t->size(0) == n && !followed(*t)
+             ? t : nullptr;
 }
 // cu_seqlens of S sequences over N rows (None: N = S)
 bool cu_of(PyObject* o, int64_t S, int64_t N, int device, const int32_t** cu) {
@@ -664,13 +711,13 @@ PyObject* paged_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return r;
 }
 
-// paged_attend(pages, D, dtype, status, table, lens, q, scale, window, out): the output, or None
+// paged_attend(pages, D, dtype, status, table, lens, q, scale, window, out, weights): the output, or None
 PyObject* paged_attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
   iq_paged p{};
   at::ScalarType dt;
   int dev;
   int64_t window;
-  if (na != 10 || !paged_of(a, &p, &dt, &dev) || !window_of(a[8], &window)) Py_RETURN_NONE;
+  if (na != 11 || !paged_of(a, &p, &dt, &dev) || !window_of(a[8], &window)) Py_RETURN_NONE;
   const at::Tensor* q = tensor_of(a[6]);
   if (!q || (q->dim() != 3 && q->dim() != 4)) Py_RETURN_NONE;
   const int nd = int(q->dim());
@@ -686,11 +733,13 @@ PyObject* paged_attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
     out = *o;
   }
+  const at::Tensor* w = nullptr;
+  if (a[10] != Py_None && (m != 1 || !(w = weights_of(a[10], p.S, p.H, int64_t(p.P) * 64, dev)))) Py_RETURN_NONE;
   void* stream;
   PyObject* key;
   if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
   Py_DECREF(key);
-  const size_t wsb = sv.ws(p.S, p.P, int(m), int(Hq), p.H, p.D);
+  const size_t wsb = w ? sv.weigh_ws(p.S, p.P, int(Hq), p.H, p.D) : sv.ws(p.S, p.P, int(m), int(Hq), p.H, p.D);
   at::Tensor ws;
   try {
     if (!out.defined()) out = like(*q);
@@ -701,17 +750,118 @@ PyObject* paged_attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const int64_t sm = nd == 3 ? 0 : q->stride(1), om = nd == 3 ? 0 : out.stride(1);
   int st;
   Py_BEGIN_ALLOW_THREADS
-  st = sv.attend(&p, q->data_ptr(), q->stride(0), sm, q->stride(nd - 2), int(m), int(Hq), float(scale), int(window),
-                 out.data_ptr(), out.stride(0), om, out.stride(nd - 2), wsb ? ws.data_ptr() : nullptr, wsb, stream);
+  st = w ? sv.weigh_attend(&p, q->data_ptr(), q->stride(0), q->stride(nd - 2), int(Hq), float(scale), int(window), out.data_ptr(),
+                           out.stride(0), out.stride(nd - 2), (float*)w->data_ptr(), w->stride(0), w->stride(1), w->size(2),
+                           ws.data_ptr(), wsb, stream)
+         : sv.attend(&p, q->data_ptr(), q->stride(0), sm, q->stride(nd - 2), int(m), int(Hq), float(scale), int(window),
+                     out.data_ptr(), out.stride(0), om, out.stride(nd - 2), wsb ? ws.data_ptr() : nullptr, wsb, stream);
   Py_END_ALLOW_THREADS
-  if (st != IQ_OK) return not_ok("iq_paged_attention", st);
+  if (st != IQ_OK) return not_ok(w ? "iq_paged_attention_weights" : "iq_paged_attention", st);
   if (a[9] != Py_None) { Py_INCREF(a[9]); return a[9]; }
   return THPVariable_Wrap(std::move(out));
 }
 
-// prompt(q, k, v, cu, scale, cu_k, causal, window, out): the output, or None
+// paged_diff_attend(pages, D, dtype, status, table, lens, q, lam, scale, window, out, weights): the output, or None
+PyObject* paged_diff_attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  iq_paged p{};
+  at::ScalarType dt;
+  int dev;
+  int64_t window;
+  if (na != 12 || !paged_of(a, &p, &dt, &dev) || !window_of(a[9], &window)) Py_RETURN_NONE;
+  const at::Tensor* q = tensor_of(a[6]);
+  if (!q || (q->dim() != 3 && q->dim() != 4)) Py_RETURN_NONE;
+  const int nd = int(q->dim());
+  q = rows_of(a[6], nd, dt, dev, p.D);
+  if (!q || q->size(0) != p.S) Py_RETURN_NONE;
+  const int64_t m = nd == 3 ? 1 : q->size(1), Hq = q->size(nd - 2);
+  if (m < 1 || m > 16 || Hq < 1 || Hq > 4096 || p.H < 2 || p.H % 2 || Hq % p.H) Py_RETURN_NONE;
+  const at::Tensor *lam = lam_of(a[7], Hq / 2, dev), *w = nullptr;
+  if (!lam || (a[11] != Py_None && (m != 1 || !(w = weights_of(a[11], p.S, p.H, int64_t(p.P) * 64, dev))))) Py_RETURN_NONE;
+  const double scale = PyFloat_AsDouble(a[8]);
+  if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  at::DimVector size(q->sizes());
+  size[nd - 2] = Hq / 2;
+  size[nd - 1] = 2 * p.D;
+  at::Tensor out;
+  if (a[10] != Py_None) {
+    const at::Tensor* o = out_rows_of(a[10], nd, dt, dev, 2 * p.D);
+    if (!o || o->sizes() != at::IntArrayRef(size)) Py_RETURN_NONE;
+    out = *o;
+  }
+  void* stream;
+  PyObject* key;
+  if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
+  Py_DECREF(key);
+  const size_t wsb = sv.diff_ws(p.S, p.P, int(m), int(Hq), p.H, p.D, w != nullptr);
+  at::Tensor ws;
+  try {
+    if (!out.defined()) out = at::empty(size, q->options().requires_grad(false));
+    if (wsb) ws = at::empty({int64_t(wsb)}, q->options().dtype(at::kByte).requires_grad(false));
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+  const int64_t sm = nd == 3 ? 0 : q->stride(1), om = nd == 3 ? 0 : out.stride(1);
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = sv.diff_attend(&p, q->data_ptr(), q->stride(0), sm, q->stride(nd - 2), int(m), int(Hq), (const float*)lam->data_ptr(),
+                      lam->stride(0), float(scale), int(window), out.data_ptr(), out.stride(0), om, out.stride(nd - 2),
+                      w ? (float*)w->data_ptr() : nullptr, w ? w->stride(0) : 0, w ? w->stride(1) : 0, w ? w->size(2) : 0,
+                      wsb ? ws.data_ptr() : nullptr, wsb, stream);
+  Py_END_ALLOW_THREADS
+  if (st != IQ_OK) return not_ok("iq_diff_paged_attention", st);
+  if (a[10] != Py_None) { Py_INCREF(a[10]); return a[10]; }
+  return THPVariable_Wrap(std::move(out));
+}
+
+// paged_evict(pages, D, dtype, status, table, lens, weights, keep, recent, sinks, shared, out, lens_out): (lens, weights), or
+// None.  out, lens_out: None or weights and lens themselves.
+PyObject* paged_evict(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  iq_paged p{};
+  at::ScalarType dt;
+  int dev;
+  int64_t v[4];
+  if (na != 13 || !paged_of(a, &p, &dt, &dev) || !ints(a, {7, 8, 9, 10}, v) || (a[11] != Py_None && a[11] != a[6]) ||
+      (a[12] != Py_None && a[12] != a[5]))
+    Py_RETURN_NONE;
+  const int64_t keep = v[0], recent = v[1], sinks = v[2], shared = v[3];
+  const at::Tensor *w = weights_of(a[6], p.S, p.H, int64_t(p.P) * 64, dev), *lens = tensor_of(a[5]);
+  if (!w || keep < 1 || keep > INT32_MAX || recent < 0 || sinks < 0 || recent > keep || sinks > keep || recent + sinks > keep ||
+      shared < 1 || shared > p.H || p.H % shared)
+    Py_RETURN_NONE;
+  void* stream;
+  PyObject* key;
+  if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
+  Py_DECREF(key);
+  const size_t wsb = sv.evict_ws(p.S, p.P, p.H, int(keep), int(recent), int(shared));
+  at::Tensor ws, out, lo;
+  try {
+    ws = at::empty({int64_t(wsb)}, w->options().dtype(at::kByte).requires_grad(false));
+    if (a[11] == Py_None) out = at::empty(w->sizes(), w->options().requires_grad(false));
+    else out = *w;
+    if (a[12] == Py_None) lo = at::empty(lens->sizes(), lens->options());
+    else lo = *lens;
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = sv.evict(&p, (const float*)w->data_ptr(), w->stride(0), w->stride(1), (float*)out.data_ptr(), out.stride(0),
+                out.stride(1), w->size(2), int(keep), int(recent), int(sinks), int(shared), (int32_t*)lo.data_ptr(),
+                ws.data_ptr(), wsb, stream);
+  Py_END_ALLOW_THREADS
+  if (st != IQ_OK) return not_ok("iq_paged_evict", st);
+  PyObject *x = a[12], *y = a[11];
+  if (x == Py_None) x = THPVariable_Wrap(std::move(lo)); else Py_INCREF(x);
+  if (y == Py_None) y = THPVariable_Wrap(std::move(out)); else Py_INCREF(y);
+  PyObject* r = x && y ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return r;
+}
+
+// prompt(q, k, v, cu, scale, cu_k, causal, window, out, weights): the output, or None
 PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
-  if (na != 9 || !PyBool_Check(a[6])) Py_RETURN_NONE;
+  if (na != 10 || !PyBool_Check(a[6])) Py_RETURN_NONE;
   const at::Tensor *q = tensor_of(a[0]), *cu = tensor_of(a[3]);
   if (!q || !cu || q->dim() != 3 || !act_dtype(q->scalar_type()) || cu->dim() != 1) Py_RETURN_NONE;
   const at::ScalarType dt = q->scalar_type();
@@ -740,37 +890,110 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
   PyObject* key;
   if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
   Py_DECREF(key);
-  if (!out.defined()) {
-    try { out = at::empty(q->sizes(), q->options().requires_grad(false)); } catch (...) { Py_RETURN_NONE; }
+  const at::Tensor* w = nullptr;
+  if (a[9] != Py_None && (!(w = weights_of(a[9], S, k->size(1), 0, dev)) || Hq > 4096 || q->stride(0) >= 1 << 23 ||
+                          q->stride(1) >= (1 << 29) / (Hq / k->size(1))))
+    Py_RETURN_NONE;
+  const size_t wsb = w ? sv.prompt_ws(int(S), int(N), int(k->size(0)), int(Hq), int(k->size(1)), int(D)) : 0;
+  at::Tensor ws;
+  try {
+    if (!out.defined()) out = at::empty(q->sizes(), q->options().requires_grad(false));
+    if (w) ws = at::empty({int64_t(wsb)}, q->options().dtype(at::kByte).requires_grad(false));
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+  const int32_t *cq = (const int32_t*)cu->data_ptr(), *ck = (const int32_t*)cu_k->data_ptr();
+  const int Nk = int(k->size(0)), H = int(k->size(1)), causal = a[6] == Py_True;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = w ? sv.weigh_prompt(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(),
+                           v->stride(0), v->stride(1), cq, ck, int(S), int(N), Nk, int(Hq), H, int(D), act_flag(dt),
+                           float(scale), causal, int(window), out.data_ptr(), out.stride(0), out.stride(1),
+                           (float*)w->data_ptr(), w->stride(0), w->stride(1), w->size(2), ws.data_ptr(), wsb, stream)
+         : sv.prompt(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(),
+                     v->stride(0), v->stride(1), cq, ck, int(S), int(N), Nk, int(Hq), H, int(D), act_flag(dt), float(scale),
+                     causal, int(window), out.data_ptr(), out.stride(0), out.stride(1), stream);
+  Py_END_ALLOW_THREADS
+  if (st != IQ_OK) return not_ok(w ? "iq_prompt_attention_weights" : "iq_prompt_attention", st);
+  if (a[8] != Py_None) { Py_INCREF(a[8]); return a[8]; }
+  return THPVariable_Wrap(std::move(out));
+}
+
+// diff_prompt(q, k, v, cu, lam, scale, cu_k, causal, window, out, weights): the output, or None
+PyObject* diff_prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  if (na != 11 || !PyBool_Check(a[7])) Py_RETURN_NONE;
+  const at::Tensor *q = tensor_of(a[0]), *cu = tensor_of(a[3]);
+  if (!q || !cu || q->dim() != 3 || !act_dtype(q->scalar_type()) || cu->dim() != 1) Py_RETURN_NONE;
+  const at::ScalarType dt = q->scalar_type();
+  const int dev = q->get_device();
+  const int64_t D = q->size(2), N = q->size(0), Hq = q->size(1), S = cu->size(0) - 1;
+  q = rows_of(a[0], 3, dt, dev, D);
+  const at::Tensor *k = rows_of(a[1], 3, dt, dev, D), *v = rows_of(a[2], 3, dt, dev, 2 * D);
+  int64_t window;
+  if (!q || !k || !v || S < 1 || S > INT32_MAX || N < 1 || N > INT32_MAX || Hq < 1 || Hq > 4096 || k->size(0) < 1 ||
+      k->size(0) > INT32_MAX || k->size(1) < 2 || k->size(1) % 2 || Hq % k->size(1) || v->size(0) != k->size(0) ||
+      v->size(1) != k->size(1) / 2 || (D != 64 && D != 128) || k->stride(0) >= 1 << 23 || v->stride(0) >= 1 << 23 ||
+      !ints_of(a[3], S + 1, dev) || !window_of(a[8], &window) || (window && a[7] == Py_False) || !current(dev))
+    Py_RETURN_NONE;
+  const int64_t Nk = k->size(0), H = k->size(1);
+  const at::Tensor *lam = lam_of(a[4], Hq / 2, dev), *cu_k = cu, *w = nullptr;
+  if (a[6] != Py_None) cu_k = ints_of(a[6], S + 1, dev);
+  if (!lam || !cu_k || (a[6] == Py_None && Nk != N)) Py_RETURN_NONE;
+  if (a[10] != Py_None && (!(w = weights_of(a[10], S, H, 0, dev)) || q->stride(0) >= 1 << 23 ||
+                           q->stride(1) >= (1 << 29) / (Hq / H)))
+    Py_RETURN_NONE;
+  const double scale = PyFloat_AsDouble(a[5]);
+  if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  at::Tensor out, ws;
+  if (a[9] != Py_None) {
+    const at::Tensor* o = out_rows_of(a[9], 3, dt, dev, 2 * D);
+    if (!o || o->size(0) != N || o->size(1) != Hq / 2) Py_RETURN_NONE;
+    out = *o;
+  }
+  void* stream;
+  PyObject* key;
+  if (!stream_of(dev, &stream, &key)) Py_RETURN_NONE;
+  Py_DECREF(key);
+  const size_t wsb = w ? sv.prompt_ws(int(S), int(N), int(Nk), int(Hq), int(H), int(D)) : 0;
+  try {
+    if (!out.defined()) out = at::empty({N, Hq / 2, 2 * D}, q->options().requires_grad(false));
+    if (w) ws = at::empty({int64_t(wsb)}, q->options().dtype(at::kByte).requires_grad(false));
+  } catch (...) {
+    Py_RETURN_NONE;
   }
   int st;
   Py_BEGIN_ALLOW_THREADS
-  st = sv.prompt(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(),
-                 v->stride(0), v->stride(1), (const int32_t*)cu->data_ptr(), (const int32_t*)cu_k->data_ptr(), int(S), int(N),
-                 int(k->size(0)), int(Hq), int(k->size(1)), int(D), act_flag(dt), float(scale), a[6] == Py_True, int(window),
-                 out.data_ptr(), out.stride(0), out.stride(1), stream);
+  st = sv.diff_prompt(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(),
+                      v->stride(0), v->stride(1), (const float*)lam->data_ptr(), lam->stride(0), (const int32_t*)cu->data_ptr(),
+                      (const int32_t*)cu_k->data_ptr(), int(S), int(N), int(Nk), int(Hq), int(H), int(D), act_flag(dt),
+                      float(scale), a[7] == Py_True, int(window), out.data_ptr(), out.stride(0), out.stride(1),
+                      w ? (float*)w->data_ptr() : nullptr, w ? w->stride(0) : 0, w ? w->stride(1) : 0, w ? w->size(2) : 0,
+                      w ? ws.data_ptr() : nullptr, wsb, stream);
   Py_END_ALLOW_THREADS
-  if (st != IQ_OK) return not_ok("iq_prompt_attention", st);
-  if (a[8] != Py_None) { Py_INCREF(a[8]); return a[8]; }
+  if (st != IQ_OK) return not_ok("iq_diff_prompt_attention", st);
+  if (a[9] != Py_None) { Py_INCREF(a[9]); return a[9]; }
   return THPVariable_Wrap(std::move(out));
 }
 
 // bind_serving(addresses): after bind()
 PyObject* bind_serving(PyObject*, PyObject* const* a, Py_ssize_t na) {
-  if (na != 1 || !PyTuple_Check(a[0]) || PyTuple_Size(a[0]) != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind_serving(five addresses)");
+  if (na != 1 || !PyTuple_Check(a[0]) || PyTuple_Size(a[0]) != 14) {
+    PyErr_SetString(PyExc_TypeError, "bind_serving(fourteen addresses)");
     return nullptr;
   }
-  void* p[5];
-  for (int i = 0; i < 5; ++i) p[i] = PyLong_AsVoidPtr(PyTuple_GetItem(a[0], i));
+  void* p[14];
+  for (int i = 0; i < 14; ++i) p[i] = PyLong_AsVoidPtr(PyTuple_GetItem(a[0], i));
   if (PyErr_Occurred()) return nullptr;
-  sv = {(paged_append_t)p[0], (paged_read_t)p[1], (paged_ws_t)p[2], (paged_attend_t)p[3], (prompt_t)p[4]};
+  sv = {(paged_append_t)p[0], (paged_read_t)p[1], (paged_ws_t)p[2], (paged_attend_t)p[3], (prompt_t)p[4], (weigh_ws_t)p[5],
+        (weigh_attend_t)p[6], (paged_ws_t)p[7], (weigh_prompt_t)p[8], (diff_ws_t)p[9], (diff_attend_t)p[10],
+        (diff_prompt_t)p[11], (paged_ws_t)p[12], (evict_t)p[13]};
   Py_RETURN_NONE;
 }
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(bind), FAST(decode), FAST(qk), FAST(av), FAST(window_append),
                          FAST(bind_serving), FAST(paged_append), FAST(paged_read), FAST(paged_attend), FAST(prompt),
+                         FAST(paged_diff_attend), FAST(diff_prompt), FAST(paged_evict),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_iqfast", nullptr, -1, methods};
 

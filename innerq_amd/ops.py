@@ -54,7 +54,9 @@ def _native(t):
     m.bind(tuple(ctypes.cast(getattr(h, n), ctypes.c_void_p).value for n in names), _WS,
            torch._C._cuda_getCurrentRawStream)
     names = ("iq_paged_append", "iq_paged_read", "iq_paged_attention_workspace_bytes", "iq_paged_attention",
-             "iq_prompt_attention")
+             "iq_prompt_attention", "iq_paged_attention_weights_workspace_bytes", "iq_paged_attention_weights",
+             "iq_prompt_weights_workspace_bytes", "iq_prompt_attention_weights", "iq_diff_paged_attention_workspace_bytes",
+             "iq_diff_paged_attention", "iq_diff_prompt_attention", "iq_paged_evict_workspace_bytes", "iq_paged_evict")
     m.bind_serving(tuple(ctypes.cast(getattr(h, n), ctypes.c_void_p).value for n in names))
     _fast = m
     return m
@@ -962,9 +964,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     sequence s (of those below T), summed over its rows and the query heads of KV head h, as PagedStore.evict goes by.
     The rows may be a prompt's last ones, behind all its keys.  The call then takes 8 bytes of memory per row and query
     head."""
-    fast = _native(q) if forward_ad._current_level < 0 and weights is None else None
+    fast = _native(q) if forward_ad._current_level < 0 else None
     if fast is not None:
-        r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out)
+        r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out, weights)
         if r is not None:
             return r
     require_act(q, "q")
@@ -1035,6 +1037,11 @@ def diff_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
     refused, ``out`` too.
 
     The steps behind such a prompt are PagedStore.diff_attend's: store.append(k, v.view(Nk, H, D), ...)."""
+    fast = _native(q) if forward_ad._current_level < 0 else None
+    if fast is not None:
+        r = fast.diff_prompt(q, k, v, cu_seqlens, lam, scale, cu_seqlens_k, causal, window, out, weights)
+        if r is not None:
+            return r
     require_act(q, "q")
     if autograd_follows(q, k, v, lam, out, weights):
         raise NotImplementedError("diff_prompt_attention has no backward: call it under torch.no_grad()")

@@ -249,9 +249,9 @@ class PagedStore:
         by the softmax weights of token j, summed over the query heads of KV head h (evict() goes by what they add up
         to).  With one new token per sequence only (a drafted token's weights could not be taken back).  The call then
         takes 4 bytes of memory per query head and place of the table."""
-        fast = ops._native(q) if forward_ad._current_level < 0 and weights is None else None
+        fast = ops._native(q) if forward_ad._current_level < 0 else None
         if fast is not None:
-            r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out)
+            r = fast.paged_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, scale, window, out, weights)
             if r is not None:
                 return r
         _no_grad(q, out, weights)
@@ -306,6 +306,12 @@ class PagedStore:
 
         weights: as attend()'s, fp32 [S, H, T]: each KV head's tokens gather the weights of its own map, whatever lam
         (evict(shared=2) keeps the same tokens for both)."""
+        fast = ops._native(q) if forward_ad._current_level < 0 else None
+        if fast is not None:
+            r = fast.paged_diff_attend(self.pages, self.D, self.dtype, self.status, table, lens, q, lam, scale, window, out,
+                                       weights)
+            if r is not None:
+                return r
         _no_grad(q, out, lam, weights)
         p = self._args(table, lens)
         if q.dim() not in (3, 4) or q.shape[0] != p.S:
@@ -357,6 +363,12 @@ class PagedStore:
         (weights itself, memory that no other argument uses, or a new tensor), 0 from ``keep`` on where tokens were
         dropped.  A sequence of a bad length is left as it is, a row that has to move from a page outside the pool becomes
         NaN (check())."""
+        fast = ops._native(weights) if forward_ad._current_level < 0 else None
+        if fast is not None:
+            r = fast.paged_evict(self.pages, self.D, self.dtype, self.status, table, lens, weights, keep, recent, sinks, shared,
+                                 out, lens_out)
+            if r is not None:
+                return r
         _no_grad(weights, out)
         p = self._args(table, lens)
         keep, recent, sinks, shared = (int(x) for x in (keep, recent, sinks, shared))
