@@ -27,7 +27,8 @@ __device__ __forceinline__ void load_to_lds(rsrc_t d, u4_t* lds, uint32_t at) {
 }
 
 // rows [r0, r1) of sequence s in a packed tensor of n rows (whatever cu holds)
-__device__ __forceinline__ void rows_of(const int32_t* cu, int s, int n, int& r0, int& r1) {
+template <typename Cu>
+__device__ __forceinline__ void rows_of(Cu cu, int s, int n, int& r0, int& r1) {
   r0 = min(max(cu[s], 0), n);
   r1 = min(max(cu[s + 1], r0), n);
 }
@@ -69,6 +70,7 @@ struct WeighArgs {
   // set by launch_prompt_weights: rows (times heads) of a workgroup, and where several share a key, their sums [..][H][Nk]
   int chunk;
   float* part;
+  int steps;  // tiles of keys of a workgroup
 };
 // its workspace: the stats, then the sums
 size_t prompt_weights_bytes(int N, int Nk, int Hq, int H);  // (a multiple of 16)

@@ -17,17 +17,21 @@ using namespace iq;
 namespace {
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, BR = 64;  // rows of a tile
-constexpr int KB = 1, BK = 2 * 32 * KB;                  // blocks of 32 keys of a wave, keys of a workgroup
+constexpr int BK = 32 * WAVES / 2;                        // keys of a workgroup
 constexpr int CHUNK = 2048, MOST_CHUNKS = 16;            // rows (times heads) of a workgroup, at least; chunks of a sequence
 
-// A slot's sequence and keys, and the rows, as rows times heads one behind the other, that see any of them.
+// Few rows over many keys: a workgroup holds up to FEW rows in LDS and walks over a.steps times BK keys, as many as leave
+// FEW_GROUPS workgroups (two per CU: their beginning, some 10 us, is then paid once).
+constexpr int FEW = 256, FEW_GROUPS = 512, MOST_STEPS = 64, FEW_WAVES = 8, FEW_THREADS = 64 * FEW_WAVES, FEW_KEYS = 32 * FEW_WAVES;
+
+// A slot's sequence and keys (of `bk` a slot), and the rows, as rows times heads one behind the other, that see any of them.
 struct Keys {
   int s, q0, k0, j0, j1, off;  // off: row i stands at key i + off
   int keys, v0, v1, rows;      // rows: [.., rows) of the sequence see any of them
 };
-__device__ __forceinline__ bool keys_of(const WeighArgs& a, int slot, Keys& x) {
+__device__ __forceinline__ bool keys_of(const WeighArgs& a, int slot, int bk, Keys& x) {
   // sequence s has the slots from first_slot(s) to first_slot(s + 1), at least as many as it has tiles of keys
-  auto first_slot = [&](int i) { return min(max(a.cu_k[i], 0), a.Nk) / BK + i; };
+  auto first_slot = [&](int i) { return min(max(a.cu_k[i], 0), a.Nk) / bk + i; };
   const int lane = threadIdx.x & 63;
   int s = 0;
   for (int m = a.S; m > 1;) {  // it is among the m from s on
@@ -37,17 +41,16 @@ __device__ __forceinline__ bool keys_of(const WeighArgs& a, int slot, Keys& x) {
     s += at * step;
   }
   x.s = __builtin_amdgcn_readfirstlane(s);
+  typedef const __attribute__((address_space(4))) int32_t* consts_t;  // (by scalar loads)
   int q1, k1;
-  rows_of(a.cu_q, x.s, a.N, x.q0, q1);
-  rows_of(a.cu_k, x.s, a.Nk, x.k0, k1);
-  x.q0 = __builtin_amdgcn_readfirstlane(x.q0);
-  x.k0 = __builtin_amdgcn_readfirstlane(x.k0);
-  const int lq = __builtin_amdgcn_readfirstlane(q1) - x.q0;
-  x.keys = __builtin_amdgcn_readfirstlane(k1) - x.k0;
+  rows_of((consts_t)a.cu_q, x.s, a.N, x.q0, q1);
+  rows_of((consts_t)a.cu_k, x.s, a.Nk, x.k0, k1);
+  const int lq = q1 - x.q0;
+  x.keys = k1 - x.k0;
   x.off = x.keys - lq;
-  x.j0 = (slot - __builtin_amdgcn_readfirstlane(first_slot(x.s))) * BK;
+  x.j0 = (slot - (x.k0 / bk + x.s)) * bk;
   if (x.j0 >= x.keys || x.j0 >= a.T) return false;
-  x.j1 = min(x.j0 + BK, x.keys);
+  x.j1 = min(x.j0 + bk, x.keys);
   const int first = a.causal ? max(x.j0 - x.off, 0) : 0;
   const int64_t seen = int64_t(x.j1) - 1 + a.window - x.off;  // rows below it see a key, in a window
   x.rows = a.window && seen < lq ? int(seen) : lq;
@@ -56,18 +59,76 @@ __device__ __forceinline__ bool keys_of(const WeighArgs& a, int slot, Keys& x) {
   return first < x.rows;
 }
 
+// Sums of 16 values over the 32 lanes of rows: halves of the values change places step by step, until lanes n and n + 16 hold
+// halves of value n's sum, then the sum.
+__device__ __forceinline__ float sum_rows(float (&acc)[16]) {
+  const int n = threadIdx.x & 31;
+#pragma unroll
+  for (int b = 8; b > 0; b /= 2) {
+    const bool up = n & b;
+#pragma unroll
+    for (int i = 0; i < b; ++i) {
+      const float x = acc[i], y = acc[i + b];
+      acc[i] = (up ? y : x) + __shfl_xor(up ? x : y, b, 64);
+    }
+  }
+  return acc[0] + __shfl_xor(acc[0], 16, 64);
+}
+
+// A block of 32 rows (in LDS, this lane's operands at qa bytes) against a wave's 32 keys: the logits, s[i] of key 8 (i / 4) +
+// 4 hi + i % 4 and row n.  st: {base, 1 / sum} of this lane's row.
 template <int D, bool BF>
-__global__ __launch_bounds__(THREADS, 4 / KB) void weigh_kernel(WeighArgs a) {
+struct Block {
+  static constexpr int KS = D / 16;
+  static __device__ __forceinline__ f16_t logits(const u4_t* lds, const int (&qa)[KS], const u4_t (&kx)[KS]) {
+    u4_t y[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) y[ks] = *reinterpret_cast<const u4_t*>(reinterpret_cast<const char*>(lds) + qa[ks]);
+    f16_t s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mma32<BF>(kx[ks], y[ks], s);
+    return s;
+  }
+  // all rows see all keys
+  static __device__ __forceinline__ void add_whole(const u4_t* lds, const int (&qa)[KS], const u4_t (&kx)[KS], float c, float2 st,
+                                                   float (&acc)[16]) {
+    const f16_t s = logits(lds, qa, kx);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      acc[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -st.x)), st.y, acc[i]);
+  }
+  // any rows: a lane's row sees the keys [first, last), counted from the lane's first key
+  static __device__ __forceinline__ void add_some(const u4_t* lds, const int (&qa)[KS], const u4_t (&kx)[KS], float c, bool big,
+                                                  float2 st, int first, int last, float (&acc)[16]) {
+    f16_t s = logits(lds, qa, kx);
+    if (big) {  // logits rounded as the base is
+      s *= c;
+      c = 1.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int j = 8 * (i / 4) + i % 4;
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -st.x)) * st.y;
+      acc[i] += j < last && j >= first ? w : 0.f;
+    }
+  }
+};
+__device__ __forceinline__ bool big_base(float2 st) { return __any(fabsf(st.x) > 65536.f); }
+
+template <int D, bool BF>
+__global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
 #pragma clang fp contract(off)  // logits times c less the base: one fma, as in the attention
   constexpr int CH = D / 8, KS = D / 16, LOADS = BR * CH / THREADS;
   __shared__ u4_t tile0[BR * CH], tile1[BR * CH];
   __shared__ float halves[BK];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
-  const int kw = wave & 1, rw = wave >> 1;
+  const int kw = wave % (WAVES / 2), rw = wave / (WAVES / 2);  // halves of the keys, of a tile's rows
   const int H = gridDim.x / a.slots, kvh = blockIdx.x % H;
   const int head0 = kvh / a.maps * a.nrep * a.maps + kvh % a.maps;  // its query heads: head0 + i * maps
   Keys x;
-  if (!keys_of(a, blockIdx.x / H, x)) return;
+  if (!keys_of(a, blockIdx.x / H, BK, x)) return;
   const int v0 = max(x.v0, int(blockIdx.y) * a.chunk), v1 = min(x.v1, int(blockIdx.y + 1) * a.chunk);
   if (v0 >= v1) return;
   const int q0 = x.q0, j0 = x.j0, tiles = (v1 - v0 + BR - 1) / BR;
@@ -76,13 +137,11 @@ __global__ __launch_bounds__(THREADS, 4 / KB) void weigh_kernel(WeighArgs a) {
   const int64_t whole = int64_t(j0) + a.window - x.off;  // rows below it, in a window
   const int vg = !a.window || whole >= x.rows ? v1 : whole <= 0 ? 0 : min(v1, int(whole) * a.nrep);
 
-  u4_t kx[KB][KS];  // A operands: key 32 kb + n of the wave's (past the last: that one again, not stored)
+  u4_t kx[KS];  // A operands: key n of the wave's (past the last: that one again, not stored)
+  {
+    const uint16_t* p = a.k + int64_t(x.k0 + min(j0 + kw * 32 + n, x.keys - 1)) * a.sk_n + kvh * a.sk_h + 8 * hi;
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    const int j = min(j0 + (kw * KB + kb) * 32 + n, x.keys - 1);
-    const uint16_t* p = a.k + int64_t(x.k0 + j) * a.sk_n + kvh * a.sk_h + 8 * hi;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) kx[kb][ks] = *reinterpret_cast<const u4_t*>(p + 16 * ks);
+    for (int ks = 0; ks < KS; ++ks) kx[ks] = *reinterpret_cast<const u4_t*>(p + 16 * ks);
   }
   // a row of the tiles in their order, as query row and head (a step of BR without a division)
   struct Place {
@@ -139,104 +198,151 @@ __global__ __launch_bounds__(THREADS, 4 / KB) void weigh_kernel(WeighArgs a) {
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) qa[ks] = chunk_at<D>(rw * 32 + n, 2 * ks + hi) * 16;
 
-  float acc[16 * KB];  // of value 16 kb + i: key 32 kb + 8 (i / 4) + 4 hi + i % 4
+  float acc[16];  // of key 8 (i / 4) + 4 hi + i % 4
 #pragma unroll
-  for (int i = 0; i < 16 * KB; ++i) acc[i] = 0.f;
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
   // this lane's row of the next tile, and its {base, 1 / sum} (past the last: that one again, not counted)
   Place mine = place_of(v0 + rw * 32 + n);
-  int mine_v = v0 + rw * 32 + n;
   const float2* stats = a.stats + int64_t(q0) * a.Hq + head0;
   auto stats_of = [&] {
     return stats[int64_t(min(mine.row, x.rows - 1)) * a.Hq + (mine.row < x.rows ? mine.head : a.nrep - 1) * a.maps];
   };
-  auto scores = [&](const u4_t* lds, f16_t (&st)[KB]) {
-    u4_t y[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) y[ks] = *reinterpret_cast<const u4_t*>(reinterpret_cast<const char*>(lds) + qa[ks]);
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) st[kb] = mma32<BF>(kx[kb][ks], y[ks], st[kb]);
-    }
-  };
-  auto add_tile = [&](int t, const u4_t* lds, int row, bool real, float2 w) {
-    f16_t st[KB];
-    const int va = v0 + t * BR;
-    if (va >= vf && va + BR <= vg && !__any(fabsf(w.x) > 65536.f)) {  // all rows see all keys
-      scores(lds, st);
-#pragma unroll
-      for (int i = 0; i < 16 * KB; ++i)
-        acc[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[i / 16][i % 16], a.scale.c, -w.x)), w.y, acc[i]);
-      return;
-    }
-    scores(lds, st);
-    float c = a.scale.c;
-    if (__any(fabsf(w.x) > 65536.f)) {  // logits rounded as the base is
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) st[kb] *= c;
-      c = 1.f;
-    }
-    // key j is seen iff first <= j < last, counted from the lane's first key
-    const int base = j0 + kw * 32 * KB + 4 * hi;
-    const int last = (real ? a.causal ? min(row + x.off + 1, x.keys) : x.keys : 0) - base;
-    const int first = (a.window ? max(row + x.off + 1 - a.window, 0) : 0) - base;
-#pragma unroll
-    for (int i = 0; i < 16 * KB; ++i) {
-      const int j = 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4;
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i / 16][i % 16], c, -w.x)) * w.y;
-      acc[i] += j < last && j >= first ? y : 0.f;
-    }
-  };
   fetch(tile0);
   float2 next = stats_of();
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) kx[kb][ks] = (kx[kb][ks] & a.scale.keep) ^ a.scale.sign;
+  for (int ks = 0; ks < KS; ++ks) kx[ks] = (kx[ks] & a.scale.keep) ^ a.scale.sign;
   // (a buffer by name in each half of the loop: reads of one would wait for the loads to the other)
   auto turn = [&](int t, u4_t* here, u4_t* other) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // the tile is there, and no wave reads the other buffer any more
     const int row = mine.row;
-    const bool real = mine_v < v1;
-    const float2 w = next;
+    const float2 st = next;
     if (t + 1 < tiles) {
       fetch(other);
-      mine_v += BR;
       advance(mine);
       next = stats_of();
     }
-    add_tile(t, here, row, real, w);
+    const int va = v0 + t * BR;
+    const bool big = big_base(st);
+    if (va >= vf && va + BR <= vg && !big) {
+      Block<D, BF>::add_whole(here, qa, kx, a.scale.c, st, acc);
+      return;
+    }
+    const int base = j0 + kw * 32 + 4 * hi;
+    const int last = (va + rw * 32 + n < v1 ? a.causal ? min(row + x.off + 1, x.keys) : x.keys : 0) - base;
+    const int first = (a.window ? max(row + x.off + 1 - a.window, 0) : 0) - base;
+    Block<D, BF>::add_some(here, qa, kx, a.scale.c, big, st, first, last, acc);
   };
   for (int t = 0; t < tiles; t += 2) {
     turn(t, tile0, tile1);
     if (t + 1 < tiles) turn(t + 1, tile1, tile0);
   }
-  // Sums over the 32 lanes of rows: halves of the values change places step by step, until lane n holds value n's sum (with
-  // 16 values: lanes n and n + 16 each a half of value n % 16's, then the sum).
-#pragma unroll
-  for (int b = 8 * KB; b > 0; b /= 2) {
-    const bool up = n & b;
-#pragma unroll
-    for (int i = 0; i < b; ++i) acc[i] = (up ? acc[i + b] : acc[i]) + __shfl_xor(up ? acc[i] : acc[i + b], b, 64);
-  }
-  if constexpr (KB == 1) acc[0] += __shfl_xor(acc[0], 16, 64);
-  const int j = kw * 32 * KB + 32 * (n / 16 % KB) + 8 * (n % 16 / 4) + 4 * hi + n % 4;
-  if (rw == 1) halves[j] = acc[0];
+  const float half = sum_rows(acc);
+  const int j = kw * 32 + 8 * (n % 16 / 4) + 4 * hi + n % 4;
+  if (rw == 1) halves[j] = half;
   __syncthreads();
-  if (rw == 1 || n >= 16 * KB || j0 + j >= x.j1 || j0 + j >= a.T) return;
-  const float sum = acc[0] + halves[j];
+  if (rw == 1 || n >= 16 || j0 + j >= x.j1 || j0 + j >= a.T) return;
+  const float sum = half + halves[j];
   if (a.part) a.part[(int64_t(blockIdx.y) * H + kvh) * a.Nk + x.k0 + j0 + j] = sum;
   else a.weights[x.s * a.sw_s + kvh * a.sw_h + j0 + j] += sum;
+}
+
+// The same for few rows over many keys.  The rows (up to FEW; more in turns) stay in LDS with their statistics in registers,
+// and a wave takes 32 of each step's 128 keys over all of them, with the next step's keys on their way: no barriers, and each
+// key's sum is one wave's.  (64 rows behind 16000 keys on 4 sequences, 8 KV heads, D = 128: 85 us by weigh_kernel, here NEW.)
+template <int D, bool BF>
+__global__ __launch_bounds__(FEW_THREADS, 4) void weigh_few_kernel(WeighArgs a) {
+#pragma clang fp contract(off)
+  constexpr int CH = D / 8, KS = D / 16, LOADS = FEW * CH / FEW_THREADS;
+  __shared__ u4_t rows[FEW * CH];
+  __shared__ float2 stats[FEW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hi = lane >> 5;
+  const int H = gridDim.x / a.slots, kvh = blockIdx.x % H;
+  const int head0 = kvh / a.maps * a.nrep * a.maps + kvh % a.maps;  // its query heads: head0 + i * maps
+  Keys x;
+  if (!keys_of(a, blockIdx.x / H, FEW_KEYS * a.steps, x)) return;
+  const uint16_t* kp = a.k + int64_t(x.k0) * a.sk_n + kvh * a.sk_h + 8 * hi;
+  auto load_keys = [&](int j, u4_t (&y)[KS]) {  // (past the last: that one again, not stored)
+    const uint16_t* p = kp + int64_t(min(j + n, x.keys - 1)) * a.sk_n;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) y[ks] = *reinterpret_cast<const u4_t*>(p + 16 * ks);
+  };
+  int qa[KS];  // this lane's operands in a block of 32 rows, in bytes
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qa[ks] = chunk_at<D>(n, 2 * ks + hi) * 16;
+  float* const to = a.weights + x.s * a.sw_s + kvh * a.sw_h;
+  for (int v0 = x.v0; v0 < x.v1; v0 += FEW) {
+    const int v1 = min(v0 + FEW, x.v1), blocks = (v1 - v0 + 31) / 32;
+    if (v0 > x.v0) __syncthreads();  // nobody reads the last rows any more
+    // (past the last row: that one again, not counted)
+    const int r0 = threadIdx.x / CH, step = FEW_THREADS / CH, step_row = step / a.nrep, step_head = step - step_row * a.nrep;
+    int row = (v0 + r0) / a.nrep, head = v0 + r0 - row * a.nrep;
+    constexpr int BATCH = LOADS < 8 ? LOADS : 8;  // loads under way together
+#pragma clang loop unroll(disable)
+    for (int i0 = 0; i0 < LOADS; i0 += BATCH) {
+      u4_t y[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const bool real = v0 + (i0 + i) * step + r0 < v1;
+        y[i] = *reinterpret_cast<const u4_t*>(a.q + int64_t(x.q0 + (real ? row : x.rows - 1)) * a.sq_n +
+                                              int64_t(head0 + (real ? head : a.nrep - 1) * a.maps) * a.sq_h +
+                                              8 * (threadIdx.x % CH));
+        row += step_row;
+        head += step_head;
+        if (head >= a.nrep) {
+          head -= a.nrep;
+          ++row;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) rows[chunk_at<D>((i0 + i) * step + r0, threadIdx.x % CH)] = y[i];
+    }
+    if (threadIdx.x < FEW) {
+      const int v = min(v0 + int(threadIdx.x), v1 - 1), row = v / a.nrep;
+      stats[threadIdx.x] = a.stats[int64_t(x.q0 + row) * a.Hq + head0 + (v - row * a.nrep) * a.maps];
+    }
+    __syncthreads();
+    for (int j0 = x.j0 + 32 * wave; j0 < x.j1; j0 += FEW_KEYS) {
+      u4_t kx[KS];
+      load_keys(j0, kx);
+      // this lane's key after the sums, and what it has gathered
+      const int key = j0 + 8 * (n % 16 / 4) + 4 * hi + n % 4;
+      const bool mine = n < 16 && key < x.j1 && key < a.T;
+      const float old = mine ? to[key] : 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kx[ks] = (kx[ks] & a.scale.keep) ^ a.scale.sign;
+      float acc[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+      // of the rows, [vf, vg) see all of these keys
+      const int vf = a.causal ? max(min(j0 + 32, x.j1) - 1 - x.off, 0) * a.nrep : 0;
+      const int64_t whole = int64_t(j0) + a.window - x.off;  // rows below it, in a window
+      const int vg = !a.window || whole >= x.rows ? v1 : whole <= 0 ? 0 : min(v1, int(whole) * a.nrep);
+#pragma clang loop unroll(disable)
+      for (int b = 0; b < blocks; ++b) {
+        const float2 st = stats[32 * b + n];
+        const int va = v0 + 32 * b;
+        const bool big = big_base(st);
+        if (va >= vf && va + 32 <= vg && !big) {
+          Block<D, BF>::add_whole(rows + 32 * b * CH, qa, kx, a.scale.c, st, acc);
+          continue;
+        }
+        const int base = j0 + 4 * hi, v = va + n, row = v / a.nrep;
+        const int last = (v < v1 ? a.causal ? min(row + x.off + 1, x.keys) : x.keys : 0) - base;
+        const int first = (a.window ? max(row + x.off + 1 - a.window, 0) : 0) - base;
+        Block<D, BF>::add_some(rows + 32 * b * CH, qa, kx, a.scale.c, big, st, first, last, acc);
+      }
+      const float sum = sum_rows(acc);
+      if (mine) to[key] = old + sum;
+    }
+  }
 }
 
 // adds the chunks' sums of BK keys
 __global__ __launch_bounds__(64) void add_kernel(WeighArgs a) {
   const int H = gridDim.x / a.slots, kvh = blockIdx.x % H;
   Keys x;
-  if (!keys_of(a, blockIdx.x / H, x)) return;
+  if (!keys_of(a, blockIdx.x / H, BK, x)) return;
   for (int j = x.j0 + threadIdx.x; j < x.j1 && j < a.T; j += 64) {
     float sum = 0.f;
     for (int z = x.v0 / a.chunk; z <= (x.v1 - 1) / a.chunk; ++z) sum += a.part[(int64_t(z) * H + kvh) * a.Nk + x.k0 + j];
@@ -250,8 +356,17 @@ inline int64_t chunk_of(int64_t rows) {
   return even < CHUNK ? CHUNK : even;
 }
 
+// Whether a call has few rows over many keys: by the mean of its sequences.
+inline bool few(int S, int N, int Nk, int Hq, int H) {
+  return int64_t(N) * (Hq / H) <= int64_t(FEW) * S && int64_t(Nk) >= int64_t(1024) * S;
+}
+
 template <int D, bool BF>
-int launch(const WeighArgs& a, dim3 grid, hipStream_t stream) {
+int launch(const WeighArgs& a, bool few, dim3 grid, hipStream_t stream) {
+  if (few) {
+    weigh_few_kernel<D, BF><<<grid, FEW_THREADS, 0, stream>>>(a);
+    return launch_status();
+  }
   weigh_kernel<D, BF><<<grid, THREADS, 0, stream>>>(a);
   if (const int st = launch_status()) return st;
   if (!a.part) return IQ_OK;
@@ -274,14 +389,16 @@ bool prompt_weights_fit(int S, int N, int Nk, int Hq, int H) {
 }
 
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream) {
-  const int64_t slots = int64_t(a.Nk) / BK + a.S;  // first_slot(S) at most
-  const int64_t rows = int64_t(a.N) * a.nrep, chunk = chunk_of(rows), chunks = ceil_div(rows, chunk);
   const int H = a.Hq / a.nrep;
-  a.slots = int(slots);
+  const bool f = few(a.S, a.N, a.Nk, a.Hq, H);
+  const int64_t steps = ceil_div(int64_t(a.Nk) * H, int64_t(FEW_KEYS) * FEW_GROUPS);
+  a.steps = !f || steps < 1 ? 1 : steps < MOST_STEPS ? int(steps) : MOST_STEPS;
+  a.slots = int(int64_t(a.Nk) / (f ? FEW_KEYS * a.steps : BK) + a.S);  // first_slot(S) at most
+  const int64_t rows = int64_t(a.N) * a.nrep, chunk = chunk_of(rows), chunks = f ? 1 : ceil_div(rows, chunk);
   a.chunk = int(chunk);
   a.part = chunks > 1 ? (float*)((char*)a.stats + (size_t(a.N) * a.Hq * sizeof(float2) + 15) / 16 * 16) : nullptr;
-  const dim3 grid(unsigned(slots * H), unsigned(chunks));
-  if (D == 128) return bf ? launch<128, true>(a, grid, stream) : launch<128, false>(a, grid, stream);
-  return bf ? launch<64, true>(a, grid, stream) : launch<64, false>(a, grid, stream);
+  const dim3 grid(unsigned(int64_t(a.slots) * H), unsigned(chunks));
+  if (D == 128) return bf ? launch<128, true>(a, f, grid, stream) : launch<128, false>(a, f, grid, stream);
+  return bf ? launch<64, true>(a, f, grid, stream) : launch<64, false>(a, f, grid, stream);
 }
 }  // namespace iq
