@@ -67,13 +67,13 @@ struct WeighArgs {
   Scale scale;
   int causal, window;
   int maps;  // 2: differential attention, KV head 2g + i's rows are those of query heads 2j + i, j in its group
-  // set by launch_prompt_weights: rows (times heads) of a workgroup, and where several share a key, their sums [..][H][Nk]
-  int chunk;
+  // set by launch_prompt_weights: workgroups that share a key, and where several do, their sums [shares][H][Nk]
+  int shares;
   float* part;
   int steps;  // tiles of keys of a workgroup
 };
 // its workspace: the stats, then the sums
-size_t prompt_weights_bytes(int N, int Nk, int Hq, int H);  // (a multiple of 16)
+size_t prompt_weights_bytes(int S, int N, int Nk, int Hq, int H);  // (a multiple of 16)
 bool prompt_weights_fit(int S, int N, int Nk, int Hq, int H);  // a launch's limits
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream);
 

@@ -528,7 +528,7 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
                sv_h, so_n, so_h, cu_q, cu_k, S, N, Nk, Hq, Hq / H, int(slots), sc.c, 8.f / sc.c, sc.keep, sc.sign,
                causal ? 1 : 0, window, weights ? (float2*)workspace : nullptr, weights ? splits_of(S, N, Nk, Hq, H) : 1,
                nullptr};
-  if (a.splits > 1) a.part = (float*)((char*)workspace + iq::prompt_weights_bytes(N, Nk, Hq, H));
+  if (a.splits > 1) a.part = (float*)((char*)workspace + iq::prompt_weights_bytes(S, N, Nk, Hq, H));
   auto launch = [&]<int D_, bool BF>() {
     const dim3 grid(unsigned(slots * H), unsigned(a.splits));
     if (a.splits == 1) {
@@ -553,7 +553,7 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
 extern "C" size_t iq_prompt_weights_workspace_bytes(int S, int N, int Nk, int Hq, int H, int D) {
   if (S <= 0 || N <= 0 || Nk < 0 || Hq <= 0 || H <= 0 || Hq % H || !d_ok(D)) return 0;
   const size_t slots = size_t(N) * (Hq / H) / BM + S, splits = splits_of(S, N, Nk, Hq, H);
-  return iq::prompt_weights_bytes(N, Nk, Hq, H) +
+  return iq::prompt_weights_bytes(S, N, Nk, Hq, H) +
          (splits > 1 ? slots * H * splits * WAVES * (32 * D + 64) * sizeof(float) : 0);
 }
 

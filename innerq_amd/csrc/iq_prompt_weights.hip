@@ -7,9 +7,10 @@
 // tile's weights are added up register by register, and lanes meet only once, at the end.  Waves: two halves of the keys by
 // two halves of a tile's rows.
 //
-// A key at the beginning of a long prompt is seen by all its rows, so a workgroup takes at most CHUNK of them; where a
-// sequence may have more, partial sums go to the workspace and a second launch adds them.  Rows are added in a fixed order:
-// no atomics.
+// A key at the beginning of a long prompt is seen by all its rows, so up to SHARES workgroups share a key: each takes every
+// so-manieth CHUNK of the rows, and a second launch adds their sums (how many rows a sequence has is not known on the host:
+// a share that finds none ends at once, and the shares are as many as leave GROUPS workgroups).  Rows are added in a fixed
+// order: no atomics.
 #include "iq_prompt.h"
 
 using namespace iq;
@@ -18,7 +19,7 @@ namespace {
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, BR = 64;  // rows of a tile
 constexpr int BK = 32 * WAVES / 2;                        // keys of a workgroup
-constexpr int CHUNK = 2048, MOST_CHUNKS = 16;            // rows (times heads) of a workgroup, at least; chunks of a sequence
+constexpr int CHUNK = 2048, SHARES = 16, GROUPS = 8192;  // rows (times heads) of a chunk; most workgroups of a key, in all
 
 // Few rows over many keys: a workgroup holds up to FEW rows in LDS and walks over a.steps times BK keys, as many as leave
 // FEW_GROUPS workgroups (two per CU: their beginning, some 10 us, is then paid once).
@@ -117,6 +118,12 @@ struct Block {
 };
 __device__ __forceinline__ bool big_base(float2 st) { return __any(fabsf(st.x) > 65536.f); }
 
+// the first chunk of a share that has rows which see the keys (or one behind them)
+__device__ __forceinline__ int share_chunk(const Keys& x, int share, int shares) {
+  const int c = x.v0 / CHUNK, ahead = share - c % shares;
+  return c + (ahead < 0 ? ahead + shares : ahead);
+}
+
 template <int D, bool BF>
 __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
 #pragma clang fp contract(off)  // logits times c less the base: one fma, as in the attention
@@ -129,13 +136,13 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
   const int head0 = kvh / a.maps * a.nrep * a.maps + kvh % a.maps;  // its query heads: head0 + i * maps
   Keys x;
   if (!keys_of(a, blockIdx.x / H, BK, x)) return;
-  const int v0 = max(x.v0, int(blockIdx.y) * a.chunk), v1 = min(x.v1, int(blockIdx.y + 1) * a.chunk);
-  if (v0 >= v1) return;
-  const int q0 = x.q0, j0 = x.j0, tiles = (v1 - v0 + BR - 1) / BR;
+  const int first_chunk = share_chunk(x, blockIdx.y, a.shares);
+  if (first_chunk * CHUNK >= x.v1) return;
+  const int q0 = x.q0, j0 = x.j0;
   // of the rows, [vf, vg) see all of the keys
   const int vf = a.causal ? max(x.j1 - 1 - x.off, 0) * a.nrep : 0;
   const int64_t whole = int64_t(j0) + a.window - x.off;  // rows below it, in a window
-  const int vg = !a.window || whole >= x.rows ? v1 : whole <= 0 ? 0 : min(v1, int(whole) * a.nrep);
+  const int vg = !a.window || whole >= x.rows ? x.v1 : whole <= 0 ? 0 : int(whole) * a.nrep;
 
   u4_t kx[KS];  // A operands: key n of the wave's (past the last: that one again, not stored)
   {
@@ -164,16 +171,12 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
   // with the sequence's last: rows past the chunk's hold anything (a later row, or zeros) and count for nothing.  Where the
   // heads divide BR a tile's rows are at the same distances from its first one in every tile.
   const int fr = threadIdx.x / CH, fc = (chunk_at<D>(fr, threadIdx.x % CH) % CH) * 16;
-  Place load[LOADS], begin = place_of(v0);
+  Place load[LOADS], begin, mine;
   uint32_t at[LOADS];
+  int v0, v1, tiles;  // of the chunk
   auto offset_of = [&](const Place& p) {
     return uint32_t(p.row - begin.row) * uint32_t(a.sq_n) * 2 + uint32_t(p.head * a.maps) * uint32_t(a.sq_h) * 2 + fc;
   };
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    load[i] = place_of(v0 + i * (THREADS / CH) + fr);
-    at[i] = offset_of(load[i]);
-  }
   const uint16_t* from = a.q + int64_t(q0) * a.sq_n + int64_t(head0) * a.sq_h;
   auto fetch = [&](u4_t* lds) {
     const int64_t bytes = 2 * (int64_t(x.rows - 1 - begin.row) * a.sq_n + int64_t((a.nrep - 1) * a.maps) * a.sq_h + D);
@@ -202,15 +205,11 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = 0.f;
   // this lane's row of the next tile, and its {base, 1 / sum} (past the last: that one again, not counted)
-  Place mine = place_of(v0 + rw * 32 + n);
   const float2* stats = a.stats + int64_t(q0) * a.Hq + head0;
   auto stats_of = [&] {
     return stats[int64_t(min(mine.row, x.rows - 1)) * a.Hq + (mine.row < x.rows ? mine.head : a.nrep - 1) * a.maps];
   };
-  fetch(tile0);
-  float2 next = stats_of();
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) kx[ks] = (kx[ks] & a.scale.keep) ^ a.scale.sign;
+  float2 next;
   // (a buffer by name in each half of the loop: reads of one would wait for the loads to the other)
   auto turn = [&](int t, u4_t* here, u4_t* other) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -224,7 +223,7 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
     }
     const int va = v0 + t * BR;
     const bool big = big_base(st);
-    if (va >= vf && va + BR <= vg && !big) {
+    if (va >= vf && va + BR <= min(vg, v1) && !big) {
       Block<D, BF>::add_whole(here, qa, kx, a.scale.c, st, acc);
       return;
     }
@@ -233,9 +232,27 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
     const int first = (a.window ? max(row + x.off + 1 - a.window, 0) : 0) - base;
     Block<D, BF>::add_some(here, qa, kx, a.scale.c, big, st, first, last, acc);
   };
-  for (int t = 0; t < tiles; t += 2) {
-    turn(t, tile0, tile1);
-    if (t + 1 < tiles) turn(t + 1, tile1, tile0);
+  for (int chunk = first_chunk; chunk * CHUNK < x.v1; chunk += a.shares) {
+    v0 = max(x.v0, chunk * CHUNK);
+    v1 = min(x.v1, (chunk + 1) * CHUNK);
+    tiles = (v1 - v0 + BR - 1) / BR;
+    begin = place_of(v0);
+    mine = place_of(v0 + rw * 32 + n);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      load[i] = place_of(v0 + i * (THREADS / CH) + fr);
+      at[i] = offset_of(load[i]);
+    }
+    if (chunk > first_chunk) __syncthreads();  // nobody reads the last tile any more
+    fetch(tile0);
+    next = stats_of();
+    if (chunk == first_chunk)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kx[ks] = (kx[ks] & a.scale.keep) ^ a.scale.sign;
+    for (int t = 0; t < tiles; t += 2) {
+      turn(t, tile0, tile1);
+      if (t + 1 < tiles) turn(t + 1, tile1, tile0);
+    }
   }
   const float half = sum_rows(acc);
   const int j = kw * 32 + 8 * (n % 16 / 4) + 4 * hi + n % 4;
@@ -338,27 +355,31 @@ __global__ __launch_bounds__(FEW_THREADS, 4) void weigh_few_kernel(WeighArgs a) 
   }
 }
 
-// adds the chunks' sums of BK keys
+// adds the shares' sums of BK keys
 __global__ __launch_bounds__(64) void add_kernel(WeighArgs a) {
   const int H = gridDim.x / a.slots, kvh = blockIdx.x % H;
   Keys x;
   if (!keys_of(a, blockIdx.x / H, BK, x)) return;
   for (int j = x.j0 + threadIdx.x; j < x.j1 && j < a.T; j += 64) {
     float sum = 0.f;
-    for (int z = x.v0 / a.chunk; z <= (x.v1 - 1) / a.chunk; ++z) sum += a.part[(int64_t(z) * H + kvh) * a.Nk + x.k0 + j];
+    for (int z = 0; z < a.shares; ++z)
+      if (share_chunk(x, z, a.shares) * CHUNK < x.v1) sum += a.part[(int64_t(z) * H + kvh) * a.Nk + x.k0 + j];
     a.weights[x.s * a.sw_s + kvh * a.sw_h + j] += sum;
   }
-}
-
-// rows (times heads) of a chunk, of a call with `rows` in all
-inline int64_t chunk_of(int64_t rows) {
-  const int64_t even = ceil_div(ceil_div(rows, MOST_CHUNKS), BR) * BR;
-  return even < CHUNK ? CHUNK : even;
 }
 
 // Whether a call has few rows over many keys: by the mean of its sequences.
 inline bool few(int S, int N, int Nk, int Hq, int H) {
   return int64_t(N) * (Hq / H) <= int64_t(FEW) * S && int64_t(Nk) >= int64_t(1024) * S;
+}
+
+inline size_t stats_bytes(int N, int Hq) { return (size_t(N) * Hq * sizeof(float2) + 15) / 16 * 16; }
+
+// workgroups that share a key
+inline int shares_of(int S, int N, int Nk, int Hq, int H) {
+  const int64_t chunks = ceil_div(int64_t(N) * (Hq / H), CHUNK), most = GROUPS / ((int64_t(Nk) / BK + S) * H);
+  const int64_t n = chunks < most ? chunks : most;
+  return few(S, N, Nk, Hq, H) || n < 1 ? 1 : n < SHARES ? int(n) : SHARES;
 }
 
 template <int D, bool BF>
@@ -377,15 +398,14 @@ int launch(const WeighArgs& a, bool few, dim3 grid, hipStream_t stream) {
 }  // namespace
 
 namespace iq {
-size_t prompt_weights_bytes(int N, int Nk, int Hq, int H) {
-  const int64_t rows = int64_t(N) * (Hq / H), chunks = ceil_div(rows, chunk_of(rows));
-  const size_t stats = (size_t(N) * Hq * sizeof(float2) + 15) / 16 * 16;
-  return chunks > 1 ? stats + (size_t(chunks) * H * Nk * sizeof(float) + 15) / 16 * 16 : stats;
+size_t prompt_weights_bytes(int S, int N, int Nk, int Hq, int H) {
+  const int shares = shares_of(S, N, Nk, Hq, H);
+  return stats_bytes(N, Hq) + (shares > 1 ? (size_t(shares) * H * Nk * sizeof(float) + 15) / 16 * 16 : 0);
 }
 
 bool prompt_weights_fit(int S, int N, int Nk, int Hq, int H) {
-  const int64_t rows = int64_t(N) * (Hq / H), chunk = chunk_of(rows), chunks = ceil_div(rows, chunk);
-  return (int64_t(Nk) / BK + S) * H <= UINT32_MAX / THREADS / chunks && chunk * chunks <= INT32_MAX;
+  return int64_t(N) * (Hq / H) <= INT32_MAX - SHARES * CHUNK &&
+         (int64_t(Nk) / BK + S) * H <= UINT32_MAX / FEW_THREADS / shares_of(S, N, Nk, Hq, H);
 }
 
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream) {
@@ -394,10 +414,9 @@ int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream) {
   const int64_t steps = ceil_div(int64_t(a.Nk) * H, int64_t(FEW_KEYS) * FEW_GROUPS);
   a.steps = !f || steps < 1 ? 1 : steps < MOST_STEPS ? int(steps) : MOST_STEPS;
   a.slots = int(int64_t(a.Nk) / (f ? FEW_KEYS * a.steps : BK) + a.S);  // first_slot(S) at most
-  const int64_t rows = int64_t(a.N) * a.nrep, chunk = chunk_of(rows), chunks = f ? 1 : ceil_div(rows, chunk);
-  a.chunk = int(chunk);
-  a.part = chunks > 1 ? (float*)((char*)a.stats + (size_t(a.N) * a.Hq * sizeof(float2) + 15) / 16 * 16) : nullptr;
-  const dim3 grid(unsigned(int64_t(a.slots) * H), unsigned(chunks));
+  a.shares = shares_of(a.S, a.N, a.Nk, a.Hq, H);
+  a.part = a.shares > 1 ? (float*)((char*)a.stats + stats_bytes(a.N, a.Hq)) : nullptr;
+  const dim3 grid(unsigned(int64_t(a.slots) * H), unsigned(a.shares));
   if (D == 128) return bf ? launch<128, true>(a, f, grid, stream) : launch<128, false>(a, f, grid, stream);
   return bf ? launch<64, true>(a, f, grid, stream) : launch<64, false>(a, f, grid, stream);
 }
