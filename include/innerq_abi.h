@@ -506,8 +506,9 @@ int iq_prompt_attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k
 /* iq_prompt_attention that also adds each key's softmax weights, summed over its sequence's rows and the query heads of its
  * KV head, to weights, fp32 [S][H][T], contiguous in T: weights[s][h][j] grows by the fp32 weights of key j of sequence s
  * (keys from T on, and those that no row sees, gather none).  A row of NaN gives NaN to the keys it sees, one that is 0 (no
- * key that counts) gives 0.  Rows are added in a fixed order.  A row stride of q below 2^23 too, a head
- * stride times Hq / H below 2^29.  workspace: iq_prompt_weights_workspace_bytes, 16-byte aligned, of this call alone while it runs. */
+ * key that counts) gives 0.  Rows are added in a fixed order.  out must not be q.  A row stride of q below 2^23 too, a head
+ * stride times Hq / H below 2^29.  workspace: iq_prompt_weights_workspace_bytes, 16-byte aligned, of this call alone while it
+ * runs. */
 size_t iq_prompt_weights_workspace_bytes(int S, int N, int Nk, int Hq, int H, int D);
 int iq_prompt_attention_weights(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n, int64_t sk_h,
                                 const void* v, int64_t sv_n, int64_t sv_h, const int32_t* cu_q, const int32_t* cu_k, int S,

@@ -387,7 +387,7 @@ extern "C" int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_
            IQ_ERR_SHAPE);
   IQ_CHECK(!window || causal, IQ_ERR_MODE);
   for (const int64_t s : {sk_n, sv_n}) IQ_CHECK(s >= 0 && s < (1 << 23), IQ_ERR_SHAPE);  // a tile of rows in 32 bits
-  IQ_CHECK(s_lam >= 0, IQ_ERR_SHAPE);
+  IQ_CHECK(s_lam >= 0 && (!N || out != q), IQ_ERR_SHAPE);
   for (const int64_t s : {sq_n, sq_h, sk_n, sk_h, sv_n, sv_h, so_n, so_h}) IQ_CHECK(s % 8 == 0, IQ_ERR_ALIGN);
   IQ_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, 4) && aligned(cu_k, 4) &&
                aligned(lam, 4), IQ_ERR_ALIGN);

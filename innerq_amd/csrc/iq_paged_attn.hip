@@ -902,6 +902,7 @@ int attention(const iq_paged* p, const void* q, int64_t sq_s, int64_t sq_m, int6
   IQ_CHECK(q && out && (MAPS == 1 || lam), IQ_ERR_NULL);
   IQ_CHECK(m > 0 && m <= 16 && Hq > 0 && Hq % p->H == 0 && p->H % MAPS == 0 && Hq <= 4096 && window >= 0 && s_lam >= 0,
            IQ_ERR_SHAPE);
+  IQ_CHECK(MAPS == 1 || out != q, IQ_ERR_SHAPE);  // an output row lies over several heads' queries
   IQ_CHECK(aligned(q, 16) && aligned(out, 16) && sq_s % 8 == 0 && sq_m % 8 == 0 && sq_h % 8 == 0 && so_s % 8 == 0 &&
                so_m % 8 == 0 && so_h % 8 == 0 && aligned(lam, 4), IQ_ERR_ALIGN);
   const int nrep = Hq / p->H, heads = p->H / MAPS;

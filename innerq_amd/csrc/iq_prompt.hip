@@ -507,6 +507,7 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
   IQ_CHECK(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, 4) && aligned(cu_k, 4),
            IQ_ERR_ALIGN);
   if (weights) {
+    IQ_CHECK(!N || out != q, IQ_ERR_SHAPE);  // q is read again after out has been written
     // a tile's rows of q in 32 bits
     IQ_CHECK(sq_n >= 0 && sq_n < (1 << 23) && sq_h >= 0 && sq_h < (1 << 29) / (Hq / H), IQ_ERR_SHAPE);
     IQ_CHECK(T >= 0 && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);

@@ -1,7 +1,8 @@
 // Native front of the per-token calls: the argument checks, segment structures
 // and launches of ops.decode_attention, ops.qk_gemv, ops.av_gemv and
 // ops.window_append for the ordinary case, without Python between them; and of
-// ops.prompt_attention and paged.PagedStore's append, read and attend.
+// ops.prompt_attention, ops.diff_prompt_attention and paged.PagedStore's append,
+// read, attend, diff_attend and evict.
 //
 // The Python wrappers build ~40 ctypes fields and ~30 small objects per call,
 // and short calls waited for them: a decode of one sequence over 1000 tokens
@@ -485,8 +486,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
 
 // ---- many sequences: 4-bit pages and packed prompts ----
 typedef int (*paged_append_t)(const iq_paged*, const int32_t*, int, const void*, int64_t, int64_t, const void*, int64_t,
-                              int64_t, const float*, const float*, int64_t, int, const void*, int64_t, int64_t, int, void*,
-                              int64_t, int64_t, void*);
+                              int64_t, const float*, const float*, int64_t, int, const int32_t*, const void*, int64_t,
+                              int64_t, int, void*, int64_t, int64_t, void*);
 typedef int (*paged_read_t)(const iq_paged*, const int32_t*, int, void*, int64_t, int64_t, void*, int64_t, int64_t, void*);
 typedef size_t (*paged_ws_t)(int, int, int, int, int, int);
 typedef int (*paged_attend_t)(const iq_paged*, const void*, int64_t, int64_t, int64_t, int, int, float, int, void*, int64_t,
@@ -621,12 +622,12 @@ bool window_of(PyObject* o, int64_t* w) {
 }
 at::Tensor like(const at::Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
 
-// paged_append(pages, D, dtype, status, table, lens, k, v, cu, cos, sin, q, q_out): (q_out or None,), or None
+// paged_append(pages, D, dtype, status, table, lens, k, v, cu, cos, sin, q, q_out, evicted): (q_out or None,), or None
 PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
   iq_paged p{};
   at::ScalarType dt;
   int dev;
-  if (na != 13 || !paged_of(a, &p, &dt, &dev)) Py_RETURN_NONE;
+  if (na != 14 || !paged_of(a, &p, &dt, &dev)) Py_RETURN_NONE;
   const at::Tensor *k = rows_of(a[6], 3, dt, dev, p.D), *v = rows_of(a[7], 3, dt, dev, p.D);
   const int32_t* cu;
   if (!k || !v || k->size(0) < 1 || k->size(0) > INT32_MAX || k->size(1) != p.H || v->sizes() != k->sizes() ||
@@ -645,6 +646,12 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
     half = t->size(1);
     if (n_pos < 1 || half < 1 || half > 128) Py_RETURN_NONE;  // (an empty table's pointer is null: no rotation)
     tab[i] = (const float*)t->data_ptr();
+  }
+  const int32_t* evicted = nullptr;
+  if (a[13] != Py_None) {
+    const at::Tensor* t = ints_of(a[13], p.S, dev);
+    if (!t || !tab[0]) Py_RETURN_NONE;
+    evicted = (const int32_t*)t->data_ptr();
   }
   const at::Tensor* q = nullptr;
   at::Tensor out;
@@ -667,10 +674,10 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
   int st;
   Py_BEGIN_ALLOW_THREADS
   st = sv.append(&p, cu, int(k->size(0)), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1),
-                 tab[0], tab[1], n_pos, int(2 * half), q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+                 tab[0], tab[1], n_pos, int(2 * half), evicted, q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
                  q ? int(q->size(1)) : 0, q ? out.data_ptr() : nullptr, q ? out.stride(0) : 0, q ? out.stride(1) : 0, stream);
   Py_END_ALLOW_THREADS
-  if (st != IQ_OK) return not_ok("iq_paged_append", st);
+  if (st != IQ_OK) return not_ok("iq_paged_append_at", st);
   if (!q) return PyTuple_Pack(1, Py_None);
   if (a[12] != Py_None) return PyTuple_Pack(1, a[12]);
   PyObject* w = THPVariable_Wrap(std::move(out));
@@ -883,7 +890,7 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
   at::Tensor out;
   if (a[8] != Py_None) {
     const at::Tensor* o = out_rows_of(a[8], 3, dt, dev, D);
-    if (!o || o->sizes() != q->sizes()) Py_RETURN_NONE;
+    if (!o || o->sizes() != q->sizes() || (a[9] != Py_None && o->data_ptr() == q->data_ptr())) Py_RETURN_NONE;
     out = *o;
   }
   void* stream;

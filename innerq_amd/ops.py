@@ -53,7 +53,7 @@ def _native(t):
              "iq_av_workspace_bytes", "iq_av_gemv", "iq_window_append")
     m.bind(tuple(ctypes.cast(getattr(h, n), ctypes.c_void_p).value for n in names), _WS,
            torch._C._cuda_getCurrentRawStream)
-    names = ("iq_paged_append", "iq_paged_read", "iq_paged_attention_workspace_bytes", "iq_paged_attention",
+    names = ("iq_paged_append_at", "iq_paged_read", "iq_paged_attention_workspace_bytes", "iq_paged_attention",
              "iq_prompt_attention", "iq_paged_attention_weights_workspace_bytes", "iq_paged_attention_weights",
              "iq_prompt_weights_workspace_bytes", "iq_prompt_attention_weights", "iq_diff_paged_attention_workspace_bytes",
              "iq_diff_paged_attention", "iq_diff_prompt_attention", "iq_paged_evict_workspace_bytes", "iq_paged_evict")
@@ -962,8 +962,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     weights: fp32 [S, H, T], memory that no other argument uses: weights[s, h, j] grows by the softmax weights of key j of
     sequence s (of those below T), summed over its rows and the query heads of KV head h, as PagedStore.evict goes by.
-    The rows may be a prompt's last ones, behind all its keys.  The call then takes 8 bytes of memory per row and query
-    head."""
+    The rows may be a prompt's last ones, behind all its keys.  ``out`` is not q then, and the call takes memory for the
+    rows' sums (8 bytes per row and query head) and for parts of the work that workgroups share."""
     fast = _native(q) if forward_ad._current_level < 0 else None
     if fast is not None:
         r = fast.prompt(q, k, v, cu_seqlens, scale, cu_seqlens_k, causal, window, out, weights)
@@ -988,8 +988,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             _shape_error(f"{name} is on {t.device}, q on {dev}")
         rows.append(readable_rows(t if t.stride(0) < 2 ** 23 else t.clone(memory_format=torch.contiguous_format)))
     q, k, v = rows
-    if weights is not None and q.stride(1) * (Hq // H) >= 2 ** 29:
-        q = q.clone(memory_format=torch.contiguous_format)
+    if weights is not None:
+        if out is not None and out.data_ptr() == q.data_ptr() and N:
+            _shape_error("out cannot be q where weights are added up")
+        if q.stride(1) * (Hq // H) >= 2 ** 29:
+            q = q.clone(memory_format=torch.contiguous_format)
     cu_q = check_cu(cu_seqlens, "cu_seqlens", None, dev)
     S = cu_q.shape[0] - 1
     cu_k = cu_q if cu_seqlens_k is None else check_cu(cu_seqlens_k, "cu_seqlens_k", S, dev)

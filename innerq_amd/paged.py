@@ -159,10 +159,10 @@ class PagedStore:
         written to q_out.  A token that cannot be appended (check()) has NaN queries, and one that only the rotation has
         no row for NaN in its page, so that read() and attend() give NaN.  Sequences that append must not share the
         pages they append to."""
-        fast = ops._native(k) if forward_ad._current_level < 0 and evicted is None else None
+        fast = ops._native(k) if forward_ad._current_level < 0 else None
         if fast is not None:
             r = fast.paged_append(self.pages, self.D, self.dtype, self.status, table, lens, k, v, cu_seqlens, cos, sin, q,
-                                  q_out)
+                                  q_out, evicted)
             if r is not None:
                 return r[0]
         _no_grad(k, v, q, cos, sin, q_out)

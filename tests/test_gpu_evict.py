@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from innerq_amd import paged
+from innerq_amd import ops, paged
 from oracle import evict_ref as E
 from oracle import serving_ref as R
 
@@ -257,3 +257,24 @@ def test_captured():
         want = *st.evict(table, ll, w, 100, 20, 1), st.pages
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_append_evicted_native(monkeypatch):
+    """append(evicted=) through the native front and without it: one token per sequence, and ragged rows."""
+    g = torch.Generator().manual_seed(40)
+    H, D, lens, gone = 2, 64, [70, 3, 130], [9, 0, 400]
+    table = torch.arange(12, dtype=torch.int32, device=DEV).view(3, 4)
+    ang = torch.rand(700, D // 2, generator=g)
+    cos, sin = ang.cos().to(DEV), ang.sin().to(DEV)
+    for cu, n in ((None, 3), (i32([0, 5, 5, 11]), 11)):
+        k, v, q = (torch.randn(n, h, D, generator=g).half().to(DEV) for h in (H, H, 4))
+        got = []
+        for native in (True, False):
+            with monkeypatch.context() as m:
+                if not native:
+                    m.setattr(ops, "_native", lambda t: None)
+                st = paged.PagedStore(12, H, D, DEV)
+                st.pages.zero_()
+                out = st.append(k, v, table, i32(lens), cu, cos, sin, q, evicted=i32(gone))
+                got.append((out, st.pages.clone(), st.check()))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and got[0][2] == got[1][2]

@@ -422,3 +422,27 @@ def test_prompt_refusals():
     assert ops.prompt_attention(none, k, v, i32([0, 0, 0]), 0.1, i32(cu), weights=w).shape == (0, 4, 64)
     ops.prompt_attention(q, k[:0], v[:0], i32(cu), 0.1, i32([0, 0, 0]), weights=w)
     assert torch.equal(w, before)
+
+
+def test_out_over_q():
+    """attend's q may become its output, with weights too; a prompt's q is read again for the weights, so it may not."""
+    lens = [300, 64]
+    st, table, cu, k, g = filled(16, lens, 2, 64, torch.float16)
+    q = torch.randn(2, 8, 64, generator=g).half().to(DEV)
+    a, b = torch.zeros(2, 2, 512, device=DEV), torch.zeros(2, 2, 512, device=DEV)
+    want, x = st.attend(q, table, i32(lens), 0.2, weights=a), q.clone()
+    assert st.attend(x, table, i32(lens), 0.2, out=x, weights=b) is x
+    assert torch.equal(x, want) and torch.equal(a, b)
+    g, q, k, v, cu, cu_k = prompts(17, [60, 40], 0, 2, 4, 64, torch.float16)
+    with pytest.raises(ValueError, match="out cannot be q"):
+        ops.prompt_attention(q, k, v, i32(cu), 0.1, out=q, weights=torch.zeros(2, 2, 60, device=DEV))
+
+
+def test_prompt_out_is_taken():
+    """An out of its own, of other strides than a new one's, holds the output, and its weights are a new one's."""
+    g, q, k, v, cu, cu_k = prompts(18, [60, 400], 0, 2, 4, 64, torch.bfloat16)
+    a, b = torch.zeros(2, 2, 400, device=DEV), torch.zeros(2, 2, 400, device=DEV)
+    want = ops.prompt_attention(q, k, v, i32(cu), 0.1, weights=a)
+    out = torch.zeros(460, 8, 64, dtype=torch.bfloat16, device=DEV)[:, ::2]
+    assert ops.prompt_attention(q, k, v, i32(cu), 0.1, out=out, weights=b) is out
+    assert torch.equal(out, want) and torch.equal(a, b)
