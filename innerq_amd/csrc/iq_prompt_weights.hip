@@ -50,7 +50,7 @@ __device__ __forceinline__ bool keys_of(const WeighArgs& a, int slot, int bk, Ke
   x.keys = k1 - x.k0;
   x.off = x.keys - lq;
   x.j0 = (slot - (x.k0 / bk + x.s)) * bk;
-  if (x.j0 >= x.keys || x.j0 >= a.T) return false;
+  if (x.j0 < 0 || x.j0 >= x.keys || x.j0 >= a.T) return false;  // (negative: a slot before the first sequence's)
   x.j1 = min(x.j0 + bk, x.keys);
   const int first = a.causal ? max(x.j0 - x.off, 0) : 0;
   const int64_t seen = int64_t(x.j1) - 1 + a.window - x.off;  // rows below it see a key, in a window

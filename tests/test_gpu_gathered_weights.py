@@ -446,3 +446,26 @@ def test_prompt_out_is_taken():
     out = torch.zeros(460, 8, 64, dtype=torch.bfloat16, device=DEV)[:, ::2]
     assert ops.prompt_attention(q, k, v, i32(cu), 0.1, out=out, weights=b) is out
     assert torch.equal(out, want) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lens,past,head", [([150], [0], (1000, 0)), ([70, 200], [0, 40], (1000, 0)), ([2900], [0], (1000, 0)),
+                                            ([3, 2], [1500, 4000], (100, 900))])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_sequences_inside(lens, past, head, causal):
+    """Rows and keys before the first sequence and behind the last one take no part, and no weight is written beside the
+    sequences' own."""
+    g, q, k, v, cu, cu_k = prompts(19, [head[0], *lens, 90], [head[1], *past, 0], 2, 4, 64, torch.float16)
+    cu, cu_k = cu[1:-1], cu_k[1:-1]
+    S, T = len(lens), max(b - a for a, b in zip(cu_k, cu_k[1:])) + 5
+    held_all = held(g, S + 2, 2, T)
+    before, w = held_all.cpu().clone(), held_all[1:-1]
+    out = torch.full_like(q, 7.0)
+    ops.prompt_attention(q, k, v, i32(cu), 0.2, i32(cu_k), causal=causal, out=out, weights=w)
+    got, qc, kc = held_all.cpu(), q.cpu(), k.cpu()
+    assert torch.equal(got[0], before[0]) and torch.equal(got[-1], before[-1])
+    assert bool((out[:cu[0]] == 7).all()) and bool((out[cu[-1]:] == 7).all())
+    for s in range(S):
+        n = cu_k[s + 1] - cu_k[s]
+        assert torch.equal(got[1 + s, :, n:], before[1 + s, :, n:])
+        want, bound = E.weights(qc[cu[s]:cu[s + 1]], kc[cu_k[s]:cu_k[s + 1]], 0.2, causal, 0)
+        check(got[1 + s, :, :n], before[1 + s, :, :n], want, bound, s)
