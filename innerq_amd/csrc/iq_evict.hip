@@ -13,6 +13,12 @@
 //   fill    rows and their weights into the free places: sources from B on, destinations below B, in any order.
 //   shift   the last `recent` rows: where they overlap their destinations one workgroup per (sequence, head), in order,
 //           each batch read whole before it is written.  Weights from `keep` on become 0.
+//
+// Bound: the latency of three launches, in each of which loads wait for each other (length, weights or plan, table, page).
+// 32 sequences of 2112 tokens to 2048, 256 of them recent (8 heads, D = 128): 12, 12 and 12 - 14 us.  8 of 32768 to 2048, 512
+// recent: 26, 25 and 13.  There a third of select's time loads the weights and counts their first digits (weights of one size share
+// bins, whose atomics take turns: one copy of the counts and single words in place of fours 30 us), and fill reads rows from
+// all over: a token's V lies in D / 8 sectors of 32 bytes with 7 other tokens', so 8 bytes come for each that is used.
 #include "iq_paged.h"
 
 using namespace iq;
@@ -23,7 +29,8 @@ constexpr int SELECT = 1024, FILL = 256, SHIFT = 1024;
 constexpr int BATCH = 4;                        // rows of a lane that are under way together
 constexpr int BITS[3] = {11, 11, 10}, BINS = 1 << 11;
 constexpr int WAVES = SELECT / 64;
-constexpr int KEYS = 32, ROUND = KEYS * SELECT, READS = 4;  // weights of a thread, of a workgroup; under way together from LDS
+constexpr int KEYS = 32, ROUND = KEYS * SELECT;  // weights of a thread, of a workgroup
+constexpr int COPIES = 2;                       // of the digits' counts, by lane: equal digits of a wave take turns
 
 typedef float f4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -69,9 +76,9 @@ __device__ __forceinline__ void all_read() {
 }
 
 __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
-  __shared__ int hist[BINS];
+  __shared__ int hist[COPIES][BINS];
   __shared__ int found[2];  // the digit, and how many of its keys are wanted
-  __shared__ uint32_t keys[ROUND + ROUND / 32];
+  __shared__ u4_t keys[ROUND / 4];
   const int runs = a.p.H / a.shared, s = blockIdx.x / runs, h0 = (blockIdx.x - s * runs) * a.shared, tid = threadIdx.x;
   const float* w = a.w + s * a.sw_s + h0 * a.sw_h;
   float* wo = a.wo + s * a.so_s + h0 * a.so_h;
@@ -89,10 +96,11 @@ __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
       for (int i = tid; i < B; i += SELECT) wo[h * a.so_h + i] = w[h * a.sw_h + i];
   // Weights as whole numbers of the same order: NaN above all, -0 as 0.  The sinks are above all too, and come first.  A
   // round's keys lie in LDS, a thread's being those of `per` neighbouring tokens, 0 (less than any weight's) past the end.
-  // (Loops over them stay loops: unrolled, with the keys in registers, the code alone took 25 us to fetch.)
   const bool one = old <= ROUND;
-  const int per = one ? (old + 4 * SELECT - 1) / (4 * SELECT) * 4 : KEYS;
-  auto key_at = [&](int j) -> uint32_t& { return keys[j + j / 32]; };  // (a thread's, 32 apart, in different banks)
+  const int groups = one ? (old + 4 * SELECT - 1) / (4 * SELECT) : KEYS / 4, per = 4 * groups;
+  // four neighbouring keys lie together: a run of them, and the threads' own ones of one place, both meet no bank twice
+  auto four_at = [&](int g) -> u4_t& { return keys[g ^ (g >> 4 & 7)]; };
+  int* const counts = hist[tid % COPIES];
   auto load = [&](int round, bool count) {  // count: the first pass's digits too
     auto four = [&](const float* p, int i) {  // weights i .. i + 3, which may be the row's last
       if (i + 4 <= a.T) return f4_t(*reinterpret_cast<const f4_any_t*>(p + i));
@@ -109,26 +117,29 @@ __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
     }
     __syncthreads();  // nobody reads the last round's keys any more
 #pragma clang loop unroll(disable)
-    for (int v = 0; v < (per + 3) / 4; ++v) {
+    for (int v = 0; v < groups; ++v) {  // (unrolled its code took 2 us more to fetch)
+      const int i = round + (v * SELECT + tid) * 4;
       f4_t y;
 #pragma unroll
       for (int u = 0; u < KEYS / 4; ++u)
         if (u == v) y = x[u];
-      const int j = (v * SELECT + tid) * 4, i = round + j;
       y += 0.f;
       if (i < old)
         for (int h = 1; h < a.shared; ++h) y += four(w + h * a.sw_h, i);
+      u4_t k;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t b = __float_as_uint(y[e]);
-        const uint32_t k = i + e < a.sinks || y[e] != y[e] ? ~0u : b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
-        key_at(j + e) = i + e < old ? k : 0u;
-        if (count && i + e < old) atomicAdd(&hist[k >> (32 - BITS[0])], 1);
+        const float z = y[e];
+        const uint32_t b = __float_as_uint(z), q = i + e < a.sinks || z != z ? ~0u : b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+        k[e] = i + e < old ? q : 0u;
+        if (count && i + e < old) atomicAdd(&counts[q >> (32 - BITS[0])], 1);
       }
+      four_at(v * SELECT + tid) = k;
     }
     __syncthreads();
   };
-  for (int i = tid; i < BINS; i += SELECT) hist[i] = 0;
+  int* const all_counts = &hist[0][0];
+  for (int i = tid; i < COPIES * BINS; i += SELECT) all_counts[i] = 0;
   if (one) load(0, B > 0);
   uint32_t least = 0;  // the B-th largest key
   int ties = 0;        // of the tokens whose key it is, the first `ties` stay
@@ -139,22 +150,26 @@ __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
       const int bits = BITS[pass];
       low -= bits;
       if (pass > 0)
-        for (int i = tid; i < BINS; i += SELECT) hist[i] = 0;
+        for (int i = tid; i < COPIES * BINS; i += SELECT) all_counts[i] = 0;
       __syncthreads();
       for (int round = 0; round < old; round += ROUND) {
         if (!one) load(round, false);
         else if (pass == 0) break;
-        for (int e0 = 0; e0 < per; e0 += READS) {
-          uint32_t k[READS];
+        for (int g = 0; g < groups; ++g) {
+          const u4_t k = four_at(g * SELECT + tid);
 #pragma unroll
-          for (int e = 0; e < READS; ++e) k[e] = key_at(min(e0 + e, per - 1) * SELECT + tid);
-#pragma unroll
-          for (int e = 0; e < READS; ++e)
-            if (e0 + e < per && k[e] && (k[e] & mask) == least) atomicAdd(&hist[k[e] >> low & ((1u << bits) - 1)], 1);
+          for (int e = 0; e < 4; ++e)
+            if (k[e] && (k[e] & mask) == least) atomicAdd(&counts[k[e] >> low & ((1u << bits) - 1)], 1);
         }
       }
       __syncthreads();
-      const int hi = BINS - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1];
+      const int hi = BINS - 1 - 2 * tid;
+      int c0 = 0, c1 = 0;
+#pragma unroll
+      for (int c = 0; c < COPIES; ++c) {
+        c0 += hist[c][hi];
+        c1 += hist[c][hi - 1];
+      }
       int total;
       const int end = group_scan(c0 + c1, total), before = end - c0 - c1;
       if (before < want && want <= end) {
@@ -175,14 +190,12 @@ __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
     if (!one) load(round, false);
     const int first = round + tid * per;
     uint32_t stay = 0, same = 0;  // a bit of each of the thread's tokens
-    for (int e0 = 0; e0 < per; e0 += READS) {
-      uint32_t k[READS];
+    for (int g = 0; g < groups; ++g) {
+      const u4_t k = four_at(tid * groups + g);
 #pragma unroll
-      for (int e = 0; e < READS; ++e) k[e] = key_at(tid * per + min(e0 + e, per - 1));
-#pragma unroll
-      for (int e = 0; e < READS; ++e) {
-        stay |= uint32_t(k[e] > least && e0 + e < per) << (e0 + e);
-        same |= uint32_t(k[e] == least && e0 + e < per) << (e0 + e);
+      for (int e = 0; e < 4; ++e) {
+        stay |= uint32_t(k[e] > least) << (4 * g + e);
+        same |= uint32_t(k[e] == least) << (4 * g + e);
       }
     }
     // (the thread's tokens below B, and below the end)
