@@ -16,6 +16,11 @@
 // matrix unit is busy 60 % of the clocks, HBM moves 0.8 GB.  With D = 64 there are half the products per exponential: the
 // vector unit is busy 79 % of the clocks, the matrix unit 50 % (1.11 - 1.18 ms, 930 - 990 TFLOP/s).  Short prompts wait for
 // their first tile: 77 tokens 7.4 us.
+//
+// iq_prompt_attention_weights: each row's {base, 1 / sum} is kept for the launches that weigh the keys (iq_prompt_weights.hip),
+// which are the second pass that a key's weight needs: a row's sum is not known before its last key.  The call brings a
+// workspace, so there a tile of few rows over many keys is shared out too (64 rows behind 16000 keys on 4 sequences, 32 query
+// heads over 8: a workgroup per tile 265 us, shared out 84 and 10 for merge_kernel).
 #include "iq_prompt.h"
 
 using namespace iq;
@@ -487,7 +492,9 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(PromptArgs a) {
 }
 
 // Workgroups that share a tile of rows: as many as make 768 of the slots (two thirds of which hold a tile where sequences are
-// short of one), while each has 512 keys, by the mean of the sequences.  Only where there is a workspace.
+// short of one), while each has 512 keys, by the mean of the sequences.  Only where there is a workspace.  (With the keys'
+// weights / the attention alone, whose tiles are whole; sequences x rows x keys, us: 1 x 64 x 4096 33 / 72, 1 x 64 x 16000
+// 66 / 265, 4 x 64 x 4096 63 / 75, 4 x 64 x 16000 153 / 270, 1 x 64 x 1100 27 / 25.)
 inline int splits_of(int S, int N, int Nk, int Hq, int H) {
   const int64_t slots = int64_t(N) * (Hq / H) / BM + S, most = 768 / (slots * H), keys = int64_t(Nk) / S / 512;
   const int64_t n = most < keys ? most : keys;

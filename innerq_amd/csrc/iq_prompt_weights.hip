@@ -10,7 +10,13 @@
 // A key at the beginning of a long prompt is seen by all its rows, so up to SHARES workgroups share a key: each takes every
 // so-manieth CHUNK of the rows, and a second launch adds their sums (how many rows a sequence has is not known on the host:
 // a share that finds none ends at once, and the shares are as many as leave GROUPS workgroups).  Rows are added in a fixed
-// order: no atomics.
+// order: no atomics.  (One share / 16 at most, a whole call, bf16, 32 heads over 8, D = 128: a prompt of 2000 tokens 134 / 90 us,
+// of 8192 947 / 845, 16 of 25 .. 2000 324 / 307, 64 of 100 59 / 63.)
+//
+// Bound: neither unit alone.  2048 rows by 2048 keys of 64 heads: vector unit busy 49 % of the clocks (16 exponentials and 32
+// multiply-adds per 16 logits of a lane, and as much again around them), matrix unit 31 %; without the tiles' loads the launch
+// took three quarters of its time, without the exponentials seven eighths.  16 packed prompts of 25 .. 2000 tokens: 110 us, 41
+// GFLOP, behind 165 of the attention's; a prompt of 77 tokens 8 us, its loads one behind the other.
 #include "iq_prompt.h"
 
 using namespace iq;
@@ -264,9 +270,10 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
   else a.weights[x.s * a.sw_s + kvh * a.sw_h + j0 + j] += sum;
 }
 
-// The same for few rows over many keys.  The rows (up to FEW; more in turns) stay in LDS with their statistics in registers,
-// and a wave takes 32 of each step's 128 keys over all of them, with the next step's keys on their way: no barriers, and each
-// key's sum is one wave's.  (64 rows behind 16000 keys on 4 sequences, 8 KV heads, D = 128: 85 us by weigh_kernel, here NEW.)
+// The same for few rows over many keys.  The rows (up to FEW; more in turns) stay in LDS with their statistics, and a wave
+// takes 32 of each step's FEW_KEYS keys over all of them: no barriers, and each key's sum is one wave's.  (64 rows behind 16000
+// keys on 4 sequences, 8 KV heads, D = 128: 85 us by weigh_kernel, 52 - 55 here, where reading the keys takes 28 at a copy's rate
+// and the products 25 at a library product's.)
 template <int D, bool BF>
 __global__ __launch_bounds__(FEW_THREADS, 4) void weigh_few_kernel(WeighArgs a) {
 #pragma clang fp contract(off)
@@ -368,9 +375,13 @@ __global__ __launch_bounds__(64) void add_kernel(WeighArgs a) {
   }
 }
 
-// Whether a call has few rows over many keys: by the mean of its sequences.
+// Whether a call has few rows over many keys, by the mean of its sequences: up to FEW rows each, and keys for seven eighths of
+// FEW_GROUPS workgroups (a whole call, us, weigh_few_kernel / weigh_kernel; 32 heads over 8, D = 128, fp16; sequences x rows x keys:
+// 1 x 64 x 4096 33.4 / 30.4, 1 x 64 x 16000 66 / 71, 4 x 64 x 4096 62.9 / 63.0, 4 x 64 x 16000 153 / 179, 16 x 64 x 1100 65 / 71,
+// 16 x 1 x 4096 100 / 125, 16 x 16 x 16000 336 / 427).
 inline bool few(int S, int N, int Nk, int Hq, int H) {
-  return int64_t(N) * (Hq / H) <= int64_t(FEW) * S && int64_t(Nk) >= int64_t(1024) * S;
+  return int64_t(N) * (Hq / H) <= int64_t(FEW) * S && int64_t(Nk) >= int64_t(1024) * S &&
+         int64_t(Nk) * H >= int64_t(FEW_KEYS) * (FEW_GROUPS - FEW_GROUPS / 8);
 }
 
 inline size_t stats_bytes(int N, int Hq) { return (size_t(N) * Hq * sizeof(float2) + 15) / 16 * 16; }
