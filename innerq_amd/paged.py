@@ -8,7 +8,10 @@ include/innerq_abi.h).  Which pages are a sequence's is the caller's ``table``, 
 * ``append`` quantizes the new tokens of every sequence into its pages, rotating keys (and the step's queries) on
   the way;
 * ``attend`` is decode attention of one or a few new tokens per sequence over its pages;
-* ``read`` gives back the values of some tokens, dense.
+* ``read`` gives back the values of some tokens, dense;
+* ``diff_attend`` is ``attend`` for differential attention, over a store whose heads come in pairs;
+* ``evict`` cuts long sequences down to a budget of tokens, by the attention weight that each has gathered: what
+  ``attend`` and ``diff_attend`` (weights=) and ops.prompt_attention (weights=) add up.
 
 A prompt attends with ops.prompt_attention over its dense K and V; a later chunk of it over what ``read`` gives.
 
