@@ -8,11 +8,12 @@
 // waves hand their normalised sums, times lam, over LDS in fp32.
 //
 // A wave holds 32 rows of 2 D sums: at D = 128 the 128 accumulators leave room for two waves per SIMD, a workgroup of 8 with
-// tiles of 32 keys; at D = 64 workgroups of 4 with tiles of 64.  (At D = 128 registers spill in the masked tiles alone.)  Bound:
-// as iq_prompt.hip the matrix unit and the softmax beside it.  A prompt of 8192 tokens, 32 query heads over 8 KV heads, D = 128,
-// fp16: 862 - 878 us, 940 - 957 TFLOP/s, where a 16384^3 library product reaches 1324; 16 packed prompts of 25 .. 2000 tokens,
-// D = 64, bf16: 132 us, 700 TFLOP/s, first and last tiles of short prompts.  Each map by a call of iq_prompt_attention over both
-// halves of V would take 1.5 times the products (K Q^T twice).
+// tiles of 32 keys; at D = 64 workgroups of 4 with tiles of 64.  (At D = 128 registers spill from the first masked tile on whose V
+// holds an infinity or NaN; when they did in every masked one, four such tiles took 40 us, now 3.)  Bound: as iq_prompt.hip the
+// matrix unit and the softmax beside it.  A prompt of 8192 tokens, 32 query heads over 8 KV heads, D = 128, fp16: 790 us, 1044
+// TFLOP/s, where a 16384^3 library product reaches 1324; 16 packed prompts of 25 .. 2000 tokens, D = 64, bf16: 132 us, 700 TFLOP/s,
+// first and last tiles of short prompts.  Each map by a call of iq_prompt_attention over both halves of V would take 1.5 times
+// the products (K Q^T twice).
 #include "iq_prompt.h"
 
 using namespace iq;
@@ -77,9 +78,17 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
   const int lq = q1 - q0, keys = k1 - k0, off = keys - lq, rows = lq * a.nrep, tiles = int((int64_t(rows) + BM - 1) / BM);
   const int tile = tiles - 1 - (slot - __builtin_amdgcn_readfirstlane(first_slot(s)));
   if (tile < 0 || tile >= tiles) return;
-  const int vrow = tile * BM + rb * 32 + n, row = min(vrow, rows - 1) / a.nrep, head = g * a.nrep + min(vrow, rows - 1) % a.nrep;
-  // key j is seen iff first <= j < last
-  const int last = a.causal ? min(row + off + 1, keys) : keys, first = a.window ? max(row + off + 1 - a.window, 0) : 0;
+  // this lane's row, and the keys that it sees: [first, last) (worked out for the queries, and once more behind the whole tiles,
+  // which have no registers to keep them)
+  int vrow, row, head, last, first;
+  auto row_of = [&](int lane_row) {
+    vrow = tile * BM + rb * 32 + lane_row;
+    row = min(vrow, rows - 1) / a.nrep;
+    head = g * a.nrep + min(vrow, rows - 1) - row * a.nrep;
+    last = a.causal ? min(row + off + 1, keys) : keys;
+    first = a.window ? max(row + off + 1 - a.window, 0) : 0;
+  };
+  row_of(n);
   // the tiles of keys that any row of the workgroup sees
   const int row_a = tile * BM / a.nrep, row_z = (min(tile * BM + BM, rows) - 1) / a.nrep;
   const int j_end = a.causal ? min(row_z + off + 1, keys) : keys, j_begin = a.window ? max(row_a + off + 1 - a.window, 0) : 0;
@@ -123,20 +132,19 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
     for (int v = 0; v < NV; ++v)
       fetch1.template operator()<VCH, LV / THREADS>(vp + 128 * v, a.sv_n, sv, vv, t, to + 2 * LK + v * LV);
   };
-  // this lane's operands in a tile, in bytes; blocks of 32 keys (K), of 16 (V) are at fixed distances from them
-  int ka[KS], va[4][2];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) ka[ks] = (map * LK + chunk_at<D>(n, 2 * ks + hi)) * 16;
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = lane & 15, d = b * 32 + (lane >> 4 & 1) * 16 + j % 4 * 4;
-      va[b][h] = (2 * LK + chunk_at<128>(h * 8 + hi * 4 + j / 4, d / 8)) * 16 + d % 8 * 2;
-    }
+  // This lane's operands in a tile, in bytes (blocks of 32 keys (K), of 16 (V) are at fixed distances from them): K's step ks is
+  // at k_own ^ 32 ks, V's block b of dims in half h of 16 keys at (v_own ^ 64 b ^ 32 h) + 8 h rows.  At D = 128 worked out where
+  // they are used: there are no registers to keep all of them.
+  const int k_own = (map * LK + chunk_at<D>(n, hi)) * 16;
+  const int v_own = (2 * LK + chunk_at<128>(hi * 4 + (lane & 15) / 4, (lane >> 4 & 1) * 2 + lane % 4 / 2)) * 16 + lane % 2 * 8;
+  auto not_kept = [&](int at) {
+    if constexpr (D == 128) asm volatile("" : "+v"(at));
+    return at;
+  };
   // S^T of a tile: st[kb][i] is key 32 kb + 8 (i/4) + 4 hi + i%4
   auto scores = [&](const u4_t* lt, f16_t (&st)[KB]) {
-    auto at = [&](int kb, int ks) { return *reinterpret_cast<const u4_t*>(reinterpret_cast<const char*>(lt) + ka[ks] + kb * 32 * CH * 16); };
+    const int ka = not_kept(k_own);
+    auto at = [&](int kb, int ks) { return *reinterpret_cast<const u4_t*>(reinterpret_cast<const char*>(lt) + (ka ^ 32 * ks) + kb * 32 * CH * 16); };
     u4_t x[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) x[ks] = at(0, ks);
@@ -152,11 +160,11 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
     }
   };
   // V^T's operand: dim 128 v + 32 b + n, keys 16 kc + 8 (e/4) + 4 hi + e%4
-  auto v_operand = [&](const u4_t* lt, int kc, int v, int b) {
+  auto v_operand = [&](const u4_t* lt, int va, int kc, int v, int b) {
     u4_t y;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const char* at = reinterpret_cast<const char*>(lt) + va[b][h] + (v * LV + kc * 16 * VCH) * 16;
+      const char* at = reinterpret_cast<const char*>(lt) + (va ^ 64 * b ^ 32 * h) + (v * LV + (kc * 16 + h * 8) * VCH) * 16;
       const u2_t w = __builtin_bit_cast(
           u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)at));
       y[2 * h] = w.x;
@@ -214,16 +222,17 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
       for (int i = 0; i < 4; ++i) p[kc][i] = pack2<BF>(st[kc / 2][8 * (kc % 2) + 2 * i], st[kc / 2][8 * (kc % 2) + 2 * i + 1]);
   };
   auto products = [&](const u4_t* lt, const u4_t (&p)[KC]) {
+    const int va = not_kept(v_own);
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) o[v][b] = mma32<BF>(v_operand(lt, kc, v, b), p[kc], o[v][b]);
+        for (int b = 0; b < 4; ++b) o[v][b] = mma32<BF>(v_operand(lt, va, kc, v, b), p[kc], o[v][b]);
   };
-  // Any tile: keys that a row does not see have weight 0.  odd: V holds an infinity or NaN, which 0 * inf would carry into
+  // Any tile: keys that a row does not see have weight 0.  ODD: V may hold an infinity or NaN, which 0 * inf would carry into
   // rows that do not see its key.
-  auto any_tile = [&](int t, const u4_t* lt, bool odd) {
+  auto any_tile = [&]<bool ODD>(int t, const u4_t* lt, bool odd) {
     const int j0 = t * BN;
     // this wave's rows: does any see the tile, do all see all of it?
     const int ra = tile * BM + rb * 32, wa = ra / a.nrep, wz = min(ra + 31, rows - 1) / a.nrep;
@@ -244,7 +253,7 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
     }
     u4_t p[KC];
     softmax(st, p);
-    if (!mask || !odd) {
+    if (!ODD || !mask || !odd) {
       products(lt, p);
       return;
     }
@@ -310,9 +319,10 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
     whole_tile(tile1);
     ++i;
   }
-  for (; i < count; ++i) {
-    u4_t* lt = i & 1 ? tile1 : tile0;
-    // each wave looks through the part of V that it has loaded itself for infinities and NaN
+  row_of(not_kept(n));
+  // tile i is there; does its V hold an infinity or NaN?  Each wave looks through the part that it has loaded itself.
+  auto next_is_odd = [&] {
+    const u4_t* lt = i & 1 ? tile1 : tile0;
     arrived();
     uint32_t top = 0;
 #pragma unroll
@@ -328,10 +338,15 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
     bool odd = false;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) odd |= lodd[i & 1][w] != 0;
-    odd = __builtin_amdgcn_readfirstlane(odd);
+    return __builtin_amdgcn_readfirstlane(odd) != 0;
+  };
+  auto tail_tile = [&]<bool ODD>(bool odd) {
     if (i + 1 < count) fetch(tile_at(i + 1), i & 1 ? tile0 : tile1);
-    any_tile(tile_at(i), lt, odd);
-  }
+    any_tile.template operator()<ODD>(tile_at(i), i & 1 ? tile1 : tile0, odd);
+  };
+  // (from the first odd tile on in a loop of its own, whose need of registers would make both spill: 40 us for four tiles)
+  for (; i < count && !next_is_odd(); ++i) tail_tile.template operator()<false>(false);
+  for (; i < count; ++i) tail_tile.template operator()<true>(next_is_odd());
   {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(y[0]) + __uint_as_float(y[1]);
