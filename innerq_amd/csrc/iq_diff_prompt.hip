@@ -444,5 +444,5 @@ extern "C" int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_
                           : (bf ? launch.operator()<64, true>() : launch.operator()<64, false>());
   if (st || !weights || !Nk) return st;
   return launch_prompt_weights({(const uint16_t*)q, (const uint16_t*)k, sq_n, sq_h, sk_n, sk_h, stats, weights, sw_s, sw_h, T,
-                                cu_q, cu_k, S, N, Nk, Hq, nrep, 0, sc, causal ? 1 : 0, window, 2, 0, nullptr, 1}, D, bf, (hipStream_t)stream);
+                                cu_q, cu_k, S, N, Nk, Hq, nrep, 0, sc, causal ? 1 : 0, window, 2, 0, nullptr, 1, 0}, D, bf, (hipStream_t)stream);
 }

@@ -71,6 +71,7 @@ struct WeighArgs {
   int shares;
   float* part;
   int steps;  // tiles of keys of a workgroup
+  int chunk_bits;  // rows of a chunk that a share takes in one go
 };
 // its workspace: the stats, then the sums
 size_t prompt_weights_bytes(int S, int N, int Nk, int Hq, int H);  // (a multiple of 16)

@@ -553,7 +553,7 @@ int attention(const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t 
                           : (bf ? launch.operator()<64, true>() : launch.operator()<64, false>());
   if (st || !weights || !Nk) return st;
   return launch_prompt_weights({a.q, a.k, sq_n, sq_h, sk_n, sk_h, a.stats, weights, sw_s, sw_h, T, cu_q, cu_k, S, N, Nk, Hq,
-                                Hq / H, 0, sc, causal ? 1 : 0, window, 1, 0, nullptr, 1}, D, bf, (hipStream_t)stream);
+                                Hq / H, 0, sc, causal ? 1 : 0, window, 1, 0, nullptr, 1, 0}, D, bf, (hipStream_t)stream);
 }
 
 }  // namespace

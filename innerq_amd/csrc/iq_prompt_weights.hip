@@ -8,7 +8,7 @@
 // two halves of a tile's rows.
 //
 // A key at the beginning of a long prompt is seen by all its rows, so up to SHARES workgroups share a key: each takes every
-// so-manieth CHUNK of the rows, and a second launch adds their sums (how many rows a sequence has is not known on the host:
+// so-manieth chunk of the rows, and a second launch adds their sums (how many rows a sequence has is not known on the host:
 // a share that finds none ends at once, and the shares are as many as leave GROUPS workgroups).  Rows are added in a fixed
 // order: no atomics.  (One share / 16 at most, a whole call, bf16, 32 heads over 8, D = 128: a prompt of 2000 tokens 134 / 90 us,
 // of 8192 947 / 845, 16 of 25 .. 2000 324 / 307, 64 of 100 59 / 63.)
@@ -25,7 +25,7 @@ namespace {
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, BR = 64;  // rows of a tile
 constexpr int BK = 32 * WAVES / 2;                        // keys of a workgroup
-constexpr int CHUNK = 2048, SHARES = 16, GROUPS = 8192;  // rows (times heads) of a chunk; most workgroups of a key, in all
+constexpr int CHUNK_BITS = 11, SHARES = 16, GROUPS = 8192;  // rows (times heads) of a chunk at most; most workgroups of a key, in all
 
 // Few rows over many keys: a workgroup holds up to FEW rows in LDS and walks over a.steps times BK keys, as many as leave
 // FEW_GROUPS workgroups (two per CU: their beginning, some 10 us, is then paid once).
@@ -125,8 +125,8 @@ struct Block {
 __device__ __forceinline__ bool big_base(float2 st) { return __any(fabsf(st.x) > 65536.f); }
 
 // the first chunk of a share that has rows which see the keys (or one behind them)
-__device__ __forceinline__ int share_chunk(const Keys& x, int share, int shares) {
-  const int c = x.v0 / CHUNK, ahead = share - c % shares;
+__device__ __forceinline__ int share_chunk(const WeighArgs& a, const Keys& x, int share) {
+  const int shares = a.shares, c = x.v0 >> a.chunk_bits, ahead = share - c % shares;
   return c + (ahead < 0 ? ahead + shares : ahead);
 }
 
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
   const int head0 = kvh / a.maps * a.nrep * a.maps + kvh % a.maps;  // its query heads: head0 + i * maps
   Keys x;
   if (!keys_of(a, blockIdx.x / H, BK, x)) return;
-  const int first_chunk = share_chunk(x, blockIdx.y, a.shares);
-  if (first_chunk * CHUNK >= x.v1) return;
+  const int first_chunk = share_chunk(a, x, blockIdx.y), chunk_rows = 1 << a.chunk_bits;
+  if (first_chunk * chunk_rows >= x.v1) return;
   const int q0 = x.q0, j0 = x.j0;
   // of the rows, [vf, vg) see all of the keys
   const int vf = a.causal ? max(x.j1 - 1 - x.off, 0) * a.nrep : 0;
@@ -238,9 +238,9 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
     const int first = (a.window ? max(row + x.off + 1 - a.window, 0) : 0) - base;
     Block<D, BF>::add_some(here, qa, kx, a.scale.c, big, st, first, last, acc);
   };
-  for (int chunk = first_chunk; chunk * CHUNK < x.v1; chunk += a.shares) {
-    v0 = max(x.v0, chunk * CHUNK);
-    v1 = min(x.v1, (chunk + 1) * CHUNK);
+  for (int chunk = first_chunk; chunk * chunk_rows < x.v1; chunk += a.shares) {
+    v0 = max(x.v0, chunk * chunk_rows);
+    v1 = min(x.v1, (chunk + 1) * chunk_rows);
     tiles = (v1 - v0 + BR - 1) / BR;
     begin = place_of(v0);
     mine = place_of(v0 + rw * 32 + n);
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64) void add_kernel(WeighArgs a) {
   for (int j = x.j0 + threadIdx.x; j < x.j1 && j < a.T; j += 64) {
     float sum = 0.f;
     for (int z = 0; z < a.shares; ++z)
-      if (share_chunk(x, z, a.shares) * CHUNK < x.v1) sum += a.part[(int64_t(z) * H + kvh) * a.Nk + x.k0 + j];
+      if (share_chunk(a, x, z) << a.chunk_bits < x.v1) sum += a.part[(int64_t(z) * H + kvh) * a.Nk + x.k0 + j];
     a.weights[x.s * a.sw_s + kvh * a.sw_h + j] += sum;
   }
 }
@@ -386,9 +386,19 @@ inline bool few(int S, int N, int Nk, int Hq, int H) {
 
 inline size_t stats_bytes(int N, int Hq) { return (size_t(N) * Hq * sizeof(float2) + 15) / 16 * 16; }
 
+// Rows of a chunk, as their logarithm: 2048, or as many fewer, 256 at least, as make 1024 workgroups of a call of long sequences
+// (by their mean; bf16, 32 heads over 8, D = 128, a whole call, us, 2048 / this: a prompt of 300 tokens 28.4 / 21.8, of 500 39.0 /
+// 27.0, of 1500 77.7 / 69.4; of 77, one chunk, 16.0).
+inline int chunk_bits(int S, int N, int Nk, int Hq, int H) {
+  const int64_t rows = int64_t(N) * (Hq / H) / S, groups = (int64_t(Nk) / BK + S) * H;
+  int bits = CHUNK_BITS;
+  while (rows >= 1024 && bits > 8 && groups * ceil_div(rows, 1 << bits) < 1024) --bits;
+  return bits;
+}
+
 // workgroups that share a key
 inline int shares_of(int S, int N, int Nk, int Hq, int H) {
-  const int64_t chunks = ceil_div(int64_t(N) * (Hq / H), CHUNK), most = GROUPS / ((int64_t(Nk) / BK + S) * H);
+  const int64_t chunks = ceil_div(int64_t(N) * (Hq / H), 1 << chunk_bits(S, N, Nk, Hq, H)), most = GROUPS / ((int64_t(Nk) / BK + S) * H);
   const int64_t n = chunks < most ? chunks : most;
   return few(S, N, Nk, Hq, H) || n < 1 ? 1 : n < SHARES ? int(n) : SHARES;
 }
@@ -415,7 +425,7 @@ size_t prompt_weights_bytes(int S, int N, int Nk, int Hq, int H) {
 }
 
 bool prompt_weights_fit(int S, int N, int Nk, int Hq, int H) {
-  return int64_t(N) * (Hq / H) <= INT32_MAX - SHARES * CHUNK &&
+  return int64_t(N) * (Hq / H) <= INT32_MAX - (SHARES << CHUNK_BITS) &&
          (int64_t(Nk) / BK + S) * H <= UINT32_MAX / FEW_THREADS / shares_of(S, N, Nk, Hq, H);
 }
 
@@ -426,6 +436,7 @@ int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream) {
   a.steps = !f || steps < 1 ? 1 : steps < MOST_STEPS ? int(steps) : MOST_STEPS;
   a.slots = int(int64_t(a.Nk) / (f ? FEW_KEYS * a.steps : BK) + a.S);  // first_slot(S) at most
   a.shares = shares_of(a.S, a.N, a.Nk, a.Hq, H);
+  a.chunk_bits = chunk_bits(a.S, a.N, a.Nk, a.Hq, H);
   a.part = a.shares > 1 ? (float*)((char*)a.stats + stats_bytes(a.N, a.Hq)) : nullptr;
   const dim3 grid(unsigned(int64_t(a.slots) * H), unsigned(a.shares));
   if (D == 128) return bf ? launch<128, true>(a, f, grid, stream) : launch<128, false>(a, f, grid, stream);
