@@ -205,3 +205,20 @@ def test_refusals():
             f(*a, 0.1)
     assert f(q[:0], k, v, i32([0, 0, 0]), lam, 0.1, c).shape == (0, 4, 128)
     assert bool((f(q, k[:0], v[:0], c, lam, 0.1, i32([0, 0, 0])) == 0).all())
+
+
+@pytest.mark.parametrize("keys", [[70], [3], [70, 100], [64, 127, 130], [199]])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,Hq", [(64, 4), (128, 4), (128, 12)])
+def test_infinities_in_some_tiles(D, Hq, dtype, keys):
+    """Tiles of keys with and without an infinity in V follow one another at the ends of the rows' keys."""
+    q, k, v, lam, cu, cu_k = prompts(17, [200, 100], 0, 4, Hq, D, dtype)
+    exact, bound = (torch.cat(x).to(DEV) for x in zip(*(X.attention(*(x[a:b].cpu() for x in (q, k, v)), lam.cpu(), 0.1)
+                                                       for a, b in zip(cu, cu[1:]))))
+    bad, hit = v.clone(), torch.zeros_like(exact, dtype=torch.bool)
+    for n, key in enumerate(keys):
+        bad[key, 1, 7 * n + 1] = float("inf") if n % 2 == 0 else float("-inf")  # of pair 1
+        hit[key:200, Hq // 4:, 7 * n + 1] = True
+    out = ops.diff_prompt_attention(q, k, bad, i32(cu), lam, 0.1)
+    assert not bool(out[hit].isfinite().any())
+    assert bool(((out.double() - exact).abs() <= bound)[~hit].all())

@@ -469,3 +469,10 @@ def test_prompt_sequences_inside(lens, past, head, causal):
         assert torch.equal(got[1 + s, :, n:], before[1 + s, :, n:])
         want, bound = E.weights(qc[cu[s]:cu[s + 1]], kc[cu_k[s]:cu_k[s + 1]], 0.2, causal, 0)
         check(got[1 + s, :, :n], before[1 + s, :, :n], want, bound, s)
+
+
+@pytest.mark.parametrize("Hq", [3, 5, 8])
+@pytest.mark.parametrize("kw", [dict(), dict(causal=False), dict(window=100), dict(window=1000)])
+def test_prompt_alone(Hq, kw):
+    """One long prompt, whose keys several workgroups share in small chunks of rows, at heads that do and do not divide them."""
+    check_prompts(*prompts(20 + Hq, [1100], 0, 1, Hq, 64, torch.float16), 0.125, **kw)
