@@ -7,18 +7,19 @@
 // A step that drops a page of 64 tokens from 2048 moves some 60 rows and the recent ones, where keeping the order would
 // move all of them.
 //
-// Three launches, one behind the other (each reads what the next one writes over):
+// Three steps, one behind the other (each reads what the next one writes over), each a launch, or all of them in one by a
+// workgroup per (sequence, run of heads):
 //   select  one workgroup per (sequence, run of heads): the B-th largest weight by three passes over the bits of the
 //           weights (11, 11, 10 from the top), then the lists of free places and of the rows that come.
 //   fill    rows and their weights into the free places: sources from B on, destinations below B, in any order.
 //   shift   the last `recent` rows: where they overlap their destinations one workgroup per (sequence, head), in order,
 //           each batch read whole before it is written.  Weights from `keep` on become 0.
 //
-// Bound: the latency of three launches, in each of which loads wait for each other (length, weights or plan, table, page).
-// 32 sequences of 2112 tokens to 2048, 256 of them recent (8 heads, D = 128): 12, 12 and 12 - 14 us.  8 of 32768 to 2048, 512
-// recent: 26, 25 and 13.  There a third of select's time loads the weights and counts their first digits (weights of one size share
-// bins, whose atomics take turns: one copy of the counts and single words in place of fours 30 us), and fill reads rows from
-// all over: a token's V lies in D / 8 sectors of 32 bytes with 7 other tokens', so 8 bytes come for each that is used.
+// Bound: latency: in each step loads wait for each other (length, weights or lists, table, page).  32 sequences of 2112 tokens to
+// 2048, 256 of them recent (8 heads, D = 128): 24.5 us in one launch, 30 where other data passes between.  8 of 32768 to 2048, 512 recent: 26, 25 and 13 us in three.
+// There a third of select's time loads the weights and counts their first digits (weights of one size share bins, whose atomics
+// take turns: one copy of the counts and single words in place of fours 30 us), and fill reads rows from all over: a token's V
+// lies in D / 8 sectors of 32 bytes with 7 other tokens', so 8 bytes come for each that is used.
 #include "iq_paged.h"
 
 using namespace iq;
@@ -29,6 +30,12 @@ constexpr int SELECT = 1024, FILL = 256, SHIFT = 1024;
 constexpr int BATCH = 4;                        // rows of a lane that are under way together
 constexpr int BITS[3] = {11, 11, 10}, BINS = 1 << 11;
 constexpr int WAVES = SELECT / 64;
+// One launch does it all for up to a workgroup per CU, where each has few rows to move or they are seven eighths of the CUs.
+// us in one launch / in three (8 heads, D = 128; sequences x tokens -> keep, recent):
+//   1 x 80 -> 64, 8  14.9 / 17.9;  1 x 2112 -> 2048, 256  20.8 / 25.1;  32 x 2112 -> 2048, 256  24.5 / 30.6
+//   32 x 8192 -> 2048, 512  84 / 98;  32 x 16384 -> 8192, 1024  246 / 256;  the heads in pairs: 32 x 2112 -> 2048, 256  32.9 / 30.4
+//   8 x 32768 -> 2048, 512  82 / 57;  2 x 16384 -> 8192, 4096  194 / 41
+constexpr int ONE = 256, FEW_ROWS = 512;
 constexpr int KEYS = 32, ROUND = KEYS * SELECT;  // weights of a thread, of a workgroup
 constexpr int COPIES = 2;                       // of the digits' counts, by lane: equal digits of a wave take turns
 
@@ -75,21 +82,23 @@ __device__ __forceinline__ void all_read() {
   __syncthreads();
 }
 
-__global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
+// What a (sequence, run of heads) keeps: the tokens of a sequence that drops any (else 0), and how many rows come; the free
+// places and the rows that come, in their order, to the plan.  By a workgroup of SELECT threads.
+struct Plan {
+  int n, count;
+};
+__device__ __forceinline__ Plan select(const EvictArgs& a, int run) {
   __shared__ int hist[COPIES][BINS];
   __shared__ int found[2];  // the digit, and how many of its keys are wanted
   __shared__ u4_t keys[ROUND / 4];
-  const int runs = a.p.H / a.shared, s = blockIdx.x / runs, h0 = (blockIdx.x - s * runs) * a.shared, tid = threadIdx.x;
+  const int runs = a.p.H / a.shared, s = run / runs, h0 = (run - s * runs) * a.shared, tid = threadIdx.x;
   const float* w = a.w + s * a.sw_s + h0 * a.sw_h;
   float* wo = a.wo + s * a.so_s + h0 * a.so_h;
-  int32_t* plan = plan_of(a, blockIdx.x);
+  int32_t* plan = plan_of(a, run);
   const int n = a.p.lens[s];
   const bool there = n >= 0 && n <= int64_t(a.p.P) * PAGE;
   if (!there && tid == 0) atomicOr(a.p.status, PAGED_BAD_TOKEN);
-  if (!there || n <= a.keep) {
-    if (tid == 0) plan[0] = plan[1] = 0;
-    return;
-  }
+  if (!there || n <= a.keep) return {0, 0};
   const int old = n - a.recent, B = a.keep - a.recent;  // B of the first `old` tokens stay
   if (a.wo != a.w)  // the weights below B (those of free places are written over by the next launch)
     for (int h = 0; h < a.shared; ++h)
@@ -218,9 +227,15 @@ __global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
       for (uint32_t left = in[list]; left; left &= left - 1) to[at++] = first + __builtin_ctz(left);
     }
   }
-  if (tid == 0) {
-    plan[0] = n;
-    plan[1] = count[0];
+  return {n, count[0]};
+}
+
+__global__ __launch_bounds__(SELECT) void select_kernel(EvictArgs a) {
+  const Plan x = select(a, blockIdx.x);
+  if (threadIdx.x == 0) {
+    int32_t* plan = plan_of(a, blockIdx.x);
+    plan[0] = x.n;
+    plan[1] = x.count;
   }
 }
 
@@ -294,18 +309,16 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int s, int h, int 
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(FILL) void fill_kernel(EvictArgs a) {
-  constexpr int U = D / 8, ROWS = FILL / U * BATCH;  // rows of a workgroup's turn
-  const int sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.p.H, h = sh - s * a.p.H;
-  const int32_t* plan = plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared);
-  const int o = threadIdx.x % U, count = plan[1];
-  if (h == 0 && chunk == 0 && threadIdx.x == 0) a.lens_out[s] = plan[0] ? a.keep : a.p.lens[s];
-  for (int r0 = chunk * ROWS + threadIdx.x / U; r0 < count; r0 += a.chunks * ROWS) {
+// the rows that come to their places, by `chunks` workgroups of THREADS
+template <int D, int THREADS>
+__device__ __forceinline__ void fill(const EvictArgs& a, int s, int h, const int32_t* plan, int count, int chunk, int chunks) {
+  constexpr int U = D / 8, ROWS = THREADS / U * BATCH;  // rows of a workgroup's turn
+  const int o = threadIdx.x % U;
+  for (int r0 = chunk * ROWS + threadIdx.x / U; r0 < count; r0 += chunks * ROWS) {
     int from[BATCH], to[BATCH];
 #pragma unroll
     for (int e = 0; e < BATCH; ++e) {
-      const int r = r0 + e * (FILL / U);
+      const int r = r0 + e * (THREADS / U);
       to[e] = plan[2 + min(r, count - 1)];
       from[e] = r < count ? plan[2 + int64_t(a.most) + r] : -1;
     }
@@ -313,13 +326,13 @@ __global__ __launch_bounds__(FILL) void fill_kernel(EvictArgs a) {
   }
 }
 
+// the last rows to their places, and zeros for the weights behind, by `chunks` workgroups of SHIFT threads
 template <int D>
-__global__ __launch_bounds__(SHIFT) void shift_kernel(EvictArgs a) {
+__device__ __forceinline__ void shift(const EvictArgs& a, int s, int h, int n, int chunk, int chunks) {
   constexpr int U = D / 8, ROWS = SHIFT / U * BATCH;
-  const int sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.p.H, h = sh - s * a.p.H;
-  const int o = threadIdx.x % U, n = plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared)[0];
+  const int o = threadIdx.x % U;
   float* wo = a.wo + s * a.so_s + h * a.so_h;
-  const int64_t first = chunk * int64_t(SHIFT) + threadIdx.x, step = int64_t(a.chunks) * SHIFT;
+  const int64_t first = chunk * int64_t(SHIFT) + threadIdx.x, step = int64_t(chunks) * SHIFT;
   if (!n) {  // a sequence that drops nothing
     if (a.wo != a.w)
       for (int64_t i = first; i < a.T; i += step) wo[i] = a.w[s * a.sw_s + h * a.sw_h + i];
@@ -328,7 +341,7 @@ __global__ __launch_bounds__(SHIFT) void shift_kernel(EvictArgs a) {
   const int src = n - a.recent;
   const bool apart = n - a.keep >= a.recent;  // the rows and their places: they move in any order
   if (apart || chunk == 0)
-    for (int r0 = chunk * ROWS; r0 < a.recent; r0 += (apart ? a.chunks : 1) * ROWS) {
+    for (int r0 = chunk * ROWS; r0 < a.recent; r0 += (apart ? chunks : 1) * ROWS) {
       int from[BATCH], to[BATCH];
 #pragma unroll
       for (int e = 0; e < BATCH; ++e) {
@@ -348,6 +361,40 @@ __global__ __launch_bounds__(SHIFT) void shift_kernel(EvictArgs a) {
     all_read();
     for (int i = max(a.keep, src) + threadIdx.x; i < n; i += SHIFT) wo[i] = 0.f;
   }
+}
+
+template <int D>
+__global__ __launch_bounds__(FILL) void fill_kernel(EvictArgs a) {
+  const int sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.p.H, h = sh - s * a.p.H;
+  const int32_t* plan = plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared);
+  if (h == 0 && chunk == 0 && threadIdx.x == 0) a.lens_out[s] = plan[0] ? a.keep : a.p.lens[s];
+  fill<D, FILL>(a, s, h, plan, plan[1], chunk, a.chunks);
+}
+
+template <int D>
+__global__ __launch_bounds__(SHIFT) void shift_kernel(EvictArgs a) {
+  const int sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.p.H, h = sh - s * a.p.H;
+  shift<D>(a, s, h, plan_of(a, int64_t(s) * (a.p.H / a.shared) + h / a.shared)[0], chunk, a.chunks);
+}
+
+// All of it in one launch, a workgroup per (sequence, run of heads).
+template <int D>
+__global__ __launch_bounds__(SELECT) void evict_kernel(EvictArgs a) {
+  static_assert(SELECT == SHIFT);
+  const int runs = a.p.H / a.shared, s = blockIdx.x / runs, h0 = (blockIdx.x - s * runs) * a.shared;
+  const Plan x = select(a, blockIdx.x);
+  all_read();  // (and written: the lists, and the weights below B)
+  for (int h = h0; h < h0 + a.shared; ++h) fill<D, SELECT>(a, s, h, plan_of(a, blockIdx.x), x.count, 0, 1);
+  all_read();
+  for (int h = h0; h < h0 + a.shared; ++h) shift<D>(a, s, h, x.n, 0, 1);
+  if (a.lens_out != a.p.lens && h0 == 0 && threadIdx.x == 0) a.lens_out[s] = x.n ? a.keep : a.p.lens[s];
+}
+// its lengths in place: behind it, as its workgroups read them
+__global__ __launch_bounds__(64) void lens_kernel(EvictArgs a) {
+  const int s = blockIdx.x * 64 + threadIdx.x;
+  if (s >= a.p.S) return;
+  const int n = a.p.lens[s];
+  if (n > a.keep && n <= int64_t(a.p.P) * PAGE) a.lens_out[s] = a.keep;
 }
 
 inline int64_t rows_that_come(int P, int keep, int recent) {
@@ -390,6 +437,15 @@ extern "C" int iq_paged_evict(const iq_paged* p, const float* weights, int64_t s
   EvictArgs a{*p, weights, sw_s, sw_h, weights_out, so_s, so_h, T, keep, recent, sinks, shared, int(most), lens_out,
               (int32_t*)workspace, chunks_of(most, FILL / lanes * BATCH)};
   const hipStream_t q = (hipStream_t)stream;
+  const int64_t groups = int64_t(p->S) * (p->H / shared);
+  if (groups <= ONE && ((most + recent) * shared <= FEW_ROWS || groups >= ONE - ONE / 8)) {
+    if (p->D == 128) evict_kernel<128><<<unsigned(groups), SELECT, 0, q>>>(a);
+    else evict_kernel<64><<<unsigned(groups), SELECT, 0, q>>>(a);
+    if (const int st = launch_status()) return st;
+    if (lens_out != p->lens) return IQ_OK;
+    lens_kernel<<<unsigned(ceil_div(p->S, 64)), 64, 0, q>>>(a);
+    return launch_status();
+  }
   select_kernel<<<p->S * (p->H / shared), SELECT, 0, q>>>(a);
   if (const int st = launch_status()) return st;
   auto rest = [&]<int D>() -> int {

@@ -278,3 +278,22 @@ def test_append_evicted_native(monkeypatch):
                 out = st.append(k, v, table, i32(lens), cu, cos, sin, q, evicted=i32(gone))
                 got.append((out, st.pages.clone(), st.check()))
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and got[0][2] == got[1][2]
+
+
+@pytest.mark.parametrize("S,H,shared", [(70, 4, 1), (300, 2, 2), (33, 8, 1)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_many_sequences_and_heads(S, H, shared, in_place):
+    """More (sequence, run of heads) pairs than CUs, of lengths from none to several pages."""
+    rng = random.Random(41 + S)
+    lens = [rng.choice([0, 1, 20, 64, 65, 100, 130, 250]) for _ in range(S)]
+    st, table, w = case(lens, H, 64, 41 + S, width=4)
+    check(st, table, lens, w, 64, 20, 3, shared, in_place)
+
+
+@pytest.mark.parametrize("shared", [1, 2])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,keep,recent", [([700], 300, 290), ([900, 40], 512, 100), ([2000, 1000], 800, 600)])
+def test_few_pairs_with_many_rows(lens, keep, recent, shared, in_place):
+    """Few (sequence, run of heads) pairs: with few rows to move, and with many, apart from their places and over them."""
+    st, table, w = case(lens, 2, 64, 50 + keep)
+    check(st, table, lens, w, keep, recent, 2, shared, in_place)
