@@ -16,10 +16,10 @@
 //           each batch read whole before it is written.  Weights from `keep` on become 0.
 //
 // Bound: latency: in each step loads wait for each other (length, weights or lists, table, page).  32 sequences of 2112 tokens to
-// 2048, 256 of them recent (8 heads, D = 128): 24.5 us in one launch, 30 where other data passes between.  8 of 32768 to 2048, 512 recent: 26, 25 and 13 us in three.
-// There a third of select's time loads the weights and counts their first digits (weights of one size share bins, whose atomics
-// take turns: one copy of the counts and single words in place of fours 30 us), and fill reads rows from all over: a token's V
-// lies in D / 8 sectors of 32 bytes with 7 other tokens', so 8 bytes come for each that is used.
+// 2048, 256 of them recent (8 heads, D = 128): 24.5 us in one launch, 30 where other data passes between.  8 of 32768 to 2048,
+// 512 recent: 26, 25 and 13 us in three.  There a third of select's time loads the weights and counts their first digits
+// (weights of one size share bins, whose atomics take turns: with one copy of the counts, and words one by one, 30 us), and fill
+// reads rows from all over: a token's V lies in D / 8 sectors of 32 bytes with 7 other tokens', so 8 bytes come for each used.
 #include "iq_paged.h"
 
 using namespace iq;
