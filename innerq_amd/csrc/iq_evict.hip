@@ -30,12 +30,12 @@ constexpr int SELECT = 1024, FILL = 256, SHIFT = 1024;
 constexpr int BATCH = 4;                        // rows of a lane that are under way together
 constexpr int BITS[3] = {11, 11, 10}, BINS = 1 << 11;
 constexpr int WAVES = SELECT / 64;
-// One launch does it all for up to a workgroup per CU, where each has few rows to move or they are seven eighths of the CUs.
-// us in one launch / in three (8 heads, D = 128; sequences x tokens -> keep, recent):
-//   1 x 80 -> 64, 8  14.9 / 17.9;  1 x 2112 -> 2048, 256  20.8 / 25.1;  32 x 2112 -> 2048, 256  24.5 / 30.6
-//   32 x 8192 -> 2048, 512  84 / 98;  32 x 16384 -> 8192, 1024  246 / 256;  the heads in pairs: 32 x 2112 -> 2048, 256  32.9 / 30.4
-//   8 x 32768 -> 2048, 512  82 / 57;  2 x 16384 -> 8192, 4096  194 / 41
-constexpr int ONE = 256, FEW_ROWS = 512;
+// One launch does it all where each (sequence, run of heads) has few rows to move, or there are as many of them as seven eighths of
+// the CUs.  us in one launch / in three (8 heads, D = 128; sequences x tokens -> keep, recent):
+//   1 x 80 -> 64, 8  14.9 / 17.9;  1 x 2112 -> 2048, 256  20.8 / 25.1;  32 of them  24.5 / 30.6;  128  86 / 91
+//   32 x 8192 -> 2048, 512  84 / 98;  32 x 16384 -> 8192, 1024  246 / 256;  64 x 4096 -> 2048, 256  118 / 125
+//   8 x 32768 -> 2048, 512  82 / 57;  2 x 16384 -> 8192, 4096  194 / 41;  32 x 2112 -> 2048, 256, heads in pairs  32.9 / 30.4
+constexpr int FULL = 224, FEW_ROWS = 512;
 constexpr int KEYS = 32, ROUND = KEYS * SELECT;  // weights of a thread, of a workgroup
 constexpr int COPIES = 2;                       // of the digits' counts, by lane: equal digits of a wave take turns
 
@@ -438,7 +438,7 @@ extern "C" int iq_paged_evict(const iq_paged* p, const float* weights, int64_t s
               (int32_t*)workspace, chunks_of(most, FILL / lanes * BATCH)};
   const hipStream_t q = (hipStream_t)stream;
   const int64_t groups = int64_t(p->S) * (p->H / shared);
-  if (groups <= ONE && ((most + recent) * shared <= FEW_ROWS || groups >= ONE - ONE / 8)) {
+  if ((most + recent) * shared <= FEW_ROWS || groups >= FULL) {
     if (p->D == 128) evict_kernel<128><<<unsigned(groups), SELECT, 0, q>>>(a);
     else evict_kernel<64><<<unsigned(groups), SELECT, 0, q>>>(a);
     if (const int st = launch_status()) return st;

@@ -297,3 +297,12 @@ def test_few_pairs_with_many_rows(lens, keep, recent, shared, in_place):
     """Few (sequence, run of heads) pairs: with few rows to move, and with many, apart from their places and over them."""
     st, table, w = case(lens, 2, 64, 50 + keep)
     check(st, table, lens, w, keep, recent, 2, shared, in_place)
+
+
+@pytest.mark.parametrize("shared", [1, 2])
+def test_some_pairs_with_many_rows(shared):
+    """More pairs than one, fewer than CUs, more rows than a workgroup moves by itself."""
+    lens = [900, 30, 640, 641, 1200, 700, 0, 1000, 800, 950]
+    for keep, recent, in_place in ((640, 64, False), (640, 500, True)):
+        st, table, w = case(lens, 4, 64, 60 + recent)
+        check(st, table, lens, w, keep, recent, 2, shared, in_place)
