@@ -10,8 +10,8 @@
 // A wave holds 32 rows of 2 D sums: at D = 128 the 128 accumulators leave room for two waves per SIMD, a workgroup of 8 with
 // tiles of 32 keys; at D = 64 workgroups of 4 with tiles of 64.  (At D = 128 registers spill from the first masked tile on whose V
 // holds an infinity or NaN; when they did in every masked one, four such tiles took 40 us, now 3.)  Bound: as iq_prompt.hip the
-// matrix unit and the softmax beside it.  A prompt of 8192 tokens, 32 query heads over 8 KV heads, D = 128, fp16: 790 us, 1044
-// TFLOP/s, where a 16384^3 library product reaches 1324; 16 packed prompts of 25 .. 2000 tokens, D = 64, bf16: 132 us, 700 TFLOP/s,
+// matrix unit and the softmax beside it.  A prompt of 8192 tokens, 32 query heads over 8 KV heads, D = 128, fp16: 790 - 801 us,
+// 1030 - 1044 TFLOP/s, where a 16384^3 library product reaches 1324; 16 packed prompts of 25 .. 2000 tokens, D = 64, bf16: 132 us, 700 TFLOP/s,
 // first and last tiles of short prompts.  Each map by a call of iq_prompt_attention over both halves of V would take 1.5 times
 // the products (K Q^T twice).
 #include "iq_prompt.h"
