@@ -306,3 +306,11 @@ def test_some_pairs_with_many_rows(shared):
     for keep, recent, in_place in ((640, 64, False), (640, 500, True)):
         st, table, w = case(lens, 4, 64, 60 + recent)
         check(st, table, lens, w, keep, recent, 2, shared, in_place)
+
+
+@pytest.mark.parametrize("shared", [1, 2])
+def test_long_cut_to_few(shared):
+    """More tokens than a workgroup holds keys of at once, of which few stay."""
+    lens = [40000, 33000, 100]
+    st, table, w = case(lens, 2, 64, 70)
+    check(st, table, lens, w, 400, 50, 4, shared, True)
