@@ -695,6 +695,7 @@ __device__ __forceinline__ void weigh_pages(const AttnArgs& a, int block) {
   const int chunk = block / (a.p.S * a.p.H), sh = block - chunk * (a.p.S * a.p.H), s = sh / a.p.H, h = sh - s * a.p.H, head = h / MAPS, map = h - head * MAPS;
   int lo;
   const int n = pages_of(a, s, lo), first = lo + chunk * a.weigh_each, len = min(a.p.lens[s], a.p.P * PAGE);
+  const int low = a.window ? len - a.window : 0;  // the row sees tokens [low, len); the others are left alone, a NaN row's too
   if (n <= 0 || first >= lo + n) return;
   int units = 0, end = 0, per = 1;
   if (a.split) {
@@ -711,7 +712,7 @@ __device__ __forceinline__ void weigh_pages(const AttnArgs& a, int block) {
 #pragma unroll
     for (int i = 0; i < WEIGH_PAGES; ++i) {
       const int page = min(p0 + i * waves, lo + n - 1), t = page * PAGE + lane;
-      there[i] = p0 + i * waves < min(first + a.weigh_each, lo + n) && t < len;
+      there[i] = p0 + i * waves < min(first + a.weigh_each, lo + n) && t < len && t >= low;
       x[i] = a.logits + ((int64_t(sh) * a.p.P + page) * PAGE + lane / 4 * 4) * a.nrep + lane % 4;
       to[i] = a.weights + s * a.sw_s + h * a.sw_h + min(t, len - 1);
       old[i] = *to[i];

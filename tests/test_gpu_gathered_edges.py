@@ -1,0 +1,81 @@
+"""Edges of gathered attention weights on the GPU: what may and may not change where rows are NaN, or only some keys
+count."""
+import random
+
+import pytest
+import torch
+
+from innerq_amd import ops, paged
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def filled(seed, lens, H, D, dtype, width):
+    """A store whose sequences hold random tokens, and its table."""
+    g, rng = torch.Generator().manual_seed(seed), random.Random(seed)
+    pool = len(lens) * width
+    table = i32(rng.sample(range(pool), pool)).view(len(lens), width)
+    st = paged.PagedStore(pool, H, D, DEV, dtype)
+    st.pages.zero_()
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    k, v = (torch.randn(cu[-1], H, D, generator=g).to(dtype).to(DEV) for _ in range(2))
+    st.append(k, v, table, i32([0] * len(lens)), i32(cu))
+    return st, table, g
+
+
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("width", [8, 40])  # a workgroup takes a whole sequence and head; workgroups share them
+@pytest.mark.parametrize("window", [1, 30, 100, 300])
+def test_rows_of_nan_leave_tokens_before_the_window(maps, D, dtype, width, window):
+    """A window that begins inside a page: the page's tokens before it gather nothing, from a row of NaN too."""
+    lens = [200, 500, 130, 64]
+    st, table, g = filled(window, lens, 2, D, dtype, width)
+    q = torch.randn(4, 8, D, generator=g).to(dtype).to(DEV)
+    lam = torch.full((4,), 0.5, device=DEV)
+    clean = torch.randn(4, 2, width * 64 + 5, generator=g).to(DEV)
+
+    def weights(q, table, lens):
+        w = clean.clone()
+        if maps == 1:
+            out = st.attend(q, table, i32(lens), 0.1, window=window, weights=w)
+        else:
+            out = st.diff_attend(q, table, i32(lens), lam, 0.1, window=window, weights=w)
+        return out, w
+
+    def check(w, s, heads, n):
+        low = max(n - window, 0)
+        for h in heads:
+            assert bool(w[s, h, low:n].isnan().all()), (s, h)
+            assert torch.equal(w[s, h, :low], clean[s, h, :low]) and torch.equal(w[s, h, n:], clean[s, h, n:]), (s, h)
+
+    plain = weights(q, table, lens)[1]
+    st.check()
+    for s, n in enumerate(lens):
+        low = max(n - window, 0)
+        assert torch.equal(plain[s, :, :low], clean[s, :, :low]) and torch.equal(plain[s, :, n:], clean[s, :, n:])
+    bad = q.clone()
+    bad[1, 0, 3] = float("nan")  # a query of KV head 0
+    bad[2] = float("inf")        # logits of infinity less infinity, in every head
+    out, w = weights(bad, table, lens)
+    assert bool(out[1, 0].isnan().all()) and bool(out[2].isnan().all())
+    check(w, 1, [0], 500)
+    check(w, 2, [0, 1], 130)
+    assert torch.equal(w[1, 1], plain[1, 1]) and torch.equal(w[0], plain[0]) and torch.equal(w[3], plain[3])
+    # a page outside the pool, and a sequence longer than its table, whose tokens are the table's then
+    bad_table = table.clone()
+    bad_table[1, 499 // 64] = 10 ** 6
+    out, w = weights(q, bad_table, [200, 500, width * 64 + 9, 64])
+    with pytest.raises(RuntimeError, match="outside the pool and a token past"):
+        st.check()
+    assert bool(out[1:3].isnan().all())
+    check(w, 1, [0, 1], 500)
+    check(w, 2, [0, 1], width * 64)
+    assert torch.equal(w[0], plain[0]) and torch.equal(w[3], plain[3])
