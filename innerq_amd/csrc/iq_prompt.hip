@@ -476,8 +476,8 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(PromptArgs a) {
     f4_t y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = part[i * 64];
-    if (st.y == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(st.x - base);
+    // (a share without a key that counts: its sums are 0, or NaN where 0 times a value is, which stays)
+    const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - base);
     l += st.y * f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] += y[i / 4][i % 4] * f;

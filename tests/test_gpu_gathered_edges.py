@@ -79,3 +79,30 @@ def test_rows_of_nan_leave_tokens_before_the_window(maps, D, dtype, width, windo
     check(w, 1, [0, 1], 500)
     check(w, 2, [0, 1], width * 64)
     assert torch.equal(w[0], plain[0]) and torch.equal(w[3], plain[3])
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("D,H,Hq,dtype", [(64, 1, 2, torch.float16), (128, 2, 8, torch.bfloat16)])
+def test_values_behind_logits_of_minus_infinity(value, D, H, Hq, dtype):
+    """An infinity or NaN in V of a key whose logits are minus infinity (0 times it) reaches the rows that see it, whether
+    or not a workgroup has only such keys: as in the call without weights."""
+    g = torch.Generator().manual_seed(3)
+    lens, keys = [6, 9], [4000, 3500]
+    cu, cu_k = i32([0, 6, 15]), i32([0, 4000, 7500])
+    q, k = torch.ones(15, Hq, D), torch.randn(7500, H, D, generator=g)
+    v = torch.randn(7500, H, D, generator=g)
+    q, k, v = (x.to(dtype).to(DEV) for x in (q, k, v))
+    k[:3900, :, 0] = float("-inf")      # of sequence 0 the last 100 keys count, of sequence 1 all
+    v[700, 0, 5] = value
+    v[3990, 0, 9] = value               # a key that counts
+    v[3997, 0, 11] = value              # that the first rows do not see
+    want = ops.prompt_attention(q, k, v, cu, 0.1, cu_k)
+    w = torch.zeros(2, H, 4000, device=DEV)
+    out = ops.prompt_attention(q, k, v, cu, 0.1, cu_k, weights=w)
+    assert bool(w.isfinite().all()) and bool((w[0, :, :3900] == 0).all())
+    r = Hq // H
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[:6, :r, 5] = hit[:6, :r, 9] = hit[3:6, :r, 11] = True
+    assert not bool(want[hit].isfinite().any()) and bool(want[~hit].isfinite().all())
+    assert not bool(out[hit].isfinite().any()) and bool(out[~hit].isfinite().all())
+    assert torch.equal(out.isnan(), want.isnan())
