@@ -354,6 +354,13 @@ __global__ __launch_bounds__(Shape<D>::THREADS, 2) void diff_kernel(DiffArgs a) 
   // The difference, 128 dims at a time: the second map's waves hand theirs to the first map's (the same rows and dims are in
   // the same lanes and registers), which store them through LDS, whole rows at a time.
   float inv = l == 0.f ? 0.f : 1.f / l;
+  if (l == 0.f)  // no key that counts: 0, whatever V holds
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[v][b][i] = 0.f;
   if (a.stats && hi == 0 && vrow < rows) a.stats[int64_t(q0 + row) * a.Hq + 2 * head + map] = float2{base_of(m), inv};
   if (map) inv *= a.lam[head * a.s_lam];
   static_assert(X::MAP_WAVES * 64 * 64 * 4 <= 2 * TILE * 16, "a part of the difference fits the two tiles");

@@ -444,6 +444,11 @@ __global__ __launch_bounds__(THREADS, 2) void prompt_kernel(PromptArgs a) {
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (l == 0.f)  // no key that counts: 0, whatever V holds
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
   if (a.stats && hi == 0 && vrow < rows) a.stats[int64_t(q0 + row) * a.Hq + head] = float2{base_of(m), inv};
   __syncthreads();  // nobody reads tiles any more
   store_rows<D, BF>(a, (wave < 2 ? lk0 : lk1) + (wave & 1) * 32 * CH, o, inv, int64_t(q0 + row) * a.so_n + head * a.so_h,
@@ -483,6 +488,9 @@ __global__ __launch_bounds__(THREADS) void merge_kernel(PromptArgs a) {
     for (int i = 0; i < 16; ++i) o[i] += y[i / 4][i % 4] * f;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (l == 0.f)  // as in prompt_kernel
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0.f;
   if (hi == 0 && b == 0) a.stats[int64_t(x.q0 + row) * a.Hq + head] = float2{base == NEG_INF ? 0.f : base, inv};
   uint16_t* to = a.out + int64_t(x.q0 + row) * a.so_n + head * a.so_h + 32 * b + 4 * hi;
 #pragma unroll

@@ -106,3 +106,38 @@ def test_values_behind_logits_of_minus_infinity(value, D, H, Hq, dtype):
     assert not bool(want[hit].isfinite().any()) and bool(want[~hit].isfinite().all())
     assert not bool(out[hit].isfinite().any()) and bool(out[~hit].isfinite().all())
     assert torch.equal(out.isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("D,H,Hq,dtype", [(64, 2, 2, torch.float16), (128, 2, 8, torch.bfloat16)])
+@pytest.mark.parametrize("past", [0, 4000])  # rows in one workgroup, and shared out
+def test_rows_without_a_key_that_counts(value, D, H, Hq, dtype, past):
+    """Rows that see only keys whose logits are minus infinity are 0, whatever V holds there; so is such a map of
+    differential attention, with the other one as it is."""
+    g = torch.Generator().manual_seed(6)
+    rows, n = 90, 90 + past
+    cu, cu_k = i32([0, rows]), i32([0, n])
+    q, k = torch.ones(rows, Hq, D), torch.randn(n, H, D, generator=g)
+    v = torch.randn(n, H, D, generator=g)
+    k[:, 0, 0] = float("-inf")  # of KV head 0, the first map's
+    v[n - 80, 0, 5] = v[n // 2, 0, 9] = value
+    q, k, v = (x.to(dtype).to(DEV) for x in (q, k, v))
+    r = Hq // H
+    for kw in (dict(), dict(causal=False)):
+        for w in (None, torch.zeros(1, H, n, device=DEV)):
+            out = ops.prompt_attention(q, k, v, cu, 0.1, cu_k, weights=w, **kw)
+            assert bool((out[:, :r] == 0).all()) and bool(out[:, r:].isfinite().all()), (kw, w is None)
+            assert w is None or bool((w[0, 0] == 0).all())
+    fine = v.clone()
+    fine[:, 0] = 0
+    lam, vv = torch.full((Hq // 2,), 0.5, device=DEV), fine.reshape(n, 1, 2 * D)
+    second = -0.5 * ops.prompt_attention(q[:, 1::2], k[:, 1:], fine[:, 1:], cu, 0.1, cu_k).float()
+    out = ops.diff_prompt_attention(q, k, vv, cu, lam, 0.1, cu_k)
+    # each call rounds every weight (by u relatively; fp16's small ones by 2^-25) and its result once
+    u, most = torch.finfo(dtype).eps / 2, float(fine.abs().max())
+    near = 2 * 0.5 * (u + n * 2.0 ** -25) * most + 2 * u * second.abs() + 2.0 ** -24
+    assert bool((out[..., :D] == 0).all()) and bool(((out[..., D:].float() - second).abs() <= 1.01 * near).all())
+    kk = k.clone()
+    kk[:, 1, 0], kk[:, 1, 1] = 0, float("-inf")  # no map has a key that counts
+    out = ops.diff_prompt_attention(q, kk, v.reshape(n, 1, 2 * D), cu, lam, 0.1, cu_k)
+    assert bool((out == 0).all())
