@@ -422,7 +422,7 @@ extern "C" int iq_diff_prompt_attention(const void* q, int64_t sq_n, int64_t sq_
                aligned(lam, 4), IQ_ERR_ALIGN);
   if (weights) {
     // a tile's rows of q in 32 bits
-    IQ_CHECK(sq_n >= 0 && sq_n < (1 << 23) && sq_h >= 0 && sq_h < (1 << 29) / (Hq / H), IQ_ERR_SHAPE);
+    IQ_CHECK(sq_n >= 0 && sq_n < (1 << 23) && sq_h >= 0 && sq_h < (1 << 29) && sq_h * (Hq / H) < (1 << 29), IQ_ERR_SHAPE);
     IQ_CHECK(T >= 0 && sw_s >= 0 && sw_h >= 0, IQ_ERR_SHAPE);
     IQ_CHECK(aligned(weights, 4), IQ_ERR_ALIGN);
   }

@@ -899,7 +899,7 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
   Py_DECREF(key);
   const at::Tensor* w = nullptr;
   if (a[9] != Py_None && (!(w = weights_of(a[9], S, k->size(1), 0, dev)) || Hq > 4096 || q->stride(0) >= 1 << 23 ||
-                          q->stride(1) >= (1 << 29) / (Hq / k->size(1))))
+                          q->stride(1) >= 1 << 29 || q->stride(1) * (Hq / k->size(1)) >= 1 << 29))
     Py_RETURN_NONE;
   const size_t wsb = w ? sv.prompt_ws(int(S), int(N), int(k->size(0)), int(Hq), int(k->size(1)), int(D)) : 0;
   at::Tensor ws;
@@ -947,7 +947,7 @@ PyObject* diff_prompt(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (a[6] != Py_None) cu_k = ints_of(a[6], S + 1, dev);
   if (!lam || !cu_k || (a[6] == Py_None && Nk != N)) Py_RETURN_NONE;
   if (a[10] != Py_None && (!(w = weights_of(a[10], S, H, 0, dev)) || q->stride(0) >= 1 << 23 ||
-                           q->stride(1) >= (1 << 29) / (Hq / H)))
+                           q->stride(1) >= 1 << 29 || q->stride(1) * (Hq / H) >= 1 << 29))
     Py_RETURN_NONE;
   const double scale = PyFloat_AsDouble(a[5]);
   if (scale == -1.0 && PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
