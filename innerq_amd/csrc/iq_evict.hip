@@ -421,7 +421,8 @@ extern "C" int iq_paged_evict(const iq_paged* p, const float* weights, int64_t s
   IQ_CHECK(keep > 0 && recent >= 0 && sinks >= 0 && int64_t(recent) + sinks <= keep, IQ_ERR_SHAPE);
   IQ_CHECK(shared > 0 && p->H % shared == 0 && T >= int64_t(p->P) * PAGE, IQ_ERR_SHAPE);
   IQ_CHECK(sw_s >= 0 && sw_h >= 0 && so_s >= 0 && so_h >= 0, IQ_ERR_SHAPE);
-  IQ_CHECK(weights != weights_out || (sw_s == so_s && sw_h == so_h), IQ_ERR_SHAPE);
+  // (the strides of one sequence, or of one head, are of no account)
+  IQ_CHECK(weights != weights_out || ((sw_s == so_s || p->S == 1) && (sw_h == so_h || p->H == 1)), IQ_ERR_SHAPE);
   IQ_CHECK(int64_t(p->S) * p->H <= INT32_MAX / SHIFT && p->P < INT32_MAX / PAGE - SELECT, IQ_ERR_SHAPE);
   IQ_CHECK(aligned(weights, 4) && aligned(weights_out, 4) && aligned(lens_out, 4), IQ_ERR_ALIGN);
   const size_t need = iq_paged_evict_workspace_bytes(p->S, p->P, p->H, keep, recent, shared);

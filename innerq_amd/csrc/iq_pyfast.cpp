@@ -588,7 +588,7 @@ bool paged_of(PyObject* const* a, iq_paged* p, at::ScalarType* dt, int* dev) {
 const at::Tensor* weights_of(PyObject* o, int64_t S, int64_t H, int64_t T, int device) {
   const at::Tensor* t = tensor_of(o);
   if (!t || t->dim() != 3 || t->scalar_type() != at::kFloat || t->get_device() != device || t->size(0) != S || t->size(1) != H ||
-      t->size(2) < T || t->size(2) < 1 || t->stride(2) != 1 || followed(*t))
+      t->size(2) < T || t->size(2) < 1 || (t->size(2) > 1 && t->stride(2) != 1) || followed(*t))
     return nullptr;
   std::pair<int64_t, int64_t> d[2];  // (stride, size), by stride
   int n = 0;

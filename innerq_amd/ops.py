@@ -164,7 +164,7 @@ def check_weights(w: torch.Tensor, name: str, S: int, H: int, T: int, device: to
     """Attention weights that tokens have gathered: fp32 [S, H, T or more] on ``device``, T contiguous; where they are
     ``written``, rows of their own."""
     require_device(w, name, torch.float32)
-    if w.dim() != 3 or w.shape[:2] != (S, H) or w.shape[2] < T or w.device != device or w.stride(2) != 1:
+    if w.dim() != 3 or w.shape[:2] != (S, H) or w.shape[2] < T or w.device != device or (w.shape[2] > 1 and w.stride(2) != 1):
         _shape_error(f"{name} must be an fp32 [{S}, {H}, {T} or more] tensor on {device}, its last dim contiguous, got "
                      f"{tuple(w.shape)} of strides {w.stride()} on {w.device}")
     if written and not _nested(zip(w.stride()[:-1], w.shape[:-1]), w.shape[-1]):

@@ -141,3 +141,34 @@ def test_rows_without_a_key_that_counts(value, D, H, Hq, dtype, past):
     kk[:, 1, 0], kk[:, 1, 1] = 0, float("-inf")  # no map has a key that counts
     out = ops.diff_prompt_attention(q, kk, v.reshape(n, 1, 2 * D), cu, lam, 0.1, cu_k)
     assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_strides_of_one_length(native, monkeypatch):
+    """The stride of a dim of length 1 says nothing: weights of one token, one sequence or one head of any such stride."""
+    if not native:
+        monkeypatch.setattr(ops, "_native", lambda t: None)
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(2, 2, 64, generator=g).half().to(DEV) for _ in range(3))
+    cu = i32([0, 1, 2])
+    a, b = torch.zeros(2, 2, 1, device=DEV), torch.zeros(2, 2, 7, device=DEV)[..., ::7]
+    assert b.shape == (2, 2, 1) and b.stride(2) == 7
+    assert torch.equal(ops.prompt_attention(q, k, v, cu, 0.1, weights=a), ops.prompt_attention(q, k, v, cu, 0.1, weights=b))
+    assert torch.equal(a, b) and bool((a == 1).all())
+    a, b = torch.zeros(2, 2, 1, device=DEV), torch.zeros(2, 2, 7, device=DEV)[..., ::7]
+    lam, vv = torch.ones(1, device=DEV), v.reshape(2, 1, 128)
+    ops.diff_prompt_attention(q, k, vv, cu, lam, 0.1, weights=a)
+    ops.diff_prompt_attention(q, k, vv, cu, lam, 0.1, weights=b)
+    assert torch.equal(a, b) and bool((a == 1).all())
+    # evict in place through another view of the same memory
+    for S, H in ((1, 1), (1, 2), (2, 1)):
+        st, table, g = filled(5, [100] * S, H, 64, torch.float16, 2)
+        w = torch.rand(S, H, 128, generator=g).to(DEV)
+        want = st.evict(table, i32([100] * S), w.clone(), 60, recent=7)[1]
+        for place in range(2):  # (strides of the dims of length 1 that no walk over them takes)
+            x = w.clone()
+            view = x.as_strided(x.shape, (x.stride(0) if S > 1 else 640, x.stride(1) if H > 1 else 1280, 1))
+            st2, table2, _ = filled(5, [100] * S, H, 64, torch.float16, 2)
+            new, out = st2.evict(table2, i32([100] * S), *((x, 60) if place else (view, 60)), recent=7,
+                                 out=view if place else x)
+            assert torch.equal(x, want) and new.tolist() == [60] * S
