@@ -18,18 +18,14 @@
 // took three quarters of its time, without the exponentials seven eighths.  16 packed prompts of 25 .. 2000 tokens: 110 us, 41
 // GFLOP, behind 165 of the attention's; a prompt of 77 tokens 8 us, its loads one behind the other.
 #include "iq_prompt.h"
+#include "iq_prompt_weights.h"
 
 using namespace iq;
 
 namespace {
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, BR = 64;  // rows of a tile
-constexpr int BK = 32 * WAVES / 2;                        // keys of a workgroup
-constexpr int CHUNK_BITS = 11, SHARES = 16, GROUPS = 8192;  // rows (times heads) of a chunk at most; most workgroups of a key, in all
-
-// Few rows over many keys: a workgroup holds up to FEW rows in LDS and walks over a.steps times BK keys, as many as leave
-// FEW_GROUPS workgroups (two per CU: their beginning, some 10 us, is then paid once).
-constexpr int FEW = 256, FEW_GROUPS = 512, MOST_STEPS = 64, FEW_WAVES = 8, FEW_THREADS = 64 * FEW_WAVES, FEW_KEYS = 32 * FEW_WAVES;
+static_assert(BK == 32 * WAVES / 2);
 
 // A slot's sequence and keys (of `bk` a slot), and the rows, as rows times heads one behind the other, that see any of them.
 struct Keys {
@@ -375,33 +371,7 @@ __global__ __launch_bounds__(64) void add_kernel(WeighArgs a) {
   }
 }
 
-// Whether a call has few rows over many keys, by the mean of its sequences: up to FEW rows each, and keys for seven eighths of
-// FEW_GROUPS workgroups (a whole call, us, weigh_few_kernel / weigh_kernel; 32 heads over 8, D = 128, fp16; sequences x rows x keys:
-// 1 x 64 x 4096 33.4 / 30.4, 1 x 64 x 16000 66 / 71, 4 x 64 x 4096 62.9 / 63.0, 4 x 64 x 16000 153 / 179, 16 x 64 x 1100 65 / 71,
-// 16 x 1 x 4096 100 / 125, 16 x 16 x 16000 336 / 427).
-inline bool few(int S, int N, int Nk, int Hq, int H) {
-  return int64_t(N) * (Hq / H) <= int64_t(FEW) * S && int64_t(Nk) >= int64_t(1024) * S &&
-         int64_t(Nk) * H >= int64_t(FEW_KEYS) * (FEW_GROUPS - FEW_GROUPS / 8);
-}
-
 inline size_t stats_bytes(int N, int Hq) { return (size_t(N) * Hq * sizeof(float2) + 15) / 16 * 16; }
-
-// Rows of a chunk, as their logarithm: 2048, or as many fewer, 256 at least, as make 1024 workgroups of a call of long sequences
-// (by their mean; bf16, 32 heads over 8, D = 128, a whole call, us, 2048 / this: a prompt of 300 tokens 28.4 / 21.8, of 500 39.0 /
-// 27.0, of 1500 77.7 / 69.4; of 77, one chunk, 16.0).
-inline int chunk_bits(int S, int N, int Nk, int Hq, int H) {
-  const int64_t rows = int64_t(N) * (Hq / H) / S, groups = (int64_t(Nk) / BK + S) * H;
-  int bits = CHUNK_BITS;
-  while (rows >= 1024 && bits > 8 && groups * ceil_div(rows, 1 << bits) < 1024) --bits;
-  return bits;
-}
-
-// workgroups that share a key
-inline int shares_of(int S, int N, int Nk, int Hq, int H) {
-  const int64_t chunks = ceil_div(int64_t(N) * (Hq / H), 1 << chunk_bits(S, N, Nk, Hq, H)), most = GROUPS / ((int64_t(Nk) / BK + S) * H);
-  const int64_t n = chunks < most ? chunks : most;
-  return few(S, N, Nk, Hq, H) || n < 1 ? 1 : n < SHARES ? int(n) : SHARES;
-}
 
 template <int D, bool BF>
 int launch(const WeighArgs& a, bool few, dim3 grid, hipStream_t stream) {
@@ -432,8 +402,7 @@ bool prompt_weights_fit(int S, int N, int Nk, int Hq, int H) {
 int launch_prompt_weights(WeighArgs a, int D, bool bf, hipStream_t stream) {
   const int H = a.Hq / a.nrep;
   const bool f = few(a.S, a.N, a.Nk, a.Hq, H);
-  const int64_t steps = ceil_div(int64_t(a.Nk) * H, int64_t(FEW_KEYS) * FEW_GROUPS);
-  a.steps = !f || steps < 1 ? 1 : steps < MOST_STEPS ? int(steps) : MOST_STEPS;
+  a.steps = f ? steps_of(a.Nk, H) : 1;
   a.slots = int(int64_t(a.Nk) / (f ? FEW_KEYS * a.steps : BK) + a.S);  // first_slot(S) at most
   a.shares = shares_of(a.S, a.N, a.Nk, a.Hq, H);
   a.chunk_bits = chunk_bits(a.S, a.N, a.Nk, a.Hq, H);
