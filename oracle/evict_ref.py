@@ -45,10 +45,11 @@ def token_words(pages, table_row, n: int, D: int):
 
 def weights(q, k, scale: float, causal=True, window=0):
     """What attention of q [lq, Hq, D] over k [lk, H, D] gives each key: (sum over rows and a group's heads of the softmax
-    weights [H, lk], bound), in 64 bits.  The bound, for a kernel whose logits, statistics and sums are fp32: a logit's dot
-    product is off by D + 8 roundings of its products' absolute sum, the exponential's argument and result by a few more,
-    which moves a weight by (D + 16) 2^-23 (1 + |logit|) relatively; its row's sum over n keys, rescaled by at most n
-    running maxima, by (2 n + 64) 2^-24, and the sum over the rows by one rounding each."""
+    weights [H, lk], bound), in 64 bits.  The bound, for a kernel whose logits, statistics and sums are fp32, is a coarse one
+    (gathered() has one that tells rounded weights from unrounded ones): every weight by (D + 16) 2^-23 (1 + the largest of
+    its row's logits' absolute sums of products) relatively, which is more than its own logit and its row's sum are off by; its
+    row's sum over n keys, rescaled by at most n running maxima, by (2 n + 64) 2^-23; the sum over the rows by one rounding of
+    2^-24 each."""
     lq, Hq, D = q.shape
     lk, H = k.shape[:2]
     r = Hq // H
@@ -68,3 +69,40 @@ def weights(q, k, scale: float, causal=True, window=0):
         out[:, j0:j1] += p.view(H, r, -1).sum(1)
         bound[:, j0:j1] += (p * rel).view(H, r, -1).sum(1)
     return out, 1.01 * (bound + (lq * r + 2) * 2.0 ** -24 * out) + 1e-30
+
+
+def gathered(q, k, scale: float, causal=True, window=0):
+    """weights() of the same arguments, on q's device, with the bound that follows from what the kernels do, small enough
+    that weights rounded to 16 bits break it.  Relatively, with u = 2^-24:
+
+      a logit: its products are exact, their sum in fp32 is off by D roundings (2 u each: the matrix unit may cut) of the
+      products' absolute sum, the factor c = RN(scale log2 e), the multiply-add and what is subtracted by 8 more; the
+      exponential by 16 u:                                 e_j = 2 u ((D + 8) sum |q k| scale + 8), which moves weight j by e_j
+      the row's sum: of weights that are off by e_j:                                            sum_j p_j e_j
+      and of its own roundings.  n keys are taken in tiles of 32 at least, each of which adds once to the sum and may change
+      the base: 2 u for the exponential of the change, u for the product, u for the change itself times what it is, and all
+      changes together are at most twice the row's largest logit; within a tile, between lanes, waves and shares fewer than
+      64 sums:                                             u (6 (n / 32 + 1) + 2 max |logit| + 64)
+      the sum over R rows and heads: in lanes of 32, then between lanes, shares and turns:       u (R / 32 + 64)"""
+    (lq, Hq, D), (lk, H) = q.shape, k.shape[:2]
+    u = 2.0 ** -24
+    out = torch.zeros(H, lk, dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    if not lq or not lk:
+        return out, bound
+    i, j = torch.arange(lq, device=q.device)[:, None], torch.arange(lk, device=q.device)[None]
+    end = i + (lk - lq + 1) if causal else torch.full_like(i, lk)
+    seen = (j < end) & ((j >= end - window) if window else (j >= 0))
+    n = seen.sum(1, keepdim=True)
+    for g in range(Hq):
+        h = g // (Hq // H)
+        x, y = q[:, g].double().contiguous(), k[:, h].double().t().contiguous()
+        s = torch.where(seen, (x @ y) * scale, -torch.inf)
+        size = torch.where(seen, (x.abs() @ y.abs()) * abs(scale), 0.0)
+        p = torch.where(seen, (s - s.amax(1, keepdim=True).clamp(min=-1e300)).exp(), 0.0)
+        p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
+        e = 2 * u * ((D + 8) * size + 8)
+        rel = e + (p * e).sum(1, keepdim=True) + u * (6 * (n / 32 + 1) + 2 * size.amax(1, keepdim=True) + 64)
+        out[h] += p.sum(0)
+        bound[h] += (p * rel).sum(0)
+    return out, 1.01 * (bound + u * (lq * (Hq // H) / 32 + 64) * out) + 1e-30
