@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from innerq_amd import ops, paged
+from oracle import evict_ref as E
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -172,3 +173,71 @@ def test_strides_of_one_length(native, monkeypatch):
             new, out = st2.evict(table2, i32([100] * S), *((x, 60) if place else (view, 60)), recent=7,
                                  out=view if place else x)
             assert torch.equal(x, want) and new.tolist() == [60] * S
+
+
+def gathered_check(st, table, lens, q, w, before, scale, maps, window=0):
+    """w = before + what the stores' keys gather, within the bound that rounded weights would break."""
+    for s, n in enumerate(lens):
+        assert torch.equal(w[s, :, n:], before[s, :, n:]), s
+        if not n:
+            continue
+        k = st.read(table[s:s + 1], i32([0]), i32([0, n]), n)[0]
+        for i in range(maps):
+            want, bound = E.gathered(q[s:s + 1, i::maps], k[:, i::maps], scale, window=window)
+            old = before[s, i::maps, :n].double()
+            worst = ((w[s, i::maps, :n].double() - old - want).abs() - bound - 2.0 ** -24 * (old + want)).amax()
+            assert worst <= 0, (s, i, float(worst))
+
+
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("lens,Hq", [([6000, 700, 1], 2), ([6000, 700, 1], 36), ([400, 500, 0], 8), ([20000], 8)])
+@pytest.mark.parametrize("window", [None, 777])
+def test_a_steps_weights_are_not_rounded(maps, D, dtype, lens, Hq, window):
+    st, table, g = filled(D, lens, 2, D, dtype, -(-max(lens) // 64))
+    q = torch.randn(len(lens), Hq, D, generator=g).to(dtype).to(DEV)
+    lam = torch.full((Hq // 2,), 0.5, device=DEV)
+    w = torch.zeros(len(lens), 2, table.shape[1] * 64, device=DEV)
+    for _ in range(2):  # from nothing, and on top of that
+        before = w.clone()
+        if maps == 1:
+            st.attend(q, table, i32(lens), D ** -0.5, window=window, weights=w)
+        else:
+            st.diff_attend(q, table, i32(lens), lam, D ** -0.5, window=window, weights=w)
+        gathered_check(st, table, lens, q, w, before, D ** -0.5, maps, window or 0)
+    st.check()
+
+
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("width", [8, 40])
+def test_captured_steps(maps, width):
+    """A captured step follows its lengths and table: every replay gives what the eager call gives, all of it finite."""
+    most = width * 64
+    st, table, g = filled(9, [most, most, most], 2, 64, torch.float16, width)
+    ll, lam = i32([most, 30, 400]), torch.full((4,), 0.5, device=DEV)
+    q = torch.randn(3, 8, 64, generator=g).half().to(DEV)
+    clean = torch.rand(3, 2, most, generator=g).to(DEV)
+    w = clean.clone()
+
+    def call(w):
+        return st.attend(q, table, ll, 0.1, weights=w) if maps == 1 else st.diff_attend(q, table, ll, lam, 0.1, weights=w)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(w)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        o = call(w)
+    for n in ([most, 30, 400], [5, most, 0], [64, 1, 65], [0, 0, 0], [400, most, 30]):
+        ll.copy_(i32(n))
+        table.copy_(table.flip(0))
+        w.copy_(clean)
+        graph.replay()
+        torch.cuda.synchronize()
+        x = clean.clone()
+        y = call(x)
+        assert bool(y.isfinite().all()) and torch.equal(o, y) and torch.equal(w, x), n
+        gathered_check(st, table, n, q, w, clean, 0.1, maps)
