@@ -10,9 +10,11 @@
 // A wave holds 32 rows of 2 D sums: at D = 128 the 128 accumulators leave room for two waves per SIMD, a workgroup of 8 with
 // tiles of 32 keys; at D = 64 workgroups of 4 with tiles of 64.  (At D = 128 registers spill from the first masked tile on whose V
 // holds an infinity or NaN; when they did in every masked one, four such tiles took 40 us, now 3.)  Bound: as iq_prompt.hip the
-// matrix unit and the softmax beside it.  A prompt of 8192 tokens, 32 query heads over 8 KV heads, D = 128, fp16: 790 - 801 us,
-// 1030 - 1044 TFLOP/s, where a 16384^3 library product reaches 1324; 16 packed prompts of 25 .. 2000 tokens, D = 64, bf16: 132 us, 700 TFLOP/s,
-// first and last tiles of short prompts.  Each map by a call of iq_prompt_attention over both halves of V would take 1.5 times
+// matrix unit and the softmax beside it.  A prompt of 8192 tokens, 32 query heads over 8 KV heads, D = 128, fp16: 765 - 801 us,
+// 1030 - 1078 TFLOP/s, where a 16384^3 library product reaches 1324; D = 64, bf16: 421 us, 980 TFLOP/s of 1380; 16 packed prompts of
+// 25 .. 2000 tokens, D = 64, bf16: 129 - 137 us, 676 - 719 TFLOP/s, what is less than a long prompt's being first and last tiles and a
+// chip that short prompts do not fill.  A workgroup walks over all keys of its rows, however few there are: 64 rows behind 16000 keys
+// on 4 sequences, D = 128, fp16: 575 us on 32 workgroups.  Each map by a call of iq_prompt_attention over both halves of V would take 1.5 times
 // the products (K Q^T twice).
 #include "iq_prompt.h"
 

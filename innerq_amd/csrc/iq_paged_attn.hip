@@ -21,11 +21,13 @@
 // 4 bytes per query head and token where the codes of a key that four heads share are 80, and the second launch reads them
 // back beside its merging (weigh_pages).  The logits of 4 tokens and all heads lie side by side, so that lanes write whole
 // lines.  8 sequences of 32768 tokens, fp16: 77 us (61 with stores that reach no memory) and 16 for merge and weights, 336 MB of
-// pages and 34 MB of logits twice; 48 of 286 .. 16001, bf16: 86 and 17.
+// pages and 34 MB of logits twice; 48 of 286 .. 16001, bf16: 86 - 91 and 17, the vector unit busy 47 % of the clocks.
 //
 // Differential attention (iq_diff_paged_attention, at the end): both maps of a pair of heads in one workgroup, so that V's
 // codes are read and converted once.  8 sequences of 32768 tokens, 32 query heads over 8, D = 64, fp16: 168 MB in 40 us, the
-// rate of a large copy; 3 new tokens on 24 of 93 .. 6001, D = 128, bf16: 40 and 6 for the merge, bound by the conversion.
+// rate of a large copy (with the keys' weights 48 and 15); 3 new tokens on 24 of 93 .. 6001, D = 128, bf16: 39 and 6 for the
+// merge, bound by no unit: a wave holds both maps' sums over 2 D dims, so that a SIMD has one wave, whose loads, conversions,
+// products and exponentials follow one another with nothing beside them (vector unit busy 33 % of the clocks, matrix unit 5 %).
 //
 // The exponentials are rounded because the matrix unit's two operands have one type, that of V's values: each weight
 // moves by half a step at most, and its sum takes it unrounded (outputs' error 1.1 - 1.4 times that of fp32 weights,
@@ -875,6 +877,14 @@ struct Launch {
 // The lengths are on the device, so the table's width P stands for them: a caller whose tables are wider than any sequence
 // passes the columns that are needed (16 sequences of 500 tokens: P = 8 8.2 us, P = 512 13.2; bf16 10.8, 16.7).
 // Two maps: a group for each where there are more than 8 rows (a tile of 8 would read its pages again for the others).
+// The same widths for two maps, whose items are half as many (P pages each, 8 KV heads, D = 128, fp16; us whole / shared out):
+//   1 x 8 13.0 / 14.6;  1 x 12 15.8 / 14.8;  8 x 16 19.1 / 15.3;  16 x 16 19.2 / 19.9;  16 x 24 25.0 / 20.0;  32 x 16 20.0 / 22.6;
+//   32 x 24 25.6 / 25.5;  64 x 32 34.3 / 40.6;  64 x 40 40.6 / 45.0;  4 new tokens, 1 x 8 17.7 / 19.8, 16 x 16 26.1 / 26.3, 64 x 32
+//   45.5 / 49.2;  bf16, 16 x 16 23.8 / 22.1
+// and with the keys' weights, where whole items take a second launch too:
+//   1 x 8 11.9 / 11.4;  1 x 12 13.4 / 11.7;  16 x 8 12.6 / 15.0;  16 x 16 16.1 / 17.7;  16 x 24 19.2 / 18.7;  32 x 24 21.0 / 26.3;
+//   64 x 32 44.1 / 47.1;  64 x 40 57.4 / 57.6;  two maps: 1 x 8 17.5 / 16.0;  16 x 8 18.4 / 18.0;  16 x 16 25.0 / 21.8;
+//   16 x 24 31.4 / 22.4;  32 x 16 26.3 / 25.8;  64 x 32 48.6 / 49.6
 inline Launch plan_of(int S, int P, int m, int nrep, int heads, int D, int maps) {
   const int64_t rows = int64_t(m) * nrep, pages = int64_t(S) * heads * P * ceil_div(rows, ROWS);
   Launch p;

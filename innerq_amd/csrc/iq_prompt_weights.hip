@@ -11,7 +11,7 @@
 // so-manieth chunk of the rows, and a second launch adds their sums (how many rows a sequence has is not known on the host:
 // a share that finds none ends at once, and the shares are as many as leave GROUPS workgroups).  Rows are added in a fixed
 // order: no atomics.  (One share / 16 at most, a whole call, bf16, 32 heads over 8, D = 128: a prompt of 2000 tokens 134 / 90 us,
-// of 8192 947 / 845, 16 of 25 .. 2000 324 / 307, 64 of 100 59 / 63.)
+// of 8192 947 / 846, 16 of 25 .. 2000 324 / 307, 64 of 100 59 / 63.)
 //
 // Bound: neither unit alone.  2048 rows by 2048 keys of 64 heads: vector unit busy 49 % of the clocks (16 exponentials and 32
 // multiply-adds per 16 logits of a lane, and as much again around them), matrix unit 31 %; without the tiles' loads the launch
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(THREADS, 4) void weigh_kernel(WeighArgs a) {
 
 // The same for few rows over many keys.  The rows (up to FEW; more in turns) stay in LDS with their statistics, and a wave
 // takes 32 of each step's FEW_KEYS keys over all of them: no barriers, and each key's sum is one wave's.  (64 rows behind 16000
-// keys on 4 sequences, 8 KV heads, D = 128: 85 us by weigh_kernel, 52 - 55 here, where reading the keys takes 28 at a copy's rate
+// keys on 4 sequences, 8 KV heads, D = 128: 85 us by weigh_kernel, 52 here, where reading the keys takes 28 at a copy's rate
 // and the products 25 at a library product's.)
 template <int D, bool BF>
 __global__ __launch_bounds__(FEW_THREADS, 4) void weigh_few_kernel(WeighArgs a) {
